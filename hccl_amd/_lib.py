@@ -39,6 +39,54 @@ class WideSeg(ctypes.Structure):
     ]
 
 
+_ranks_field = ctypes.POINTER(ctypes.c_void_p)
+
+
+class RmsNorm(ctypes.Structure):
+    """hcclx_rms_norm_t of include/hcclx_ops.h."""
+    _fields_ = [(k, ctypes.c_uint32) for k in ("n", "rows", "row_elems")] + [
+        ("dtype", ctypes.c_int), ("out_dtype", ctypes.c_int), ("eps", ctypes.c_float)] + [
+        (k, _ranks_field) for k in ("x", "residual", "weight", "total", "out")]
+
+
+class RmsNormGrad(ctypes.Structure):
+    """hcclx_rms_norm_grad_t."""
+    _fields_ = [(k, ctypes.c_uint32) for k in ("n", "rows", "row_elems")] + [
+        ("dtype", ctypes.c_int), ("eps", ctypes.c_float)] + [
+        (k, _ranks_field) for k in ("dy", "total", "weight", "dtotal", "dx", "dweight")]
+
+
+class FfnShape(ctypes.Structure):
+    """hcclx_ffn_shape_t."""
+    _fields_ = [(k, ctypes.c_uint32) for k in ("n", "capacity", "dim", "hidden")] + [
+        ("rows", ctypes.c_uint64), ("dtype", ctypes.c_int), ("activation", ctypes.c_int), ("counts", ctypes.c_void_p),
+        ("counts_per_rank", ctypes.c_uint32), ("count_unit", ctypes.c_uint32)]
+
+
+class GatedFfn(ctypes.Structure):
+    """hcclx_gated_ffn_t."""
+    _fields_ = [("shape", FfnShape), ("x_dtype", ctypes.c_int)] + [
+        (k, _ranks_field) for k in ("x", "w_gate", "w_up", "w_down", "out")] + [("saved", ctypes.c_void_p)]
+
+
+class GatedFfnGrad(ctypes.Structure):
+    """hcclx_gated_ffn_grad_t."""
+    _fields_ = [("shape", FfnShape)] + [(k, _ranks_field) for k in ("dy", "x", "w_gate", "w_up", "w_down")] + [
+        ("saved", ctypes.c_void_p)] + [(k, _ranks_field) for k in ("dx", "dw_gate", "dw_up", "dw_down")]
+
+
+class AdamWTensor(ctypes.Structure):
+    """hcclx_adamw_tensor_t."""
+    _fields_ = [("count", ctypes.c_uint64)] + [
+        (k, ctypes.c_void_p) for k in ("param", "grad", "m", "v", "m_scale", "v_scale", "copy")] + [("weight_decay", ctypes.c_float)]
+
+
+class AdamWStep(ctypes.Structure):
+    """hcclx_adamw_step_t."""
+    _fields_ = [(k, ctypes.c_double) for k in ("lr", "beta1", "beta2", "eps")] + [
+        ("step", ctypes.c_uint32), ("seed", ctypes.c_uint32), ("grad_scale", ctypes.c_void_p)]
+
+
 _lib = None
 
 
@@ -112,6 +160,18 @@ def load():
     lib.hcclx_allgatherv.restype = ctypes.c_int
     lib.hcclx_allgatherv.argtypes = [vpp, vpp, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_int,
                                      ctypes.c_int, ctypes.c_void_p]
+    plan_p = ctypes.POINTER(ctypes.c_void_p)
+    for name, arg in (("rms_norm", RmsNorm), ("rms_norm_grad", RmsNormGrad), ("gated_ffn", GatedFfn), ("gated_ffn_grad", GatedFfnGrad)):
+        fn = getattr(lib, f"hcclx_{name}_plan_create")
+        fn.restype = ctypes.c_int
+        fn.argtypes = [ctypes.POINTER(arg), plan_p]
+    lib.hcclx_gated_ffn_saved_bytes.restype = ctypes.c_uint64
+    lib.hcclx_gated_ffn_saved_bytes.argtypes = [ctypes.c_uint64, ctypes.c_uint32]
+    lib.hcclx_adamw_plan_create.restype = ctypes.c_int
+    lib.hcclx_adamw_plan_create.argtypes = [ctypes.POINTER(AdamWTensor), ctypes.c_uint32, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                            plan_p]
+    lib.hcclx_adamw_step.restype = ctypes.c_int
+    lib.hcclx_adamw_step.argtypes = [ctypes.c_void_p, ctypes.POINTER(AdamWStep), ctypes.c_void_p]
     _lib = lib
     return lib
 

@@ -1264,7 +1264,27 @@ struct hcclx_plan {
     uint64_t algo_bytes = 0;
     std::vector<Batch> batches;
     std::vector<size_t> offsets;
+    std::unique_ptr<PlanWork> work;
 };
+
+namespace hcclx {
+
+int plan_of(const DeviceCtx *ctx, std::unique_ptr<PlanWork> work, uint64_t algo_bytes, uint64_t device_bytes, hcclx_plan_t **plan)
+{
+    hcclx_plan *p = new hcclx_plan;
+    p->device = ctx->device;
+    p->algo_bytes = algo_bytes;
+    p->table_bytes = device_bytes;
+    p->work = std::move(work);
+    *plan = p;
+    return HCCL_SUCCESS;
+}
+
+const PlanWork *work_of(const hcclx_plan_t *plan) { return plan->work.get(); }
+
+int plan_device(const hcclx_plan_t *plan) { return plan->device; }
+
+}  // namespace hcclx
 
 extern "C" {
 
@@ -1531,6 +1551,7 @@ int hcclx_plan_launch(const hcclx_plan_t *plan, void *stream)
     DeviceCtx *ctx = device_ctx();
     if (!ctx) return HCCL_E_RUNTIME;
     if (ctx->device != plan->device) return fail(HCCL_E_PARA, "plan belongs to another device");
+    if (plan->work) return plan->work->launch(ctx, static_cast<hipStream_t>(stream));
     for (size_t i = 0; i < plan->batches.size(); ++i) {
         int rc = launch_batch(ctx, plan->batches[i], plan->d_table + plan->offsets[i], static_cast<hipStream_t>(stream));
         if (rc != HCCL_SUCCESS) return rc;

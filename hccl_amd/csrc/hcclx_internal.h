@@ -2,6 +2,8 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <memory>
+#include <new>
 #include <string>
 #include <vector>
 #include "hccl_types.h"
@@ -147,6 +149,48 @@ struct BlockLaunch {
     void fill(char *h) const;
     BlockTable table(const char *d) const;   // the arrays of a launch table at d
 };
+
+// What a plan launches that is no list of folds and copies (the operators of hcclx_ops.h).
+struct PlanWork {
+    virtual ~PlanWork() = default;
+    virtual int launch(const DeviceCtx *ctx, hipStream_t stream) const = 0;
+};
+// A plan over `work`; algo_bytes and device_bytes are what hcclx_plan_bytes and hcclx_plan_table_bytes answer.
+int plan_of(const DeviceCtx *ctx, std::unique_ptr<PlanWork> work, uint64_t algo_bytes, uint64_t device_bytes, hcclx_plan_t **plan);
+const PlanWork *work_of(const hcclx_plan_t *plan);   // nullptr: a plan of folds and copies
+int plan_device(const hcclx_plan_t *plan);
+
+// Device memory of a plan.
+struct DeviceBlock {
+    char *p = nullptr;
+    DeviceBlock() = default;
+    DeviceBlock(const DeviceBlock &) = delete;
+    DeviceBlock &operator=(const DeviceBlock &) = delete;
+    ~DeviceBlock()
+    {
+        if (p) (void)hipFree(p);
+    }
+    int get(size_t bytes)
+    {
+        HCCLX_HIP(hipMalloc(reinterpret_cast<void **>(&p), bytes));
+        return 0;
+    }
+};
+
+// Runs the body of a C entry point: what C++ throws there (out of host memory) becomes a result.
+template <typename F>
+int guarded(F &&body)
+{
+    try {
+        return body();
+    } catch (const std::bad_alloc &) {
+        set_error("out of memory");   // short enough to need none
+        return HCCL_E_MEMORY;
+    } catch (...) {
+        set_error("internal error");
+        return HCCL_E_INTERNAL;
+    }
+}
 
 // Queues the copy of a launch table from the pinned ring to its place in device memory.
 int upload_table(char *d, const char *h, size_t bytes, hipStream_t stream);

@@ -228,3 +228,110 @@ def moe_gather_combine(expert, dest, perm, tokens, topk, row_elems, dtype, sdisp
     check(_lib.load().hcclx_moe_gather_combine(_ptr_array(expert), _ptr_array(dest), _ptr_array(perm), len(expert), tokens,
                                                topk, row_elems, int(dtype), ctypes.c_void_p(sdispls),
                                                ctypes.c_void_p(rdispls), _ptr_array(out), ctypes.c_void_p(stream)))
+
+
+# ---- Operators next to the collectives (include/hcclx_ops.h).  Each is a plan: created once, launched many times. ----------
+
+ROW8_TAIL = 16       # bytes behind the codes of an 8-bit row: its scale (a float) and zeros
+ADAMW_BLOCK = 256    # elements of a tensor that share the scales of 8-bit states
+ACT_SILU = 0
+ACT_GELU_TANH = 1
+
+
+def _ranks(what, ptrs, n):
+    """An array of n device addresses for a structure's field (None: null)."""
+    if ptrs is None:
+        return None
+    if len(ptrs) != n:
+        raise ValueError(f"{what} has {len(ptrs)} addresses for {n} ranks")
+    return _ptr_array(ptrs)
+
+
+class _OperatorPlan(Plan):
+    def _create(self, entry, *args):
+        self._h = None
+        h = ctypes.c_void_p()
+        check(getattr(_lib.load(), entry)(*args, ctypes.byref(h)))
+        self._h = h
+
+
+class RmsNormPlan(_OperatorPlan):
+    """total = x + residual;  out = total * weight / sqrt(mean(total^2) + eps), for every row of every rank (hcclx_rms_norm_t).
+    x, weight, out, residual and total are lists of device addresses, one per rank; residual and total may be left out.
+    out_dtype FP8E4M3: rows of row_elems codes, the scale and padding (ROW8_TAIL bytes), as moe_dispatch can carry them."""
+
+    def __init__(self, x, weight, out, rows, row_elems, dtype, residual=None, total=None, out_dtype=None, eps=1e-6):
+        n = len(x)
+        a = _lib.RmsNorm(n, rows, row_elems, int(dtype), int(dtype if out_dtype is None else out_dtype), eps, _ranks("x", x, n),
+                         _ranks("residual", residual, n), _ranks("weight", weight, n), _ranks("total", total, n), _ranks("out", out, n))
+        self._create("hcclx_rms_norm_plan_create", ctypes.byref(a))
+
+
+class RmsNormGradPlan(_OperatorPlan):
+    """The norm's gradient: dx of x and of residual, dweight of weight (may be left out), from dy of out, the stored total and,
+    optionally, dtotal, the gradient that reaches total from elsewhere (hcclx_rms_norm_grad_t)."""
+
+    def __init__(self, dy, total, weight, dx, dweight, rows, row_elems, dtype, dtotal=None, eps=1e-6):
+        n = len(dy)
+        a = _lib.RmsNormGrad(n, rows, row_elems, int(dtype), eps, _ranks("dy", dy, n), _ranks("total", total, n),
+                             _ranks("weight", weight, n), _ranks("dtotal", dtotal, n), _ranks("dx", dx, n), _ranks("dweight", dweight, n))
+        self._create("hcclx_rms_norm_grad_plan_create", ctypes.byref(a))
+
+
+def gated_ffn_saved_bytes(rows, hidden):
+    """Bytes that the forward pass of `rows` rows saves for the gradient."""
+    return _lib.load().hcclx_gated_ffn_saved_bytes(rows, hidden)
+
+
+def _ffn_shape(n, capacity, dim, hidden, dtype, rows, counts, counts_per_rank, count_unit, activation):
+    return _lib.FfnShape(n, capacity, dim, hidden, rows, int(dtype), int(activation), counts or None, counts_per_rank, count_unit)
+
+
+class GatedFfnPlan(_OperatorPlan):
+    """out = (act(x w_gate^T) * (x w_up^T)) w_down^T for the rows that every rank has (hcclx_gated_ffn_t): counts is the device
+    address of counts_per_rank numbers per rank, whose sum / count_unit is the rank's number of rows when the plan is launched
+    (moe_route's recv_counts, the number of ranks and its row_elems); 0: capacity rows each.  rows: at most so many in all
+    ranks together.  saved: device address of gated_ffn_saved_bytes(rows, hidden) bytes for GatedFfnGradPlan, or 0."""
+
+    def __init__(self, x, w_gate, w_up, w_down, out, capacity, dim, hidden, dtype, rows=0, counts=0, counts_per_rank=1, count_unit=1,
+                 x_dtype=None, activation=ACT_SILU, saved=0):
+        n = len(x)
+        a = _lib.GatedFfn(_ffn_shape(n, capacity, dim, hidden, dtype, rows, counts, counts_per_rank, count_unit, activation),
+                          int(dtype if x_dtype is None else x_dtype), _ranks("x", x, n), _ranks("w_gate", w_gate, n),
+                          _ranks("w_up", w_up, n), _ranks("w_down", w_down, n), _ranks("out", out, n), saved or None)
+        self._create("hcclx_gated_ffn_plan_create", ctypes.byref(a))
+
+
+class GatedFfnGradPlan(_OperatorPlan):
+    """The gradients of x and of the three weights, from dy of out and what GatedFfnPlan saved for the same shape
+    (hcclx_gated_ffn_grad_t)."""
+
+    def __init__(self, dy, x, w_gate, w_up, w_down, saved, dx, dw_gate, dw_up, dw_down, capacity, dim, hidden, dtype, rows=0, counts=0,
+                 counts_per_rank=1, count_unit=1, activation=ACT_SILU):
+        n = len(dy)
+        a = _lib.GatedFfnGrad(_ffn_shape(n, capacity, dim, hidden, dtype, rows, counts, counts_per_rank, count_unit, activation),
+                              _ranks("dy", dy, n), _ranks("x", x, n), _ranks("w_gate", w_gate, n), _ranks("w_up", w_up, n),
+                              _ranks("w_down", w_down, n), saved or None, _ranks("dx", dx, n), _ranks("dw_gate", dw_gate, n),
+                              _ranks("dw_up", dw_up, n), _ranks("dw_down", dw_down, n))
+        self._create("hcclx_gated_ffn_grad_plan_create", ctypes.byref(a))
+
+
+class AdamWPlan(_OperatorPlan):
+    """The AdamW step over many tensors (hcclx_adamw_tensor_t).  tensors: dicts with count, param, grad, m, v, weight_decay and,
+    optionally, copy (the new parameters in copy_dtype), m_scale and v_scale (state_dtype FP8E4M3: one float each per
+    ADAMW_BLOCK elements); addresses on the device.  step() launches it; launch() is refused."""
+
+    def __init__(self, tensors, grad_dtype, state_dtype, copy_dtype=None):
+        arr = (_lib.AdamWTensor * max(1, len(tensors)))()
+        for a, t in zip(arr, tensors):
+            a.count, a.weight_decay = t["count"], t.get("weight_decay", 0.0)
+            for k in ("param", "grad", "m", "v", "m_scale", "v_scale", "copy"):
+                setattr(a, k, t.get(k) or None)
+        self._create("hcclx_adamw_plan_create", arr, len(tensors), int(grad_dtype), int(state_dtype),
+                     int(grad_dtype if copy_dtype is None else copy_dtype))
+
+    def step(self, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, seed=0, grad_scale=0, stream=0):
+        """step: 1, 2, ...; seed: 32 bits, another one every step (8-bit states); grad_scale: device address of a float that
+        multiplies the gradients, or 0."""
+        a = _lib.AdamWStep(lr, beta1, beta2, eps, step, seed & 0xFFFFFFFF, grad_scale or None)
+        check(_lib.load().hcclx_adamw_step(self._h, ctypes.byref(a), ctypes.c_void_p(stream)))

@@ -29,6 +29,7 @@ class DataType(enum.IntEnum):
     FP64 = 10
     BFP16 = 11
     INT128 = 12
+    FP8E4M3 = 15
 
 
 class ReduceOp(enum.IntEnum):
@@ -47,8 +48,8 @@ def dtype_size(dt):
 
 # the enumerators under their short names, so that `from hccl_amd import types as T; T.BFP16, T.SUM` reads like the
 # C header's HCCL_DATA_TYPE_BFP16 / HCCL_REDUCE_SUM
-INT8, INT16, INT32, FP16, FP32, INT64, UINT64, UINT8, UINT16, UINT32, FP64, BFP16, INT128 = (
+INT8, INT16, INT32, FP16, FP32, INT64, UINT64, UINT8, UINT16, UINT32, FP64, BFP16, INT128, FP8E4M3 = (
     int(DataType.INT8), int(DataType.INT16), int(DataType.INT32), int(DataType.FP16), int(DataType.FP32),
     int(DataType.INT64), int(DataType.UINT64), int(DataType.UINT8), int(DataType.UINT16), int(DataType.UINT32),
-    int(DataType.FP64), int(DataType.BFP16), int(DataType.INT128))
+    int(DataType.FP64), int(DataType.BFP16), int(DataType.INT128), int(DataType.FP8E4M3))
 SUM, PROD, MAX, MIN = int(ReduceOp.SUM), int(ReduceOp.PROD), int(ReduceOp.MAX), int(ReduceOp.MIN)
