@@ -1,4 +1,4 @@
-// Launch interface of the experts' feed-forward kernels (ffn_gemm.h, instantiated per type in ffn_bf16.hip and ffn_f16.hip).
+// Launch interface of the experts' feed-forward kernels (ffn_launch.h, instantiated per type in ffn_bf16.hip and ffn_f16.hip).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -34,6 +34,7 @@ struct FfnArgs {
     char *dproj;    // packed rows of 2 x `hidden` elements: gradients of both products of the forward pass
     float *saved;   // packed rows of 2 x `hidden` floats: both products of the forward pass; may be nullptr (kFfnGateUp)
     char *x16;      // 8-bit rows: packed rows of `dim` elements that hold their codes' values; else nullptr
+    bool x8;        // kFfnGateUp: rows of 8-bit codes
     int act;
 };
 

@@ -60,7 +60,7 @@ struct FfnWork : PlanWork {
     int launch(const DeviceCtx *ctx, hipStream_t st) const override
     {
         hipError_t e = hipSuccess;
-        if (up.x16 != nullptr) {
+        if (up.x8) {
             e = dtype == HCCL_DATA_TYPE_FP16 ? launch_ffn_widen<HCCL_DATA_TYPE_FP16>(up, st) : launch_ffn_widen<HCCL_DATA_TYPE_BFP16>(up, st);
         }
         if (e == hipSuccess) e = product(dtype, kFfnGateUp, up, ctx->num_cus, st);
@@ -113,6 +113,7 @@ int make_ffn(const hcclx_gated_ffn_t &f, hcclx_plan_t **plan)
     const uint64_t held = h_bytes + (small ? round256(static_cast<uint64_t>(rows.most) * rows.dim * 2) : 0);
     if (held != 0 && (rc = w->scratch.get(held)) != HCCL_SUCCESS) return rc;
     w->up.h = w->down.h = w->scratch.p;
+    w->up.x8 = small;
     if (small) w->up.x16 = w->scratch.p + h_bytes;
     const uint64_t weights = 3ull * rows.n * rows.dim * rows.hidden * 2;
     return plan_of(ctx, std::move(w), weights + static_cast<uint64_t>(rows.most) * rows.dim * (small ? 3 : 4), held, plan);

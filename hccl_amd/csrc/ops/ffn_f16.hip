@@ -1,6 +1,6 @@
 // The experts' feed-forward kernels for fp16.
 #include "hccl_types.h"
-#include "ops/ffn_gemm.h"
+#include "ops/ffn_launch.h"
 
 namespace hcclx {
 template hipError_t launch_ffn_widen<HCCL_DATA_TYPE_FP16>(const FfnArgs &, hipStream_t);

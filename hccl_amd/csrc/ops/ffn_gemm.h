@@ -30,8 +30,16 @@ typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 
-constexpr uint32_t kBK = 64;             // k of a stage
 constexpr uint32_t kOut = 0x80000000u;   // an offset behind every range
+constexpr uint32_t kRaw = 0x00027000u;        // last word of a buffer resource: plain bytes, range-checked
+constexpr uint32_t kMostRange = 0x7fffffffu;
+constexpr uint32_t kBK = 64;             // k of a stage: a cache line of a k-wise row
+constexpr uint32_t kWaves = 8;           // of a workgroup, two by four
+constexpr uint32_t kWaveRows = 2;
+constexpr uint32_t kWaveCols = 4;
+constexpr uint32_t kTile = 256;          // rows and columns of a whole tile
+constexpr uint32_t kTableBytes = 1024;
+constexpr uint32_t kLdsBytes = 160 * 1024 - kTableBytes;        // for stages
 
 template <int DT> struct Mma;
 template <> struct Mma<HCCL_DATA_TYPE_BFP16> {
@@ -61,7 +69,53 @@ __device__ __forceinline__ uint2 narrow4(f32x4 v)
     return __builtin_bit_cast(uint2, r);
 }
 
+// Eight codes' values.
+template <int DT>
+__device__ __forceinline__ u32x4 widen8(uint32_t low, uint32_t high)
+{
+    float f[4];
+    from_e4m3(low, f);
+    const uint2 lo = narrow4<DT>(f32x4{f[0], f[1], f[2], f[3]});
+    from_e4m3(high, f);
+    const uint2 hi = narrow4<DT>(f32x4{f[0], f[1], f[2], f[3]});
+    return u32x4{lo.x, lo.y, hi.x, hi.y};
+}
+
+// Two fragments of C as 16-bit values, four columns to a lane: afterwards lanes 0..15 and 32..47 hold columns 0..7 and 8..15 of the
+// first, the others of the second.  16-byte stores of half a cache line per row instead of 8-byte ones of a quarter.
+__device__ __forceinline__ u32x4 pair_up(uint2 first, uint2 second)
+{
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 x = __builtin_amdgcn_permlane16_swap(first.x, second.x, false, false);
+    const u32x2 y = __builtin_amdgcn_permlane16_swap(first.y, second.y, false, false);
+    return u32x4{x[0], y[0], x[1], y[1]};
+}
+// A stretch of memory that results go to or come from, at offsets of 32 bits; what does not exist has the offset kOut, where loads
+// give zeros and stores do nothing.  (No branches: the number of stores of a tile is known when they are waited for.)
+struct Window {
+    __amdgpu_buffer_rsrc_t rsrc;
+    __device__ __forceinline__ explicit Window(const void *base, uint32_t range = kMostRange)
+        : rsrc(__builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, static_cast<int>(range), kRaw))
+    {
+    }
+    __device__ __forceinline__ void store(uint32_t offset, u32x4 v) const { __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, offset, 0, 0); }
+    __device__ __forceinline__ void store_half(uint32_t offset, uint2 v) const
+    {
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{v.x, v.y}, rsrc, offset, 0, 0);
+    }
+    __device__ __forceinline__ f32x4 load(uint32_t offset) const
+    {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, offset, 0, 0));
+    }
+};
+
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ const char *uniform(const char *p)
+{
+    const uint64_t x = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<const char *>(static_cast<uint64_t>(uniform(static_cast<uint32_t>(x >> 32))) << 32 | uniform(static_cast<uint32_t>(x)));
+}
 __device__ __forceinline__ uint32_t of_lane(uint32_t x, uint32_t lane) { return __builtin_amdgcn_readlane(x, lane); }
 
 __device__ __forceinline__ uint32_t inclusive_sum(uint32_t v)
@@ -87,7 +141,14 @@ struct RankRows {
             r = s.capacity;
             if (s.counts != nullptr) {
                 uint64_t sum = 0;
-                for (uint32_t i = 0; i < s.per_rank; ++i) sum += s.counts[static_cast<uint64_t>(j) * s.per_rank + i];
+                const uint64_t *mine = s.counts + static_cast<uint64_t>(j) * s.per_rank;
+                for (uint32_t i = 0; i < s.per_rank; i += 8) {   // eight loads at a time
+                    uint64_t c[8];
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; ++e) c[e] = mine[i + e < s.per_rank ? i + e : i];
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; ++e) sum += i + e < s.per_rank ? c[e] : 0;
+                }
                 const uint64_t rows64 = (sum >> 32) == 0 ? static_cast<uint32_t>(sum) / s.unit : sum / s.unit;
                 r = rows64 < s.capacity ? static_cast<uint32_t>(rows64) : s.capacity;
             }
@@ -111,86 +172,104 @@ struct RankRows {
     }
 };
 
+// A tile of C, or a part of one.
 struct Tile {
     uint32_t rank;
-    uint32_t m0;      // first row, of the rank
     uint32_t rows;    // of the rank
     uint32_t start;   // the rank's first packed row
-    uint32_t nt;      // number of the column tile
+    uint32_t m0;      // first row and column
+    uint32_t n0;
+    uint32_t weight;  // kFfnGradWeights: of w_gate, w_up or w_down
 };
 
-// Which tile workgroup `id` computes.  The eight XCDs take workgroups in turn and have an L2 each: every XCD gets a stretch of
-// tiles of its own, and neighbours in a stretch are kGroup row tiles by a few column tiles, which share operands.
+// Tiles are numbered rank by rank, kGroup rows of tiles at a time, down these first: 32 neighbours are 4 x 8 tiles, which share
+// operands.
 constexpr uint32_t kGroup = 4;
-template <uint32_t BM>
-__device__ __forceinline__ bool locate(const FfnRows &s, uint32_t nts, Tile *t)
+__device__ __forceinline__ void in_groups(uint32_t at, uint32_t mts, uint32_t nts, uint32_t *mt, uint32_t *nt)
 {
-    const RankRows mine(s);
-    const uint32_t tiles = (mine.rows + BM - 1) / BM;
-    const uint32_t upto = inclusive_sum(tiles);
-    const uint32_t total = of_lane(upto, 63);
-    const uint32_t all = total * nts;
-    const uint32_t per = (all + 7) / 8;
-    const uint32_t slot = blockIdx.x / 8;
-    const uint32_t at = (blockIdx.x % 8) * per + slot;
-    if (slot >= per || at >= all) return false;
-    const uint32_t group = at / (kGroup * nts);
-    const uint32_t first = group * kGroup;
-    const uint32_t height = total - first < kGroup ? total - first : kGroup;
+    const uint32_t first = at / (kGroup * nts) * kGroup;
+    const uint32_t height = mts - first < kGroup ? mts - first : kGroup;
     const uint32_t inside = at - first * nts;
-    const uint32_t mt = first + inside % height;
-    t->nt = inside / height;
-    t->rank = __builtin_ctzll(__ballot(upto > mt));
-    t->rows = of_lane(mine.rows, t->rank);
-    t->start = of_lane(mine.start, t->rank);
-    t->m0 = (mt - (of_lane(upto, t->rank) - of_lane(tiles, t->rank))) * BM;
-    return true;
+    *mt = uniform(first + inside % height);   // (a division leaves them in vector registers)
+    *nt = uniform(inside / height);
 }
 
-// Brings R rows (k-wise: of the operand; crosswise: R columns of 64 rows) of a stage to LDS, 16 bytes per lane and load.
-template <uint32_t R, uint32_t WAVES, bool KWISE, bool PAIR>
-struct Stager {
-    static constexpr uint32_t kLoads = R / 8 / WAVES;
-    static_assert(kLoads * 8 * WAVES == R, "every wavefront loads as much");
-    uint32_t offset[kLoads];
-    uint32_t k_at;   // k-wise: of this lane's chunk in a stage
-
-    // ld: bytes of a row of the buffer; cols: crosswise, columns that exist from the tile's first on
-    __device__ __forceinline__ void init(uint32_t wave, uint32_t lane, uint32_t ld, uint32_t cols)
+// How whole tiles are shared out.  T of them on W CUs take T / W rounds and one more for what is left, however little; so what is
+// left is cut into parts, of which a CU has at most one: quarters of up to W / 4 tiles, halves (of the columns) of up to W / 2.
+// The eight XCDs take workgroups in turn and have an L2 each: every XCD gets a run of neighbours out of each round.
+struct Share {
+    uint32_t whole;   // tiles that are not cut
+    uint32_t parts;   // of each tile that is: 2 or 4
+    uint32_t left;    // tiles that are
+    __device__ __forceinline__ Share(uint32_t tiles, uint32_t groups)
     {
-        if constexpr (KWISE) {
-            const uint32_t chunk = (lane % 8) ^ (lane / 8);
-            k_at = chunk * 8;
-#pragma unroll
-            for (uint32_t i = 0; i < kLoads; ++i) {
-                uint32_t row = (wave * kLoads + i) * 8 + lane / 8;
-                if (PAIR) row %= R / 2;
-                offset[i] = row * ld + chunk * 16;
-            }
-        } else {
-            constexpr uint32_t kChunks = R / 8;   // of a row
-            k_at = 0;
-#pragma unroll
-            for (uint32_t i = 0; i < kLoads; ++i) {
-                const uint32_t at = (wave * kLoads + i) * 64 + lane;
-                const uint32_t k = at / kChunks;
-                const uint32_t place = at % kChunks;
-                const uint32_t turn = (k & 3) | ((k >> 3) & 1) << 2;
-                const uint32_t chunk = ((place / 2) ^ turn) * 2 + place % 2;
-                offset[i] = chunk * 8 < cols ? k * ld + chunk * 16 : kOut;
-            }
-        }
+        left = uniform(tiles % groups);
+        parts = left <= groups / 4 ? 4 : 2;
+        if (left > groups / 2) left = 0;
+        whole = tiles - left;
     }
-    // base: of the stage (uniform); range: bytes from there on that exist; left: k-wise, k that exist from the stage's first on
-    __device__ __forceinline__ void issue(const char *base, uint32_t range, uint32_t left, lds_char *lds, uint32_t wave) const
+};
+
+// Columns of C, and of a whole tile.
+template <int KIND>
+__host__ __device__ inline uint32_t columns(const FfnRows &s)
+{
+    return KIND == kFfnGateUp || KIND == kFfnGradHidden ? s.hidden : s.dim;
+}
+template <int KIND> constexpr uint32_t kTileCols = KIND == kFfnGateUp ? kTile / 2 : kTile;   // half of a tile from either weight
+
+// Two loads of 16 bytes per lane, from the range-checked buffer at the lanes' offsets to lds + 16 * lane and 1024 behind.  Written
+// out because the compiler waits for every such load that it knows of before it lets a transposing LDS read go, whatever that
+// reads; here loads and reads keep apart by meet().  There is no register that the loads write.  s_nop: five wait states between
+// a vector instruction that may have written the scalar operands and the first load, one behind a write of m0.
+typedef uint32_t Resource __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void load_to_lds(Resource buffer, uint32_t lds, uint32_t first, uint32_t second)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %4, 0 offen lds\n\t"
+                 "s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %4, 0 offen lds" ::"s"(lds), "s"(lds + 1024), "v"(first), "v"(second),
+                 "s"(buffer) : "memory");
+}
+
+// Brings R rows (k-wise: of the operand; crosswise: R columns of kBK rows) of a stage to LDS.
+template <uint32_t R, bool KWISE, bool PAIR>
+struct Stager {
+    static constexpr uint32_t kLoads = R * kBK * 2 / 1024 / kWaves;
+    static constexpr uint32_t kChunks = KWISE ? kBK / 8 : R / 8;   // of 16 bytes, of a row
+    static constexpr uint32_t kRows = 64 / kChunks;                // of a load
+    static_assert(kLoads * 1024 * kWaves == R * kBK * 2 && kRows * kChunks == 64 && kLoads % 2 == 0, "every wavefront loads as much, in whole rows");
+    uint32_t row_at;   // offset of the first load's row
+    uint32_t chunk;    // and the chunk of it
+
+    // ld: bytes of a row of the buffer
+    __device__ __forceinline__ void init(uint32_t wave, uint32_t lane, uint32_t ld)
     {
-        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, static_cast<int>(range), 0x00027000);
-        const bool beyond = KWISE && k_at >= left;
+        uint32_t row = wave * kLoads * kRows + lane / kChunks;
+        if constexpr (KWISE) {
+            chunk = (lane % 8) ^ (lane / 8);
+            if (PAIR) row %= R / 2;
+        } else {
+            const uint32_t turn = (row & 3) | ((row >> 3) & 1) << 2;
+            chunk = ((lane % kChunks / 2) ^ turn) * 2 + lane % 2;
+        }
+        row_at = row * ld;
+    }
+    // base: of the stage; range: bytes from there on that exist; end: k (k-wise) or columns (crosswise) that do
+    __device__ __forceinline__ void issue(const char *base, uint32_t range, uint32_t end, uint32_t ld, uint32_t lds, uint32_t wave) const
+    {
+        const uint64_t at = reinterpret_cast<uint64_t>(base);
+        const Resource buffer = {uniform(static_cast<uint32_t>(at)), uniform(static_cast<uint32_t>(at >> 32) & 0xffffu), uniform(range), kRaw};
+        uint32_t offset[kLoads];
 #pragma unroll
         for (uint32_t i = 0; i < kLoads; ++i) {
-            const uint32_t o = beyond ? kOut : offset[i];
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void *)(lds + (wave * kLoads + i) * 1024), 16, o, 0, 0, 0);
+            // (crosswise: of the row's number, the first two bits and the fourth turn the chunks; a load is kRows rows further on)
+            constexpr bool kTurns = !KWISE && kRows < 4;
+            static_assert(KWISE || kRows * kLoads <= 8, "the fourth bit is the wavefront's");
+            const uint32_t c = kTurns ? chunk ^ ((i * kRows) & 3) * 2 : chunk;
+            const uint32_t o = c * 8 < end ? row_at + c * 16 : kOut;
+            offset[i] = o + i * kRows * ld;
         }
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads; i += 2) load_to_lds(buffer, uniform(lds + (wave * kLoads + i) * 1024), offset[i], offset[i + 1]);
     }
 };
 
@@ -202,21 +281,23 @@ struct Reader {
     __device__ __forceinline__ explicit Reader(uint32_t lane)
     {
         if constexpr (KWISE) {
-            base = (lane % 16) * 128 + (((lane / 16) ^ (lane & 7)) * 16);
+            base = (lane % 16) * (kBK * 2) + ((lane / 16) ^ (lane % 8)) * 16;
             turn = 0;
         } else {
             const uint32_t k = lane / 16 * 8 + lane % 16 / 4;
-            turn = (k & 3) | ((k >> 3) & 1) << 2;
+            turn = ((k & 3) | ((k >> 3) & 1) << 2) * 32;
             base = k * (R * 2) + lane % 4 * 8;
         }
     }
-    // f: number of the 16 rows in the tile; half: which 32 of the stage's 64 k
+    // f: number of the 16 rows in the tile; half: which 32 k of the stage's
     __device__ __forceinline__ u32x4 operator()(const lds_char *tile, uint32_t f, uint32_t half) const
     {
         if constexpr (KWISE) {
-            return *(const lds_u32x4 *)(tile + (base ^ (half * 64)) + f * 2048);
+            return *(const lds_u32x4 *)(tile + (base ^ (half * 64)) + f * (kBK * 32));
         } else {
-            const lds_char *p = tile + base + (f ^ turn) * 32 + half * (32 * R * 2);
+            uint32_t t = turn;
+            asm("" : "+v"(t));   // (computed for each read: kept for every fragment it would take a register each)
+            const lds_char *p = tile + base + ((f * 32) ^ t) + half * (32 * R * 2);
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p));
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 4 * R * 2));
             struct Both {
@@ -246,141 +327,298 @@ struct Act {
     }
 };
 
-// One operand of a product: where its tile begins and how its stages follow each other.
-struct Operand {
-    const char *base;
-    uint32_t ld;      // bytes of a row
-    uint32_t extent;  // k-wise: rows from the tile's first on; crosswise: columns
+// Where the stages of a tile come from: two pairs of operands along k, one after the other (the second of kFfnGradInput alone).
+struct Feed {
+    const char *a[2];
+    const char *b[2];
+    uint32_t a_ld;       // bytes of a row
+    uint32_t b_ld;
+    uint32_t a_extent;   // k-wise: rows from the tile's first on; crosswise: columns
+    uint32_t b_extent;
+    uint32_t k;          // of each pair
 };
-template <bool KWISE>
-__device__ __forceinline__ void stage_of(const Operand &o, uint32_t rows, uint32_t k0, uint32_t k, const char **base, uint32_t *range)
+template <int KIND, uint32_t BN>
+__device__ __forceinline__ Feed feed_of(const FfnArgs &a, const Tile &t, uint32_t wave)
 {
-    if constexpr (KWISE) {
-        const uint32_t have = o.extent < rows ? o.extent : rows;
-        *base = o.base + static_cast<uint64_t>(k0) * 2;
-        *range = (have - 1) * o.ld + (k - k0) * 2;
+    const uint32_t dim = a.rows.dim;
+    const uint32_t hidden = a.rows.hidden;
+    const uint64_t n0 = t.n0;
+    Feed f;
+    f.a[1] = f.b[1] = nullptr;
+    if constexpr (KIND == kFfnGradWeights) {
+        f.k = t.rows;
+        if (t.weight < 2) {
+            f.a[0] = a.dproj + static_cast<uint64_t>(t.start) * hidden * 4 + (static_cast<uint64_t>(t.weight) * hidden + t.m0) * 2;
+            f.b[0] = a.p[0][t.rank] + n0 * 2;
+            f.a_ld = hidden * 4;
+            f.b_ld = dim * 2;
+            f.a_extent = hidden - t.m0;
+            f.b_extent = dim - t.n0;
+        } else {
+            f.a[0] = a.p[1][t.rank] + static_cast<uint64_t>(t.m0) * 2;
+            f.b[0] = a.h + static_cast<uint64_t>(t.start) * hidden * 2 + n0 * 2;
+            f.a_ld = dim * 2;
+            f.b_ld = hidden * 2;
+            f.a_extent = dim - t.m0;
+            f.b_extent = hidden - t.n0;
+        }
     } else {
-        const uint32_t have = k - k0 < kBK ? k - k0 : kBK;
-        *base = o.base + static_cast<uint64_t>(k0) * o.ld;
-        *range = (have - 1) * o.ld + o.extent * 2;
+        const uint64_t row = static_cast<uint64_t>(t.start) + t.m0;
+        f.a_extent = t.rows - t.m0;
+        if constexpr (KIND == kFfnGateUp) {
+            f.k = dim;
+            f.a[0] = a.x16 != nullptr ? a.x16 + row * dim * 2 : a.p[0][t.rank] + static_cast<uint64_t>(t.m0) * dim * 2;
+            f.b[0] = a.p[wave * (BN / kWaves) >= BN / 2 ? 2 : 1][t.rank] + n0 * dim * 2;   // of the rows that this wavefront stages
+            f.a_ld = f.b_ld = dim * 2;
+            f.b_extent = hidden - t.n0;
+        } else if constexpr (KIND == kFfnDown) {
+            f.k = hidden;
+            f.a[0] = a.h + row * hidden * 2;
+            f.b[0] = a.p[0][t.rank] + n0 * hidden * 2;
+            f.a_ld = f.b_ld = hidden * 2;
+            f.b_extent = dim - t.n0;
+        } else if constexpr (KIND == kFfnGradHidden) {
+            f.k = dim;
+            f.a[0] = a.p[0][t.rank] + static_cast<uint64_t>(t.m0) * dim * 2;
+            f.b[0] = a.p[1][t.rank] + n0 * 2;
+            f.a_ld = dim * 2;
+            f.b_ld = hidden * 2;
+            f.b_extent = hidden - t.n0;
+        } else {
+            f.k = hidden;
+            f.a[0] = a.dproj + row * hidden * 4;
+            f.a[1] = f.a[0] + static_cast<uint64_t>(hidden) * 2;
+            f.b[0] = a.p[0][t.rank] + n0 * 2;
+            f.b[1] = a.p[1][t.rank] + n0 * 2;
+            f.a_ld = hidden * 4;
+            f.b_ld = dim * 2;
+            f.b_extent = dim - t.n0;
+        }
+    }
+    // all of it is the same for the whole wavefront, which the compiler does not always see
+    f.a[0] = uniform(f.a[0]);
+    f.b[0] = uniform(f.b[0]);
+    f.a_ld = uniform(f.a_ld);
+    f.b_ld = uniform(f.b_ld);
+    f.a_extent = uniform(f.a_extent);
+    f.b_extent = uniform(f.b_extent);
+    f.k = uniform(f.k);
+    return f;
+}
+
+// All but the youngest LOADS loads of this wavefront and all its LDS reads are done, and everybody has got here.
+template <int LOADS>
+__device__ __forceinline__ void meet()
+{
+    __builtin_amdgcn_sched_barrier(0);   // the matrix instructions in front stay there and run while this waits
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Asks the scheduler to issue a row's LDS reads, then its matrix instructions.
+template <int ROWS, int MFMAS, int READS>
+__device__ __forceinline__ void spread()
+{
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);   // LDS reads
+        __builtin_amdgcn_sched_group_barrier(0x008, MFMAS, 0);   // matrix instructions
     }
 }
 
-// WM x WN wavefronts of FM x FN fragments each.
-template <int DT, int KIND, int WM, int WN, int FM, int FN>
-__global__ void __launch_bounds__(WM *WN * 64)
-k_ffn(FfnArgs a)
+// Writes a tile of C, or what becomes of it.
+template <int DT, int KIND, int FM, int FN>
+__device__ __forceinline__ void results(const FfnArgs &a, const Tile &t, const f32x4 (&acc)[FM][FN], uint32_t wm, uint32_t wn, uint32_t lane)
 {
-    constexpr uint32_t BM = WM * FM * 16;
-    constexpr uint32_t BN = WN * FN * 16;
-    constexpr uint32_t kWaves = WM * WN;
+    const uint32_t dim = a.rows.dim;
+    const uint32_t hidden = a.rows.hidden;
+    asm volatile("" : "+v"(lane));   // what follows from it is not computed ahead of the products, which need the registers
+    // A lane holds columns 4 (lane / 16) .. + 3 of row lane % 16 of every fragment of C (col_of), and after pair_up() eight columns
+    // of one fragment of two (col_in of the first).  Offsets are from the tile's first row on, in bytes.
+    const uint32_t row_in = wm * (FM * 16) + lane % 16;
+    const uint32_t col_in = (lane / 16 % 2) * 16 + lane / 32 * 8;
+    const uint32_t col_of = lane / 16 * 4;
+    constexpr int kOwn = KIND == kFfnGateUp ? FN / 2 : FN;   // fragments of C across
+    const uint32_t first = t.n0 + wn * (kOwn * 16);
+    if constexpr (KIND == kFfnGradWeights) {
+        const uint32_t width = t.weight == 2 ? hidden : dim;
+        const uint32_t height = t.weight == 2 ? dim : hidden;
+        const Window c(a.p[2 + t.weight][t.rank] + static_cast<uint64_t>(t.m0) * width * 2);
+#pragma unroll
+        for (int m = 0; m < FM; ++m) {
+            const uint32_t row = row_in + m * 16;
+            const bool live = t.m0 + row < height;
+#pragma unroll
+            for (int n = 0; n < FN; n += 2) {
+                const uint32_t col = first + n * 16 + col_in;
+                c.store(live && col < width ? row * width * 2 + col * 2 : kOut, pair_up(narrow4<DT>(acc[m][n]), narrow4<DT>(acc[m][n + 1])));
+            }
+        }
+    } else {
+        const uint64_t packed = static_cast<uint64_t>(t.start) + t.m0;
+        if constexpr (KIND == kFfnGateUp) {
+            const Window to_h(a.h + packed * hidden * 2);
+            const Window to_saved(a.saved + packed * 2 * hidden);
+            const char *wire = a.p[0][t.rank] + static_cast<uint64_t>(t.m0) * (dim + HCCLX_ROW8_TAIL) + dim;   // the scale of row m0, if rows are of 8 bits
+#pragma unroll
+            for (int m = 0; m < FM; ++m) {
+                const uint32_t row = row_in + m * 16;
+                const bool live = t.m0 + row < t.rows;
+                float scale = 1.0f;
+                if (a.x16 != nullptr && live) scale = *reinterpret_cast<const float *>(wire + static_cast<uint64_t>(row) * (dim + HCCLX_ROW8_TAIL));
+                uint2 h[kOwn];
+#pragma unroll
+                for (int n = 0; n < kOwn; ++n) {
+                    const f32x4 g = acc[m][n] * scale;
+                    const f32x4 u = acc[m][n + kOwn] * scale;
+                    const uint32_t col = first + n * 16 + col_of;
+                    if (a.saved != nullptr) {
+                        const bool there = live && col < hidden;
+                        to_saved.store(there ? row * hidden * 8 + col * 4 : kOut, __builtin_bit_cast(u32x4, g));
+                        to_saved.store(there ? row * hidden * 8 + (hidden + col) * 4 : kOut, __builtin_bit_cast(u32x4, u));
+                    }
+                    f32x4 r;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) r[e] = Act(g[e], a.act).value * u[e];
+                    h[n] = narrow4<DT>(r);
+                }
+                if constexpr (kOwn == 2) {
+                    const uint32_t col = first + col_in;
+                    to_h.store(live && col < hidden ? row * hidden * 2 + col * 2 : kOut, pair_up(h[0], h[1]));
+                } else {
+                    const uint32_t col = first + col_of;
+                    to_h.store_half(live && col < hidden ? row * hidden * 2 + col * 2 : kOut, h[0]);
+                }
+            }
+        } else if constexpr (KIND == kFfnGradHidden) {
+            const Window to_h(a.h + packed * hidden * 2);
+            const Window to_d(a.dproj + packed * 2 * hidden * 2);
+            const Window from(a.saved + packed * 2 * hidden);
+#pragma unroll
+            for (int m = 0; m < FM; ++m) {
+                const uint32_t row = row_in + m * 16;
+                const bool live = t.m0 + row < t.rows;
+                f32x4 g[FN], u[FN];
+#pragma unroll
+                for (int n = 0; n < FN; ++n) {
+                    const uint32_t col = first + n * 16 + col_of;
+                    const bool there = live && col < hidden;
+                    g[n] = from.load(there ? row * hidden * 8 + col * 4 : kOut);
+                    u[n] = from.load(there ? row * hidden * 8 + (hidden + col) * 4 : kOut);
+                }
+                uint2 h[FN], dg[FN], du[FN];
+#pragma unroll
+                for (int n = 0; n < FN; ++n) {
+                    f32x4 r, d0, d1;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const Act f(g[n][e], a.act);
+                        r[e] = f.value * u[n][e];
+                        d0[e] = acc[m][n][e] * u[n][e] * f.slope;
+                        d1[e] = acc[m][n][e] * f.value;
+                    }
+                    h[n] = narrow4<DT>(r);
+                    dg[n] = narrow4<DT>(d0);
+                    du[n] = narrow4<DT>(d1);
+                }
+#pragma unroll
+                for (int n = 0; n < FN; n += 2) {
+                    const uint32_t col = first + n * 16 + col_in;
+                    const bool there = live && col < hidden;
+                    to_h.store(there ? row * hidden * 2 + col * 2 : kOut, pair_up(h[n], h[n + 1]));
+                    to_d.store(there ? row * hidden * 4 + col * 2 : kOut, pair_up(dg[n], dg[n + 1]));
+                    to_d.store(there ? row * hidden * 4 + (hidden + col) * 2 : kOut, pair_up(du[n], du[n + 1]));
+                }
+            }
+        } else {
+            const Window c((KIND == kFfnDown ? a.p[1][t.rank] : a.p[2][t.rank]) + static_cast<uint64_t>(t.m0) * dim * 2);
+#pragma unroll
+            for (int m = 0; m < FM; ++m) {
+                const uint32_t row = row_in + m * 16;
+                const bool live = t.m0 + row < t.rows;
+#pragma unroll
+                for (int n = 0; n < FN; n += 2) {
+                    const uint32_t col = first + n * 16 + col_in;
+                    c.store(live && col < dim ? row * dim * 2 + col * 2 : kOut, pair_up(narrow4<DT>(acc[m][n]), narrow4<DT>(acc[m][n + 1])));
+                }
+            }
+        }
+    }
+}
+
+// Tiles of wavefronts of FM x FN fragments each: t and what next(&t) gives after it, until it says no.  The stages of one tile
+// follow those of the one before without a break, so that the first of them are on their way while results are written.
+template <int DT, int KIND, int FM, int FN, typename Next>
+__device__ __forceinline__ void products(const FfnArgs &a, Tile t, char *s_tile, Next &&next)
+{
+    constexpr uint32_t BM = kWaveRows * FM * 16;
+    constexpr uint32_t BN = kWaveCols * FN * 16;
     constexpr bool kPair = KIND == kFfnGateUp;             // half of the columns from either weight
     constexpr bool kAk = KIND != kFfnGradWeights;          // A lies k-wise
     constexpr bool kBk = KIND == kFfnGateUp || KIND == kFfnDown;
     constexpr uint32_t kCols = kPair ? BN / 2 : BN;        // columns of C
     constexpr uint32_t kStage = (BM + BN) * kBK * 2;
-    __shared__ __attribute__((aligned(1024))) char s_tile[2][kStage];
+    constexpr uint32_t kStages = kLdsBytes / kStage;
+    constexpr uint32_t kPairs = KIND == kFfnGradInput ? 2 : 1;
 
-    const FfnRows &s = a.rows;
     const uint32_t wave = uniform(threadIdx.x / 64);
     const uint32_t lane = threadIdx.x & 63;
-    const uint32_t dim = s.dim;
-    const uint32_t hidden = s.hidden;
+    const uint32_t wm = wave / kWaveCols;
+    const uint32_t wn = wave % kWaveCols;
+    auto place = [&](uint32_t slot) { return (lds_char *)s_tile + slot * kStage; };
 
-    // what is multiplied: up to two pairs of operands along k, one after the other
-    Operand oa[2], ob[2];
-    uint32_t ks = 0;          // length of k, of each pair
-    uint32_t pairs = 1;
-    Tile t;
-    uint32_t n0 = 0;
-    uint32_t weight = 0;      // kFfnGradWeights: 0 the projections', 1 w_down's
-    if constexpr (KIND == kFfnGradWeights) {
-        const uint32_t first_tiles = (2 * hidden + BM - 1) / BM * ((dim + BN - 1) / BN);
-        const uint32_t second_tiles = (dim + BM - 1) / BM * ((hidden + BN - 1) / BN);
-        const uint32_t per = (first_tiles + second_tiles + 7) / 8;   // of an XCD and rank
-        const uint32_t rank = blockIdx.x / (per * 8);
-        const uint32_t inside = blockIdx.x % (per * 8);
-        uint32_t at = inside % 8 * per + inside / 8;
-        if (at >= first_tiles + second_tiles) return;
-        weight = at >= first_tiles ? 1 : 0;
-        if (weight != 0) at -= first_tiles;
-        const uint32_t mts = ((weight != 0 ? dim : 2 * hidden) + BM - 1) / BM;
-        const uint32_t nts = ((weight != 0 ? hidden : dim) + BN - 1) / BN;
-        const uint32_t first = at / (kGroup * nts) * kGroup;
-        const uint32_t height = mts - first < kGroup ? mts - first : kGroup;
-        const uint32_t left = at - first * nts;
-        const RankRows mine(s);
-        t.rank = rank;
-        t.rows = of_lane(mine.rows, rank);
-        t.start = of_lane(mine.start, rank);
-        t.m0 = (first + left % height) * BM;
-        t.nt = left / height;
-        n0 = t.nt * BN;
-        ks = t.rows;
-        if (weight == 0) {
-            oa[0] = {a.dproj + static_cast<uint64_t>(t.start) * hidden * 4 + static_cast<uint64_t>(t.m0) * 2, hidden * 4, 2 * hidden - t.m0};
-            ob[0] = {a.p[0][rank] + static_cast<uint64_t>(n0) * 2, dim * 2, dim - n0};
-        } else {
-            oa[0] = {a.p[1][rank] + static_cast<uint64_t>(t.m0) * 2, dim * 2, dim - t.m0};
-            ob[0] = {a.h + static_cast<uint64_t>(t.start) * hidden * 2 + static_cast<uint64_t>(n0) * 2, hidden * 2, hidden - n0};
-        }
-    } else {
-        const uint32_t cols = KIND == kFfnGateUp || KIND == kFfnGradHidden ? hidden : dim;
-        if (!locate<BM>(s, (cols + kCols - 1) / kCols, &t)) return;
-        n0 = t.nt * kCols;
-        const uint64_t row = static_cast<uint64_t>(t.start) + t.m0;
-        const uint32_t rows = t.rows - t.m0;
-        if constexpr (KIND == kFfnGateUp) {
-            ks = dim;
-            const char *x = a.x16 != nullptr ? a.x16 + row * dim * 2 : a.p[0][t.rank] + static_cast<uint64_t>(t.m0) * dim * 2;
-            oa[0] = {x, dim * 2, rows};
-            const char *w = a.p[wave * (BN / kWaves) >= BN / 2 ? 2 : 1][t.rank];   // of the rows that this wavefront stages
-            ob[0] = {w + static_cast<uint64_t>(n0) * dim * 2, dim * 2, hidden - n0};
-        } else if constexpr (KIND == kFfnDown) {
-            ks = hidden;
-            oa[0] = {a.h + row * hidden * 2, hidden * 2, rows};
-            ob[0] = {a.p[0][t.rank] + static_cast<uint64_t>(n0) * hidden * 2, hidden * 2, dim - n0};
-        } else if constexpr (KIND == kFfnGradHidden) {
-            ks = dim;
-            oa[0] = {a.p[0][t.rank] + static_cast<uint64_t>(t.m0) * dim * 2, dim * 2, rows};
-            ob[0] = {a.p[1][t.rank] + static_cast<uint64_t>(n0) * 2, hidden * 2, hidden - n0};
-        } else {
-            ks = hidden;
-            pairs = 2;
-            oa[0] = {a.dproj + row * hidden * 4, hidden * 4, rows};
-            oa[1] = {oa[0].base + static_cast<uint64_t>(hidden) * 2, hidden * 4, rows};
-            ob[0] = {a.p[0][t.rank] + static_cast<uint64_t>(n0) * 2, dim * 2, dim - n0};
-            ob[1] = {a.p[1][t.rank] + static_cast<uint64_t>(n0) * 2, dim * 2, dim - n0};
-        }
-    }
+    Stager<BM, kAk, false> sa;
+    Stager<BN, kBk, kPair> sb;
+    constexpr int kReads = (kAk ? 1 : 2) + (kBk ? 1 : 2);
+    constexpr int kLoads = decltype(sa)::kLoads + decltype(sb)::kLoads;
+    static_assert(kStages >= 2 && kLoads * (kStages - 1) < 64, "two stages fit; the counter of loads holds what is on its way");
 
-    Stager<BM, kWaves, kAk, false> sa;
-    Stager<BN, kWaves, kBk, kPair> sb;
-    sa.init(wave, lane, oa[0].ld, oa[0].extent);
-    sb.init(wave, lane, ob[0].ld, ob[0].extent);
-    const uint32_t steps = (ks + kBK - 1) / kBK;   // of a pair
-    const uint32_t total = steps * pairs;
-    auto stage = [&](uint32_t step, lds_char *lds) {
-        const bool second = KIND == kFfnGradInput && step >= steps;
-        const uint32_t k0 = (second ? step - steps : step) * kBK;
-        const char *base;
-        uint32_t range;
-        stage_of<kAk>(second ? oa[1] : oa[0], BM, k0, ks, &base, &range);
-        sa.issue(base, range, ks - k0, lds, wave);
-        stage_of<kBk>(second ? ob[1] : ob[0], kCols, k0, ks, &base, &range);
-        sb.issue(base, range, ks - k0, lds + BM * kBK * 2, wave);
+    // The loads run ahead of the products: `from` is where they are, `then` what follows (if `more`), `left` k of this pair are to
+    // come in `steps` stages.  A tile has kStages stages at least (of zeros, if need be): when its products begin, all of those
+    // are its own.
+    auto stages_of = [&](const Feed &f) {
+        const uint32_t n = (f.k + kBK - 1) / kBK * kPairs;
+        return n < kStages ? kStages : n;
+    };
+    Feed from = feed_of<KIND, BN>(a, t, wave);
+    Feed then = from;
+    bool more = false;
+    uint32_t left = from.k;
+    uint32_t steps = stages_of(from);
+    uint32_t pair = 0;
+    auto follow = [&] {   // on to the next tile
+        if (!more) return;
+        more = false;
+        from = then;
+        left = from.k;
+        steps = stages_of(from);
+        pair = 0;
+    };
+    auto stage = [&](uint32_t slot) {
+        const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)s_tile)) + slot * kStage;
+        const uint32_t k = left < kBK ? left : kBK;
+        const uint32_t a_rows = kAk ? (from.a_extent < BM ? from.a_extent : BM) : k;
+        const uint32_t b_rows = kBk ? (from.b_extent < kCols ? from.b_extent : kCols) : k;
+        const uint32_t a_range = k == 0 ? 0 : (a_rows - 1) * from.a_ld + (kAk ? k : from.a_extent) * 2;
+        const uint32_t b_range = k == 0 ? 0 : (b_rows - 1) * from.b_ld + (kBk ? k : from.b_extent) * 2;
+        sa.issue(from.a[0], a_range, kAk ? k : from.a_extent, from.a_ld, lds, wave);
+        sb.issue(from.b[0], b_range, kBk ? k : from.b_extent, from.b_ld, lds + BM * kBK * 2, wave);
+        left -= k;
+        from.a[0] += kAk ? kBK * 2 : static_cast<uint64_t>(from.a_ld) * kBK;
+        from.b[0] += kBk ? kBK * 2 : static_cast<uint64_t>(from.b_ld) * kBK;
+        if (KIND == kFfnGradInput && left == 0 && pair == 0) {
+            pair = 1;
+            left = from.k;
+            from.a[0] = from.a[1];
+            from.b[0] = from.b[1];
+        }
+        if (steps != 0) --steps;
+        if (steps == 0) follow();
     };
 
-    const uint32_t wm = wave / WN;
-    const uint32_t wn = wave % WN;
     const Reader<kAk, BM> ra(lane);
     const Reader<kBk, BN> rb(lane);
-    f32x4 acc[FM][FN];
-#pragma unroll
-    for (int m = 0; m < FM; ++m) {
-#pragma unroll
-        for (int n = 0; n < FN; ++n) acc[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
     // the fragments of B that this wavefront takes: of a pair, half from either weight
     auto b_frag = [&](int n) -> uint32_t {
         if constexpr (kPair) {
@@ -390,95 +628,193 @@ k_ffn(FfnArgs a)
             return wn * FN + n;
         }
     };
-
-    if (total != 0) stage(0, (lds_char *)s_tile[0]);
-    for (uint32_t step = 0; step < total; ++step) {
-        __syncthreads();   // this stage's loads have landed, and everybody has read the one before
-        const lds_char *tile = (const lds_char *)s_tile[step & 1];
-        if (step + 1 < total) stage(step + 1, (lds_char *)s_tile[(step + 1) & 1]);
+    // Fragments of 32 k at a time.  While they are multiplied, row of fragments by row, the next ones are read: one of A into the
+    // registers of the row just done, and B's into a second set.  When everybody has read the last of a stage, the one kStages
+    // behind it is loaded into its place; it has the time of kStages - 1 stages to land.
+    f32x4 acc[FM][FN];
+    // (A's rows of fragments take turns with FM + 1 sets of registers, so that the last of a stage is read a row before its end.)
+    u32x4 fa[FM + 1], fb[2][FN];
+    static_assert(FM >= FN, "every row of fragments reads one of B, until it has them all");
+    auto first_half = [&](const lds_char *tile) {   // multiplies it, reads the second half of the stage at `tile`
 #pragma unroll
-        for (uint32_t half = 0; half < 2; ++half) {
-            u32x4 fa[FM], fb[FN];
+        for (int m = 0; m < FM; ++m) {
+            fa[m == 0 ? FM : m - 1] = ra(tile, wm * FM + m, 1);
+            if (m < FN) fb[1][m] = rb(tile + BM * kBK * 2, b_frag(m), 1);
 #pragma unroll
-            for (int m = 0; m < FM; ++m) fa[m] = ra(tile, wm * FM + m, half);
-#pragma unroll
-            for (int n = 0; n < FN; ++n) fb[n] = rb(tile + BM * kBK * 2, b_frag(n), half);
-#pragma unroll
-            for (int m = 0; m < FM; ++m) {
-#pragma unroll
-                for (int n = 0; n < FN; ++n) acc[m][n] = Mma<DT>::run(fb[n], fa[m], acc[m][n]);
-            }
+            for (int n = 0; n < FN; ++n) acc[m][n] = Mma<DT>::run(fb[0][n], fa[m], acc[m][n]);
         }
-    }
+        spread<FM, FN, kReads>();
+    };
+    auto second_half = [&](const lds_char *tile) {   // multiplies it, reads the first half of the stage at `tile`
+#pragma unroll
+        for (int m = 0; m < FM; ++m) {
+            // (row m of the second half has the registers of row m - 1 of the first)
+            const int free = m == 0 ? FM - 1 : m - 2;
+            if (free >= 0) fa[free] = ra(tile, wm * FM + free, 0);
+            if (m < FN) fb[0][m] = rb(tile + BM * kBK * 2, b_frag(m), 0);
+#pragma unroll
+            for (int n = 0; n < FN; ++n) acc[m][n] = Mma<DT>::run(fb[1][n], fa[m == 0 ? FM : m - 1], acc[m][n]);
+        }
+        fa[FM - 2] = ra(tile, wm * FM + FM - 2, 0);
+        spread<FM, FN, kReads>();
+    };
+    // The stores of a tile's results, which are younger than the loads of the next one's first stages.
+    constexpr int kStores = KIND == kFfnGateUp ? FM * (FN == 4 ? 1 : FN / 2) : KIND == kFfnGradHidden ? 3 * FM * FN / 2 : FM * FN / 2;
+    constexpr int kSavedStores = KIND == kFfnGateUp ? FM * FN : 0;
 
-    // a lane holds columns 4 (lane / 16) .. + 3 of row lane % 16 of every fragment
-    const uint32_t row_in = wm * (FM * 16) + lane % 16;
-    const uint32_t col_in = lane / 16 * 4;
+    bool joined = false;   // the stages that lie in LDS already are this tile's
+    uint32_t slot = 0;
+    for (;;) {
+        const uint32_t total = (joined ? stages_of(then) : steps);
+        Tile after = t;
+        const bool last = !next(&after);
+        const bool apart = !last && KIND == kFfnGradWeights && (after.weight == 2) != (t.weight == 2);   // its rows have other lengths
+        const Feed its = last ? then : feed_of<KIND, BN>(a, after, wave);
+        if (!joined) {
+            sa.init(wave, lane, from.a_ld);
+            sb.init(wave, lane, from.b_ld);
+        }
+        then = its;
+        more = !last && !apart;
+        if (steps == 0) follow();
+        if (!joined) {
+            slot = 0;
 #pragma unroll
-    for (int m = 0; m < FM; ++m) {
-        const uint32_t row = t.m0 + row_in + m * 16;
-        if constexpr (KIND == kFfnGradWeights) {
-            if (row >= (weight != 0 ? dim : 2 * hidden)) continue;
-            const uint32_t width = weight != 0 ? hidden : dim;
-            const char *to = weight != 0 ? a.p[4][t.rank] : row < hidden ? a.p[2][t.rank] : a.p[3][t.rank];
-            const uint32_t r = weight == 0 && row >= hidden ? row - hidden : row;
-            char *c = const_cast<char *>(to) + static_cast<uint64_t>(r) * width * 2;
+            for (uint32_t k = 0; k < kStages; ++k) stage(k);
+            meet<kLoads *(kStages - 1)>();
+        }
+        {   // (read here, not by the last turn of the tile before: writing results needs the registers)
+            const lds_char *tile = place(slot);
 #pragma unroll
-            for (int n = 0; n < FN; ++n) {
-                const uint32_t col = n0 + (wn * FN + n) * 16 + col_in;
-                if (col < width) *reinterpret_cast<uint2 *>(c + static_cast<uint64_t>(col) * 2) = narrow4<DT>(acc[m][n]);
-            }
-        } else {
-            if (row >= t.rows) continue;
-            const uint64_t packed = static_cast<uint64_t>(t.start) + row;
-            if constexpr (KIND == kFfnGateUp) {
-                float scale = 1.0f;
-                if (a.x16 != nullptr) scale = *reinterpret_cast<const float *>(a.p[0][t.rank] + static_cast<uint64_t>(row) * (dim + HCCLX_ROW8_TAIL) + dim);
+            for (int m = 0; m < FM; ++m) fa[m] = ra(tile, wm * FM + m, 0);
 #pragma unroll
-                for (int n = 0; n < FN / 2; ++n) {
-                    const uint32_t col = n0 + (wn * (FN / 2) + n) * 16 + col_in;
-                    if (col >= hidden) continue;
-                    const f32x4 g = acc[m][n] * scale;
-                    const f32x4 u = acc[m][n + FN / 2] * scale;
-                    if (a.saved != nullptr) {
-                        float *to = a.saved + packed * 2 * hidden + col;
-                        *reinterpret_cast<f32x4 *>(to) = g;
-                        *reinterpret_cast<f32x4 *>(to + hidden) = u;
-                    }
-                    f32x4 h;
+            for (int n = 0; n < FN; ++n) fb[0][n] = rb(tile + BM * kBK * 2, b_frag(n), 0);
+        }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) h[e] = Act(g[e], a.act).value * u[e];
-                    *reinterpret_cast<uint2 *>(a.h + (packed * hidden + col) * 2) = narrow4<DT>(h);
-                }
-            } else if constexpr (KIND == kFfnGradHidden) {
+        for (int m = 0; m < FM; ++m) {
 #pragma unroll
-                for (int n = 0; n < FN; ++n) {
-                    const uint32_t col = n0 + (wn * FN + n) * 16 + col_in;
-                    if (col >= hidden) continue;
-                    const float *from = a.saved + packed * 2 * hidden + col;
-                    const f32x4 g = *reinterpret_cast<const f32x4 *>(from);
-                    const f32x4 u = *reinterpret_cast<const f32x4 *>(from + hidden);
-                    f32x4 h, dg, du;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const Act f(g[e], a.act);
-                        h[e] = f.value * u[e];
-                        dg[e] = acc[m][n][e] * u[e] * f.slope;
-                        du[e] = acc[m][n][e] * f.value;
-                    }
-                    *reinterpret_cast<uint2 *>(a.h + (packed * hidden + col) * 2) = narrow4<DT>(h);
-                    char *to = a.dproj + (packed * 2 * hidden + col) * 2;
-                    *reinterpret_cast<uint2 *>(to) = narrow4<DT>(dg);
-                    *reinterpret_cast<uint2 *>(to + static_cast<uint64_t>(hidden) * 2) = narrow4<DT>(du);
+            for (int n = 0; n < FN; ++n) acc[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        for (uint32_t step = 0; step < total; ++step) {
+            first_half(place(slot));
+            if (step == 0 && joined) {
+                if (kSavedStores != 0 && a.saved != nullptr) {
+                    meet<kLoads *(kStages - 2) + kStores + kSavedStores>();
+                } else {
+                    meet<kLoads *(kStages - 2) + kStores>();
                 }
             } else {
-                char *c = const_cast<char *>(KIND == kFfnDown ? a.p[1][t.rank] : a.p[2][t.rank]) + static_cast<uint64_t>(row) * dim * 2;
-#pragma unroll
-                for (int n = 0; n < FN; ++n) {
-                    const uint32_t col = n0 + (wn * FN + n) * 16 + col_in;
-                    if (col < dim) *reinterpret_cast<uint2 *>(c + static_cast<uint64_t>(col) * 2) = narrow4<DT>(acc[m][n]);
-                }
+                meet<kLoads *(kStages - 2)>();
             }
+            stage(slot);
+            slot = slot + 1 == kStages ? 0 : slot + 1;
+            second_half(place(slot));
+        }
+        results<DT, KIND, FM, FN>(a, t, acc, wm, wn, lane);
+        if (last) break;
+        t = after;
+        joined = !apart;
+        if (apart) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            from = then;
+            left = from.k;
+            steps = stages_of(from);
+            pair = 0;
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // nothing may be on its way to LDS when it is given back
+}
+
+// One workgroup per CU.  It takes its share of the whole tiles, one of every round, and then of the parts.  SMALL: of tiles of 128 x
+// 128 alone, for ranks of fewer rows than a whole tile has; then four stages are on their way instead of two.
+template <int DT, int KIND, bool SMALL>
+__global__ void __launch_bounds__(kWaves * 64, 2)
+k_ffn(FfnArgs a)
+{
+    constexpr uint32_t kEdge = SMALL ? kTile / 2 : kTile;
+    constexpr uint32_t kWide = SMALL ? kTileCols<KIND> / 2 : kTileCols<KIND>;
+    __shared__ __attribute__((aligned(1024))) char s_tile[kLdsBytes];
+    struct Rank {
+        uint32_t rows;
+        uint32_t start;
+        uint32_t down;   // tiles
+        uint32_t upto;   // tiles of this rank and those before it
+    };
+    __shared__ Rank s_rank[kFfnRanks];   // (one wavefront's registers would hold it, had the products any to spare)
+    static_assert(sizeof(s_rank) <= kTableBytes, "beside the stages");
+    const FfnRows &s = a.rows;
+    auto count = [](uint32_t size, uint32_t edge) { return (size + edge - 1) / edge; };
+    // kFfnGradWeights: all ranks' tiles of the projections' gradients, then those of w_down's
+    const uint32_t across = count(KIND == kFfnGradWeights ? s.dim : columns<KIND>(s), KIND == kFfnGradWeights ? kEdge : kWide);
+    const uint32_t across1 = count(s.hidden, kEdge);
+    const uint32_t tiles0 = 2 * across1 * across;
+    const uint32_t tiles1 = count(s.dim, kEdge) * across1;
+    if (threadIdx.x < 64) {
+        const RankRows mine(s);
+        const uint32_t down = count(mine.rows, kEdge);
+        s_rank[threadIdx.x] = {mine.rows, mine.start, down, inclusive_sum(down * across)};
+    }
+    __syncthreads();
+    auto tile = [&](uint32_t at, Tile *t) {
+        t->weight = 0;
+        if constexpr (KIND == kFfnGradWeights) {
+            const bool down = at >= s.n * tiles0;
+            at -= down ? s.n * tiles0 : 0;
+            t->rank = uniform(at / (down ? tiles1 : tiles0));
+            in_groups(at % (down ? tiles1 : tiles0), down ? across : 2 * across1, down ? across1 : across, &t->m0, &t->n0);
+            t->weight = uniform(down ? 2 : t->m0 >= across1 ? 1 : 0);
+            t->m0 = uniform(t->m0 - (t->weight == 1 ? across1 : 0));
+        } else {
+            t->rank = __builtin_ctzll(__ballot(s_rank[threadIdx.x & 63].upto > at));
+            const uint32_t down = uniform(s_rank[t->rank].down);
+            in_groups(at - (uniform(s_rank[t->rank].upto) - down * across), down, across, &t->m0, &t->n0);
+        }
+        t->rows = uniform(s_rank[t->rank].rows);
+        t->start = uniform(s_rank[t->rank].start);
+        t->m0 *= kEdge;
+        t->n0 *= kWide;
+    };
+    const uint32_t tiles = KIND == kFfnGradWeights ? s.n * (tiles0 + tiles1) : uniform(s_rank[kFfnRanks - 1].upto);
+    const uint32_t turned = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
+    uint32_t at = turned;
+    uint32_t end = tiles;
+    auto next = [&](Tile *then) {
+        at += gridDim.x;
+        if (at >= end) return false;
+        tile(at, then);
+        return true;
+    };
+    Tile t;
+    if constexpr (SMALL) {
+        if (at >= end) return;
+        tile(at, &t);
+        products<DT, KIND, 4, 2>(a, t, s_tile, next);
+    } else {
+        const Share share(tiles, gridDim.x);
+        end = share.whole;
+        if (at < end) {
+            tile(at, &t);
+            products<DT, KIND, 8, 4>(a, t, s_tile, next);
+        }
+        if (turned >= share.left * share.parts) return;
+        const uint32_t part = uniform(turned % share.parts);
+        tile(uniform(share.whole + turned / share.parts), &t);
+        t.n0 += part % 2 * (kTileCols<KIND> / 2);
+        if (share.parts == 4) t.m0 += part / 2 * (kTile / 2);
+        // a part may have no column or row
+        if constexpr (KIND == kFfnGradWeights) {
+            if (t.n0 >= (t.weight == 2 ? s.hidden : s.dim) || t.m0 >= (t.weight == 2 ? s.dim : s.hidden)) return;
+        } else {
+            if (t.n0 >= columns<KIND>(s) || t.m0 >= t.rows) return;
+        }
+        __syncthreads();   // everybody is done with the last whole tile's LDS
+        auto none = [](Tile *) { return false; };
+        if (share.parts == 2) {
+            products<DT, KIND, 8, 2>(a, t, s_tile, none);
+        } else {
+            products<DT, KIND, 4, 2>(a, t, s_tile, none);
         }
     }
 }
@@ -503,76 +839,24 @@ k_ffn_widen(FfnArgs a)
         const u32x4 codes = *reinterpret_cast<const u32x4 *>(from + c);
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-            float f[8];
-            from_e4m3(codes[2 * q], *reinterpret_cast<float(*)[4]>(f));
-            from_e4m3(codes[2 * q + 1], *reinterpret_cast<float(*)[4]>(f + 4));
-            const uint2 lo = narrow4<DT>(f32x4{f[0], f[1], f[2], f[3]});
-            const uint2 hi = narrow4<DT>(f32x4{f[4], f[5], f[6], f[7]});
-            *reinterpret_cast<u32x4 *>(to + (c + q * 8) * 2) = u32x4{lo.x, lo.y, hi.x, hi.y};
+            *reinterpret_cast<u32x4 *>(to + (c + q * 8) * 2) = widen8<DT>(codes[2 * q], codes[2 * q + 1]);
         }
     }
 }
 
-// Workgroups of a product in tiles of bm x (columns of C per tile): at most one tile more per rank than the rows fill.
-inline uint64_t row_tiles(const FfnRows &s, uint64_t bm)
-{
-    const uint64_t by_rows = s.most / bm + s.n;
-    const uint64_t by_rank = s.n * ((s.capacity + bm - 1) / bm);
-    return by_rows < by_rank ? by_rows : by_rank;
-}
-
-template <int DT, int KIND, int WM, int WN, int FM, int FN>
-hipError_t run(const FfnArgs &a, hipStream_t st)
-{
-    constexpr uint64_t BM = WM * FM * 16;
-    constexpr uint64_t BN = WN * FN * 16;
-    const FfnRows &s = a.rows;
-    uint64_t groups;
-    if (KIND == kFfnGradWeights) {
-        const uint64_t tiles = (2ull * s.hidden + BM - 1) / BM * ((s.dim + BN - 1) / BN) + (s.dim + BM - 1) / BM * ((s.hidden + BN - 1) / BN);
-        groups = (tiles + 7) / 8 * 8 * s.n;
-    } else {
-        const uint64_t cols = KIND == kFfnGateUp || KIND == kFfnGradHidden ? s.hidden : s.dim;
-        const uint64_t width = KIND == kFfnGateUp ? BN / 2 : BN;
-        groups = (row_tiles(s, BM) * ((cols + width - 1) / width) + 7) / 8 * 8;
-    }
-    if (groups > 0xffffffffull / (WM * WN * 64)) return hipErrorInvalidValue;
-    if (groups == 0) return hipSuccess;
-    HCCLX_LAUNCH((k_ffn<DT, KIND, WM, WN, FM, FN>), dim3(static_cast<uint32_t>(groups)), dim3(WM * WN * 64), 0, st, a);
-    return hipGetLastError();
-}
-
 template <int DT, int KIND>
-hipError_t pick(const FfnArgs &a, uint32_t num_cus, hipStream_t st)
+hipError_t run(const FfnArgs &a, bool small, uint32_t num_cus, hipStream_t st)
 {
-    const FfnRows &s = a.rows;
-    const uint64_t cols = KIND == kFfnGateUp || KIND == kFfnGradHidden ? s.hidden : s.dim;
-    const uint64_t rows = KIND == kFfnGradWeights ? 3ull * s.hidden * s.n : s.most;
-    const bool large = (rows / 256) * (cols / 256) >= num_cus && (KIND == kFfnGradWeights || s.most / s.n >= 128);
-    if (large) return run<DT, KIND, 2, 4, 8, 4>(a, st);
-    return run<DT, KIND, 2, 2, 4, 4>(a, st);
+    if (a.rows.most == 0 && KIND != kFfnGradWeights) return hipSuccess;
+    const uint32_t groups = num_cus < 32 ? 32 : num_cus / 32 * 32;   // a multiple of eight, and its half and quarter too
+    if (small) {
+        HCCLX_LAUNCH((k_ffn<DT, KIND, true>), dim3(groups), dim3(kWaves * 64), 0, st, a);
+    } else {
+        HCCLX_LAUNCH((k_ffn<DT, KIND, false>), dim3(groups), dim3(kWaves * 64), 0, st, a);
+    }
+    return hipGetLastError();
 }
 
 }  // namespace ffn
-
-template <int DT>
-hipError_t launch_ffn_widen(const FfnArgs &a, hipStream_t st)
-{
-    if (a.rows.most == 0) return hipSuccess;
-    HCCLX_LAUNCH((ffn::k_ffn_widen<DT>), dim3((a.rows.most + 3) / 4), dim3(256), 0, st, a);
-    return hipGetLastError();
-}
-
-template <int DT>
-hipError_t launch_ffn(FfnKind kind, const FfnArgs &a, uint32_t num_cus, hipStream_t st)
-{
-    switch (kind) {
-        case kFfnGateUp: return ffn::pick<DT, kFfnGateUp>(a, num_cus, st);
-        case kFfnDown: return ffn::pick<DT, kFfnDown>(a, num_cus, st);
-        case kFfnGradHidden: return ffn::pick<DT, kFfnGradHidden>(a, num_cus, st);
-        case kFfnGradInput: return ffn::pick<DT, kFfnGradInput>(a, num_cus, st);
-        default: return ffn::pick<DT, kFfnGradWeights>(a, num_cus, st);
-    }
-}
 
 }  // namespace hcclx

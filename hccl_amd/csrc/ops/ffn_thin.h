@@ -1,0 +1,166 @@
+// The forward products for few rows per rank (a decoding step), where the time is that of reading the weights once.
+//
+// A workgroup takes 16 columns of C (of both weights) of one rank and all its rows, 16 x MB at a time; its eight wavefronts share
+// out k in turns of 64 and add up their parts in LDS.  Weights go from memory to the matrix instruction's registers without LDS:
+// nobody else needs them.  A lane's two chunks of 16 bytes of a turn lie next to each other (k = 16 (lane / 16) .. + 15), so that
+// four lanes read a cache line of a row; the same k of the rows of x, which come from the L2.
+//
+// Bounds as in ffn_gemm.h: range-checked loads give zeros behind the last row, column and k.
+#pragma once
+#include "ops/ffn_gemm.h"
+
+namespace hcclx {
+namespace ffn {
+
+constexpr uint32_t kThinWaves = 8;
+constexpr uint32_t kTurnK = 64;
+constexpr int kAhead = 4;   // turns whose loads are on their way together
+
+template <int DT, int KIND, int MB, bool X8>
+__global__ void __launch_bounds__(kThinWaves * 64)
+k_ffn_thin(FfnArgs a)
+{
+    constexpr int kWeights = KIND == kFfnGateUp ? 2 : 1;
+    static_assert(KIND == kFfnGateUp || (KIND == kFfnDown && !X8), "the forward products");
+    __shared__ f32x4 s_part[kThinWaves][MB * kWeights][64];
+    __shared__ uint32_t s_rows[2];
+    const FfnRows &s = a.rows;
+    const uint32_t rank = blockIdx.y;
+    const uint32_t wave = uniform(threadIdx.x / 64);
+    const uint32_t lane = threadIdx.x & 63;
+    if (wave == 0) {
+        const RankRows mine(s);
+        if (lane == rank) {
+            s_rows[0] = mine.rows;
+            s_rows[1] = mine.start;
+        }
+    }
+    __syncthreads();
+    const uint32_t rows = uniform(s_rows[0]);
+    const uint32_t start = uniform(s_rows[1]);
+    const uint32_t dim = s.dim;
+    const uint32_t hidden = s.hidden;
+    const uint32_t ks = KIND == kFfnGateUp ? dim : hidden;
+    const uint32_t cols = KIND == kFfnGateUp ? hidden : dim;
+    const uint32_t n0 = blockIdx.x * 16;
+    const uint32_t w_ld = ks * 2;
+    const uint32_t x_ld = X8 ? dim + HCCLX_ROW8_TAIL : ks * 2;
+    const uint32_t have = cols - n0 < 16 ? cols - n0 : 16;
+    const Window gate((KIND == kFfnGateUp ? a.p[1][rank] : a.p[0][rank]) + static_cast<uint64_t>(n0) * w_ld, have * w_ld);
+    const Window up((KIND == kFfnGateUp ? a.p[2][rank] : a.p[0][rank]) + static_cast<uint64_t>(n0) * w_ld, have * w_ld);
+    const char *x = KIND == kFfnGateUp ? a.p[0][rank] : a.h + static_cast<uint64_t>(start) * w_ld;
+    const uint32_t w_row = lane % 16 * w_ld;
+    const uint32_t x_row = lane % 16 * x_ld;
+    const uint32_t k_in = lane / 16 * 16;
+    const uint32_t turns = (ks + kTurnK * kThinWaves - 1) / (kTurnK * kThinWaves);
+
+    for (uint32_t m0 = 0; m0 < rows; m0 += 16 * MB) {
+        const uint32_t here = rows - m0 < 16 * MB ? rows - m0 : 16 * MB;
+        const Window in(x + static_cast<uint64_t>(m0) * x_ld, here * x_ld);
+        f32x4 acc[MB][kWeights];
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+#pragma unroll
+            for (int w = 0; w < kWeights; ++w) acc[m][w] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        u32x4 fw[kAhead][kWeights][2];
+        u32x4 fx[kAhead][MB][X8 ? 1 : 2];
+        auto load = [&](uint32_t turn, int to) {
+            const uint32_t k = (turn * kThinWaves + wave) * kTurnK + k_in;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t o = k + h * 8 < ks ? w_row + (k + h * 8) * 2 : kOut;
+                fw[to][0][h] = __builtin_bit_cast(u32x4, gate.load(o));
+                if constexpr (kWeights == 2) fw[to][1][h] = __builtin_bit_cast(u32x4, up.load(o));
+            }
+#pragma unroll
+            for (int m = 0; m < MB; ++m) {
+                const uint32_t row = x_row + m * 16 * x_ld;
+                if constexpr (X8) {
+                    fx[to][m][0] = __builtin_bit_cast(u32x4, in.load(k < ks ? row + k : kOut));   // (dim is a multiple of 16)
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        fx[to][m][h] = __builtin_bit_cast(u32x4, in.load(k + h * 8 < ks ? row + (k + h * 8) * 2 : kOut));
+                    }
+                }
+            }
+        };
+        auto multiply = [&](int from) {
+#pragma unroll
+            for (int m = 0; m < MB; ++m) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const u32x4 f = X8 ? widen8<DT>(fx[from][m][0][2 * h], fx[from][m][0][2 * h + 1]) : fx[from][m][X8 ? 0 : h];
+#pragma unroll
+                    for (int w = 0; w < kWeights; ++w) acc[m][w] = Mma<DT>::run(fw[from][w][h], f, acc[m][w]);
+                }
+            }
+        };
+#pragma unroll
+        for (int t = 0; t < kAhead; ++t) load(t, t);
+        for (uint32_t turn = 0; turn < turns; turn += kAhead) {
+#pragma unroll
+            for (int t = 0; t < kAhead; ++t) {
+                multiply(t);
+                load(turn + t + kAhead, t);   // (behind the last turn: nothing, which loads zeros)
+            }
+        }
+
+        __syncthreads();   // the parts of the rows before have been read
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+#pragma unroll
+            for (int w = 0; w < kWeights; ++w) s_part[wave][m * kWeights + w][lane] = acc[m][w];
+        }
+        __syncthreads();
+        if (wave >= MB) continue;
+        f32x4 sum[kWeights];
+#pragma unroll
+        for (int w = 0; w < kWeights; ++w) {
+            sum[w] = s_part[0][wave * kWeights + w][lane];
+#pragma unroll
+            for (uint32_t v = 1; v < kThinWaves; ++v) sum[w] += s_part[v][wave * kWeights + w][lane];
+        }
+        const uint32_t row = m0 + wave * 16 + lane % 16;
+        const uint32_t col = n0 + lane / 16 * 4;
+        if (row >= rows || col >= cols) continue;
+        if constexpr (KIND == kFfnGateUp) {
+            if constexpr (X8) {
+                const float scale = *reinterpret_cast<const float *>(x + static_cast<uint64_t>(row) * x_ld + dim);
+                sum[0] *= scale;
+                sum[kWeights - 1] *= scale;
+            }
+            const uint64_t packed = static_cast<uint64_t>(start) + row;
+            if (a.saved != nullptr) {
+                float *to = a.saved + packed * 2 * hidden + col;
+                *reinterpret_cast<f32x4 *>(to) = sum[0];
+                *reinterpret_cast<f32x4 *>(to + hidden) = sum[kWeights - 1];
+            }
+            f32x4 h;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = Act(sum[0][e], a.act).value * sum[kWeights - 1][e];
+            *reinterpret_cast<uint2 *>(a.h + (packed * hidden + col) * 2) = narrow4<DT>(h);
+        } else {
+            char *c = const_cast<char *>(a.p[1][rank]);
+            *reinterpret_cast<uint2 *>(c + (static_cast<uint64_t>(row) * dim + col) * 2) = narrow4<DT>(sum[0]);
+        }
+    }
+}
+
+template <int DT, int KIND, int MB>
+void launch_thin(const FfnArgs &a, bool x8, hipStream_t st)
+{
+    const uint32_t cols = columns<KIND>(a.rows);
+    const dim3 grid((cols + 15) / 16, a.rows.n);
+    if constexpr (KIND == kFfnGateUp) {
+        if (x8) {
+            HCCLX_LAUNCH((k_ffn_thin<DT, KIND, MB, true>), grid, dim3(kThinWaves * 64), 0, st, a);
+            return;
+        }
+    }
+    HCCLX_LAUNCH((k_ffn_thin<DT, KIND, MB, false>), grid, dim3(kThinWaves * 64), 0, st, a);
+}
+
+}  // namespace ffn
+}  // namespace hcclx
