@@ -111,10 +111,12 @@ struct Window {
 };
 
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ const char *uniform(const char *p)
+// The same where the compiler, knowing that x is uniform, would drop the instruction and keep x and all that is computed from it in
+// vector registers (quotients of the tiles' numbers).
+__device__ __forceinline__ uint32_t scalar(uint32_t x)
 {
-    const uint64_t x = reinterpret_cast<uint64_t>(p);
-    return reinterpret_cast<const char *>(static_cast<uint64_t>(uniform(static_cast<uint32_t>(x >> 32))) << 32 | uniform(static_cast<uint32_t>(x)));
+    asm("" : "+v"(x));
+    return uniform(x);
 }
 __device__ __forceinline__ uint32_t of_lane(uint32_t x, uint32_t lane) { return __builtin_amdgcn_readlane(x, lane); }
 
@@ -190,8 +192,8 @@ __device__ __forceinline__ void in_groups(uint32_t at, uint32_t mts, uint32_t nt
     const uint32_t first = at / (kGroup * nts) * kGroup;
     const uint32_t height = mts - first < kGroup ? mts - first : kGroup;
     const uint32_t inside = at - first * nts;
-    *mt = uniform(first + inside % height);   // (a division leaves them in vector registers)
-    *nt = uniform(inside / height);
+    *mt = scalar(first + inside % height);
+    *nt = scalar(inside / height);
 }
 
 // How whole tiles are shared out.  T of them on W CUs take T / W rounds and one more for what is left, however little; so what is
@@ -203,7 +205,7 @@ struct Share {
     uint32_t left;    // tiles that are
     __device__ __forceinline__ Share(uint32_t tiles, uint32_t groups)
     {
-        left = uniform(tiles % groups);
+        left = scalar(tiles % groups);
         parts = left <= groups / 4 ? 4 : 2;
         if (left > groups / 2) left = 0;
         whole = tiles - left;
@@ -395,14 +397,6 @@ __device__ __forceinline__ Feed feed_of(const FfnArgs &a, const Tile &t, uint32_
             f.b_extent = dim - t.n0;
         }
     }
-    // all of it is the same for the whole wavefront, which the compiler does not always see
-    f.a[0] = uniform(f.a[0]);
-    f.b[0] = uniform(f.b[0]);
-    f.a_ld = uniform(f.a_ld);
-    f.b_ld = uniform(f.b_ld);
-    f.a_extent = uniform(f.a_extent);
-    f.b_extent = uniform(f.b_extent);
-    f.k = uniform(f.k);
     return f;
 }
 
@@ -547,7 +541,8 @@ __device__ __forceinline__ void results(const FfnArgs &a, const Tile &t, const f
     }
 }
 
-// Tiles of wavefronts of FM x FN fragments each: t and what next(&t) gives after it, until it says no.  The stages of one tile
+// Tiles of wavefronts of FM x FN fragments each: t and what next(&t) gives after it, until it says no; their operands' rows have the
+// same lengths.  The stages of one tile
 // follow those of the one before without a break, so that the first of them are on their way while results are written.
 template <int DT, int KIND, int FM, int FN, typename Next>
 __device__ __forceinline__ void products(const FfnArgs &a, Tile t, char *s_tile, Next &&next)
@@ -570,6 +565,9 @@ __device__ __forceinline__ void products(const FfnArgs &a, Tile t, char *s_tile,
 
     Stager<BM, kAk, false> sa;
     Stager<BN, kBk, kPair> sb;
+    Feed from = feed_of<KIND, BN>(a, t, wave);
+    sa.init(wave, lane, from.a_ld);
+    sb.init(wave, lane, from.b_ld);
     constexpr int kReads = (kAk ? 1 : 2) + (kBk ? 1 : 2);
     constexpr int kLoads = decltype(sa)::kLoads + decltype(sb)::kLoads;
     static_assert(kStages >= 2 && kLoads * (kStages - 1) < 64, "two stages fit; the counter of loads holds what is on its way");
@@ -581,7 +579,6 @@ __device__ __forceinline__ void products(const FfnArgs &a, Tile t, char *s_tile,
         const uint32_t n = (f.k + kBK - 1) / kBK * kPairs;
         return n < kStages ? kStages : n;
     };
-    Feed from = feed_of<KIND, BN>(a, t, wave);
     Feed then = from;
     bool more = false;
     uint32_t left = from.k;
@@ -668,14 +665,9 @@ __device__ __forceinline__ void products(const FfnArgs &a, Tile t, char *s_tile,
         const uint32_t total = (joined ? stages_of(then) : steps);
         Tile after = t;
         const bool last = !next(&after);
-        const bool apart = !last && KIND == kFfnGradWeights && (after.weight == 2) != (t.weight == 2);   // its rows have other lengths
         const Feed its = last ? then : feed_of<KIND, BN>(a, after, wave);
-        if (!joined) {
-            sa.init(wave, lane, from.a_ld);
-            sb.init(wave, lane, from.b_ld);
-        }
         then = its;
-        more = !last && !apart;
+        more = !last;
         if (steps == 0) follow();
         if (!joined) {
             slot = 0;
@@ -713,16 +705,7 @@ __device__ __forceinline__ void products(const FfnArgs &a, Tile t, char *s_tile,
         results<DT, KIND, FM, FN>(a, t, acc, wm, wn, lane);
         if (last) break;
         t = after;
-        joined = !apart;
-        if (apart) {
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            from = then;
-            left = from.k;
-            steps = stages_of(from);
-            pair = 0;
-        }
+        joined = true;
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // nothing may be on its way to LDS when it is given back
 }
@@ -751,6 +734,8 @@ k_ffn(FfnArgs a)
     const uint32_t across1 = count(s.hidden, kEdge);
     const uint32_t tiles0 = 2 * across1 * across;
     const uint32_t tiles1 = count(s.dim, kEdge) * across1;
+    const uint32_t both0 = scalar(s.n) * tiles0;   // of all ranks (read by a part of the workgroup too, which makes it a vector)
+    const uint32_t both1 = scalar(s.n) * tiles1;
     if (threadIdx.x < 64) {
         const RankRows mine(s);
         const uint32_t down = count(mine.rows, kEdge);
@@ -760,23 +745,23 @@ k_ffn(FfnArgs a)
     auto tile = [&](uint32_t at, Tile *t) {
         t->weight = 0;
         if constexpr (KIND == kFfnGradWeights) {
-            const bool down = at >= s.n * tiles0;
-            at -= down ? s.n * tiles0 : 0;
-            t->rank = uniform(at / (down ? tiles1 : tiles0));
+            const bool down = at >= both0;
+            at -= down ? both0 : 0;
+            t->rank = scalar(at / (down ? tiles1 : tiles0));
             in_groups(at % (down ? tiles1 : tiles0), down ? across : 2 * across1, down ? across1 : across, &t->m0, &t->n0);
-            t->weight = uniform(down ? 2 : t->m0 >= across1 ? 1 : 0);
-            t->m0 = uniform(t->m0 - (t->weight == 1 ? across1 : 0));
+            t->weight = down ? 2 : t->m0 >= across1 ? 1 : 0;
+            t->m0 -= t->weight == 1 ? across1 : 0;
         } else {
             t->rank = __builtin_ctzll(__ballot(s_rank[threadIdx.x & 63].upto > at));
             const uint32_t down = uniform(s_rank[t->rank].down);
             in_groups(at - (uniform(s_rank[t->rank].upto) - down * across), down, across, &t->m0, &t->n0);
         }
-        t->rows = uniform(s_rank[t->rank].rows);
-        t->start = uniform(s_rank[t->rank].start);
+        t->rows = scalar(s_rank[t->rank].rows);
+        t->start = scalar(s_rank[t->rank].start);
         t->m0 *= kEdge;
         t->n0 *= kWide;
     };
-    const uint32_t tiles = KIND == kFfnGradWeights ? s.n * (tiles0 + tiles1) : uniform(s_rank[kFfnRanks - 1].upto);
+    const uint32_t tiles = KIND == kFfnGradWeights ? both0 + both1 : uniform(s_rank[kFfnRanks - 1].upto);
     const uint32_t turned = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
     uint32_t at = turned;
     uint32_t end = tiles;
@@ -788,19 +773,25 @@ k_ffn(FfnArgs a)
     };
     Tile t;
     if constexpr (SMALL) {
-        if (at >= end) return;
-        tile(at, &t);
-        products<DT, KIND, 4, 2>(a, t, s_tile, next);
+        for (uint32_t group = 0; group < (KIND == kFfnGradWeights ? 2 : 1); ++group) {
+            end = group == 0 && KIND == kFfnGradWeights ? both0 : tiles;
+            if (at >= end) continue;
+            __syncthreads();
+            tile(at, &t);
+            products<DT, KIND, 4, 2>(a, t, s_tile, next);
+        }
     } else {
         const Share share(tiles, gridDim.x);
-        end = share.whole;
-        if (at < end) {
+        for (uint32_t group = 0; group < (KIND == kFfnGradWeights ? 2 : 1); ++group) {
+            end = group == 0 && KIND == kFfnGradWeights && share.whole > both0 ? both0 : share.whole;
+            if (at >= end) continue;
+            __syncthreads();   // everybody is done with the LDS of the tiles before
             tile(at, &t);
             products<DT, KIND, 8, 4>(a, t, s_tile, next);
         }
         if (turned >= share.left * share.parts) return;
-        const uint32_t part = uniform(turned % share.parts);
-        tile(uniform(share.whole + turned / share.parts), &t);
+        const uint32_t part = scalar(turned % share.parts);
+        tile(scalar(share.whole + turned / share.parts), &t);
         t.n0 += part % 2 * (kTileCols<KIND> / 2);
         if (share.parts == 4) t.m0 += part / 2 * (kTile / 2);
         // a part may have no column or row

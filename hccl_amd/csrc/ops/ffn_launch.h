@@ -1,6 +1,5 @@
 // Which kernel computes a product: instantiated per type in ffn_bf16.hip and ffn_f16.hip.
 #pragma once
-#include <stdlib.h>
 #include "ops/ffn_gemm.h"
 #include "ops/ffn_thin.h"
 
@@ -10,7 +9,9 @@ namespace hcclx {
 constexpr uint32_t kThinRows = 32;
 inline bool thin(const FfnRows &s) { return s.most <= static_cast<uint64_t>(s.n) * kThinRows; }
 
-inline bool small_tiles(const FfnRows &s) { return getenv("FFN_SMALL") ? atoi(getenv("FFN_SMALL")) : s.most <= s.n * 128ull; }
+// Rows per rank up to which products take tiles of half a whole tile's height and width.
+constexpr uint32_t kSmallRows = 128;
+inline bool small_tiles(const FfnRows &s) { return s.most <= static_cast<uint64_t>(s.n) * kSmallRows; }
 
 template <int DT, int KIND>
 hipError_t launch_forward(const FfnArgs &a, uint32_t num_cus, hipStream_t st)
