@@ -1,8 +1,9 @@
 // The AdamW step over many tensors in one launch (include/hcclx_ops.h: hcclx_adamw_*).
 //
 // Bound: HBM bandwidth: 28 bytes per element with 16-bit gradients, states in 32 bits and a 16-bit copy, 16 with states in 8 bits.
-// A workgroup takes a tile of one tensor; a wavefront takes kPieces blocks of 256 elements of it, a lane four neighbouring
-// elements of each, so that every access of a wavefront is one run of memory and a block's scale is a reduction in registers.
+// A workgroup takes a tile of one tensor; a wavefront takes 256 elements of it, a lane four neighbouring ones, so that every access
+// of a wavefront is one run of memory and a block's scale is a reduction in registers.  (Two such blocks per wavefront, which ends
+// later and holds more registers: 100 M elements 632 us, one 522.)
 #include "hcclx_internal.h"
 #include "hcclx_ops.h"
 #include "kernels/elem.h"
@@ -19,8 +20,7 @@ namespace {
 
 constexpr uint32_t kBlock = HCCLX_ADAMW_BLOCK;
 constexpr uint32_t kThreads256 = 256;
-constexpr uint32_t kPieces = 2;                                 // blocks per wavefront
-constexpr uint32_t kTile = kPieces * kBlock * (kThreads256 / 64);   // elements per workgroup
+constexpr uint32_t kTile = kBlock * (kThreads256 / 64);   // elements per workgroup
 static_assert(kBlock == 64 * 4, "a lane holds four elements of a block");
 
 struct TensorDev {
@@ -38,7 +38,7 @@ struct TensorDev {
 };
 
 struct StepArgs {
-    float lr, beta1, rest1, beta2, rest2, eps, unbias1, unbias2;   // rest = 1 - beta, unbias = 1 / (1 - beta^step)
+    float lr, beta1, rest1, beta2, rest2, eps, unbias1, root2;   // rest = 1 - beta, unbias = 1 / (1 - beta^step), root2 = sqrt(unbias2)
     uint32_t seed;
     const float *grad_scale;
 };
@@ -73,73 +73,110 @@ typedef uint32_t u32_u __attribute__((aligned(1)));
 typedef float f32x4v __attribute__((ext_vector_type(4)));
 typedef f32x4v f32x4_u __attribute__((aligned(4)));
 
+// The tensors' addresses come out of a table, which does not say that they are in global memory.
+template <typename T>
+using Global = __attribute__((address_space(1))) T *;
+template <typename T>
+__device__ __forceinline__ Global<T> global(const void *p)
+{
+    return reinterpret_cast<Global<T>>(reinterpret_cast<uint64_t>(p));
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, HcclDataType dt)
+{
+    if (dt == HCCL_DATA_TYPE_BFP16) {
+        typedef __bf16 B2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, B2{static_cast<__bf16>(a), static_cast<__bf16>(b)});
+    }
+    typedef _Float16 H2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, H2{static_cast<_Float16>(a), static_cast<_Float16>(b)});
+}
+
 // Four elements at `at` as floats; only the first `have` exist.
 template <int DT>
-__device__ __forceinline__ void load4(const char *p, uint64_t at, uint32_t have, float (&f)[4])
+__device__ __forceinline__ void load4(const void *base, uint64_t at, uint32_t have, float (&f)[4])
 {
     using D = DTypeOf<DT>;
     using S = typename D::S;
-    p += at * sizeof(S);
+    const Global<const S> p = global<const S>(base) + at;
     if (have >= 4) {
         if constexpr (sizeof(S) == 4) {
-            const f32x4v x = __builtin_nontemporal_load(reinterpret_cast<const f32x4_u *>(p));
+            const f32x4v x = __builtin_nontemporal_load(reinterpret_cast<Global<const f32x4_u>>(p));
 #pragma unroll
             for (int e = 0; e < 4; ++e) f[e] = x[e];
         } else {
-            const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2_u *>(p));
+            const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<Global<const u32x2_u>>(p));
 #pragma unroll
             for (int e = 0; e < 4; ++e) f[e] = D::widen(static_cast<S>(x[e / 2] >> (16 * (e & 1))));
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = static_cast<uint32_t>(e) < have ? D::widen(reinterpret_cast<const S *>(p)[e]) : 0.0f;
+        for (int e = 0; e < 4; ++e) f[e] = static_cast<uint32_t>(e) < have ? D::widen(p[e]) : 0.0f;
     }
 }
 template <int DT>
-__device__ __forceinline__ void store4(char *p, uint64_t at, uint32_t have, const float (&f)[4])
+__device__ __forceinline__ void store4(void *base, uint64_t at, uint32_t have, const float (&f)[4])
 {
     using D = DTypeOf<DT>;
     using S = typename D::S;
-    p += at * sizeof(S);
+    const Global<S> p = global<S>(base) + at;
     if (have >= 4) {
         if constexpr (sizeof(S) == 4) {
-            const f32x4v x = {f[0], f[1], f[2], f[3]};
-            __builtin_nontemporal_store(x, reinterpret_cast<f32x4_u *>(p));
+            __builtin_nontemporal_store(f32x4v{f[0], f[1], f[2], f[3]}, reinterpret_cast<Global<f32x4_u>>(p));
         } else {
-            const u32x2 x = {static_cast<uint32_t>(D::narrow(f[0])) | static_cast<uint32_t>(D::narrow(f[1])) << 16,
-                             static_cast<uint32_t>(D::narrow(f[2])) | static_cast<uint32_t>(D::narrow(f[3])) << 16};
-            __builtin_nontemporal_store(x, reinterpret_cast<u32x2_u *>(p));
+            constexpr HcclDataType kDt = static_cast<HcclDataType>(DT);
+            __builtin_nontemporal_store(u32x2{pack2(f[0], f[1], kDt), pack2(f[2], f[3], kDt)}, reinterpret_cast<Global<u32x2_u>>(p));
         }
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            if (static_cast<uint32_t>(e) < have) reinterpret_cast<S *>(p)[e] = D::narrow(f[e]);
+            if (static_cast<uint32_t>(e) < have) p[e] = D::narrow(f[e]);
         }
     }
 }
-__device__ __forceinline__ uint32_t load_codes(const char *p, uint64_t at, uint32_t have)
+__device__ __forceinline__ uint32_t load_codes(const void *base, uint64_t at, uint32_t have)
 {
-    p += at;
-    if (have >= 4) return __builtin_nontemporal_load(reinterpret_cast<const u32_u *>(p));
+    const Global<const uint8_t> p = global<const uint8_t>(base) + at;
+    if (have >= 4) return __builtin_nontemporal_load(reinterpret_cast<Global<const u32_u>>(p));
     uint32_t c = 0;
 #pragma unroll
     for (uint32_t e = 0; e < 3; ++e) {
-        if (e < have) c |= static_cast<uint32_t>(static_cast<uint8_t>(p[e])) << (8 * e);
+        if (e < have) c |= static_cast<uint32_t>(p[e]) << (8 * e);
     }
     return c;
 }
-__device__ __forceinline__ void store_codes(char *p, uint64_t at, uint32_t have, uint32_t c)
+__device__ __forceinline__ void store_codes(void *base, uint64_t at, uint32_t have, uint32_t c)
 {
-    p += at;
+    const Global<uint8_t> p = global<uint8_t>(base) + at;
     if (have >= 4) {
-        __builtin_nontemporal_store(c, reinterpret_cast<u32_u *>(p));
+        __builtin_nontemporal_store(c, reinterpret_cast<Global<u32_u>>(p));
     } else {
 #pragma unroll
         for (uint32_t e = 0; e < 3; ++e) {
-            if (e < have) p[e] = static_cast<char>(c >> (8 * e));
+            if (e < have) p[e] = static_cast<uint8_t>(c >> (8 * e));
         }
     }
 }
+
+// x / scale, rounded as a division is, for a whole block: with the scale's inverse, one step of the quotient's remainder gives the
+// nearest float (Markstein).  Where the products would leave the range of normal floats it is a division.
+struct Quotient {
+    float by;
+    float inverse;
+    bool plain;
+    __device__ __forceinline__ explicit Quotient(float scale)
+    {
+        by = scale > 0.0f ? scale : 1.0f;
+        inverse = 1.0f / by;
+        plain = !(by > 0x1p-90f && by < 0x1p90f);
+    }
+    __device__ __forceinline__ float operator()(float x) const
+    {
+        if (plain) return x / by;
+        const float q = x * inverse;
+        return __builtin_fmaf(__builtin_fmaf(-q, by, x), inverse, q);
+    }
+};
 
 template <int GRAD, bool SMALL, int COPY>   // COPY: a 16-bit type, or fp32 for none
 __global__ void __launch_bounds__(kThreads256)
@@ -147,78 +184,73 @@ k_adamw(const TensorDev *tensors, const uint32_t *tensor_of_tile, StepArgs a)
 {
     const TensorDev t = tensors[tensor_of_tile[blockIdx.x]];
     const uint32_t lane = threadIdx.x & 63;
-    const uint64_t start = (blockIdx.x - t.first_tile) * kTile + static_cast<uint64_t>(threadIdx.x / 64) * kPieces * kBlock;
+    const uint64_t start = (blockIdx.x - t.first_tile) * kTile + static_cast<uint64_t>(threadIdx.x / 64) * kBlock;
     const float scale = a.grad_scale != nullptr ? *a.grad_scale : 1.0f;
     const uint32_t key = mix(a.seed + (t.index + 1) * 0x9E3779B9u);
-    float g[kPieces][4], p[kPieces][4], m[kPieces][4], v[kPieces][4];
-    uint32_t have[kPieces];
-#pragma unroll
-    for (uint32_t k = 0; k < kPieces; ++k) {
-        const uint64_t at = start + k * kBlock + lane * 4;
-        have[k] = at >= t.count ? 0u : t.count - at >= 4 ? 4u : static_cast<uint32_t>(t.count - at);
-        load4<GRAD>(t.grad, at, have[k], g[k]);
-        load4<HCCL_DATA_TYPE_FP32>(reinterpret_cast<const char *>(t.param), at, have[k], p[k]);
-        if constexpr (SMALL) {
-            const uint64_t block = (start + k * kBlock) / kBlock;
-            const bool any = start + k * kBlock < t.count;
-            const float ms = any ? t.m_scale[block] : 0.0f;
-            const float vs = any ? t.v_scale[block] : 0.0f;
-            from_e4m3(load_codes(t.m, at, have[k]), m[k]);
-            from_e4m3(load_codes(t.v, at, have[k]), v[k]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                m[k][e] *= ms;
-                v[k][e] *= vs;
-                v[k][e] *= v[k][e];
-            }
-        } else {
-            load4<HCCL_DATA_TYPE_FP32>(t.m, at, have[k], m[k]);
-            load4<HCCL_DATA_TYPE_FP32>(t.v, at, have[k], v[k]);
-        }
-    }
-#pragma unroll
-    for (uint32_t k = 0; k < kPieces; ++k) {
-        const uint64_t at = start + k * kBlock + lane * 4;
+    const uint64_t at = start + lane * 4;
+    const uint32_t have = at >= t.count ? 0u : t.count - at >= 4 ? 4u : static_cast<uint32_t>(t.count - at);
+    if (start >= t.count) return;   // the wavefront's whole block is behind the end
+    const uint64_t block = start / kBlock;
+    float g[4], p[4], m[4], v[4];
+    load4<GRAD>(t.grad, at, have, g);
+    load4<HCCL_DATA_TYPE_FP32>(t.param, at, have, p);
+    if constexpr (SMALL) {
+        const uint32_t cm = load_codes(t.m, at, have);
+        const uint32_t cv = load_codes(t.v, at, have);
+        const float ms = global<const float>(t.m_scale)[block];
+        const float vs = global<const float>(t.v_scale)[block];
+        from_e4m3(cm, m);
+        from_e4m3(cv, v);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float x = g[k][e] * scale;
-            m[k][e] = a.beta1 * m[k][e] + a.rest1 * x;
-            v[k][e] = a.beta2 * v[k][e] + a.rest2 * x * x;
-            const float update = (m[k][e] * a.unbias1) / (sqrtf(v[k][e] * a.unbias2) + a.eps);
-            p[k][e] = p[k][e] - a.lr * (t.weight_decay * p[k][e] + update);
+            m[e] *= ms;
+            v[e] *= vs;
+            v[e] *= v[e];
         }
-        store4<HCCL_DATA_TYPE_FP32>(reinterpret_cast<char *>(t.param), at, have[k], p[k]);
-        if constexpr (COPY != HCCL_DATA_TYPE_FP32) store4<COPY>(t.copy, at, have[k], p[k]);
-        if constexpr (SMALL) {
-            float most_m = 0.0f;
-            float most_r = 0.0f;
+    } else {
+        load4<HCCL_DATA_TYPE_FP32>(t.m, at, have, m);
+        load4<HCCL_DATA_TYPE_FP32>(t.v, at, have, v);
+    }
+    float r[4];   // sqrt(v)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {   // (elements behind the end are zeros throughout)
-                v[k][e] = sqrtf(v[k][e]);
-                most_m = fmaxf(most_m, fabsf(m[k][e]));
-                most_r = fmaxf(most_r, v[k][e]);
-            }
-            const float scale_m = wave_max(most_m) * (1.0f / kE4m3Most);
-            const float scale_r = wave_max(most_r) * (1.0f / kE4m3Most);
-            const float by_m = scale_m > 0.0f ? scale_m : 1.0f;
-            const float by_r = scale_r > 0.0f ? scale_r : 1.0f;
+    for (int e = 0; e < 4; ++e) {
+        const float x = g[e] * scale;
+        m[e] = a.beta1 * m[e] + a.rest1 * x;
+        v[e] = a.beta2 * v[e] + a.rest2 * x * x;
+        r[e] = sqrtf(v[e]);
+        // (the hardware's reciprocal is good to a rounding, of an update that is small against the parameter)
+        const float update = (m[e] * a.unbias1) * __builtin_amdgcn_rcpf(r[e] * a.root2 + a.eps);
+        p[e] = p[e] - a.lr * (t.weight_decay * p[e] + update);
+    }
+    store4<HCCL_DATA_TYPE_FP32>(t.param, at, have, p);
+    if constexpr (COPY != HCCL_DATA_TYPE_FP32) store4<COPY>(t.copy, at, have, p);
+    if constexpr (SMALL) {
+        float most_m = 0.0f;
+        float most_r = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t word = mix(static_cast<uint32_t>(at) + e + key);
-                m[k][e] = round_by(m[k][e] / by_m, static_cast<float>(word & 0xffffu) * 0x1p-16f);
-                v[k][e] = round_by(v[k][e] / by_r, static_cast<float>(word >> 16) * 0x1p-16f);
-            }
-            store_codes(t.m, at, have[k], to_e4m3(m[k][0], m[k][1], m[k][2], m[k][3]));
-            store_codes(t.v, at, have[k], to_e4m3(v[k][0], v[k][1], v[k][2], v[k][3]));
-            if (lane == 0 && have[k] != 0) {
-                const uint64_t block = (start + k * kBlock) / kBlock;
-                t.m_scale[block] = scale_m;
-                t.v_scale[block] = scale_r;
-            }
-        } else {
-            store4<HCCL_DATA_TYPE_FP32>(t.m, at, have[k], m[k]);
-            store4<HCCL_DATA_TYPE_FP32>(t.v, at, have[k], v[k]);
+        for (int e = 0; e < 4; ++e) {   // (elements behind the end are zeros throughout)
+            most_m = fmaxf(most_m, fabsf(m[e]));
+            most_r = fmaxf(most_r, r[e]);
         }
+        const float scale_m = wave_max(most_m) * (1.0f / kE4m3Most);
+        const float scale_r = wave_max(most_r) * (1.0f / kE4m3Most);
+        const Quotient of_m(scale_m);
+        const Quotient of_r(scale_r);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t word = mix(static_cast<uint32_t>(at) + e + key);
+            m[e] = round_by(of_m(m[e]), static_cast<float>(word & 0xffffu) * 0x1p-16f);
+            v[e] = round_by(of_r(r[e]), static_cast<float>(word >> 16) * 0x1p-16f);
+        }
+        store_codes(t.m, at, have, to_e4m3(m[0], m[1], m[2], m[3]));
+        store_codes(t.v, at, have, to_e4m3(v[0], v[1], v[2], v[3]));
+        if (lane == 0) {
+            global<float>(t.m_scale)[block] = scale_m;
+            global<float>(t.v_scale)[block] = scale_r;
+        }
+    } else {
+        store4<HCCL_DATA_TYPE_FP32>(t.m, at, have, m);
+        store4<HCCL_DATA_TYPE_FP32>(t.v, at, have, v);
     }
 }
 
@@ -363,7 +395,7 @@ int hcclx_adamw_step(const hcclx_plan_t *plan, const hcclx_adamw_step_t *step, v
     a.rest2 = static_cast<float>(1.0 - step->beta2);
     a.eps = static_cast<float>(step->eps);
     a.unbias1 = static_cast<float>(1.0 / (1.0 - std::pow(step->beta1, step->step)));
-    a.unbias2 = static_cast<float>(1.0 / (1.0 - std::pow(step->beta2, step->step)));
+    a.root2 = static_cast<float>(std::sqrt(1.0 / (1.0 - std::pow(step->beta2, step->step))));
     a.seed = step->seed;
     a.grad_scale = step->grad_scale;
     return work->step(a, static_cast<hipStream_t>(stream));

@@ -41,19 +41,23 @@ constexpr uint32_t kMostVectors = 4;
 template <int DT> constexpr int kMostThreads = HCCLX_NORM_MAX_ROW / (Vec16<DT>::NE * kMostVectors);
 static_assert(kMostThreads<HCCL_DATA_TYPE_FP32> <= 1024, "a workgroup holds the longest row");
 
-// Vector v of a row of `elems` elements as 32-bit floats; zeros behind the row's end.
-template <int DT>
-__device__ __forceinline__ void load_vec(const char *row, uint32_t v, uint32_t elems, float (&f)[Vec16<DT>::NE])
+// Vector v of a row of `elems` elements as it lies in memory; zeros behind the row's end.  WARM: it is read again (weights).
+template <int DT, bool WARM>
+__device__ __forceinline__ u32x4 load_vec(const char *row, uint32_t v, uint32_t elems)
 {
     using V = Vec16<DT>;
     using S = typename V::S;
     const uint32_t at = v * V::NE;
     if (at + V::NE <= elems) {
-        V::unpack(ld16_cached(row + static_cast<size_t>(v) * 16), f);
-    } else {
-#pragma unroll
-        for (int e = 0; e < V::NE; ++e) f[e] = at + e < elems ? V::D::widen(reinterpret_cast<const S *>(row)[at + e]) : 0.0f;
+        const char *p = row + static_cast<size_t>(v) * 16;
+        return WARM ? ld16_cached(p) : __builtin_nontemporal_load(as_global(p));
     }
+    S tmp[V::NE];
+#pragma unroll
+    for (int e = 0; e < V::NE; ++e) tmp[e] = at + e < elems ? reinterpret_cast<const S *>(row)[at + e] : S(0);
+    u32x4 raw;
+    __builtin_memcpy(&raw, tmp, 16);
+    return raw;
 }
 
 template <int DT>
@@ -72,20 +76,27 @@ __device__ __forceinline__ void store_vec(char *row, uint32_t v, uint32_t elems,
     }
 }
 
-// Sum / maximum over the threads of a row (blockDim.x of them, whole wavefronts).  s: one float per wavefront of the workgroup.
-template <bool MAX>
-__device__ __forceinline__ float row_reduce(float v, float *s)
+// Sums of N values over the threads of a row (blockDim.x of them, whole wavefronts), or the largest of N magnitudes.  s: N floats per
+// wavefront of the workgroup, of which no reader is left.
+template <bool MAX, int N>
+__device__ __forceinline__ void row_reduce(float (&v)[N], float (*s)[N])
 {
-    v = MAX ? wave_max(v) : wave_sum(v);
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = MAX ? wave_max(v[k]) : wave_sum(v[k]);
     const uint32_t waves = blockDim.x / 64;
-    if (waves == 1) return v;
-    float *mine = s + threadIdx.y * waves;
-    __syncthreads();   // the last reduction's values have been read
-    if ((threadIdx.x & 63) == 0) mine[threadIdx.x / 64] = v;
+    if (waves == 1) return;
+    float(*mine)[N] = s + threadIdx.y * waves;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) mine[threadIdx.x / 64][k] = v[k];
+    }
     __syncthreads();
-    v = mine[0];
-    for (uint32_t w = 1; w < waves; ++w) v = MAX ? fmaxf(v, mine[w]) : v + mine[w];
-    return v;
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = mine[0][k];
+    for (uint32_t w = 1; w < waves; ++w) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = MAX ? fmaxf(v[k], mine[w][k]) : v[k] + mine[w][k];
+    }
 }
 
 template <int DT, bool QUANT, int NV>
@@ -94,7 +105,7 @@ k_rms_norm(NormPtrs ptrs, uint32_t rows, uint32_t elems, float eps)
 {
     using V = Vec16<DT>;
     constexpr int NE = V::NE;
-    __shared__ float s_part[16];
+    __shared__ float s_part[2][16][1];
     const uint32_t rank = blockIdx.y;
     const uint32_t row = blockIdx.x * blockDim.y + threadIdx.y;
     const bool live = row < rows;
@@ -102,42 +113,53 @@ k_rms_norm(NormPtrs ptrs, uint32_t rows, uint32_t elems, float eps)
     const char *x = ptrs.x[rank] + at;
     const char *residual = ptrs.residual[rank];
     char *total = ptrs.total[rank];
+    u32x4 w[NV];
     float t[NV][NE];
-    float square = 0.0f;
+    float square[1] = {0.0f};
+    {   // everything that is read, together: small launches are little more than this round trip
+        u32x4 rx[NV], rr[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const uint32_t v = threadIdx.x + i * blockDim.x;
-        load_vec<DT>(x, v, elems, t[i]);
+        for (int i = 0; i < NV; ++i) rx[i] = load_vec<DT, false>(x, threadIdx.x + i * blockDim.x, elems);
         if (residual != nullptr) {
-            float r[NE];
-            load_vec<DT>(residual + at, v, elems, r);
 #pragma unroll
-            for (int e = 0; e < NE; ++e) t[i][e] = V::D::widen(V::D::narrow(t[i][e] + r[e]));
+            for (int i = 0; i < NV; ++i) rr[i] = load_vec<DT, false>(residual + at, threadIdx.x + i * blockDim.x, elems);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) w[i] = load_vec<DT, true>(ptrs.weight[rank], threadIdx.x + i * blockDim.x, elems);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            V::unpack(rx[i], t[i]);
+            if (residual != nullptr) {
+                float r[NE];
+                V::unpack(rr[i], r);
+#pragma unroll
+                for (int e = 0; e < NE; ++e) t[i][e] = V::D::widen(V::D::narrow(t[i][e] + r[e]));
+            }
         }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         if (total != nullptr && live) store_vec<DT>(total + at, threadIdx.x + i * blockDim.x, elems, t[i]);
 #pragma unroll
-        for (int e = 0; e < NE; ++e) square += t[i][e] * t[i][e];
+        for (int e = 0; e < NE; ++e) square[0] += t[i][e] * t[i][e];
     }
-    square = row_reduce<false>(square, s_part);
-    const float r = 1.0f / sqrtf(square / static_cast<float>(elems) + eps);
-    float most = 0.0f;
+    row_reduce<false, 1>(square, s_part[0]);
+    const float r = 1.0f / sqrtf(square[0] / static_cast<float>(elems) + eps);
+    float most[1] = {0.0f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        float w[NE];
-        load_vec<DT>(ptrs.weight[rank], threadIdx.x + i * blockDim.x, elems, w);
+        float f[NE];
+        V::unpack(w[i], f);
 #pragma unroll
         for (int e = 0; e < NE; ++e) {
-            t[i][e] = t[i][e] * r * w[e];
-            if (QUANT) most = fmaxf(most, fabsf(t[i][e]));
+            t[i][e] = t[i][e] * r * f[e];
+            if (QUANT) most[0] = fmaxf(most[0], fabsf(t[i][e]));
         }
     }
     if constexpr (QUANT) {
-        most = row_reduce<true>(most, s_part);
+        row_reduce<true, 1>(most, s_part[1]);
         if (!live) return;
-        const CodeScale code(most);
+        const CodeScale code(most[0]);
         char *out = ptrs.out[rank] + static_cast<size_t>(row) * (elems + kTail);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -160,81 +182,99 @@ k_rms_norm(NormPtrs ptrs, uint32_t rows, uint32_t elems, float eps)
 }
 
 // Slot s of a rank (threadIdx.y of a workgroup) takes the rows s, s + slots, ...; it adds up its part of dweight in registers
-// and writes it to partial[rank][slot][elems].
-template <int DT, int NV>
-__global__ void __launch_bounds__(kMostThreads<DT>)
+// and writes it to partial[rank][slot][elems].  AHEAD: a row is read while the one before it is computed.
+template <int DT, int NV, bool AHEAD>
+__global__ void __launch_bounds__(AHEAD ? 1024 : kMostThreads<DT>)
 k_rms_norm_grad(GradPtrs ptrs, uint32_t rows, uint32_t elems, float eps, float *partial)
 {
     using V = Vec16<DT>;
     constexpr int NE = V::NE;
-    __shared__ float s_part[2][16];
+    __shared__ float s_part[2][16][2];   // of the rows in turn
     const uint32_t rank = blockIdx.y;
     const uint32_t slots = gridDim.x * blockDim.y;
-    const uint32_t slot = blockIdx.x * blockDim.y + threadIdx.y;
     const char *dtotal = ptrs.dtotal[rank];
+    const char *dys = ptrs.dy[rank];
+    const char *totals = ptrs.total[rank];
     float acc[NV][NE];
+    u32x4 w[NV], rt[NV], ra[NV], rd[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
 #pragma unroll
         for (int e = 0; e < NE; ++e) acc[i][e] = 0.0f;
     }
+    auto read = [&](uint32_t row) {   // (behind the last row: it again)
+        const size_t at = static_cast<size_t>(row < rows ? row : rows - 1) * elems * sizeof(typename V::S);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) rt[i] = load_vec<DT, false>(totals + at, threadIdx.x + i * blockDim.x, elems);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) ra[i] = load_vec<DT, false>(dys + at, threadIdx.x + i * blockDim.x, elems);
+        if (dtotal != nullptr) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) rd[i] = load_vec<DT, false>(dtotal + at, threadIdx.x + i * blockDim.x, elems);
+        }
+    };
+    read(blockIdx.x * blockDim.y + threadIdx.y);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) w[i] = load_vec<DT, true>(ptrs.weight[rank], threadIdx.x + i * blockDim.x, elems);
+    uint32_t turn = 0;
     // as many turns for every slot of a workgroup: they meet at barriers
-    for (uint32_t first = blockIdx.x * blockDim.y; first < rows; first += slots) {
+    for (uint32_t first = blockIdx.x * blockDim.y; first < rows; first += slots, turn ^= 1) {
         const uint32_t row = first + threadIdx.y;
         const bool live = row < rows;
         const size_t at = static_cast<size_t>(live ? row : rows - 1) * elems * sizeof(typename V::S);
-        float t[NV][NE];
-        float a[NV][NE];
-        float square = 0.0f;
-        float dot = 0.0f;
+        // (the row stays as it was read and is widened twice: in 16 bits that is half the registers)
+        u32x4 ct[NV], ca[NV], cd[NV];
+        float sums[2] = {0.0f, 0.0f};   // of total^2 and of total * dy * weight
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            load_vec<DT>(ptrs.total[rank] + at, threadIdx.x + i * blockDim.x, elems, t[i]);
-            load_vec<DT>(ptrs.dy[rank] + at, threadIdx.x + i * blockDim.x, elems, a[i]);
+            ct[i] = rt[i];
+            ca[i] = ra[i];
+            cd[i] = rd[i];
         }
+        if (AHEAD && first + slots < rows) read(row + slots);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            float w[NE];
-            load_vec<DT>(ptrs.weight[rank], threadIdx.x + i * blockDim.x, elems, w);
+            float f[NE], t[NE], g[NE];
+            V::unpack(w[i], f);
+            V::unpack(ct[i], t);
+            V::unpack(ca[i], g);
 #pragma unroll
             for (int e = 0; e < NE; ++e) {
-                square += t[i][e] * t[i][e];
-                dot += t[i][e] * (a[i][e] * w[e]);
+                sums[0] += t[e] * t[e];
+                sums[1] += t[e] * (g[e] * f[e]);
             }
         }
-        square = row_reduce<false>(square, s_part[0]);
-        dot = row_reduce<false>(dot, s_part[1]);
-        const float r = 1.0f / sqrtf(square / static_cast<float>(elems) + eps);
-        const float c = (r * r) * (dot / static_cast<float>(elems));
-        if (!live) continue;
+        row_reduce<false, 2>(sums, s_part[turn]);
+        const float r = 1.0f / sqrtf(sums[0] / static_cast<float>(elems) + eps);
+        const float c = (r * r) * (sums[1] / static_cast<float>(elems));
+        if (live) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t v = threadIdx.x + i * blockDim.x;
-            float w[NE];
-            load_vec<DT>(ptrs.weight[rank], v, elems, w);
-            float d[NE];
+            for (int i = 0; i < NV; ++i) {
+                float f[NE], t[NE], g[NE], d[NE];
+                asm("" : "+v"(ct[i]), "+v"(ca[i]));   // widened again, not kept
+                V::unpack(w[i], f);
+                V::unpack(ct[i], t);
+                V::unpack(ca[i], g);
+                if (dtotal != nullptr) V::unpack(cd[i], d);
 #pragma unroll
-            for (int e = 0; e < NE; ++e) {
-                acc[i][e] += a[i][e] * (t[i][e] * r);
-                d[e] = r * (a[i][e] * w[e] - t[i][e] * c);
+                for (int e = 0; e < NE; ++e) {
+                    acc[i][e] += g[e] * (t[e] * r);
+                    const float x = r * (g[e] * f[e] - t[e] * c);
+                    d[e] = dtotal != nullptr ? x + d[e] : x;
+                }
+                store_vec<DT>(ptrs.dx[rank] + at, threadIdx.x + i * blockDim.x, elems, d);
             }
-            if (dtotal != nullptr) {
-                float more[NE];
-                load_vec<DT>(dtotal + at, v, elems, more);
-#pragma unroll
-                for (int e = 0; e < NE; ++e) d[e] += more[e];
-            }
-            store_vec<DT>(ptrs.dx[rank] + at, v, elems, d);
         }
+        if (!AHEAD && first + slots < rows) read(row + slots);
     }
     if (partial == nullptr) return;
-    char *mine = reinterpret_cast<char *>(partial + (static_cast<size_t>(rank) * slots + slot) * elems);
+    float *mine = partial + (static_cast<size_t>(rank) * slots + blockIdx.x * blockDim.y + threadIdx.y) * elems;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const uint32_t at = (threadIdx.x + i * blockDim.x) * NE;
 #pragma unroll
         for (int e = 0; e < NE; ++e) {
-            if (at + e < elems) reinterpret_cast<float *>(mine)[at + e] = acc[i][e];
+            if (at + e < elems) mine[at + e] = acc[i][e];
         }
     }
 }
@@ -251,7 +291,7 @@ k_rms_norm_join(OutPtrs dweight, uint32_t slots, uint32_t elems, const float *pa
     float sum = 0.0f;
     if (col < elems) {
         const float *p = partial + static_cast<size_t>(rank) * slots * elems + col;
-#pragma unroll 4
+#pragma unroll 8
         for (uint32_t s = threadIdx.y; s < slots; s += 16) sum += p[static_cast<size_t>(s) * elems];
     }
     s_sum[threadIdx.y][threadIdx.x] = sum;
@@ -261,18 +301,19 @@ k_rms_norm_join(OutPtrs dweight, uint32_t slots, uint32_t elems, const float *pa
     reinterpret_cast<typename D::S *>(dweight.p[rank])[col] = D::narrow(sum);
 }
 
-// Threads per row and vectors per thread: a row is held by as few wavefronts as leave a thread at most four vectors of it;
-// workgroups of short rows hold several.
+// Threads per row and vectors per thread: a row is held by as few wavefronts as leave a thread at most so many vectors of it (1024
+// threads: more); workgroups of short rows hold several.  The norm takes four; its gradient, which holds three rows, the next
+// ones and a part of dweight, two.
 struct RowShape {
     uint32_t threads;
     uint32_t per_group;
     uint32_t vectors;
 };
-RowShape shape_of(uint32_t elems, int ne)
+RowShape shape_of(uint32_t elems, int ne, uint32_t most_vectors)
 {
     const uint32_t vecs = (elems + ne - 1) / ne;
     uint32_t threads = 64;
-    while (threads * kMostVectors < vecs) threads *= 2;
+    while (threads < 1024 && threads * most_vectors < vecs) threads *= 2;
     return {threads, std::max(1u, 256u / threads), (vecs + threads - 1) / threads};
 }
 
@@ -292,11 +333,12 @@ template <int DT>
 void launch_grad(const RowShape &s, dim3 grid, hipStream_t st, const GradPtrs &p, uint32_t rows, uint32_t elems, float eps, float *partial)
 {
     const dim3 block(s.threads, s.per_group);
-    switch (s.vectors) {
-        case 1: HCCLX_LAUNCH((k_rms_norm_grad<DT, 1>), grid, block, 0, st, p, rows, elems, eps, partial); break;
-        case 2: HCCLX_LAUNCH((k_rms_norm_grad<DT, 2>), grid, block, 0, st, p, rows, elems, eps, partial); break;
-        case 3: HCCLX_LAUNCH((k_rms_norm_grad<DT, 3>), grid, block, 0, st, p, rows, elems, eps, partial); break;
-        default: HCCLX_LAUNCH((k_rms_norm_grad<DT, 4>), grid, block, 0, st, p, rows, elems, eps, partial); break;
+    if (s.vectors == 1) {
+        HCCLX_LAUNCH((k_rms_norm_grad<DT, 1, true>), grid, block, 0, st, p, rows, elems, eps, partial);
+    } else if (s.vectors == 2) {
+        HCCLX_LAUNCH((k_rms_norm_grad<DT, 2, true>), grid, block, 0, st, p, rows, elems, eps, partial);
+    } else if constexpr (Vec16<DT>::NE == 4) {   // 32-bit rows that 1024 threads hold with four vectors each
+        HCCLX_LAUNCH((k_rms_norm_grad<DT, 4, false>), grid, block, 0, st, p, rows, elems, eps, partial);
     }
 }
 
@@ -411,7 +453,7 @@ int make_norm(const hcclx_rms_norm_t &a, hcclx_plan_t **plan)
     w->dtype = a.dtype;
     w->quant = quant;
     w->eps = a.eps;
-    w->shape = shape_of(a.row_elems, 16 / static_cast<int>(size));
+    w->shape = shape_of(a.row_elems, 16 / static_cast<int>(size), kMostVectors);
     const uint64_t elements = static_cast<uint64_t>(a.n) * a.rows * a.row_elems;
     const uint64_t algo = elements * (size * (1 + (a.residual != nullptr) + (a.total != nullptr)) + (quant ? 1 : size));
     return plan_of(ctx, std::move(w), algo, 0, plan);
@@ -437,9 +479,10 @@ int make_norm_grad(const hcclx_rms_norm_grad_t &a, hcclx_plan_t **plan)
     w->elems = a.row_elems;
     w->dtype = a.dtype;
     w->eps = a.eps;
-    w->shape = shape_of(a.row_elems, 16 / static_cast<int>(size));
+    w->shape = shape_of(a.row_elems, 16 / static_cast<int>(size), 2);
     const uint32_t most = (a.rows + w->shape.per_group - 1) / w->shape.per_group;
-    w->groups = std::min(most, std::max(1u, 4u * ctx->num_cus / a.n));
+    // a slot takes two rows at least, while there are workgroups for every CU: each slot's part of dweight is as long as a row of floats
+    w->groups = std::min(std::max((most + 1) / 2, std::min(most, ctx->num_cus / a.n)), std::max(1u, 4u * ctx->num_cus / a.n));
     uint64_t held = 0;
     if (w->want_dweight && a.rows != 0) {
         held = static_cast<uint64_t>(a.n) * w->groups * w->shape.per_group * a.row_elems * sizeof(float);
