@@ -101,11 +101,11 @@ __device__ __forceinline__ void load4(const void *base, uint64_t at, uint32_t ha
     const Global<const S> p = global<const S>(base) + at;
     if (have >= 4) {
         if constexpr (sizeof(S) == 4) {
-            const f32x4v x = __builtin_nontemporal_load(reinterpret_cast<Global<const f32x4_u>>(p));
+            const f32x4v x = *reinterpret_cast<Global<const f32x4_u>>(p);
 #pragma unroll
             for (int e = 0; e < 4; ++e) f[e] = x[e];
         } else {
-            const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<Global<const u32x2_u>>(p));
+            const u32x2 x = *reinterpret_cast<Global<const u32x2_u>>(p);
 #pragma unroll
             for (int e = 0; e < 4; ++e) f[e] = D::widen(static_cast<S>(x[e / 2] >> (16 * (e & 1))));
         }
@@ -137,7 +137,7 @@ __device__ __forceinline__ void store4(void *base, uint64_t at, uint32_t have, c
 __device__ __forceinline__ uint32_t load_codes(const void *base, uint64_t at, uint32_t have)
 {
     const Global<const uint8_t> p = global<const uint8_t>(base) + at;
-    if (have >= 4) return __builtin_nontemporal_load(reinterpret_cast<Global<const u32_u>>(p));
+    if (have >= 4) return *reinterpret_cast<Global<const u32_u>>(p);
     uint32_t c = 0;
 #pragma unroll
     for (uint32_t e = 0; e < 3; ++e) {

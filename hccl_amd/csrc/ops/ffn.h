@@ -38,8 +38,6 @@ struct FfnArgs {
     int act;
 };
 
-// Rows of 8-bit codes to x16 (kFfnGateUp's arguments).
-template <int DT> hipError_t launch_ffn_widen(const FfnArgs &a, hipStream_t st);
 template <int DT> hipError_t launch_ffn(FfnKind kind, const FfnArgs &a, uint32_t num_cus, hipStream_t st);
 
 }  // namespace hcclx

@@ -1,7 +1,7 @@
 // C entry points of the experts' gated feed-forward block (include/hcclx_ops.h: hcclx_gated_ffn_*): checks, the plans' scratch
 // memory and the order of the products.
 //
-// Forward: two launches, one per product pair (three for 8-bit rows).  Gradient: three; with T rows in all, the products of the
+// Forward: two launches (three where 8-bit rows are widened first).  Gradient: three; with T rows in all, the products of the
 // forward pass are 6 T dim hidden operations, those of the gradient twice as many.
 #include "hcclx_internal.h"
 #include "hcclx_ops.h"
@@ -59,11 +59,7 @@ struct FfnWork : PlanWork {
 
     int launch(const DeviceCtx *ctx, hipStream_t st) const override
     {
-        hipError_t e = hipSuccess;
-        if (up.x8) {
-            e = dtype == HCCL_DATA_TYPE_FP16 ? launch_ffn_widen<HCCL_DATA_TYPE_FP16>(up, st) : launch_ffn_widen<HCCL_DATA_TYPE_BFP16>(up, st);
-        }
-        if (e == hipSuccess) e = product(dtype, kFfnGateUp, up, ctx->num_cus, st);
+        hipError_t e = product(dtype, kFfnGateUp, up, ctx->num_cus, st);
         if (e == hipSuccess) e = product(dtype, kFfnDown, down, ctx->num_cus, st);
         return e == hipSuccess ? HCCL_SUCCESS : fail_hip(e, "feed-forward kernels");
     }

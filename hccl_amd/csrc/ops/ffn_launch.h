@@ -1,50 +1,63 @@
-// Which kernel computes a product: instantiated per type in ffn_bf16.hip and ffn_f16.hip.
+// Which kernel computes a product: instantiated per type in ffn_bf16.hip and ffn_f16.hip.  A choice goes by the sizes and by the
+// bound on the rows of all ranks, from which the rows of a rank are taken as if all had as many; whatever they turn out to be on
+// the device, every kernel is right for them.
 #pragma once
 #include "ops/ffn_gemm.h"
 #include "ops/ffn_thin.h"
 
 namespace hcclx {
+namespace ffn {
 
-// Rows per rank, if all have as many, up to which the forward products read the weights straight into registers.
-constexpr uint32_t kThinRows = 32;
-inline bool thin(const FfnRows &s) { return s.most <= static_cast<uint64_t>(s.n) * kThinRows; }
+// Products with few rows read the weights; what counts is how many bytes are on their way.  Tiles of 128 x 128 keep 48 KiB of
+// weights per CU on their way and read the rows' operand once per tile, but have to be as many as the CUs; the thin kernel
+// has eight wavefronts per 16 columns and reads the rows' operand that often.  Weights of dim x 2048, both products, thin : tiles,
+// us: 8 ranks x 7168 (256 tiles of the first product), 1 row 138 : 132, 16 rows 182 : 134; 4 ranks x 7168 (128), 1 row
+// 75 : 89, 8 rows 84 : 90, 16 rows 96 : 91; 2 ranks x 4096 (64), 1 row 26 : 59, 64 rows 55 : 61; 1 rank (32), 64 rows 39 : 56.
+template <int KIND>
+bool thin(const FfnRows &s, uint32_t cus)
+{
+    const uint64_t tiles = static_cast<uint64_t>(s.n) * ((columns<KIND>(s) + kTileCols<KIND> / 2 - 1) / (kTileCols<KIND> / 2));
+    const uint64_t rows = (s.most + s.n - 1) / s.n;
+    return (rows <= 64 && tiles <= cus / 4) || (rows <= 8 && tiles < cus);
+}
 
-// Rows per rank up to which products take tiles of half a whole tile's height and width.
+// Rows of a rank up to which tiles of 128 x 128 are taken: a whole tile would be half empty.
 constexpr uint32_t kSmallRows = 128;
-inline bool small_tiles(const FfnRows &s) { return s.most <= static_cast<uint64_t>(s.n) * kSmallRows; }
 
 template <int DT, int KIND>
-hipError_t launch_forward(const FfnArgs &a, uint32_t num_cus, hipStream_t st)
+hipError_t launch(const FfnArgs &a, uint32_t cus, hipStream_t st)
 {
     const FfnRows &s = a.rows;
-    if (s.most == 0) return hipSuccess;
-    if (!thin(s)) return ffn::run<DT, KIND>(a, small_tiles(s), num_cus, st);
-    const bool x8 = a.x8;
-    if (s.most <= static_cast<uint64_t>(s.n) * 16) {
-        ffn::launch_thin<DT, KIND, 1>(a, x8, st);
-    } else {
-        ffn::launch_thin<DT, KIND, 2>(a, x8, st);
+    if constexpr (KIND == kFfnGateUp || KIND == kFfnDown) {
+        if (s.most != 0 && thin<KIND>(s, cus)) {
+            const uint64_t rows = (s.most + s.n - 1) / s.n;
+            if (rows <= 16) {
+                launch_thin<DT, KIND, 1>(a, st);
+            } else if (rows <= 32) {
+                launch_thin<DT, KIND, 2>(a, st);
+            } else {
+                launch_thin<DT, KIND, 4>(a, st);
+            }
+            return hipGetLastError();
+        }
+        if (KIND == kFfnGateUp && a.x8 && s.most != 0) {   // (the thin kernel reads the codes)
+            HCCLX_LAUNCH((k_ffn_widen<DT>), dim3((s.most + 3) / 4), dim3(256), 0, st, a);
+        }
     }
-    return hipGetLastError();
+    return run<DT, KIND>(a, s.most <= static_cast<uint64_t>(s.n) * kSmallRows, cus, st);
 }
 
-template <int DT>
-hipError_t launch_ffn_widen(const FfnArgs &a, hipStream_t st)
-{
-    if (a.rows.most == 0 || thin(a.rows)) return hipSuccess;   // the thin kernel reads the codes
-    HCCLX_LAUNCH((ffn::k_ffn_widen<DT>), dim3((a.rows.most + 3) / 4), dim3(256), 0, st, a);
-    return hipGetLastError();
-}
+}  // namespace ffn
 
 template <int DT>
 hipError_t launch_ffn(FfnKind kind, const FfnArgs &a, uint32_t num_cus, hipStream_t st)
 {
     switch (kind) {
-        case kFfnGateUp: return launch_forward<DT, kFfnGateUp>(a, num_cus, st);
-        case kFfnDown: return launch_forward<DT, kFfnDown>(a, num_cus, st);
-        case kFfnGradHidden: return ffn::run<DT, kFfnGradHidden>(a, small_tiles(a.rows), num_cus, st);
-        case kFfnGradInput: return ffn::run<DT, kFfnGradInput>(a, small_tiles(a.rows), num_cus, st);
-        default: return ffn::run<DT, kFfnGradWeights>(a, small_tiles(a.rows), num_cus, st);
+        case kFfnGateUp: return ffn::launch<DT, kFfnGateUp>(a, num_cus, st);
+        case kFfnDown: return ffn::launch<DT, kFfnDown>(a, num_cus, st);
+        case kFfnGradHidden: return ffn::launch<DT, kFfnGradHidden>(a, num_cus, st);
+        case kFfnGradInput: return ffn::launch<DT, kFfnGradInput>(a, num_cus, st);
+        default: return ffn::launch<DT, kFfnGradWeights>(a, num_cus, st);
     }
 }
 

@@ -1,7 +1,7 @@
 // The forward products for few rows per rank (a decoding step), where the time is that of reading the weights once.
 //
 // A workgroup takes 16 columns of C (of both weights) of one rank and all its rows, 16 x MB at a time; its eight wavefronts share
-// out k in turns of 64 and add up their parts in LDS.  Weights go from memory to the matrix instruction's registers without LDS:
+// out k in turns of 64 and add up their parts in LDS, in the order of the wavefronts.  Weights go from memory to the matrix instruction's registers without LDS:
 // nobody else needs them.  A lane's two chunks of 16 bytes of a turn lie next to each other (k = 16 (lane / 16) .. + 15), so that
 // four lanes read a cache line of a row; the same k of the rows of x, which come from the L2.
 //
@@ -14,7 +14,10 @@ namespace ffn {
 
 constexpr uint32_t kThinWaves = 8;
 constexpr uint32_t kTurnK = 64;
-constexpr int kAhead = 4;   // turns whose loads are on their way together
+// Turns whose loads are on their way together.  (Two, four, eight: 8 ranks x 1 row x 7168 x 2048, second product 67, 80, 113 us; first
+// 95, 93, 104.  More registers leave fewer wavefronts on a CU, and a turn behind the last costs as much as any.  Sixteen
+// wavefronts instead of eight: 73 and 101.)
+constexpr int kAhead = 2;
 
 template <int DT, int KIND, int MB, bool X8>
 __global__ void __launch_bounds__(kThinWaves * 64)
@@ -149,12 +152,12 @@ k_ffn_thin(FfnArgs a)
 }
 
 template <int DT, int KIND, int MB>
-void launch_thin(const FfnArgs &a, bool x8, hipStream_t st)
+void launch_thin(const FfnArgs &a, hipStream_t st)
 {
     const uint32_t cols = columns<KIND>(a.rows);
     const dim3 grid((cols + 15) / 16, a.rows.n);
     if constexpr (KIND == kFfnGateUp) {
-        if (x8) {
+        if (a.x8) {
             HCCLX_LAUNCH((k_ffn_thin<DT, KIND, MB, true>), grid, dim3(kThinWaves * 64), 0, st, a);
             return;
         }

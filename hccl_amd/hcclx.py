@@ -250,9 +250,16 @@ def _ranks(what, ptrs, n):
 class _OperatorPlan(Plan):
     def _create(self, entry, *args):
         self._h = None
+        lib = _lib.load()
         h = ctypes.c_void_p()
-        check(getattr(_lib.load(), entry)(*args, ctypes.byref(h)))
+        check(getattr(lib, entry)(*args, ctypes.byref(h)))
         self._h = h
+        self._launch = lib.hcclx_plan_launch
+
+    def launch(self, stream=0):
+        rc = self._launch(self._h, stream)
+        if rc:
+            check(rc)
 
 
 class RmsNormPlan(_OperatorPlan):
@@ -329,9 +336,14 @@ class AdamWPlan(_OperatorPlan):
                 setattr(a, k, t.get(k) or None)
         self._create("hcclx_adamw_plan_create", arr, len(tensors), int(grad_dtype), int(state_dtype),
                      int(grad_dtype if copy_dtype is None else copy_dtype))
+        self._args = _lib.AdamWStep()
+        self._args_ref = ctypes.byref(self._args)
+        self._step = _lib.load().hcclx_adamw_step
 
     def step(self, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, seed=0, grad_scale=0, stream=0):
         """step: 1, 2, ...; seed: 32 bits, another one every step (8-bit states); grad_scale: device address of a float that
         multiplies the gradients, or 0."""
-        a = _lib.AdamWStep(lr, beta1, beta2, eps, step, seed & 0xFFFFFFFF, grad_scale or None)
-        check(_lib.load().hcclx_adamw_step(self._h, ctypes.byref(a), ctypes.c_void_p(stream)))
+        self._args.__init__(lr, beta1, beta2, eps, step, seed & 0xFFFFFFFF, grad_scale or None)
+        rc = self._step(self._h, self._args_ref, stream)
+        if rc:
+            check(rc)
