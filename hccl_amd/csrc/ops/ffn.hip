@@ -23,7 +23,7 @@ int check_shape(const hcclx_ffn_shape_t &s, FfnRows *out)
     }
     const uint64_t all = static_cast<uint64_t>(s.n) * s.capacity;
     const uint64_t most = s.rows == 0 || s.rows > all ? all : s.rows;
-    if (most > 0x7fffffffull) return fail(HCCL_E_PARA, "too many rows");
+    if (most > 0xffffffffull / 256) return fail(HCCL_E_PARA, "too many rows");   // a workgroup of 256 for each, in one launch
     if (s.counts != nullptr && (s.counts_per_rank == 0 || s.counts_per_rank > kFfnRanks)) {
         return fail(HCCL_E_PARA, "counts per rank outside 1.." + std::to_string(kFfnRanks));
     }

@@ -41,7 +41,7 @@ hipError_t launch(const FfnArgs &a, uint32_t cus, hipStream_t st)
             return hipGetLastError();
         }
         if (KIND == kFfnGateUp && a.x8 && s.most != 0) {   // (the thin kernel reads the codes)
-            HCCLX_LAUNCH((k_ffn_widen<DT>), dim3((s.most + 3) / 4), dim3(256), 0, st, a);
+            HCCLX_LAUNCH((k_ffn_widen<DT>), dim3(s.most), dim3(256), 0, st, a);
         }
     }
     return run<DT, KIND>(a, s.most <= static_cast<uint64_t>(s.n) * kSmallRows, cus, st);
