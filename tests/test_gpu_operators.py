@@ -476,6 +476,29 @@ def test_ffn_of_many_rows(rows, dim, hidden, dtype):
     f.check()
 
 
+# On both sides of where another kernel, tile or split of what is left of a round takes over (256 CUs).
+FFN_EDGES = [([16], 16, 264, 520), ([17], 17, 264, 520), ([32], 32, 520, 264), ([33], 33, 520, 264), ([64], 64, 1032, 136), ([65], 65, 1032, 136),
+             ([128, 128], 128, 264, 136), ([128, 129], 129, 264, 136), ([100, 0, 20, 128], 128, 1032, 520), ([0, 0], 400, 264, 136),
+             ([0, 700, 0], 700, 136, 264), ([2000], 2000, 648, 1272), ([3900], 3900, 1288, 1272), ([1], 700, 520, 264)]
+
+
+@pytest.mark.parametrize("dtype", [T.FP16, T.BFP16])
+@pytest.mark.parametrize("rows,capacity,dim,hidden", FFN_EDGES)
+def test_ffn_at_the_edges_of_its_kernels(rows, capacity, dim, hidden, dtype):
+    f = Ffn(rows, capacity, dim, hidden, dtype, 3 * dim + hidden)
+    f.run()
+    f.check()
+    if capacity > max(rows):                                       # the same rows in plans made for capacity
+        f.run(bound=0)
+        f.check()
+
+
+def test_ffn_of_rows_from_many_senders():
+    f = Ffn([5, 164, 0], 170, 72, 136, T.BFP16, 12, per_rank=63)
+    f.run()
+    f.check()
+
+
 def test_ffn_rows_are_counted_on_the_device():
     """One plan, launched after the counts change; rows beyond capacity, and beyond the bound on all rows, are left alone."""
     f = Ffn([9, 4, 7], 9, 64, 48, T.BFP16, 4, per_rank=3)
@@ -533,6 +556,17 @@ def test_ffn_gradient_against_differences():
 @pytest.mark.parametrize("rows,dim,hidden", [([1], 16, 8), ([3, 0, 70], 1040, 136), ([2, 2], 2048, 512), ([600, 900], 528, 264)])
 def test_ffn_of_8_bit_rows(rows, dim, hidden, dtype):
     """Rows as the norm writes them: codes and a scale each; counts in elements of those rows."""
+    check_8_bit_rows(rows, dim, hidden, dtype)
+
+
+@pytest.mark.parametrize("dtype", [T.FP16, T.BFP16])
+@pytest.mark.parametrize("rows,dim,hidden", [([16], 272, 136), ([17], 272, 136), ([20, 40, 3], 528, 72), ([64], 1040, 136), ([65], 1040, 136),
+                                             ([100, 0, 9, 128], 1040, 264), ([129], 272, 136)])
+def test_ffn_of_8_bit_rows_at_the_edges_of_its_kernels(rows, dim, hidden, dtype):
+    check_8_bit_rows(rows, dim, hidden, dtype)
+
+
+def check_8_bit_rows(rows, dim, hidden, dtype):
     n, cap, g, td = len(rows), max(rows), gen(dim), TD[dtype]
     x = [normal((cap, dim), torch.float32, g, 4.0) for _ in range(n)]
     w = torch.ones(dim, device=DEV)
