@@ -3,7 +3,16 @@
 // Every product is  C[m][n] = sum over k of A[m][k] B[n][k]  in tiles of BM x BN, with the operands as they lie in memory: "k-wise"
 // (k runs along a row of the buffer) or "crosswise" (k counts the rows of the buffer).  A tile of either operand comes to LDS by
 // loads that write LDS directly, 64 k at a time, two stages deep; crosswise tiles are read back with the transposing LDS read.
-// v_mfma 16x16x32 takes B as its first operand, so that a lane ends up with four neighbouring columns of C.
+// v_mfma 16x16x32 takes B as its first operand, so that a lane ends up with four neighbouring columns of C.  (From registers alone
+// it reaches 2100 TFLOP/s here, 32x32x16 1350.)
+//
+// What bounds it: the matrix instructions, of which 70 % of the time is full, at the clock that the card's power leaves (1.9 GHz).
+// 8 ranks x 4096 rows x 7168 x 2048 1400 us for the first product (1370 TFLOP/s), 750 for the second (1280).  A wavefront has 128 x
+// 128 of a tile of 256 x 256, which is one wavefront per SIMD, 256 accumulators in the second half of its registers and one LDS
+// read of 1 KiB for four matrix instructions; eight wavefronts of 128 x 64 read half as much again and took 1580 and 820.  With
+// nobody else on its SIMD a wavefront has to keep the matrix pipe busy by itself: between two matrix instructions there is one
+// LDS read, or one load, or a few scalar instructions (all of a stage's loads at once: as slow as eight wavefronts), and what is
+// read is a row of fragments ahead.  Stages of 32 k, more of them, took 1890.
 //
 // LDS layout: chunks of 16 bytes (k-wise) or 32 bytes (crosswise) of a row are permuted by an exclusive or with the row's number,
 // so that the lanes of a read meet different banks.  The loads write LDS in lane order, hence the permutation is applied to the
@@ -34,12 +43,11 @@ constexpr uint32_t kOut = 0x80000000u;   // an offset behind every range
 constexpr uint32_t kRaw = 0x00027000u;        // last word of a buffer resource: plain bytes, range-checked
 constexpr uint32_t kMostRange = 0x7fffffffu;
 constexpr uint32_t kBK = 64;             // k of a stage: a cache line of a k-wise row
-constexpr uint32_t kWaves = 8;           // of a workgroup, two by four
+constexpr uint32_t kWaves = 4;           // of a workgroup, two by two
 constexpr uint32_t kWaveRows = 2;
-constexpr uint32_t kWaveCols = 4;
+constexpr uint32_t kWaveCols = 2;
 constexpr uint32_t kTile = 256;          // rows and columns of a whole tile
-constexpr uint32_t kTableBytes = 1024;
-constexpr uint32_t kLdsBytes = 160 * 1024 - kTableBytes;        // for stages
+constexpr uint32_t kLdsBytes = 160 * 1024;
 
 template <int DT> struct Mma;
 template <> struct Mma<HCCL_DATA_TYPE_BFP16> {
@@ -49,6 +57,7 @@ template <> struct Mma<HCCL_DATA_TYPE_BFP16> {
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
     }
+    static __device__ __forceinline__ void add(f32x4 &c, u32x4 a, u32x4 b) { asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b)); }
 };
 template <> struct Mma<HCCL_DATA_TYPE_FP16> {
     typedef _Float16 E;
@@ -57,6 +66,7 @@ template <> struct Mma<HCCL_DATA_TYPE_FP16> {
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
     }
+    static __device__ __forceinline__ void add(f32x4 &c, u32x4 a, u32x4 b) { asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b)); }
 };
 
 // Four floats rounded to nearest even, as 8 bytes.
@@ -99,11 +109,6 @@ struct Window {
     {
     }
     __device__ __forceinline__ void store(uint32_t offset, u32x4 v) const { __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, offset, 0, 0); }
-    __device__ __forceinline__ void store_half(uint32_t offset, uint2 v) const
-    {
-        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-        __builtin_amdgcn_raw_buffer_store_b64(u32x2{v.x, v.y}, rsrc, offset, 0, 0);
-    }
     __device__ __forceinline__ f32x4 load(uint32_t offset) const
     {
         return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, offset, 0, 0));
@@ -197,7 +202,9 @@ __device__ __forceinline__ void in_groups(uint32_t at, uint32_t mts, uint32_t nt
 }
 
 // How whole tiles are shared out.  T of them on W CUs take T / W rounds and one more for what is left, however little; so what is
-// left is cut into parts, of which a CU has at most one: quarters of up to W / 4 tiles, halves (of the columns) of up to W / 2.
+// left is cut into parts, of which a CU has at most one: quarters of up to W / 4 tiles, halves (of the columns) of up to W / 2.  One
+// rank, bf16, cut : whole, forward and gradients: 1024 rows x 2048 x 2048 53 + 120 : 102 + 220 us, 2048 x 4096 x 2048 (a round and
+// halves or quarters of one) 101 + 220 : 156 + 343.  More than W / 2 are left whole: three quarters of a tile take as long as it.
 // The eight XCDs take workgroups in turn and have an L2 each: every XCD gets a run of neighbours out of each round.
 struct Share {
     uint32_t whole;   // tiles that are not cut
@@ -220,16 +227,14 @@ __host__ __device__ inline uint32_t columns(const FfnRows &s)
 }
 template <int KIND> constexpr uint32_t kTileCols = KIND == kFfnGateUp ? kTile / 2 : kTile;   // half of a tile from either weight
 
-// Two loads of 16 bytes per lane, from the range-checked buffer at the lanes' offsets to lds + 16 * lane and 1024 behind.  Written
-// out because the compiler waits for every such load that it knows of before it lets a transposing LDS read go, whatever that
-// reads; here loads and reads keep apart by meet().  There is no register that the loads write.  s_nop: five wait states between
-// a vector instruction that may have written the scalar operands and the first load, one behind a write of m0.
+// A load of 16 bytes per lane, from the range-checked buffer at the lanes' offsets to lds + 16 * lane.  Written out because the
+// compiler waits for every such load that it knows of before it lets a transposing LDS read go, whatever that reads; here loads and
+// reads keep apart by meet().  There is no register that the load writes.  s_nop: a wait state behind a write of m0.  A buffer
+// whose scalars a vector instruction may have written takes five, which are between the making of a buffer and its first load.
 typedef uint32_t Resource __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ void load_to_lds(Resource buffer, uint32_t lds, uint32_t first, uint32_t second)
+__device__ __forceinline__ void load_to_lds(Resource buffer, uint32_t lds, uint32_t offset)
 {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %4, 0 offen lds\n\t"
-                 "s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %4, 0 offen lds" ::"s"(lds), "s"(lds + 1024), "v"(first), "v"(second),
-                 "s"(buffer) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory");
 }
 
 // Brings R rows (k-wise: of the operand; crosswise: R columns of kBK rows) of a stage to LDS.
@@ -238,7 +243,7 @@ struct Stager {
     static constexpr uint32_t kLoads = R * kBK * 2 / 1024 / kWaves;
     static constexpr uint32_t kChunks = KWISE ? kBK / 8 : R / 8;   // of 16 bytes, of a row
     static constexpr uint32_t kRows = 64 / kChunks;                // of a load
-    static_assert(kLoads * 1024 * kWaves == R * kBK * 2 && kRows * kChunks == 64 && kLoads % 2 == 0, "every wavefront loads as much, in whole rows");
+    static_assert(kLoads * 1024 * kWaves == R * kBK * 2 && kRows * kChunks == 64, "every wavefront loads as much, in whole rows");
     uint32_t row_at;   // offset of the first load's row
     uint32_t chunk;    // and the chunk of it
 
@@ -255,25 +260,29 @@ struct Stager {
         }
         row_at = row * ld;
     }
-    // base: of the stage; range: bytes from there on that exist; end: k (k-wise) or columns (crosswise) that do
-    __device__ __forceinline__ void issue(const char *base, uint32_t range, uint32_t end, uint32_t ld, uint32_t lds, uint32_t wave) const
+    // Load i of a stage in `buffer`.  end: k (k-wise) or columns (crosswise) that exist
+    __device__ __forceinline__ void issue(uint32_t i, Resource buffer, uint32_t end, uint32_t ld, uint32_t lds, uint32_t wave) const
     {
-        const uint64_t at = reinterpret_cast<uint64_t>(base);
-        const Resource buffer = {uniform(static_cast<uint32_t>(at)), uniform(static_cast<uint32_t>(at >> 32) & 0xffffu), uniform(range), kRaw};
-        uint32_t offset[kLoads];
-#pragma unroll
-        for (uint32_t i = 0; i < kLoads; ++i) {
-            // (crosswise: of the row's number, the first two bits and the fourth turn the chunks; a load is kRows rows further on)
-            constexpr bool kTurns = !KWISE && kRows < 4;
-            static_assert(KWISE || kRows * kLoads <= 8, "the fourth bit is the wavefront's");
-            const uint32_t c = kTurns ? chunk ^ ((i * kRows) & 3) * 2 : chunk;
-            const uint32_t o = c * 8 < end ? row_at + c * 16 : kOut;
-            offset[i] = o + i * kRows * ld;
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < kLoads; i += 2) load_to_lds(buffer, uniform(lds + (wave * kLoads + i) * 1024), offset[i], offset[i + 1]);
+        load_to_lds(buffer, uniform(lds + (wave * kLoads + i) * 1024), at(i, end, ld));
+    }
+
+private:
+    __device__ __forceinline__ uint32_t at(uint32_t i, uint32_t end, uint32_t ld) const
+    {
+        // (crosswise: of the row's number, the first two bits and the fourth turn the chunks; a load is kRows rows further on)
+        constexpr bool kTurns = !KWISE;
+        
+        const uint32_t c = kTurns ? chunk ^ (((i * kRows) & 3) | (((i * kRows) >> 3) & 1) << 2) * 2 : chunk;
+        return (c * 8 < end ? row_at + c * 16 : kOut) + i * kRows * ld;
     }
 };
+
+// base: of a stage; range: bytes from there on that exist
+__device__ __forceinline__ Resource resource(const char *base, uint32_t range)
+{
+    const uint64_t at = reinterpret_cast<uint64_t>(base);
+    return {uniform(static_cast<uint32_t>(at)), uniform(static_cast<uint32_t>(at >> 32) & 0xffffu), uniform(range), kRaw};
+}
 
 // A fragment of 16 rows by 32 k out of a staged tile.
 template <bool KWISE, uint32_t R>
@@ -310,22 +319,27 @@ struct Reader {
     }
 };
 
-// act(a) and its derivative.
+// act(a) = a / (1 + exp(-w(a))) and its derivative: both activations with w = a (p + q a^2), SILU with 1 and 0, and GELU_TANH, whose
+// (1 + tanh z) / 2 is 1 / (1 + exp(-2 z)).
+struct ActTerms {
+    float p;
+    float q;
+    __device__ __forceinline__ explicit ActTerms(int act)
+    {
+        constexpr float kTwice = 1.5957691216057308f;   // 2 sqrt(2 / pi)
+        p = act == HCCLX_ACT_SILU ? 1.0f : kTwice;
+        q = act == HCCLX_ACT_SILU ? 0.0f : kTwice * 0.044715f;
+    }
+};
 struct Act {
     float value;
     float slope;
-    __device__ __forceinline__ Act(float a, int act)
+    __device__ __forceinline__ Act(float a, const ActTerms &t)
     {
-        if (act == HCCLX_ACT_SILU) {
-            const float s = 1.0f / (1.0f + __expf(-a));
-            value = a * s;
-            slope = s * (1.0f + a * (1.0f - s));
-        } else {
-            constexpr float kRoot = 0.7978845608028654f;   // sqrt(2 / pi)
-            const float t = 1.0f - 2.0f / (__expf(2.0f * kRoot * (a + 0.044715f * a * a * a)) + 1.0f);
-            value = 0.5f * a * (1.0f + t);
-            slope = 0.5f * (1.0f + t) + 0.5f * a * (1.0f - t * t) * (kRoot * (1.0f + 3.0f * 0.044715f * a * a));
-        }
+        const float square = __builtin_fminf(a * a, 1e30f);   // (0 times infinity is not 0; the exponential is 0 long before)
+        const float s = 1.0f / (1.0f + __expf(-a * (t.p + t.q * square)));
+        value = a * s;
+        slope = s * (1.0f + a * (1.0f - s) * (t.p + 3.0f * t.q * square));
     }
 };
 
@@ -404,21 +418,11 @@ __device__ __forceinline__ Feed feed_of(const FfnArgs &a, const Tile &t, uint32_
 template <int LOADS>
 __device__ __forceinline__ void meet()
 {
+    static_assert(LOADS < 64, "the counter's range");
     __builtin_amdgcn_sched_barrier(0);   // the matrix instructions in front stay there and run while this waits
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-}
-
-// Asks the scheduler to issue a row's LDS reads, then its matrix instructions.
-template <int ROWS, int MFMAS, int READS>
-__device__ __forceinline__ void spread()
-{
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);   // LDS reads
-        __builtin_amdgcn_sched_group_barrier(0x008, MFMAS, 0);   // matrix instructions
-    }
 }
 
 // Writes a tile of C, or what becomes of it.
@@ -435,6 +439,7 @@ __device__ __forceinline__ void results(const FfnArgs &a, const Tile &t, const f
     const uint32_t col_of = lane / 16 * 4;
     constexpr int kOwn = KIND == kFfnGateUp ? FN / 2 : FN;   // fragments of C across
     const uint32_t first = t.n0 + wn * (kOwn * 16);
+    const ActTerms terms(a.act);
     if constexpr (KIND == kFfnGradWeights) {
         const uint32_t width = t.weight == 2 ? hidden : dim;
         const uint32_t height = t.weight == 2 ? dim : hidden;
@@ -474,15 +479,13 @@ __device__ __forceinline__ void results(const FfnArgs &a, const Tile &t, const f
                     }
                     f32x4 r;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) r[e] = Act(g[e], a.act).value * u[e];
+                    for (int e = 0; e < 4; ++e) r[e] = Act(g[e], terms).value * u[e];
                     h[n] = narrow4<DT>(r);
                 }
-                if constexpr (kOwn == 2) {
-                    const uint32_t col = first + col_in;
-                    to_h.store(live && col < hidden ? row * hidden * 2 + col * 2 : kOut, pair_up(h[0], h[1]));
-                } else {
-                    const uint32_t col = first + col_of;
-                    to_h.store_half(live && col < hidden ? row * hidden * 2 + col * 2 : kOut, h[0]);
+#pragma unroll
+                for (int n = 0; n < kOwn; n += 2) {
+                    const uint32_t col = first + n * 16 + col_in;
+                    to_h.store(live && col < hidden ? row * hidden * 2 + col * 2 : kOut, pair_up(h[n], h[n + 1]));
                 }
             }
         } else if constexpr (KIND == kFfnGradHidden) {
@@ -507,7 +510,7 @@ __device__ __forceinline__ void results(const FfnArgs &a, const Tile &t, const f
                     f32x4 r, d0, d1;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const Act f(g[n][e], a.act);
+                        const Act f(g[n][e], terms);
                         r[e] = f.value * u[n][e];
                         d0[e] = acc[m][n][e] * u[n][e] * f.slope;
                         d1[e] = acc[m][n][e] * f.value;
@@ -541,9 +544,22 @@ __device__ __forceinline__ void results(const FfnArgs &a, const Tile &t, const f
     }
 }
 
+// Waits until the accumulators' last products, or zeros, are in their registers: what the compiler does by itself for instructions
+// that it knows.
+template <int FM, int FN>
+__device__ __forceinline__ void settle(f32x4 (&acc)[FM][FN])
+{
+    asm volatile("s_nop 15\n\ts_nop 7" ::: "memory");
+#pragma unroll
+    for (int m = 0; m < FM; ++m) {
+#pragma unroll
+        for (int n = 0; n < FN; n += 4) asm volatile("" : "+a"(acc[m][n]), "+a"(acc[m][n + 1]), "+a"(acc[m][n + 2]), "+a"(acc[m][n + 3]));
+    }
+}
+
 // Tiles of wavefronts of FM x FN fragments each: t and what next(&t) gives after it, until it says no; their operands' rows have the
-// same lengths.  The stages of one tile
-// follow those of the one before without a break, so that the first of them are on their way while results are written.
+// same lengths.  The stages of one tile follow those of the one before without a break, so that the first of them are on their way
+// while results are written.
 template <int DT, int KIND, int FM, int FN, typename Next>
 __device__ __forceinline__ void products(const FfnArgs &a, Tile t, char *s_tile, Next &&next)
 {
@@ -553,65 +569,135 @@ __device__ __forceinline__ void products(const FfnArgs &a, Tile t, char *s_tile,
     constexpr bool kAk = KIND != kFfnGradWeights;          // A lies k-wise
     constexpr bool kBk = KIND == kFfnGateUp || KIND == kFfnDown;
     constexpr uint32_t kCols = kPair ? BN / 2 : BN;        // columns of C
-    constexpr uint32_t kStage = (BM + BN) * kBK * 2;
-    constexpr uint32_t kStages = kLdsBytes / kStage;
+    constexpr uint32_t kStageA = BM * kBK * 2;
+    constexpr uint32_t kStageB = BN * kBK * 2;
+    // As many stages as fit, with one more of A: A's loads go out in the first half of a stage's products and B's in the second.
+    constexpr uint32_t kStages = (kLdsBytes - kStageA) / (kStageA + kStageB);
     constexpr uint32_t kPairs = KIND == kFfnGradInput ? 2 : 1;
 
     const uint32_t wave = uniform(threadIdx.x / 64);
     const uint32_t lane = threadIdx.x & 63;
     const uint32_t wm = wave / kWaveCols;
     const uint32_t wn = wave % kWaveCols;
-    auto place = [&](uint32_t slot) { return (lds_char *)s_tile + slot * kStage; };
+    auto place_a = [&](uint32_t slot) { return (lds_char *)s_tile + slot * kStageA; };
+    auto place_b = [&](uint32_t slot) { return (lds_char *)s_tile + (kStages + 1) * kStageA + slot * kStageB; };
+    auto after_a = [](uint32_t slot) { return slot == kStages ? 0 : slot + 1; };
+    auto after_b = [](uint32_t slot) { return slot + 1 == kStages ? 0 : slot + 1; };
 
     Stager<BM, kAk, false> sa;
     Stager<BN, kBk, kPair> sb;
     Feed from = feed_of<KIND, BN>(a, t, wave);
     sa.init(wave, lane, from.a_ld);
     sb.init(wave, lane, from.b_ld);
-    constexpr int kReads = (kAk ? 1 : 2) + (kBk ? 1 : 2);
-    constexpr int kLoads = decltype(sa)::kLoads + decltype(sb)::kLoads;
-    static_assert(kStages >= 2 && kLoads * (kStages - 1) < 64, "two stages fit; the counter of loads holds what is on its way");
+    constexpr int kLoadsA = decltype(sa)::kLoads;
+    constexpr int kLoadsB = decltype(sb)::kLoads;
+    constexpr int kLoads = kLoadsA + kLoadsB;
+    static_assert(kStages >= 2 && kLoadsA <= FM && kLoadsB <= FM, "two stages fit; every row of fragments issues a load of each");
 
     // The loads run ahead of the products: `from` is where they are, `then` what follows (if `more`), `left` k of this pair are to
     // come in `steps` stages.  A tile has kStages stages at least (of zeros, if need be): when its products begin, all of those
-    // are its own.
-    auto stages_of = [&](const Feed &f) {
+    // are its own.  Without branches, and in pieces that fit between two matrix instructions; the empty asm keeps the compiler
+    // from moving a piece.
+    auto stages_of = [&](const Feed &f) -> int {
         const uint32_t n = (f.k + kBK - 1) / kBK * kPairs;
         return n < kStages ? kStages : n;
     };
     Feed then = from;
-    bool more = false;
+    uint32_t more = 0;
     uint32_t left = from.k;
-    uint32_t steps = stages_of(from);
+    int steps = stages_of(from);
     uint32_t pair = 0;
-    auto follow = [&] {   // on to the next tile
-        if (!more) return;
-        more = false;
-        from = then;
-        left = from.k;
-        steps = stages_of(from);
-        pair = 0;
+    struct Stage {
+        Resource r;
+        uint32_t end, ld;
     };
-    auto stage = [&](uint32_t slot) {
-        const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)s_tile)) + slot * kStage;
-        const uint32_t k = left < kBK ? left : kBK;
-        const uint32_t a_rows = kAk ? (from.a_extent < BM ? from.a_extent : BM) : k;
-        const uint32_t b_rows = kBk ? (from.b_extent < kCols ? from.b_extent : kCols) : k;
-        const uint32_t a_range = k == 0 ? 0 : (a_rows - 1) * from.a_ld + (kAk ? k : from.a_extent) * 2;
-        const uint32_t b_range = k == 0 ? 0 : (b_rows - 1) * from.b_ld + (kBk ? k : from.b_extent) * 2;
-        sa.issue(from.a[0], a_range, kAk ? k : from.a_extent, from.a_ld, lds, wave);
-        sb.issue(from.b[0], b_range, kBk ? k : from.b_extent, from.b_ld, lds + BM * kBK * 2, wave);
-        left -= k;
-        from.a[0] += kAk ? kBK * 2 : static_cast<uint64_t>(from.a_ld) * kBK;
-        from.b[0] += kBk ? kBK * 2 : static_cast<uint64_t>(from.b_ld) * kBK;
-        if (KIND == kFfnGradInput && left == 0 && pair == 0) {
-            pair = 1;
-            left = from.k;
-            from.a[0] = from.a[1];
-            from.b[0] = from.b[1];
+    Stage ga, gb;   // the next of A to be loaded, and of B
+    uint32_t k = 0, rows = 0, range = 0, on = 0;
+    auto k_left = [&] { return left < kBK ? left : kBK; };
+    constexpr int kPiecesA = 3;
+    auto next_a = [&](int i) {
+        if (i == 0) {
+            k = k_left();
+            rows = kAk ? (from.a_extent < BM ? from.a_extent : BM) : k;
+            asm volatile("" : "+s"(k), "+s"(rows));
         }
-        if (steps != 0) --steps;
-        if (steps == 0) follow();
+        if (i == 1) {
+            range = k == 0 ? 0 : (rows - 1) * from.a_ld + (kAk ? k : from.a_extent) * 2;
+            asm volatile("" : "+s"(range));
+        }
+        if (i == 2) {
+            ga = {resource(from.a[0], range), kAk ? k : from.a_extent, from.a_ld};
+            asm volatile("" : "+s"(ga.r));
+        }
+    };
+    constexpr int kPiecesB = 11;
+    constexpr int kPiecesOfB = 3;   // the others take `from` on to the next stage, or to the next tile if this one's are all on their way
+    auto next_b = [&](int i) {
+        if (i == 0) {
+            k = k_left();
+            rows = kBk ? (from.b_extent < kCols ? from.b_extent : kCols) : k;
+            asm volatile("" : "+s"(k), "+s"(rows));
+        }
+        if (i == 1) {
+            range = k == 0 ? 0 : (rows - 1) * from.b_ld + (kBk ? k : from.b_extent) * 2;
+            asm volatile("" : "+s"(range));
+        }
+        if (i == 2) {
+            gb = {resource(from.b[0], range), kBk ? k : from.b_extent, from.b_ld};
+            asm volatile("" : "+s"(gb.r));
+        }
+        if (i == 3) {
+            left -= k;
+            from.a[0] += kAk ? kBK * 2 : static_cast<uint64_t>(from.a_ld) * kBK;
+            asm volatile("" : "+s"(left), "+s"(from.a[0]));
+        }
+        if (i == 4) {
+            from.b[0] += kBk ? kBK * 2 : static_cast<uint64_t>(from.b_ld) * kBK;
+            asm volatile("" : "+s"(from.b[0]));
+        }
+        if (KIND == kFfnGradInput && i == 5) {
+            const bool second = left == 0 && pair == 0;
+            pair = second ? 1 : pair;
+            left = second ? from.k : left;
+            from.a[0] = second ? from.a[1] : from.a[0];
+            from.b[0] = second ? from.b[1] : from.b[0];
+            asm volatile("" : "+s"(left), "+s"(pair), "+s"(from.a[0]), "+s"(from.b[0]));
+        }
+        if (i == 6) {
+            --steps;
+            on = steps <= 0 ? more : 0;
+            more -= on;
+            asm volatile("" : "+s"(steps), "+s"(on), "+s"(more));
+        }
+        if (i == 7) {
+            from.a[0] = on != 0 ? then.a[0] : from.a[0];
+            from.a[1] = on != 0 ? then.a[1] : from.a[1];
+            asm volatile("" : "+s"(from.a[0]), "+s"(from.a[1]));
+        }
+        if (i == 8) {
+            from.b[0] = on != 0 ? then.b[0] : from.b[0];
+            from.b[1] = on != 0 ? then.b[1] : from.b[1];
+            asm volatile("" : "+s"(from.b[0]), "+s"(from.b[1]));
+        }
+        if (i == 9) {
+            from.a_extent = on != 0 ? then.a_extent : from.a_extent;
+            from.b_extent = on != 0 ? then.b_extent : from.b_extent;
+            from.k = on != 0 ? then.k : from.k;
+            asm volatile("" : "+s"(from.a_extent), "+s"(from.b_extent), "+s"(from.k));
+        }
+        if (i == 10) {
+            left = on != 0 ? then.k : left;
+            steps = on != 0 ? stages_of(then) : steps;
+            pair = on != 0 ? 0 : pair;
+            asm volatile("" : "+s"(left), "+s"(steps), "+s"(pair));
+        }
+    };
+
+    auto issue_a = [&](int i, uint32_t slot) {
+        if (i < kLoadsA) sa.issue(i, ga.r, ga.end, ga.ld, static_cast<uint32_t>(reinterpret_cast<uintptr_t>(place_a(slot))), wave);
+    };
+    auto issue_b = [&](int i, uint32_t slot) {
+        if (i < kLoadsB) sb.issue(i, gb.r, gb.end, gb.ld, static_cast<uint32_t>(reinterpret_cast<uintptr_t>(place_b(slot))), wave);
     };
 
     const Reader<kAk, BM> ra(lane);
@@ -625,87 +711,115 @@ __device__ __forceinline__ void products(const FfnArgs &a, Tile t, char *s_tile,
             return wn * FN + n;
         }
     };
-    // Fragments of 32 k at a time.  While they are multiplied, row of fragments by row, the next ones are read: one of A into the
-    // registers of the row just done, and B's into a second set.  When everybody has read the last of a stage, the one kStages
-    // behind it is loaded into its place; it has the time of kStages - 1 stages to land.
+    // Fragments of 32 k at a time.  While they are multiplied, row of fragments by row, the next ones are read: A's into the
+    // registers of the rows done, of which there are kEarly more than rows, so that the last of a stage is read kEarly rows before
+    // its end, and B's into a second set.  When everybody has read the last of a stage, the one kStages behind it is loaded into its
+    // place, B's in the half that follows and A's in the one after.
     f32x4 acc[FM][FN];
-    // (A's rows of fragments take turns with FM + 1 sets of registers, so that the last of a stage is read a row before its end.)
-    u32x4 fa[FM + 1], fb[2][FN];
-    static_assert(FM >= FN, "every row of fragments reads one of B, until it has them all");
-    auto first_half = [&](const lds_char *tile) {   // multiplies it, reads the second half of the stage at `tile`
+    constexpr int kEarly = 2;
+    u32x4 fa[FM + kEarly], fb[2][FN];
+    static_assert(FM >= FN && FN >= 4, "every row of fragments reads one of B, until it has them all");
+    auto second_of = [](int m) { return m < kEarly ? FM + m : m - kEarly; };   // registers of row m of the second half
+    auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
+    // Does its share of the pieces before product (m, n) of a half, where nothing is read or loaded.
+    auto pieces = [&](int m, int n, int count, auto &&piece) {
+        constexpr int kPer = FN == 8 ? 3 : 1;              // places of a row
+        constexpr int kPlaces = FM == 4 ? 4 : kPer * 4;
+        if (FN == 8 ? n != 1 && n != 3 && n != 6 : n != 1) return;
+        const int place = m * kPer + n / 3;
+#pragma unroll
+        for (int i = 0; i < kPiecesB; ++i) {
+            if (i * kPlaces / kPiecesB == place && i < count) piece(i);
+        }
+    };
+    // multiplies the first half of a stage, reads its second half, loads A into slot `to`
+    auto first_half = [&](const lds_char *pa, const lds_char *pb, uint32_t to) {
 #pragma unroll
         for (int m = 0; m < FM; ++m) {
-            fa[m == 0 ? FM : m - 1] = ra(tile, wm * FM + m, 1);
-            if (m < FN) fb[1][m] = rb(tile + BM * kBK * 2, b_frag(m), 1);
 #pragma unroll
-            for (int n = 0; n < FN; ++n) acc[m][n] = Mma<DT>::run(fb[0][n], fa[m], acc[m][n]);
+            for (int n = 0; n < FN; ++n) {
+                if (m == 0 && n < kEarly) fa[second_of(n)] = ra(pa, wm * FM + n, 1);
+                if (m > 0 && n == 0 && m + kEarly - 1 < FM) fa[second_of(m + kEarly - 1)] = ra(pa, wm * FM + m + kEarly - 1, 1);
+                if (n * 2 == FN && m * 2 < FN) fb[1][m * 2] = rb(pb, b_frag(m * 2), 1);
+                if (n * 2 == FN + 2 && m * 2 + 1 < FN) fb[1][m * 2 + 1] = rb(pb, b_frag(m * 2 + 1), 1);
+                if (n == FN - 1) issue_a(m, to);
+                pieces(m, n, kPiecesB, next_b);
+                Mma<DT>::add(acc[m][n], fb[0][n], fa[m]);
+                fence();
+            }
         }
-        spread<FM, FN, kReads>();
     };
-    auto second_half = [&](const lds_char *tile) {   // multiplies it, reads the first half of the stage at `tile`
+    // multiplies the second half, reads the first half of the next stage, loads B into slot `to`
+    auto second_half = [&](const lds_char *pa, const lds_char *pb, uint32_t to) {
 #pragma unroll
         for (int m = 0; m < FM; ++m) {
-            // (row m of the second half has the registers of row m - 1 of the first)
-            const int free = m == 0 ? FM - 1 : m - 2;
-            if (free >= 0) fa[free] = ra(tile, wm * FM + free, 0);
-            if (m < FN) fb[0][m] = rb(tile + BM * kBK * 2, b_frag(m), 0);
 #pragma unroll
-            for (int n = 0; n < FN; ++n) acc[m][n] = Mma<DT>::run(fb[1][n], fa[m == 0 ? FM : m - 1], acc[m][n]);
+            for (int n = 0; n < FN; ++n) {
+                if (n == 0 && m < kEarly) fa[FM - kEarly + m] = ra(pa, wm * FM + FM - kEarly + m, 0);
+                if (n == 0 && m > kEarly) fa[m - 1 - kEarly] = ra(pa, wm * FM + m - 1 - kEarly, 0);
+                if (n * 2 == FN && m < FN) fb[0][m] = rb(pb, b_frag(m), 0);
+                if (n == FN - 1) issue_b(m, to);
+                pieces(m, n, kPiecesA, next_a);
+                Mma<DT>::add(acc[m][n], fb[1][n], fa[second_of(m)]);
+                fence();
+            }
         }
-        fa[FM - 2] = ra(tile, wm * FM + FM - 2, 0);
-        spread<FM, FN, kReads>();
+        fa[FM - 1 - kEarly] = ra(pa, wm * FM + FM - 1 - kEarly, 0);
     };
-    // The stores of a tile's results, which are younger than the loads of the next one's first stages.
-    constexpr int kStores = KIND == kFfnGateUp ? FM * (FN == 4 ? 1 : FN / 2) : KIND == kFfnGradHidden ? 3 * FM * FN / 2 : FM * FN / 2;
-    constexpr int kSavedStores = KIND == kFfnGateUp ? FM * FN : 0;
-
-    bool joined = false;   // the stages that lie in LDS already are this tile's
-    uint32_t slot = 0;
+    int total = steps;
+    uint32_t at_a = 0, at_b = 0;
+#pragma unroll 1
+    for (uint32_t slot = 0; slot < kStages; ++slot) {   // (a loop: this runs once, and takes as long as its instructions take to come)
+        for (int i = 0; i < kPiecesA; ++i) next_a(i);
+        for (int i = 0; i < kPiecesOfB; ++i) next_b(i);
+        asm volatile("s_nop 4" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < kLoadsA; ++i) issue_a(i, slot);
+#pragma unroll
+        for (int i = 0; i < kLoadsB; ++i) issue_b(i, slot);
+        for (int i = kPiecesOfB; i < kPiecesB; ++i) next_b(i);
+    }
+    bool landed = false;   // the tile's first stage, with the others
     for (;;) {
-        const uint32_t total = (joined ? stages_of(then) : steps);
         Tile after = t;
         const bool last = !next(&after);
-        const Feed its = last ? then : feed_of<KIND, BN>(a, after, wave);
-        then = its;
-        more = !last;
-        if (steps == 0) follow();
-        if (!joined) {
-            slot = 0;
-#pragma unroll
-            for (uint32_t k = 0; k < kStages; ++k) stage(k);
-            meet<kLoads *(kStages - 1)>();
+        if (!last) then = feed_of<KIND, BN>(a, after, wave);
+        more = scalar(last ? 0 : 1);
+        if (steps <= 0 && more != 0) {   // this tile's stages are all on their way already
+            more = 0;
+            from = then;
+            left = from.k;
+            steps = stages_of(from);
+            pair = 0;
         }
+        if (!landed) meet<kLoads *(kStages - 1)>();
+        landed = true;
         {   // (read here, not by the last turn of the tile before: writing results needs the registers)
-            const lds_char *tile = place(slot);
 #pragma unroll
-            for (int m = 0; m < FM; ++m) fa[m] = ra(tile, wm * FM + m, 0);
+            for (int m = 0; m < FM; ++m) fa[m] = ra(place_a(at_a), wm * FM + m, 0);
 #pragma unroll
-            for (int n = 0; n < FN; ++n) fb[0][n] = rb(tile + BM * kBK * 2, b_frag(n), 0);
+            for (int n = 0; n < FN; ++n) fb[0][n] = rb(place_b(at_b), b_frag(n), 0);
         }
 #pragma unroll
         for (int m = 0; m < FM; ++m) {
 #pragma unroll
             for (int n = 0; n < FN; ++n) acc[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        for (uint32_t step = 0; step < total; ++step) {
-            first_half(place(slot));
-            if (step == 0 && joined) {
-                if (kSavedStores != 0 && a.saved != nullptr) {
-                    meet<kLoads *(kStages - 2) + kStores + kSavedStores>();
-                } else {
-                    meet<kLoads *(kStages - 2) + kStores>();
-                }
-            } else {
-                meet<kLoads *(kStages - 2)>();
-            }
-            stage(slot);
-            slot = slot + 1 == kStages ? 0 : slot + 1;
-            second_half(place(slot));
+        for (int i = 0; i < kPiecesA; ++i) next_a(i);
+        settle<FM, FN>(acc);
+        for (int step = 0; step < total; ++step) {
+            first_half(place_a(at_a), place_b(at_b), at_a == 0 ? kStages : at_a - 1);
+            meet<kLoads *(kStages - 2) + kLoadsA>();   // the next stage has landed; of a new tile's first, the results before it have left, too
+            const uint32_t to = at_b;
+            at_a = after_a(at_a);
+            at_b = after_b(at_b);
+            second_half(place_a(at_a), place_b(at_b), to);
         }
+        settle<FM, FN>(acc);
         results<DT, KIND, FM, FN>(a, t, acc, wm, wn, lane);
         if (last) break;
         t = after;
-        joined = true;
+        total = stages_of(then);
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // nothing may be on its way to LDS when it is given back
 }
@@ -713,21 +827,17 @@ __device__ __forceinline__ void products(const FfnArgs &a, Tile t, char *s_tile,
 // One workgroup per CU.  It takes its share of the whole tiles, one of every round, and then of the parts.  SMALL: of tiles of 128 x
 // 128 alone, for ranks of fewer rows than a whole tile has; then four stages are on their way instead of two.
 template <int DT, int KIND, bool SMALL>
-__global__ void __launch_bounds__(kWaves * 64, 2)
+__global__ void __launch_bounds__(kWaves * 64, 1)
 k_ffn(FfnArgs a)
 {
+    static_assert(!SMALL || KIND != kFfnGradWeights, "whose tiles are full however few the rows");
     constexpr uint32_t kEdge = SMALL ? kTile / 2 : kTile;
     constexpr uint32_t kWide = SMALL ? kTileCols<KIND> / 2 : kTileCols<KIND>;
     __shared__ __attribute__((aligned(1024))) char s_tile[kLdsBytes];
-    struct Rank {
-        uint32_t rows;
-        uint32_t start;
-        uint32_t down;   // tiles
-        uint32_t upto;   // tiles of this rank and those before it
-    };
-    __shared__ Rank s_rank[kFfnRanks];   // (one wavefront's registers would hold it, had the products any to spare)
-    static_assert(sizeof(s_rank) <= kTableBytes, "beside the stages");
     const FfnRows &s = a.rows;
+    // (read together; otherwise the way to the first load is a row of waits for one argument each)
+    asm volatile("" ::"s"(s.counts), "s"(s.per_rank), "s"(s.unit), "s"(s.n), "s"(s.capacity), "s"(s.most), "s"(s.dim), "s"(s.hidden), "s"(a.h),
+                 "s"(a.dproj), "s"(a.saved), "s"(a.x16), "s"(a.act));
     auto count = [](uint32_t size, uint32_t edge) { return (size + edge - 1) / edge; };
     // kFfnGradWeights: all ranks' tiles of the projections' gradients, then those of w_down's
     const uint32_t across = count(KIND == kFfnGradWeights ? s.dim : columns<KIND>(s), KIND == kFfnGradWeights ? kEdge : kWide);
@@ -736,12 +846,9 @@ k_ffn(FfnArgs a)
     const uint32_t tiles1 = count(s.dim, kEdge) * across1;
     const uint32_t both0 = scalar(s.n) * tiles0;   // of all ranks (read by a part of the workgroup too, which makes it a vector)
     const uint32_t both1 = scalar(s.n) * tiles1;
-    if (threadIdx.x < 64) {
-        const RankRows mine(s);
-        const uint32_t down = count(mine.rows, kEdge);
-        s_rank[threadIdx.x] = {mine.rows, mine.start, down, inclusive_sum(down * across)};
-    }
-    __syncthreads();
+    const RankRows mine(s);   // (of the lane's rank)
+    const uint32_t mine_down = count(mine.rows, kEdge);
+    const uint32_t mine_upto = inclusive_sum(mine_down * across);   // tiles of this rank and those before it
     auto tile = [&](uint32_t at, Tile *t) {
         t->weight = 0;
         if constexpr (KIND == kFfnGradWeights) {
@@ -752,16 +859,16 @@ k_ffn(FfnArgs a)
             t->weight = down ? 2 : t->m0 >= across1 ? 1 : 0;
             t->m0 -= t->weight == 1 ? across1 : 0;
         } else {
-            t->rank = __builtin_ctzll(__ballot(s_rank[threadIdx.x & 63].upto > at));
-            const uint32_t down = uniform(s_rank[t->rank].down);
-            in_groups(at - (uniform(s_rank[t->rank].upto) - down * across), down, across, &t->m0, &t->n0);
+            t->rank = __builtin_ctzll(__ballot(mine_upto > at));
+            const uint32_t down = of_lane(mine_down, t->rank);
+            in_groups(at - (of_lane(mine_upto, t->rank) - down * across), down, across, &t->m0, &t->n0);
         }
-        t->rows = scalar(s_rank[t->rank].rows);
-        t->start = scalar(s_rank[t->rank].start);
+        t->rows = of_lane(mine.rows, t->rank);
+        t->start = of_lane(mine.start, t->rank);
         t->m0 *= kEdge;
         t->n0 *= kWide;
     };
-    const uint32_t tiles = KIND == kFfnGradWeights ? both0 + both1 : uniform(s_rank[kFfnRanks - 1].upto);
+    const uint32_t tiles = KIND == kFfnGradWeights ? both0 + both1 : of_lane(mine_upto, kFfnRanks - 1);
     const uint32_t turned = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
     uint32_t at = turned;
     uint32_t end = tiles;
@@ -773,13 +880,9 @@ k_ffn(FfnArgs a)
     };
     Tile t;
     if constexpr (SMALL) {
-        for (uint32_t group = 0; group < (KIND == kFfnGradWeights ? 2 : 1); ++group) {
-            end = group == 0 && KIND == kFfnGradWeights ? both0 : tiles;
-            if (at >= end) continue;
-            __syncthreads();
-            tile(at, &t);
-            products<DT, KIND, 4, 2>(a, t, s_tile, next);
-        }
+        if (at >= end) return;
+        tile(at, &t);
+        products<DT, KIND, 4, 4>(a, t, s_tile, next);
     } else {
         const Share share(tiles, gridDim.x);
         for (uint32_t group = 0; group < (KIND == kFfnGradWeights ? 2 : 1); ++group) {
@@ -787,7 +890,7 @@ k_ffn(FfnArgs a)
             if (at >= end) continue;
             __syncthreads();   // everybody is done with the LDS of the tiles before
             tile(at, &t);
-            products<DT, KIND, 8, 4>(a, t, s_tile, next);
+            products<DT, KIND, 8, 8>(a, t, s_tile, next);
         }
         if (turned >= share.left * share.parts) return;
         const uint32_t part = scalar(turned % share.parts);
@@ -803,9 +906,9 @@ k_ffn(FfnArgs a)
         __syncthreads();   // everybody is done with the last whole tile's LDS
         auto none = [](Tile *) { return false; };
         if (share.parts == 2) {
-            products<DT, KIND, 8, 2>(a, t, s_tile, none);
+            products<DT, KIND, 8, 4>(a, t, s_tile, none);
         } else {
-            products<DT, KIND, 4, 2>(a, t, s_tile, none);
+            products<DT, KIND, 4, 4>(a, t, s_tile, none);
         }
     }
 }
@@ -837,11 +940,13 @@ hipError_t run(const FfnArgs &a, bool small, uint32_t num_cus, hipStream_t st)
 {
     if (a.rows.most == 0 && KIND != kFfnGradWeights) return hipSuccess;
     const uint32_t groups = num_cus < 32 ? 32 : num_cus / 32 * 32;   // a multiple of eight, and its half and quarter too
-    if (small) {
-        HCCLX_LAUNCH((k_ffn<DT, KIND, true>), dim3(groups), dim3(kWaves * 64), 0, st, a);
-    } else {
-        HCCLX_LAUNCH((k_ffn<DT, KIND, false>), dim3(groups), dim3(kWaves * 64), 0, st, a);
+    if constexpr (KIND != kFfnGradWeights) {
+        if (small) {
+            HCCLX_LAUNCH((k_ffn<DT, KIND, true>), dim3(groups), dim3(kWaves * 64), 0, st, a);
+            return hipGetLastError();
+        }
     }
+    HCCLX_LAUNCH((k_ffn<DT, KIND, false>), dim3(groups), dim3(kWaves * 64), 0, st, a);
     return hipGetLastError();
 }
 

@@ -11,8 +11,8 @@ namespace ffn {
 // Products with few rows read the weights; what counts is how many bytes are on their way.  Tiles of 128 x 128 keep 48 KiB of
 // weights per CU on their way and read the rows' operand once per tile, but have to be as many as the CUs; the thin kernel
 // has eight wavefronts per 16 columns and reads the rows' operand that often.  Weights of dim x 2048, both products, thin : tiles,
-// us: 8 ranks x 7168 (256 tiles of the first product), 1 row 138 : 132, 16 rows 182 : 134; 4 ranks x 7168 (128), 1 row
-// 75 : 89, 8 rows 84 : 90, 16 rows 96 : 91; 2 ranks x 4096 (64), 1 row 26 : 59, 64 rows 55 : 61; 1 rank (32), 64 rows 39 : 56.
+// us: 8 ranks x 7168 (256 tiles of the first product), 1 row 138 : 142, 16 rows 175 : 140; 4 ranks x 7168 (128), 1 row 76 : 97,
+// 8 rows 83 : 93, 16 rows 93 : 94; 2 ranks x 4096 (64), 1 row 26 : 63, 64 rows 55 : 63; 1 rank (32), 64 rows 39 : 59.
 template <int KIND>
 bool thin(const FfnRows &s, uint32_t cus)
 {
@@ -21,7 +21,8 @@ bool thin(const FfnRows &s, uint32_t cus)
     return (rows <= 64 && tiles <= cus / 4) || (rows <= 8 && tiles < cus);
 }
 
-// Rows of a rank up to which tiles of 128 x 128 are taken: a whole tile would be half empty.
+// Rows of a rank up to which tiles of 128 x 128 are taken: a whole tile would be half empty.  8 ranks x 4096 x 2048, small : whole
+// tiles, us: 64 rows, forward 99 : 121, gradients of the rows 134 : 144; 128 rows 115 : 125, 140 : 152; 160 rows, forward 146 : 124.
 constexpr uint32_t kSmallRows = 128;
 
 template <int DT, int KIND>

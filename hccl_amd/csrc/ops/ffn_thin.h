@@ -142,7 +142,7 @@ k_ffn_thin(FfnArgs a)
             }
             f32x4 h;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) h[e] = Act(sum[0][e], a.act).value * sum[kWeights - 1][e];
+            for (int e = 0; e < 4; ++e) h[e] = Act(sum[0][e], ActTerms(a.act)).value * sum[kWeights - 1][e];
             *reinterpret_cast<uint2 *>(a.h + (packed * hidden + col) * 2) = narrow4<DT>(h);
         } else {
             char *c = const_cast<char *>(a.p[1][rank]);
