@@ -11,8 +11,8 @@ namespace ffn {
 // Products with few rows read the weights; what counts is how many bytes are on their way.  Tiles of 128 x 128 keep 48 KiB of
 // weights per CU on their way and read the rows' operand once per tile, but have to be as many as the CUs; the thin kernel
 // has eight wavefronts per 16 columns and reads the rows' operand that often.  Weights of dim x 2048, both products, thin : tiles,
-// us: 8 ranks x 7168 (256 tiles of the first product), 1 row 138 : 142, 16 rows 175 : 140; 4 ranks x 7168 (128), 1 row 76 : 97,
-// 8 rows 83 : 93, 16 rows 93 : 94; 2 ranks x 4096 (64), 1 row 26 : 63, 64 rows 55 : 63; 1 rank (32), 64 rows 39 : 59.
+// us: 8 ranks x 7168 (256 tiles of the first product), 1 row 136 : 142, 16 rows 174 : 139; 4 ranks x 7168 (128), 1 row 75 : 95,
+// 8 rows 82 : 93, 16 rows 92 : 94; 2 ranks x 4096 (64), 1 row 25 : 63, 64 rows 54 : 64; 1 rank (32), 64 rows 38 : 60.
 template <int KIND>
 bool thin(const FfnRows &s, uint32_t cus)
 {
@@ -20,6 +20,10 @@ bool thin(const FfnRows &s, uint32_t cus)
     const uint64_t rows = (s.most + s.n - 1) / s.n;
     return (rows <= 64 && tiles <= cus / 4) || (rows <= 8 && tiles < cus);
 }
+
+// Workgroups of eight columns instead of sixteen, while no CU gets two of them.  The block, 1 row, halves : sixteens, us: 1 rank
+// 4096 x 512 14.5 : 15.6, 4096 x 2048 (128 workgroups of sixteen) 16.2 : 17.3, 16 rows 18.9 : 20.3; 2 ranks (256) 31 : 25.
+inline bool halves(const FfnRows &s, uint32_t cus) { return static_cast<uint64_t>(s.n) * ((s.hidden + 15) / 16) <= cus / 2; }
 
 // Rows of a rank up to which tiles of 128 x 128 are taken: a whole tile would be half empty.  8 ranks x 4096 x 2048, small : whole
 // tiles, us: 64 rows, forward 99 : 121, gradients of the rows 134 : 144; 128 rows 115 : 125, 140 : 152; 160 rows, forward 146 : 124.
@@ -33,11 +37,15 @@ hipError_t launch(const FfnArgs &a, uint32_t cus, hipStream_t st)
         if (s.most != 0 && thin<KIND>(s, cus)) {
             const uint64_t rows = (s.most + s.n - 1) / s.n;
             if (rows <= 16) {
-                launch_thin<DT, KIND, 1>(a, st);
+                if (KIND == kFfnGateUp && halves(s, cus)) {
+                    launch_thin<DT, KIND, 1, KIND == kFfnGateUp>(a, st);
+                } else {
+                    launch_thin<DT, KIND, 1, false>(a, st);
+                }
             } else if (rows <= 32) {
-                launch_thin<DT, KIND, 2>(a, st);
+                launch_thin<DT, KIND, 2, false>(a, st);
             } else {
-                launch_thin<DT, KIND, 4>(a, st);
+                launch_thin<DT, KIND, 4, false>(a, st);
             }
             return hipGetLastError();
         }
