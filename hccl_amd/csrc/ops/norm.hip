@@ -36,7 +36,8 @@ struct OutPtrs {
     char *p[kMostRanks];
 };
 
-// A thread holds at most so many vectors of 16 bytes of a row.
+// A thread holds at most so many vectors of 16 bytes of a row.  (Two: 8 ranks x 4096 x 7168 to 8 bits 351 us instead of 305, in one
+// run; 8 x 2048 x 4096 91 instead of 93, 8 x 64 x 7168 the same.)
 constexpr uint32_t kMostVectors = 4;
 template <int DT> constexpr int kMostThreads = HCCLX_NORM_MAX_ROW / (Vec16<DT>::NE * kMostVectors);
 static_assert(kMostThreads<HCCL_DATA_TYPE_FP32> <= 1024, "a workgroup holds the longest row");
