@@ -39,6 +39,7 @@ struct OutPtrs {
 // A thread holds at most so many vectors of 16 bytes of a row.  (Two: 8 ranks x 4096 x 7168 to 8 bits 351 us instead of 305, in one
 // run; 8 x 2048 x 4096 91 instead of 93, 8 x 64 x 7168 the same.)
 constexpr uint32_t kMostVectors = 4;
+constexpr uint32_t kGroup = 256;   // threads of a workgroup that holds several rows, at most
 template <int DT> constexpr int kMostThreads = HCCLX_NORM_MAX_ROW / (Vec16<DT>::NE * kMostVectors);
 static_assert(kMostThreads<HCCL_DATA_TYPE_FP32> <= 1024, "a workgroup holds the longest row");
 
@@ -186,7 +187,7 @@ k_rms_norm(NormPtrs ptrs, uint32_t rows, uint32_t elems, float eps)
 }
 
 // Slot s of a rank (threadIdx.y of a workgroup) takes the rows s, s + slots, ...; it adds up its part of dweight in registers
-// and writes it to partial[rank][slot][elems].  AHEAD: a row is read while the one before it is computed (dtotal, which is wanted
+// and the workgroup writes the sum of its slots' to partial[rank][workgroup][elems].  AHEAD: a row is read while the one before it is computed (dtotal, which is wanted
 // last, when its turn begins: ahead too it has no registers).  With x = total and r = 1 / sqrt(mean x^2 + eps):
 // dx = r (dy w - x r^2 mean(x dy w)) + dtotal,  dw = sum over the rows of dy x r.
 // Bound: how many rows are on their way, four workgroups of 256 threads per CU at 128 registers.  bf16, 8 ranks x 2048 x 4096 110 us
@@ -198,6 +199,7 @@ k_rms_norm_grad(GradPtrs ptrs, uint32_t rows, uint32_t elems, float eps, float *
     using V = Vec16<DT>;
     constexpr int NE = V::NE;
     __shared__ float s_part[2][16][2];   // of the rows in turn
+    __shared__ float s_join[NE][kGroup];
     const uint32_t rank = blockIdx.y;
     const uint32_t slots = gridDim.x * blockDim.y;
     const char *dtotal = ptrs.dtotal[rank];
@@ -275,7 +277,22 @@ k_rms_norm_grad(GradPtrs ptrs, uint32_t rows, uint32_t elems, float eps, float *
         if (!AHEAD && first + slots < rows) read(row + slots);
     }
     if (partial == nullptr) return;
-    float *mine = partial + (static_cast<size_t>(rank) * slots + blockIdx.x * blockDim.y + threadIdx.y) * elems;
+    if (blockDim.y > 1) {   // the workgroup's slots first, in their order
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < NE; ++e) s_join[e][threadIdx.y * blockDim.x + threadIdx.x] = acc[i][e];
+            __syncthreads();
+            if (threadIdx.y != 0) continue;
+            for (uint32_t y = 1; y < blockDim.y; ++y) {
+#pragma unroll
+                for (int e = 0; e < NE; ++e) acc[i][e] += s_join[e][y * blockDim.x + threadIdx.x];
+            }
+        }
+        if (threadIdx.y != 0) return;
+    }
+    float *mine = partial + (static_cast<size_t>(rank) * gridDim.x + blockIdx.x) * elems;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const uint32_t at = (threadIdx.x + i * blockDim.x) * NE;
@@ -286,10 +303,10 @@ k_rms_norm_grad(GradPtrs ptrs, uint32_t rows, uint32_t elems, float eps, float *
     }
 }
 
-// dweight = the slots' parts, added in their order: 64 columns per workgroup, every 16th slot per row of threads, then the rows.
+// dweight = the workgroups' parts, added in their order: 64 columns per workgroup, every 16th part per row of threads, then the rows.
 template <int DT>
 __global__ void __launch_bounds__(1024)
-k_rms_norm_join(OutPtrs dweight, uint32_t slots, uint32_t elems, const float *partial)
+k_rms_norm_join(OutPtrs dweight, uint32_t parts, uint32_t elems, const float *partial)
 {
     using D = DTypeOf<DT>;
     __shared__ float s_sum[16][64];
@@ -297,9 +314,9 @@ k_rms_norm_join(OutPtrs dweight, uint32_t slots, uint32_t elems, const float *pa
     const uint32_t col = blockIdx.x * 64 + threadIdx.x;
     float sum = 0.0f;
     if (col < elems) {
-        const float *p = partial + static_cast<size_t>(rank) * slots * elems + col;
+        const float *p = partial + static_cast<size_t>(rank) * parts * elems + col;
 #pragma unroll 8
-        for (uint32_t s = threadIdx.y; s < slots; s += 16) sum += p[static_cast<size_t>(s) * elems];
+        for (uint32_t s = threadIdx.y; s < parts; s += 16) sum += p[static_cast<size_t>(s) * elems];
     }
     s_sum[threadIdx.y][threadIdx.x] = sum;
     __syncthreads();
@@ -309,7 +326,8 @@ k_rms_norm_join(OutPtrs dweight, uint32_t slots, uint32_t elems, const float *pa
 }
 
 // Threads per row and vectors per thread: a row is held by as few wavefronts as leave a thread at most so many vectors of it (1024
-// threads: more); workgroups of short rows hold several.  The norm takes four; its gradient, which holds three rows, the next
+// threads: more), one, two or a multiple of four of them, one for every SIMD (five: gradient of 8 x 1024 x 4097 bf16 137 us, eight
+// 108); workgroups of short rows hold several.  The norm takes four; its gradient, which holds three rows, the next
 // ones and a part of dweight, two.
 struct RowShape {
     uint32_t threads;
@@ -320,8 +338,8 @@ RowShape shape_of(uint32_t elems, int ne, uint32_t most_vectors)
 {
     const uint32_t vecs = (elems + ne - 1) / ne;
     uint32_t threads = 64;
-    while (threads < 1024 && threads * most_vectors < vecs) threads *= 2;
-    return {threads, std::max(1u, 256u / threads), (vecs + threads - 1) / threads};
+    while (threads < 1024 && threads * most_vectors < vecs) threads += std::min(threads, kGroup);
+    return {threads, std::max(1u, kGroup / threads), (vecs + threads - 1) / threads};
 }
 
 template <int DT, bool QUANT>
@@ -384,16 +402,15 @@ struct NormGradWork : PlanWork {
     int dtype = 0;
     float eps = 0.0f;
     RowShape shape{};
-    DeviceBlock partial;   // float[n][slots][elems]
+    DeviceBlock partial;   // float[n][groups][elems]
 
     template <int DT>
     void run(hipStream_t st) const
     {
         float *part = reinterpret_cast<float *>(partial.p);
-        const uint32_t slots = groups * shape.per_group;
         if (rows != 0) launch_grad<DT>(shape, dim3(groups, n), st, ptrs, rows, elems, eps, part);
         if (want_dweight) {
-            HCCLX_LAUNCH((k_rms_norm_join<DT>), dim3((elems + 63) / 64, n), dim3(64, 16), 0, st, dweight, rows != 0 ? slots : 0u, elems, part);
+            HCCLX_LAUNCH((k_rms_norm_join<DT>), dim3((elems + 63) / 64, n), dim3(64, 16), 0, st, dweight, rows != 0 ? groups : 0u, elems, part);
         }
     }
 
@@ -488,11 +505,13 @@ int make_norm_grad(const hcclx_rms_norm_grad_t &a, hcclx_plan_t **plan)
     w->eps = a.eps;
     w->shape = shape_of(a.row_elems, 16 / static_cast<int>(size), 2);
     const uint32_t most = (a.rows + w->shape.per_group - 1) / w->shape.per_group;
-    // a slot takes two rows at least, while there are workgroups for every CU: each slot's part of dweight is as long as a row of floats
-    w->groups = std::min(std::max((most + 1) / 2, std::min(most, ctx->num_cus / a.n)), std::max(1u, 4u * ctx->num_cus / a.n));
+    // A workgroup takes four rows at least, while there are workgroups for every CU: its part of dweight is as long as a row of floats
+    // (8 ranks x 256 x 4096 bf16, two rows 32 us, four 25; 3 x 777 x 1001 fp32, two at a time, four 15.7, eight 20.7).  Four workgroups
+    // per CU: of 256 threads a CU holds as many; of longer rows' the others follow (8 x 1024 x 8192 118 us, as many as it holds 131).
+    w->groups = std::min(std::max((a.rows + 3) / 4, std::min(most, ctx->num_cus / a.n)), std::max(1u, 4u * ctx->num_cus / a.n));
     uint64_t held = 0;
     if (w->want_dweight && a.rows != 0) {
-        held = static_cast<uint64_t>(a.n) * w->groups * w->shape.per_group * a.row_elems * sizeof(float);
+        held = static_cast<uint64_t>(a.n) * w->groups * a.row_elems * sizeof(float);
         if ((rc = w->partial.get(held)) != HCCL_SUCCESS) return rc;
     }
     const uint64_t elements = static_cast<uint64_t>(a.n) * a.rows * a.row_elems;
