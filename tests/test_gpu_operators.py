@@ -67,6 +67,10 @@ NORM_SIZES = [(1, 1, 1), (2, 3, 7), (1, 5, 8), (3, 2, 100), (2, 4, 511), (1, 9, 
 @pytest.mark.parametrize("n,rows,elems", NORM_SIZES)
 @pytest.mark.parametrize("skew", [0, 1])
 def test_norm_and_its_gradient(n, rows, elems, dtype, skew):
+    check_norm(n, rows, elems, dtype, skew)
+
+
+def check_norm(n, rows, elems, dtype, skew):
     g, td, eps = gen(n * 7 + elems), TD[dtype], 1e-6
     x = [normal((rows, elems), td, g) for _ in range(n)]
     res = [normal((rows, elems), td, g, 3.0) for _ in range(n)]
@@ -118,6 +122,13 @@ def test_norm_gradient_of_many_rows_per_workgroup(rows):
     hcclx.RmsNormGradPlan(ptrs(dy), ptrs(t), ptrs(w), ptrs(dy), None, rows, elems, T.BFP16, eps=1e-5).launch()   # dx on top of dy
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(dx, dy))
+
+
+@pytest.mark.parametrize("dtype", [T.FP32, T.BFP16])
+@pytest.mark.parametrize("n,rows,elems", [(64, 9, 40), (2, 37, 300), (1, 5, 6000), (3, 6, 8200), (1, 3, 12300), (2, 4, 16384)])
+def test_norm_gradient_of_every_workgroup_shape(n, rows, elems, dtype):
+    """One to four wavefronts per row, several rows per workgroup, eight, twelve and sixteen wavefronts."""
+    check_norm(n, rows, elems, dtype, 0)
 
 
 def test_norm_gradient_against_differences():
@@ -491,6 +502,14 @@ def test_ffn_at_the_edges_of_its_kernels(rows, capacity, dim, hidden, dtype):
     if capacity > max(rows):                                       # the same rows in plans made for capacity
         f.run(bound=0)
         f.check()
+
+
+@pytest.mark.parametrize("capacity", [4, 100, 300])
+def test_ffn_of_64_ranks(capacity):
+    """As many ranks as there are, some without rows, in plans for few rows, small tiles and whole ones."""
+    f = Ffn([k * 7 % 5 for k in range(64)], capacity, 72, 136, T.BFP16, capacity, per_rank=3)
+    f.run(bound=0)
+    f.check()
 
 
 def test_ffn_of_rows_from_many_senders():
