@@ -2,11 +2,11 @@
 //
 // A workgroup takes 16 columns of C (of both weights) of one rank and all its rows, 16 x MB at a time; its eight wavefronts share
 // out k in turns of 64 and add up their parts in LDS, in the order of the wavefronts.  Weights go from memory to the matrix
-// instruction's registers without LDS: nobody else needs them.  A lane's two chunks of 16 bytes of a turn lie next to each other (k = 16 (lane / 16) .. + 15), so that
-// four lanes read a cache line of a row; the same k of the rows of x, which come from the L2.
+// instruction's registers without LDS: nobody else needs them.  A lane's two chunks of 16 bytes of a turn lie next to each other
+// (k = 16 (lane / 16) .. + 15), so that four lanes read a cache line of a row; the same k of the rows of x, which come from the L2.
 //
-// What bounds it: the weights' way from memory, with too little time to reach its rate: 1 row x 4096 x 2048 10.9 and 5.5 us (3.1 TB/s), 2 ranks
-// 25 (4.0), 8 ranks x 7168 x 2048 136 (5.2).
+// What bounds it: the weights' way from memory, with too little time to reach its rate: 1 row x 4096 x 2048 10.9 and 5.5 us
+// (3.1 TB/s), 2 ranks 25 (4.0), 8 ranks x 7168 x 2048 136 (5.2).
 //
 // Limits as in ffn_gemm.h: range-checked loads give zeros behind the last row, column and k.
 #pragma once
@@ -115,7 +115,9 @@ k_ffn_thin(FfnArgs a)
                 for (int h = 0; h < 2; ++h) {
                     const u32x4 f = X8 ? widen8<DT>(fx[from][m][0][2 * h], fx[from][m][0][2 * h + 1]) : fx[from][m][X8 ? 0 : h];
 #pragma unroll
-                    for (int w = 0; w < kWeights; ++w) acc[m][w] = Mma<DT>::run(HALF ? fw[from][w][h] | fu[from][h] : fw[from][w][h], f, acc[m][w]);
+                    for (int w = 0; w < kWeights; ++w) {
+                        acc[m][w] = Mma<DT>::run(HALF ? fw[from][w][h] | fu[from][h] : fw[from][w][h], f, acc[m][w]);
+                    }
                 }
             }
         };

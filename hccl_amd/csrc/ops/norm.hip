@@ -187,11 +187,12 @@ k_rms_norm(NormPtrs ptrs, uint32_t rows, uint32_t elems, float eps)
 }
 
 // Slot s of a rank (threadIdx.y of a workgroup) takes the rows s, s + slots, ...; it adds up its part of dweight in registers
-// and the workgroup writes the sum of its slots' to partial[rank][workgroup][elems].  AHEAD: a row is read while the one before it is computed (dtotal, which is wanted
-// last, when its turn begins: ahead too it has no registers).  With x = total and r = 1 / sqrt(mean x^2 + eps):
+// and the workgroup writes the sum of its slots' to partial[rank][workgroup][elems].  AHEAD: a row is read while the one before it is
+// computed (dtotal, which is wanted last, when its turn begins: ahead too it has no registers).  With x = total and
+// r = 1 / sqrt(mean x^2 + eps):
 // dx = r (dy w - x r^2 mean(x dy w)) + dtotal,  dw = sum over the rows of dy x r.
-// Bound: how many rows are on their way, four workgroups of 256 threads per CU at 128 registers.  bf16, 8 ranks x 2048 x 4096 110 us
-// (4.9 TB/s; two workgroups per CU 163, three 137; dtotal ahead 123).
+// Bound: how many rows are on their way, four workgroups of 256 threads per CU at 128 registers.  bf16, 8 ranks x 2048 x 4096 108 us
+// (5.0 TB/s; two workgroups per CU 163, three 137; dtotal ahead 123).
 template <int DT, int NV, bool AHEAD>
 __global__ void __launch_bounds__(AHEAD ? 1024 : kMostThreads<DT>)
 k_rms_norm_grad(GradPtrs ptrs, uint32_t rows, uint32_t elems, float eps, float *partial)
