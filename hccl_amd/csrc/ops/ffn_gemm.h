@@ -601,7 +601,7 @@ __device__ __forceinline__ void products(const FfnArgs &a, Tile t, char *s_tile,
     constexpr int kLoadsA = decltype(sa)::kLoads;
     constexpr int kLoadsB = decltype(sb)::kLoads;
     constexpr int kLoads = kLoadsA + kLoadsB;
-    static_assert(kStages >= 2 && kLoadsA <= FM && kLoadsB <= FM, "two stages fit; every row of fragments issues a load of each");
+    static_assert(kStages >= 2, "two stages fit");
 
     // The loads run ahead of the products: `from` is where they are, `then` what follows (if `more`), `left` k of this pair are to
     // come in `steps` stages.  A tile has kStages stages at least (of zeros, if need be): when its products begin, all of those
@@ -703,10 +703,10 @@ __device__ __forceinline__ void products(const FfnArgs &a, Tile t, char *s_tile,
     };
 
     auto issue_a = [&](int i, uint32_t slot) {
-        if (i < kLoadsA) sa.issue(i, ga.r, ga.end, ga.ld, static_cast<uint32_t>(reinterpret_cast<uintptr_t>(place_a(slot))), wave);
+        sa.issue(i, ga.r, ga.end, ga.ld, static_cast<uint32_t>(reinterpret_cast<uintptr_t>(place_a(slot))), wave);
     };
     auto issue_b = [&](int i, uint32_t slot) {
-        if (i < kLoadsB) sb.issue(i, gb.r, gb.end, gb.ld, static_cast<uint32_t>(reinterpret_cast<uintptr_t>(place_b(slot))), wave);
+        sb.issue(i, gb.r, gb.end, gb.ld, static_cast<uint32_t>(reinterpret_cast<uintptr_t>(place_b(slot))), wave);
     };
 
     const Reader<kAk, BM> ra(lane);
@@ -727,13 +727,13 @@ __device__ __forceinline__ void products(const FfnArgs &a, Tile t, char *s_tile,
     f32x4 acc[FM][FN];
     constexpr int kEarly = 2;
     u32x4 fa[FM + kEarly], fb[2][FN];
-    static_assert(FM >= FN && FN >= 4, "every row of fragments reads one of B, until it has them all");
+    static_assert(FM * 2 >= FN && FN >= 4, "every row of fragments reads two of B at most");
     auto second_of = [](int m) { return m < kEarly ? FM + m : m - kEarly; };   // registers of row m of the second half
     auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
     // Does its share of the pieces before product (m, n) of a half, where nothing is read or loaded.
     auto pieces = [&](int m, int n, int count, auto &&piece) {
         constexpr int kPer = FN == 8 ? 3 : 1;              // places of a row
-        constexpr int kPlaces = FM == 4 ? 4 : kPer * 4;
+        constexpr int kPlaces = kPer * 4;
         if (FN == 8 ? n != 1 && n != 3 && n != 6 : n != 1) return;
         const int place = m * kPer + n / 3;
 #pragma unroll
@@ -751,7 +751,10 @@ __device__ __forceinline__ void products(const FfnArgs &a, Tile t, char *s_tile,
                 if (m > 0 && n == 0 && m + kEarly - 1 < FM) fa[second_of(m + kEarly - 1)] = ra(pa, wm * FM + m + kEarly - 1, 1);
                 if (n * 2 == FN && m * 2 < FN) fb[1][m * 2] = rb(pb, b_frag(m * 2), 1);
                 if (n * 2 == FN + 2 && m * 2 + 1 < FN) fb[1][m * 2 + 1] = rb(pb, b_frag(m * 2 + 1), 1);
-                if (n == FN - 1) issue_a(m, to);
+                if (n == FN - 1) {
+#pragma unroll
+                    for (int i = m; i < kLoadsA; i += FM) issue_a(i, to);
+                }
                 pieces(m, n, kPiecesB, next_b);
                 Mma<DT>::add(acc[m][n], fb[0][n], fa[m]);
                 fence();
@@ -766,8 +769,14 @@ __device__ __forceinline__ void products(const FfnArgs &a, Tile t, char *s_tile,
             for (int n = 0; n < FN; ++n) {
                 if (n == 0 && m < kEarly) fa[FM - kEarly + m] = ra(pa, wm * FM + FM - kEarly + m, 0);
                 if (n == 0 && m > kEarly) fa[m - 1 - kEarly] = ra(pa, wm * FM + m - 1 - kEarly, 0);
-                if (n * 2 == FN && m < FN) fb[0][m] = rb(pb, b_frag(m), 0);
-                if (n == FN - 1) issue_b(m, to);
+                if (n * 2 == FN) {
+#pragma unroll
+                    for (int i = m; i < FN; i += FM) fb[0][i] = rb(pb, b_frag(i), 0);
+                }
+                if (n == FN - 1) {
+#pragma unroll
+                    for (int i = m; i < kLoadsB; i += FM) issue_b(i, to);
+                }
                 pieces(m, n, kPiecesA, next_a);
                 Mma<DT>::add(acc[m][n], fb[1][n], fa[second_of(m)]);
                 fence();
@@ -833,15 +842,18 @@ __device__ __forceinline__ void products(const FfnArgs &a, Tile t, char *s_tile,
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // nothing may be on its way to LDS when it is given back
 }
 
-// One workgroup per CU.  It takes its share of the whole tiles, one of every round, and then of the parts.  SMALL: of tiles of 128 x
-// 128 alone, for ranks of fewer rows than a whole tile has; then four stages are on their way instead of two.
-template <int DT, int KIND, bool SMALL>
+// How C is cut: into whole tiles and their parts; or, for ranks of fewer rows than a whole tile has, into tiles of 128 x 128 (four
+// stages on their way instead of two) or of 128 x 256 (three).
+enum Cut { kCutWhole, kCutSmall, kCutWide };
+
+// One workgroup per CU.  It takes its share of the tiles, one of every round, and then of the parts.
+template <int DT, int KIND, Cut CUT>
 __global__ void __launch_bounds__(kWaves * 64, 1)
 k_ffn(FfnArgs a)
 {
-    static_assert(!SMALL || KIND != kFfnGradWeights, "whose tiles are full however few the rows");
-    constexpr uint32_t kEdge = SMALL ? kTile / 2 : kTile;
-    constexpr uint32_t kWide = SMALL ? kTileCols<KIND> / 2 : kTileCols<KIND>;
+    static_assert(CUT == kCutWhole || KIND != kFfnGradWeights, "whose tiles are full however few the rows");
+    constexpr uint32_t kEdge = CUT == kCutWhole ? kTile : kTile / 2;
+    constexpr uint32_t kWide = CUT == kCutSmall ? kTileCols<KIND> / 2 : kTileCols<KIND>;
     __shared__ __attribute__((aligned(1024))) char s_tile[kLdsBytes];
     const FfnRows &s = a.rows;
     // (read together; otherwise the way to the first load is a row of waits for one argument each)
@@ -888,10 +900,10 @@ k_ffn(FfnArgs a)
         return true;
     };
     Tile t;
-    if constexpr (SMALL) {
+    if constexpr (CUT != kCutWhole) {
         if (at >= end) return;
         tile(at, &t);
-        products<DT, KIND, 4, 4>(a, t, s_tile, next);
+        products<DT, KIND, 4, CUT == kCutWide ? 8 : 4>(a, t, s_tile, next);
     } else {
         const Share share(tiles, gridDim.x);
         for (uint32_t group = 0; group < (KIND == kFfnGradWeights ? 2 : 1); ++group) {
@@ -945,17 +957,20 @@ k_ffn_widen(FfnArgs a)
 }
 
 template <int DT, int KIND>
-hipError_t run(const FfnArgs &a, bool small, uint32_t num_cus, hipStream_t st)
+hipError_t run(const FfnArgs &a, Cut cut, uint32_t num_cus, hipStream_t st)
 {
     if (a.rows.most == 0 && KIND != kFfnGradWeights) return hipSuccess;
-    const uint32_t groups = num_cus < 32 ? 32 : num_cus / 32 * 32;   // a multiple of eight, and its half and quarter too
-    if constexpr (KIND != kFfnGradWeights) {
-        if (small) {
-            HCCLX_LAUNCH((k_ffn<DT, KIND, true>), dim3(groups), dim3(kWaves * 64), 0, st, a);
-            return hipGetLastError();
-        }
+    const dim3 groups(num_cus < 32 ? 32 : num_cus / 32 * 32);   // a multiple of eight, and its half and quarter too
+    const dim3 block(kWaves * 64);
+    if constexpr (KIND == kFfnGradWeights) {
+        HCCLX_LAUNCH((k_ffn<DT, KIND, kCutWhole>), groups, block, 0, st, a);
+    } else if (cut == kCutWhole) {
+        HCCLX_LAUNCH((k_ffn<DT, KIND, kCutWhole>), groups, block, 0, st, a);
+    } else if (cut == kCutSmall) {
+        HCCLX_LAUNCH((k_ffn<DT, KIND, kCutSmall>), groups, block, 0, st, a);
+    } else {
+        HCCLX_LAUNCH((k_ffn<DT, KIND, kCutWide>), groups, block, 0, st, a);
     }
-    HCCLX_LAUNCH((k_ffn<DT, KIND, false>), dim3(groups), dim3(kWaves * 64), 0, st, a);
     return hipGetLastError();
 }
 

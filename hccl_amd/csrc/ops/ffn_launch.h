@@ -29,6 +29,20 @@ inline bool halves(const FfnRows &s, uint32_t cus) { return static_cast<uint64_t
 // tiles, us: 64 rows, forward 99 : 121, gradients of the rows 134 : 144; 128 rows 115 : 125, 140 : 152; 160 rows, forward 146 : 124.
 constexpr uint32_t kSmallRows = 128;
 
+// Of those, which: a round of tiles of 128 x 256 takes 1.3 times as long as one of 128 x 128, and there are as many rounds as the
+// fullest CU has tiles.  Block of 8 ranks, 64 rows, wide in both products : small, us: 7168 x 2112 (132 tiles in a round : 264 in
+// two) 174 : 195, 6144 x 2560 180 : 200; 7168 x 2048 (256 in a round) 180 : 152, 4096 x 1024 91 : 64.
+template <int KIND>
+Cut cut_of(const FfnRows &s, uint32_t cus)
+{
+    if (s.most > static_cast<uint64_t>(s.n) * kSmallRows) return kCutWhole;
+    auto rounds = [&](uint32_t cols) {
+        const uint64_t tiles = static_cast<uint64_t>(s.n) * ((columns<KIND>(s) + cols - 1) / cols);
+        return (tiles + cus - 1) / cus;
+    };
+    return 13 * rounds(kTileCols<KIND>) < 10 * rounds(kTileCols<KIND> / 2) ? kCutWide : kCutSmall;
+}
+
 template <int DT, int KIND>
 hipError_t launch(const FfnArgs &a, uint32_t cus, hipStream_t st)
 {
@@ -53,7 +67,7 @@ hipError_t launch(const FfnArgs &a, uint32_t cus, hipStream_t st)
             HCCLX_LAUNCH((k_ffn_widen<DT>), dim3(s.most), dim3(256), 0, st, a);
         }
     }
-    return run<DT, KIND>(a, s.most <= static_cast<uint64_t>(s.n) * kSmallRows, cus, st);
+    return run<DT, KIND>(a, cut_of<KIND>(s, cus), cus, st);
 }
 
 }  // namespace ffn

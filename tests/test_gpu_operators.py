@@ -490,7 +490,8 @@ def test_ffn_of_many_rows(rows, dim, hidden, dtype):
 # On both sides of where another kernel, tile or split of what is left of a round takes over (256 CUs).
 FFN_EDGES = [([16], 16, 264, 520), ([17], 17, 264, 520), ([32], 32, 520, 264), ([33], 33, 520, 264), ([64], 64, 1032, 136), ([65], 65, 1032, 136),
              ([128, 128], 128, 264, 136), ([128, 129], 129, 264, 136), ([100, 0, 20, 128], 128, 1032, 520), ([0, 0], 400, 264, 136),
-             ([0, 700, 0], 700, 136, 264), ([2000], 2000, 648, 1272), ([3900], 3900, 1288, 1272), ([1], 700, 520, 264)]
+             ([0, 700, 0], 700, 136, 264), ([2000], 2000, 648, 1272), ([3900], 3900, 1288, 1272), ([1], 700, 520, 264),
+             ([90, 0, 128, 33, 70, 1, 65, 120], 128, 5128, 2120), ([100, 3] * 16, 100, 1288, 1096)]
 
 
 @pytest.mark.parametrize("dtype", [T.FP16, T.BFP16])
