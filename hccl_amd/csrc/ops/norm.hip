@@ -456,6 +456,26 @@ int take(P *const *in, uint32_t n, uint64_t align, bool optional, const char *wh
     return HCCL_SUCCESS;
 }
 
+// Rows and ranks run in any order and at once, so what a launch writes may lie on what it reads only where nobody else reads it: `own`
+// says whether rank i's may lie on that rank's part, given how far behind it begins.  to: n pointers to `bytes` each, from (may be
+// all null): n to `from_bytes`.
+template <typename Own>
+int check_apart(uint32_t n, const char *to_what, char *const *to, uint64_t bytes, const char *from_what, const char *const *from,
+                uint64_t from_bytes, Own &&own)
+{
+    if (to[0] == nullptr || from[0] == nullptr) return HCCL_SUCCESS;
+    for (uint32_t i = 0; i < n; ++i) {
+        for (uint32_t j = 0; j < n; ++j) {
+            const uint64_t t = reinterpret_cast<uint64_t>(to[i]);
+            const uint64_t f = reinterpret_cast<uint64_t>(from[j]);
+            if (t >= f + from_bytes || f >= t + bytes || (i == j && own(t - f))) continue;
+            return fail(HCCL_E_PARA, std::string(to_what) + "[" + std::to_string(i) + "] overlaps " + from_what + "[" + std::to_string(j) +
+                                         "], which others read or write");
+        }
+    }
+    return HCCL_SUCCESS;
+}
+
 int make_norm(const hcclx_rms_norm_t &a, hcclx_plan_t **plan)
 {
     int rc = check_norm(a.n, a.row_elems, a.dtype);
@@ -472,6 +492,27 @@ int make_norm(const hcclx_rms_norm_t &a, hcclx_plan_t **plan)
     if ((rc = take(a.out, a.n, quant ? 16 : size, false, "out", w->ptrs.out)) != HCCL_SUCCESS) return rc;
     DeviceCtx *ctx = device_ctx();
     if (!ctx) return HCCL_E_RUNTIME;
+    if (a.rows != 0) {
+        const uint64_t row = a.row_elems * size;
+        const uint64_t bytes = a.rows * row;
+        const uint64_t out_bytes = quant ? static_cast<uint64_t>(a.rows) * (a.row_elems + kTail) : bytes;
+        const NormPtrs &p = w->ptrs;
+        // a row's threads have read all of it before the first of them writes out, but not before total; rows of out begin where those
+        // of x do unless they are of 8 bits
+        const bool one = a.rows == 1;
+        const auto out_on_rows = [&](uint64_t behind) { return one || (!quant && behind == 0); };
+        const auto out_on_total = [&](uint64_t behind) { return !quant && behind == 0; };   // out is what stays
+        const auto out_on_weight = [&](uint64_t) { return one; };
+        const auto total_on_rows = [](uint64_t behind) { return behind == 0; };
+        const auto total_on_weight = [&](uint64_t behind) { return one && behind == 0; };
+        if ((rc = check_apart(a.n, "out", p.out, out_bytes, "x", p.x, bytes, out_on_rows)) != HCCL_SUCCESS) return rc;
+        if ((rc = check_apart(a.n, "out", p.out, out_bytes, "residual", p.residual, bytes, out_on_rows)) != HCCL_SUCCESS) return rc;
+        if ((rc = check_apart(a.n, "out", p.out, out_bytes, "weight", p.weight, row, out_on_weight)) != HCCL_SUCCESS) return rc;
+        if ((rc = check_apart(a.n, "out", p.out, out_bytes, "total", p.total, bytes, out_on_total)) != HCCL_SUCCESS) return rc;
+        if ((rc = check_apart(a.n, "total", p.total, bytes, "x", p.x, bytes, total_on_rows)) != HCCL_SUCCESS) return rc;
+        if ((rc = check_apart(a.n, "total", p.total, bytes, "residual", p.residual, bytes, total_on_rows)) != HCCL_SUCCESS) return rc;
+        if ((rc = check_apart(a.n, "total", p.total, bytes, "weight", p.weight, row, total_on_weight)) != HCCL_SUCCESS) return rc;
+    }
     w->n = a.n;
     w->rows = a.rows;
     w->elems = a.row_elems;

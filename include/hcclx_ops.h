@@ -28,8 +28,9 @@ extern "C" {
  * nearest; a row of zeros has scale 0.  Such rows are multiples of 16 bytes (row_elems has to be one), so that an MoE
  * dispatch of row_elems + HCCLX_ROW8_TAIL elements of HCCL_DATA_TYPE_FP8E4M3 carries codes and scale, and the experts' block
  * reads them where they arrive.
- * x, residual and weight have one pointer per rank (several may be the same); total may be x or residual, out may be any of
- * them that total is not. */
+ * x, residual and weight have one pointer per rank (several may be the same).  Where no other rank reads them, total may be x or
+ * residual, and out may be the one of them that total is not; not so 8-bit rows, which lie at other places than those of x (a single
+ * row may).  Results that overlap anything else the launch reads or writes are refused (HCCL_E_PARA). */
 #define HCCLX_ROW8_TAIL 16
 #define HCCLX_NORM_MAX_ROW 16384
 typedef struct {

@@ -1,0 +1,64 @@
+"""What the operators' entry points refuse because a launch could not give the right answer: results on top of what is still to
+be read, sizes that no launch holds.  Plans are made and never launched, from addresses that nothing dereferences."""
+import pytest
+
+from hccl_amd import hcclx
+from hccl_amd import types as T
+from hccl_amd._lib import HcclError
+
+pytestmark = pytest.mark.gpu   # (the checks of addresses come behind the one for a GPU)
+PARA = 1
+A, B, C, D, W = (0x7F0000000000 + (k << 32) for k in range(5))
+
+
+def refused(make, *words):
+    with pytest.raises(HcclError) as e:
+        make()
+    assert e.value.code == PARA, str(e.value)
+    for w in words:
+        assert w in str(e.value)
+
+
+def norm(rows=4, elems=64, dtype=T.BFP16, **more):
+    args = dict(x=[A], weight=[W], out=[B], rows=rows, row_elems=elems, dtype=dtype)
+    args.update(more)
+    return lambda: hcclx.RmsNormPlan(**args)
+
+
+ROW = 64 * 2   # bytes of a row of norm()
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(out=[A], out_dtype=T.FP8E4M3), ("out[0]", "x[0]")),                       # rows of another length than x's
+    (dict(out=[C], residual=[C], out_dtype=T.FP8E4M3), ("out[0]", "residual[0]")),
+    (dict(out=[C], total=[C], out_dtype=T.FP8E4M3), ("out[0]", "total[0]")),
+    (dict(out=[A], out_dtype=T.FP8E4M3, dtype=T.FP32), ("out[0]", "x[0]")),
+    (dict(out=[A + 3 * ROW + 112], out_dtype=T.FP8E4M3), ("out[0]", "x[0]")),       # the last 16 bytes of x
+    (dict(out=[A - 4 * 80 + 16], out_dtype=T.FP8E4M3), ("out[0]", "x[0]")),         # and the first
+    (dict(out=[W]), ("out[0]", "weight[0]")),                                       # other rows read it
+    (dict(out=[W - 4 * ROW + 2]), ("out[0]", "weight[0]")),
+    (dict(total=[W]), ("total[0]", "weight[0]")),
+    (dict(out=[A + ROW]), ("out[0]", "x[0]")),                                      # a row off
+    (dict(total=[A - 2]), ("total[0]", "x[0]")),
+    (dict(total=[A + 2], rows=1), ("total[0]", "x[0]")),
+    (dict(x=[A, A], weight=[W, W], out=[A, B]), ("out[0]", "x[1]")),                # another rank's
+    (dict(x=[A, C], weight=[W, W], out=[C, B]), ("out[0]", "x[1]")),
+    (dict(x=[A, A], weight=[W, W], out=[B, D], total=[C, A]), ("total[1]", "x[0]")),
+    (dict(x=[A, B], weight=[W, W], out=[W, C], rows=1), ("out[0]", "weight[1]")),
+    (dict(x=[A, B], weight=[W, W], out=[C, D], residual=[C, C]), ("out[0]", "residual[1]")),
+])
+def test_norm_refuses_results_on_what_is_still_read(change, words):
+    refused(norm(**change), *words)
+
+
+@pytest.mark.parametrize("change", [
+    {}, dict(out=[A]), dict(total=[A]), dict(residual=[C], total=[C], out=[A]), dict(residual=[C], total=[A], out=[C]),
+    dict(residual=[A]), dict(out=[A], total=[A]),
+    dict(out_dtype=T.FP8E4M3), dict(out=[A + 4 * ROW], out_dtype=T.FP8E4M3), dict(out=[A - 4 * 80], out_dtype=T.FP8E4M3),   # next to x
+    dict(out=[A], out_dtype=T.FP8E4M3, rows=1), dict(out=[W], rows=1),              # one row: all is read before it is written
+    dict(out=[A], out_dtype=T.FP8E4M3, rows=0),
+    dict(x=[A, A], weight=[W, W], out=[B, C]), dict(x=[A, B], weight=[W, W], out=[A, B]),
+    dict(x=[A, B], weight=[W, W], out=[C, D], residual=[B, A], total=[C, D]),
+])
+def test_norm_takes_results_in_place_of_what_only_their_row_reads(change):
+    norm(**change)()
