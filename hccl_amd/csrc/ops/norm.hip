@@ -334,6 +334,7 @@ struct RowShape {
     uint32_t threads;
     uint32_t per_group;
     uint32_t vectors;
+    uint64_t groups(uint64_t rows) const { return (rows + per_group - 1) / per_group; }
 };
 RowShape shape_of(uint32_t elems, int ne, uint32_t most_vectors)
 {
@@ -379,7 +380,7 @@ struct NormWork : PlanWork {
     int launch(const DeviceCtx *, hipStream_t st) const override
     {
         if (rows == 0) return HCCL_SUCCESS;
-        const dim3 grid((rows + shape.per_group - 1) / shape.per_group, n);
+        const dim3 grid(static_cast<uint32_t>(shape.groups(rows)), n);
         if (dtype == HCCL_DATA_TYPE_FP32) {
             quant ? launch_norm<HCCL_DATA_TYPE_FP32, true>(shape, grid, st, ptrs, rows, elems, eps)
                   : launch_norm<HCCL_DATA_TYPE_FP32, false>(shape, grid, st, ptrs, rows, elems, eps);
@@ -485,6 +486,8 @@ int make_norm(const hcclx_rms_norm_t &a, hcclx_plan_t **plan)
     if (quant && a.row_elems % 16 != 0) return fail(HCCL_E_PARA, "8-bit rows are multiples of 16 elements");
     auto w = std::make_unique<NormWork>();
     const uint64_t size = dtype_size(a.dtype);
+    w->shape = shape_of(a.row_elems, 16 / static_cast<int>(size), kMostVectors);
+    if (w->shape.groups(a.rows) * w->shape.threads > 0xffffffffull) return fail(HCCL_E_PARA, "too many rows");   // of a launch along x
     if ((rc = take(a.x, a.n, size, false, "x", w->ptrs.x)) != HCCL_SUCCESS) return rc;
     if ((rc = take(a.residual, a.n, size, true, "residual", w->ptrs.residual)) != HCCL_SUCCESS) return rc;
     if ((rc = take(a.weight, a.n, size, false, "weight", w->ptrs.weight)) != HCCL_SUCCESS) return rc;
@@ -519,7 +522,6 @@ int make_norm(const hcclx_rms_norm_t &a, hcclx_plan_t **plan)
     w->dtype = a.dtype;
     w->quant = quant;
     w->eps = a.eps;
-    w->shape = shape_of(a.row_elems, 16 / static_cast<int>(size), kMostVectors);
     const uint64_t elements = static_cast<uint64_t>(a.n) * a.rows * a.row_elems;
     const uint64_t algo = elements * (size * (1 + (a.residual != nullptr) + (a.total != nullptr)) + (quant ? 1 : size));
     return plan_of(ctx, std::move(w), algo, 0, plan);
@@ -546,11 +548,12 @@ int make_norm_grad(const hcclx_rms_norm_grad_t &a, hcclx_plan_t **plan)
     w->dtype = a.dtype;
     w->eps = a.eps;
     w->shape = shape_of(a.row_elems, 16 / static_cast<int>(size), 2);
-    const uint32_t most = (a.rows + w->shape.per_group - 1) / w->shape.per_group;
+    const uint32_t most = static_cast<uint32_t>(w->shape.groups(a.rows));
     // A workgroup takes four rows at least, while there are workgroups for every CU: its part of dweight is as long as a row of floats
     // (8 ranks x 256 x 4096 bf16, two rows 32 us, four 25; 3 x 777 x 1001 fp32, two at a time, four 15.7, eight 20.7).  Four workgroups
     // per CU: of 256 threads a CU holds as many; of longer rows' the others follow (8 x 1024 x 8192 118 us, as many as it holds 131).
-    w->groups = std::min(std::max((a.rows + 3) / 4, std::min(most, ctx->num_cus / a.n)), std::max(1u, 4u * ctx->num_cus / a.n));
+    w->groups = std::min(std::max(a.rows / 4 + (a.rows % 4 != 0), std::min(most, ctx->num_cus / a.n)), std::max(1u, 4u * ctx->num_cus / a.n));
+    if (a.rows > 0xffffffffu - w->groups * w->shape.per_group) return fail(HCCL_E_PARA, "too many rows");   // a slot's next row has 32 bits
     uint64_t held = 0;
     if (w->want_dweight && a.rows != 0) {
         held = static_cast<uint64_t>(a.n) * w->groups * a.row_elems * sizeof(float);

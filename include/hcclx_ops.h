@@ -35,7 +35,7 @@ extern "C" {
 #define HCCLX_NORM_MAX_ROW 16384
 typedef struct {
     uint32_t n;         /* ranks, 1 .. 64 */
-    uint32_t rows;      /* of each rank; 0: nothing to do */
+    uint32_t rows;      /* of each rank, as many as fit a launch (2^22 - 1 of any length, 2^28 - 4 of the shortest); 0: nothing to do */
     uint32_t row_elems; /* 1 .. HCCLX_NORM_MAX_ROW */
     int dtype;          /* of x, residual, weight and total */
     int out_dtype;      /* dtype or HCCL_DATA_TYPE_FP8E4M3 */

@@ -1,6 +1,7 @@
 """What the operators' entry points refuse because a launch could not give the right answer: results on top of what is still to
 be read, sizes that no launch holds.  Plans are made and never launched, from addresses that nothing dereferences."""
 import pytest
+import torch
 
 from hccl_amd import hcclx
 from hccl_amd import types as T
@@ -62,3 +63,22 @@ def test_norm_refuses_results_on_what_is_still_read(change, words):
 ])
 def test_norm_takes_results_in_place_of_what_only_their_row_reads(change):
     norm(**change)()
+
+
+@pytest.mark.parametrize("n,elems", [(1, 8), (64, 8), (1, 16384)])
+def test_norm_gradient_refuses_rows_whose_numbers_wrap(n, elems):
+    def make(rows):
+        return lambda: hcclx.RmsNormGradPlan(*([at << 50] * n for at in (1, 2, 3, 4)), [5 << 50] * n, rows, elems, T.BFP16)
+    make(0xFFFF0000)()
+    for rows in (0xFFFFFFFF, 0xFFFFFFFE, 0xFFFFFFFC):
+        refused(make(rows), "rows")
+
+
+def test_norm_of_as_many_rows_as_a_launch_holds():
+    """The limit is the launch's: one row less is normed."""
+    rows = (1 << 28) - 4
+    x = torch.randint(1, 100, (rows,), device="cuda:0", dtype=torch.bfloat16)
+    w, out = torch.full((1,), 3, device="cuda:0", dtype=torch.bfloat16), torch.zeros_like(x)
+    hcclx.RmsNormPlan([x.data_ptr()], [w.data_ptr()], [out.data_ptr()], rows, 1, T.BFP16).launch()
+    torch.cuda.synchronize()
+    assert bool((out == 3).all())                                  # x * 3 / sqrt(x^2 + 1e-6): 3 but for 2^-21 of it
