@@ -541,6 +541,17 @@ int make_norm_grad(const hcclx_rms_norm_grad_t &a, hcclx_plan_t **plan)
     if ((rc = take(a.dweight, a.n, size, true, "dweight", w->dweight.p)) != HCCL_SUCCESS) return rc;
     DeviceCtx *ctx = device_ctx();
     if (!ctx) return HCCL_E_RUNTIME;
+    if (a.rows != 0) {
+        const uint64_t row = a.row_elems * size;
+        const uint64_t bytes = a.rows * row;
+        const GradPtrs &p = w->ptrs;
+        const auto on_rows = [](uint64_t behind) { return behind == 0; };
+        const auto on_weight = [&](uint64_t behind) { return a.rows == 1 && behind == 0; };
+        if ((rc = check_apart(a.n, "dx", p.dx, bytes, "dy", p.dy, bytes, on_rows)) != HCCL_SUCCESS) return rc;
+        if ((rc = check_apart(a.n, "dx", p.dx, bytes, "total", p.total, bytes, on_rows)) != HCCL_SUCCESS) return rc;
+        if ((rc = check_apart(a.n, "dx", p.dx, bytes, "dtotal", p.dtotal, bytes, on_rows)) != HCCL_SUCCESS) return rc;
+        if ((rc = check_apart(a.n, "dx", p.dx, bytes, "weight", p.weight, row, on_weight)) != HCCL_SUCCESS) return rc;
+    }
     w->want_dweight = a.dweight != nullptr;
     w->n = a.n;
     w->rows = a.rows;

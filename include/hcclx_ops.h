@@ -52,7 +52,9 @@ int hcclx_rms_norm_plan_create(const hcclx_rms_norm_t *norm, hcclx_plan_t **plan
  *     dx      = r * (dy * weight - total * r^2 * mean(dy * weight * total)) + dtotal
  *     dweight = sum over the rank's rows of dy * total * r
  * dx is the gradient of x and of residual alike; dtotal is what reaches total from elsewhere (NULL: nothing).  Sums are held
- * in 32 bits and added in a fixed order.  dx may be dy or dtotal; dweight NULL: not wanted. */
+ * in 32 bits and added in a fixed order.  dx may be its rank's dy, total or dtotal where no other rank reads it; on top of anything
+ * else that is read it is refused (HCCL_E_PARA).  dweight, which is written when all has been read, may be weight; NULL: not
+ * wanted. */
 typedef struct {
     uint32_t n;
     uint32_t rows; /* 0: dweight becomes zeros */

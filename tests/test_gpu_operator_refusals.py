@@ -65,6 +65,30 @@ def test_norm_takes_results_in_place_of_what_only_their_row_reads(change):
     norm(**change)()
 
 
+def norm_grad(rows=4, **more):
+    args = dict(dy=[A], total=[B], weight=[W], dx=[C], dweight=[D], rows=rows, row_elems=64, dtype=T.BFP16)
+    args.update(more)
+    return lambda: hcclx.RmsNormGradPlan(**args)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(dx=[W]), ("dx[0]", "weight[0]")), (dict(dx=[W - 3 * ROW]), ("dx[0]", "weight[0]")), (dict(dx=[A + ROW]), ("dx[0]", "dy[0]")),
+    (dict(dx=[B - 2]), ("dx[0]", "total[0]")), (dict(dx=[D + 2 * ROW], dtotal=[D], dweight=None), ("dx[0]", "dtotal[0]")),
+    (dict(dy=[A, A], total=[B, B], weight=[W, W], dx=[A, C], dweight=[D, D + ROW]), ("dx[0]", "dy[1]")),
+    (dict(dy=[A, B], total=[C, C], weight=[W, W], dx=[D, C], dweight=None), ("dx[1]", "total[0]")),
+    (dict(dy=[A, B], total=[C, D], weight=[W, W], dx=[B, A], dweight=None), ("dx[0]", "dy[1]")),
+])
+def test_norm_gradient_refuses_results_on_what_is_still_read(change, words):
+    refused(norm_grad(**change), *words)
+
+
+@pytest.mark.parametrize("change", [{}, dict(dx=[A]), dict(dx=[B]), dict(dtotal=[C]), dict(dtotal=[A]), dict(dx=[W], rows=1), dict(dx=[W], rows=0),
+                                    dict(dweight=[W]), dict(dx=[A + 4 * ROW]), dict(dx=[W + ROW]),
+                                    dict(dy=[A, B], total=[C, D], weight=[W, W], dx=[A, B], dweight=None)])
+def test_norm_gradient_takes_results_in_place_of_what_only_their_row_reads(change):
+    norm_grad(**change)()
+
+
 @pytest.mark.parametrize("n,elems", [(1, 8), (64, 8), (1, 16384)])
 def test_norm_gradient_refuses_rows_whose_numbers_wrap(n, elems):
     def make(rows):
