@@ -7,6 +7,7 @@
 #include "hcclx_ops.h"
 #include "ops/ffn.h"
 
+#include <algorithm>
 #include <string>
 
 using namespace hcclx;
@@ -70,13 +71,15 @@ struct FfnGradWork : PlanWork {
     FfnArgs hidden{};
     FfnArgs input{};
     FfnArgs weights{};
-    DeviceBlock scratch;   // h, dproj
+    bool weights_first = false;   // dx lies on what the weights' products read
+    DeviceBlock scratch;          // h, dproj
 
     int launch(const DeviceCtx *ctx, hipStream_t st) const override
     {
         hipError_t e = product(dtype, kFfnGradHidden, hidden, ctx->num_cus, st);
+        if (e == hipSuccess && weights_first) e = product(dtype, kFfnGradWeights, weights, ctx->num_cus, st);
         if (e == hipSuccess) e = product(dtype, kFfnGradInput, input, ctx->num_cus, st);
-        if (e == hipSuccess) e = product(dtype, kFfnGradWeights, weights, ctx->num_cus, st);
+        if (e == hipSuccess && !weights_first) e = product(dtype, kFfnGradWeights, weights, ctx->num_cus, st);
         return e == hipSuccess ? HCCL_SUCCESS : fail_hip(e, "feed-forward gradient kernels");
     }
 };
@@ -115,6 +118,12 @@ int make_ffn(const hcclx_gated_ffn_t &f, hcclx_plan_t **plan)
     return plan_of(ctx, std::move(w), weights + static_cast<uint64_t>(rows.most) * rows.dim * (small ? 3 : 4), held, plan);
 }
 
+// How many of n pointers are among n others.
+uint32_t among(uint32_t n, const char *const *a, const char *const *b)
+{
+    return static_cast<uint32_t>(std::count_if(a, a + n, [&](const char *p) { return std::find(b, b + n, p) != b + n; }));
+}
+
 int make_ffn_grad(const hcclx_gated_ffn_grad_t &f, hcclx_plan_t **plan)
 {
     FfnRows rows;
@@ -137,6 +146,21 @@ int make_ffn_grad(const hcclx_gated_ffn_grad_t &f, hcclx_plan_t **plan)
     if ((rc = take(const_cast<const void *const *>(f.dw_gate), rows.n, "dw_gate", w->weights.p[2])) != HCCL_SUCCESS) return rc;
     if ((rc = take(const_cast<const void *const *>(f.dw_up), rows.n, "dw_up", w->weights.p[3])) != HCCL_SUCCESS) return rc;
     if ((rc = take(const_cast<const void *const *>(f.dw_down), rows.n, "dw_down", w->weights.p[4])) != HCCL_SUCCESS) return rc;
+    // What a product writes may lie on what only products before it read.  How many rows a buffer has is known on the device only, and
+    // one without rows may begin where another ends, so nothing is refused for a single rank's address.
+    const uint32_t n = rows.n;
+    const char *const *x = w->weights.p[0], *const *dy = w->weights.p[1], *const *dx = w->input.p[2];
+    const char *const *w_gate = w->input.p[0], *const *w_up = w->input.p[1];
+    const uint32_t dx_on_x = among(n, dx, x), dx_on_dy = among(n, dx, dy);
+    w->weights_first = dx_on_x != 0 || dx_on_dy != 0;
+    if (rows.most != 0 && (among(n, dx, w_gate) == n || among(n, dx, w_up) == n)) return fail(HCCL_E_PARA, "dx on w_gate or w_up");
+    for (uint32_t k = 2; k < 5 && rows.most != 0; ++k) {
+        const char *const *dw = w->weights.p[k];
+        if (among(n, dw, x) == n || among(n, dw, dy) == n) return fail(HCCL_E_PARA, "the gradient of a weight on x or dy");
+        if ((dx_on_x == n || dx_on_dy == n) && among(n, dw, w_gate) + among(n, dw, w_up) != 0) {
+            return fail(HCCL_E_PARA, "dx on x or dy and the gradient of a weight on w_gate or w_up at once");
+        }
+    }
     DeviceCtx *ctx = device_ctx();
     if (!ctx) return HCCL_E_RUNTIME;
     const uint64_t h_bytes = round256(static_cast<uint64_t>(rows.most) * rows.hidden * 2);

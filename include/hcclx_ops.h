@@ -117,7 +117,9 @@ int hcclx_gated_ffn_plan_create(const hcclx_gated_ffn_t *ffn, hcclx_plan_t **pla
 
 /* Its gradients, from dy of out and what the forward pass saved for the same shape and counts.  The gradients of the weights
  * are sums over the rank's rows (zeros where it has none), rounded once; the operands of their products are rounded to dtype
- * (the gradients of both products of the forward pass, and h). */
+ * (the gradients of both products of the forward pass, and h).  The buffers of dx may be those of dy or of x, and
+ * those of dw_gate, dw_up and dw_down the weights', but not both at once (w_down's always); what is written on other inputs is refused
+ * where an address says so (HCCL_E_PARA). */
 typedef struct {
     hcclx_ffn_shape_t shape;
     const void *const *dy;

@@ -33,3 +33,36 @@ def test_norm_gradient_in_place(n, rows, elems, dtype, on):
         O.assert_close(dw[i], wdw, bdw)
     launch(src[on], w)
     assert all(torch.equal(a, b) for a, b in zip(src[on] + w, dx + dw))
+
+
+# ---- the experts' gradient on top of its inputs ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [T.FP16, T.BFP16])
+@pytest.mark.parametrize("rows,dim,hidden", [([3, 0, 2], 72, 40), ([130, 1, 129], 136, 264), ([700, 300], 264, 520)])
+@pytest.mark.parametrize("on", ["dx on dy", "dx on x", "dx on dy of another rank", "dw on the weights"])
+def test_ffn_gradient_in_place(rows, dim, hidden, dtype, on):
+    f = Ffn(rows, max(rows), dim, hidden, dtype, dim)
+    f.run()
+    f.check()
+    n, shape = len(rows), {**f.shape, "rows": f.total}
+    want = [f.dx[i][:r * dim].clone() for i, r in enumerate(rows)] + [d[i].clone() for d in f.dw for i in range(n)]
+    at = [k.ptrs for k in (f.dw[0], f.dw[1], f.dw[2])]
+    if on == "dx on dy":
+        dx, dw = f.dy, f.dw
+    elif on == "dx on x":
+        dx, dw = f.x, f.dw
+    elif on == "dx on dy of another rank":
+        dx, dw = f.dy, f.dw
+    else:
+        dx, dw = f.dx, f.w
+        at = [ptrs(k) for k in f.w]
+    turn = 1 if on == "dx on dy of another rank" else 0
+    place = [(i + turn) % n for i in range(n)]
+    for k in (f.dx, *f.dw):
+        if k is not dx:
+            k.raw.fill_(0xFF)
+    hcclx.GatedFfnGradPlan(f.dy.ptrs, f.x.ptrs, *[ptrs(k) for k in f.w], f.saved.data_ptr(), [dx.ptrs[p] for p in place], *at, **shape).launch()
+    torch.cuda.synchronize()
+    got = [dx[p][:r * dim] for p, r in zip(place, rows)] + [d[i].view(-1) for d in dw for i in range(n)]
+    for k, (a, b) in enumerate(zip(got, want)):
+        assert torch.equal(a, b), k

@@ -89,6 +89,34 @@ def test_norm_gradient_takes_results_in_place_of_what_only_their_row_reads(chang
     norm_grad(**change)()
 
 
+def ffn_grad():
+    names = ("dy", "x", "w_gate", "w_up", "w_down", "dx", "dw_gate", "dw_up", "dw_down")
+    return dict({k: [A + (i << 32), A + (i << 32) + (1 << 20)] for i, k in enumerate(names)}, saved=A + (1 << 40), capacity=8, dim=64, hidden=32,
+                dtype=T.BFP16)
+
+
+@pytest.mark.parametrize("dx", ["dy", "x"])
+@pytest.mark.parametrize("dw", ["dw_gate", "dw_up"])
+@pytest.mark.parametrize("weight", ["w_gate", "w_up"])
+def test_ffn_gradient_refuses_dx_and_dw_in_place_at_once(dx, dw, weight):
+    args = ffn_grad()
+    args["dx"] = args[dx]
+    hcclx.GatedFfnGradPlan(**args)
+    hcclx.GatedFfnGradPlan(**{**args, "dw_down": args["w_down"]})
+    refused(lambda: hcclx.GatedFfnGradPlan(**{**args, dw: args[weight]}), "at once")
+    refused(lambda: hcclx.GatedFfnGradPlan(**{**args, dw: [args[dw][0], args[weight][0]]}), "at once")
+
+
+@pytest.mark.parametrize("result,on", [("dx", "w_gate"), ("dx", "w_up")] + [(r, k) for r in ("dw_gate", "dw_up", "dw_down") for k in ("x", "dy")])
+def test_ffn_gradient_refuses_results_on_what_their_product_reads(result, on):
+    args = ffn_grad()
+    refused(lambda: hcclx.GatedFfnGradPlan(**{**args, result: args[on]}), result[:1])
+    refused(lambda: hcclx.GatedFfnGradPlan(**{**args, result: args[on][::-1]}), " on ")
+    hcclx.GatedFfnGradPlan(**{**args, result: args[on], "capacity": 0})
+    # a rank without rows, whose buffer begins where those of the others end
+    hcclx.GatedFfnGradPlan(**{**args, result: [args[result][0], args[on][0]]})
+
+
 @pytest.mark.parametrize("n,elems", [(1, 8), (64, 8), (1, 16384)])
 def test_norm_gradient_refuses_rows_whose_numbers_wrap(n, elems):
     def make(rows):
