@@ -343,10 +343,12 @@ struct Act {
     float slope;
     __device__ __forceinline__ Act(float a, const ActTerms &t)
     {
-        const float square = __builtin_fminf(a * a, 1e30f);   // (0 times infinity is not 0; the exponential is 0 long before)
+        // (0 times infinity is not 0.  Far out, where s is 0 or 1, so is value or 1 - s, and what it is multiplied by is finite: the
+        // square by its limit, which s has long ceased to notice, and not times a, which has none.)
+        const float square = __builtin_fminf(a * a, 1e30f);
         const float s = 1.0f / (1.0f + __expf(-a * (t.p + t.q * square)));
         value = a * s;
-        slope = s * (1.0f + a * (1.0f - s) * (t.p + 3.0f * t.q * square));
+        slope = s + value * (1.0f - s) * (t.p + 3.0f * t.q * square);
     }
 };
 

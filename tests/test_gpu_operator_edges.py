@@ -66,3 +66,29 @@ def test_ffn_gradient_in_place(rows, dim, hidden, dtype, on):
     got = [dx[p][:r * dim] for p, r in zip(place, rows)] + [d[i].view(-1) for d in dw for i in range(n)]
     for k, (a, b) in enumerate(zip(got, want)):
         assert torch.equal(a, b), k
+
+
+# ---- gates far out ---------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("act", [0, 1])
+@pytest.mark.parametrize("rows", [1, 100, 300])
+def test_ffn_gates_to_the_end_of_the_range(rows, act):
+    """Gates of +-2^43 .. 2^123, whose cube passes the range of 32 bits: the activation and its derivative are 0 and 0, or the gate
+    and 1.  Every number is a power of two or a small multiple of one, so that results are exact."""
+    dim, hidden, powers = 64, 168, torch.arange(20, 101, device=DEV)
+    e = torch.cat([powers, powers, powers[:6]]).double()
+    sign = torch.ones(hidden, device=DEV, dtype=torch.float64)
+    sign[81:162] = -1
+    f = Ffn([rows], rows, dim, hidden, T.BFP16, 1)
+    x, dy = torch.zeros((rows, dim), device=DEV, dtype=torch.bfloat16), torch.zeros((rows, dim), device=DEV, dtype=torch.bfloat16)
+    x[:, 0], dy[:, 0] = 2.0 ** 23, 1
+    f.x[0].copy_(x.view(-1)), f.dy[0].copy_(dy.view(-1))
+    for w in f.w:
+        w[0].zero_()
+    f.w[0][0][:, 0] = sign * 2.0 ** e          # gate +-2^(e + 23)
+    f.w[1][0][:, 0] = 2.0 ** -23               # up 1
+    f.w[2][0][0] = 2.0 ** -(e + 23)
+    f.run(act)
+    got = [f.out[0].view(rows, dim), f.dx[0].view(rows, dim)] + [d[0].view(w[0].shape) for d, w in zip(f.dw, f.w)]
+    for a, (b, _) in zip(got, O.ffn(x, f.w[0][0], f.w[1][0], f.w[2][0], act, torch.bfloat16, dy)):
+        assert bool(b.isfinite().all()) and torch.equal(a, b.to(torch.bfloat16))   # (some sums round to infinity)
