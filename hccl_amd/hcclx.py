@@ -336,14 +336,12 @@ class AdamWPlan(_OperatorPlan):
                 setattr(a, k, t.get(k) or None)
         self._create("hcclx_adamw_plan_create", arr, len(tensors), int(grad_dtype), int(state_dtype),
                      int(grad_dtype if copy_dtype is None else copy_dtype))
-        self._args = _lib.AdamWStep()
-        self._args_ref = ctypes.byref(self._args)
         self._step = _lib.load().hcclx_adamw_step
 
     def step(self, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, seed=0, grad_scale=0, stream=0):
         """step: 1, 2, ...; seed: 32 bits, another one every step (8-bit states); grad_scale: device address of a float that
         multiplies the gradients, or 0."""
-        self._args.__init__(lr, beta1, beta2, eps, step, seed & 0xFFFFFFFF, grad_scale or None)
-        rc = self._step(self._h, self._args_ref, stream)
+        args = _lib.AdamWStep(lr, beta1, beta2, eps, step, seed & 0xFFFFFFFF, grad_scale or None)
+        rc = self._step(self._h, ctypes.byref(args), stream)
         if rc:
             check(rc)
