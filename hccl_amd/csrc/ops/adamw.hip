@@ -43,6 +43,7 @@ struct StepArgs {
     const float *grad_scale;
 };
 
+// (shifts and factors: of C. Wellons' published search for 32-bit mixers whose output bits depend on all input bits alike)
 __device__ __forceinline__ uint32_t mix(uint32_t x)
 {
     x ^= x >> 16;

@@ -6,8 +6,10 @@
 // v_mfma 16x16x32 takes B as its first operand, so that a lane ends up with four neighbouring columns of C.  (From registers alone
 // it reaches 2100 TFLOP/s here, 32x32x16 1350.)
 //
-// What bounds it: the matrix instructions, of which 70 % of the time is full, at the clock that the card's power leaves (1.9 GHz).
-// 8 ranks x 4096 rows x 7168 x 2048 1400 us for the first product (1370 TFLOP/s), 750 for the second (1280).  A wavefront has 128 x
+// What bounds it: the matrix instructions, at the clock that the card's power leaves.  8 ranks x 4096 rows x 7168 x 2048: 1400 us for
+// the first product (1370 TFLOP/s; its pipes are busy 71 % of the time, at 1.75 to 1.9 GHz), 750 for the second (1280; 66 %).  With
+// rows of 4096 they are busy for 59 to 61 %, with those of the hidden rows' gradient, which reads and writes four streams between its
+// tiles while nothing is multiplied, for 38 %.  A wavefront has 128 x
 // 128 of a tile of 256 x 256, which is one wavefront per SIMD, 256 accumulators in the second half of its registers and one LDS
 // read of 1 KiB for four matrix instructions; eight wavefronts of 128 x 64 read half as much again and took 1580 and 820.  With
 // nobody else on its SIMD a wavefront has to keep the matrix pipe busy by itself: between two matrix instructions there is one
@@ -278,7 +280,6 @@ private:
     {
         // (crosswise: of the row's number, the first two bits and the fourth turn the chunks; a load is kRows rows further on)
         constexpr bool kTurns = !KWISE;
-        
         const uint32_t c = kTurns ? chunk ^ (((i * kRows) & 3) | (((i * kRows) >> 3) & 1) << 2) * 2 : chunk;
         return (c * 8 < end ? row_at + c * 16 : kOut) + i * kRows * ld;
     }

@@ -1,6 +1,6 @@
 // Which kernel computes a product: instantiated per type in ffn_bf16.hip and ffn_f16.hip.  A choice goes by the sizes and by the
 // bound on the rows of all ranks, from which the rows of a rank are taken as if all had as many; whatever they turn out to be on
-// the device, every kernel is right for them.
+// the device, every kernel is right for them.  (A plan whose bound is far above what a launch then has runs the kernels of the bound.)
 #pragma once
 #include "ops/ffn_gemm.h"
 #include "ops/ffn_thin.h"
@@ -10,9 +10,12 @@ namespace ffn {
 
 // Products with few rows read the weights; what counts is how many bytes are on their way.  Tiles of 128 x 128 keep 48 KiB of
 // weights per CU on their way and read the rows' operand once per tile, but have to be as many as the CUs; the thin kernel
-// has eight wavefronts per 16 columns and reads the rows' operand that often.  Weights of dim x 2048, both products, thin : tiles,
-// us: 8 ranks x 7168 (256 tiles of the first product), 1 row 136 : 142, 16 rows 174 : 139; 4 ranks x 7168 (128), 1 row 75 : 95,
-// 8 rows 82 : 93, 16 rows 92 : 94; 2 ranks x 4096 (64), 1 row 25 : 63, 64 rows 54 : 64; 1 rank (32), 64 rows 38 : 60.
+// has eight wavefronts per 16 columns and reads the rows' operand that often.  Both products, weights from memory, thin : tiles, us:
+// up to a quarter of a round of tiles, 2 ranks x 4096 x 2048 (64 tiles of the first product), 1 row 26.5 : 60, 64 rows 55 : 64; 1 rank
+// (32), 64 rows 42 : 62; 1 x 7168 x 2048, 64 rows 74 : 88.  Up to a round, 4 ranks x 7168 x 2048 (128 tiles), 1 row 75 : 95, 8 rows
+// 82 : 96, 64 rows 182 : 106; 8 x 4096 x 1024 (128), 8 rows 52 : 60, 64 rows 115 : 64.  A full round, 8 x 7168 x 2048 (256), 1 row
+// 138 : 146, 4 rows 144 : 138, 16 rows 174 : 139; 16 x 2048 x 1024 (256), 1 row 50 : 56, 8 rows 55 : 56, 16 rows 60 : 57.  What the rule
+// leaves: a single row at a full round, and 9 to 16 rows at half of one (4 x 16 x 7168 x 2048 92 : 97, 8 x 16 x 4096 x 1024 58 : 60.5).
 template <int KIND>
 bool thin(const FfnRows &s, uint32_t cus)
 {

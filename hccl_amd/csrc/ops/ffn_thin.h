@@ -5,8 +5,9 @@
 // instruction's registers without LDS: nobody else needs them.  A lane's two chunks of 16 bytes of a turn lie next to each other
 // (k = 16 (lane / 16) .. + 15), so that four lanes read a cache line of a row; the same k of the rows of x, which come from the L2.
 //
-// What bounds it: the weights' way from memory, with too little time to reach its rate: 1 row x 4096 x 2048 10.9 and 5.5 us
-// (3.1 TB/s), 2 ranks 25 (4.0), 8 ranks x 7168 x 2048 136 (5.2).
+// What bounds it: the weights' way from memory, with too little time to reach its rate.  Block of 1 row x 4096 x 2048 16 us (3.1 TB/s;
+// 10.9 and 5.5 us of kernels) where the last-level cache holds the weights, 17.7 (2.8) from memory; 2 ranks 26.5 (3.8), 4 ranks x
+// 7168 x 2048 74.5 (4.7).
 //
 // Limits as in ffn_gemm.h: range-checked loads give zeros behind the last row, column and k.
 #pragma once
@@ -17,8 +18,8 @@ namespace ffn {
 
 constexpr uint32_t kThinWaves = 8;
 constexpr uint32_t kTurnK = 64;
-// Turns whose loads are on their way together.  (Two, four, eight: 8 ranks x 1 row x 7168 x 2048, second product 67, 80, 113 us; first
-// 95, 93, 104.  More registers leave fewer wavefronts on a CU, and a turn behind the last costs as much as any.  Sixteen
+// Turns whose loads are on their way together.  (Two, four, eight: 8 ranks x 1 row x 7168 x 2048, for which tiles are taken otherwise,
+// second product 67, 80, 113 us; first 95, 93, 104.  More registers leave fewer wavefronts on a CU, and a turn behind the last costs as much as any.  Sixteen
 // wavefronts instead of eight: 73 and 101.)
 constexpr int kTurnsAhead = 2;
 

@@ -102,8 +102,9 @@ __device__ __forceinline__ void row_reduce(float (&v)[N], float (*s)[N])
 }
 
 // A row per blockDim.x threads and no second row: what a workgroup waits for, others have on their way.  bf16, 8 ranks x 4096 x 7168
-// with residual and 8-bit rows 284 us (5.8 TB/s), 8 x 2048 x 4096 in 16 bits 93 us (5.8); 8 x 64 x 7168 10 us, a launch and one
-// trip to memory.
+// with residual and 8-bit rows 285 us (5.8 TB/s), 8 x 2048 x 4096 in 16 bits 93 us (5.8).  8 x 64 x 7168 to 8 bits 10 us with the rows
+// in the last-level cache, 13 from memory (2.0 TB/s), in 16 bits 10: neither the bytes nor one trip to memory make that up; the chain
+// of a rank's addresses, its rows and two reductions has not been taken apart.
 template <int DT, bool QUANT, int NV>
 __global__ void __launch_bounds__(kMostThreads<DT>)
 k_rms_norm(NormPtrs ptrs, uint32_t rows, uint32_t elems, float eps)

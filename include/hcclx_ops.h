@@ -95,7 +95,8 @@ typedef struct {
     uint32_t capacity; /* rows that fit a rank's buffers */
     uint32_t dim;
     uint32_t hidden;
-    uint64_t rows;     /* at most so many in all ranks together; 0: n * capacity.  Scratch memory is sized by it */
+    uint64_t rows;     /* at most so many in all ranks together; 0: n * capacity.  Scratch memory is sized by it, and kernels are
+                          chosen by it: a decoding step's plan should say how many rows it has at most */
     int dtype;
     int activation;    /* hcclx_act_t */
     const uint64_t *counts; /* device */
@@ -150,7 +151,10 @@ int hcclx_gated_ffn_grad_plan_create(const hcclx_gated_ffn_grad_t *ffn, hcclx_pl
  * of tensor t is  mix(k + mix(seed + (t + 1) * 0x9E3779B9)),  in 32-bit arithmetic, its low half for m and its high half for
  * sqrt(v), with
  *     mix(x):  x ^= x >> 16;  x *= 0x7FEB352D;  x ^= x >> 15;  x *= 0x846CA68B;  x ^= x >> 16
- * so that a step is a function of its arguments; give every step another seed. */
+ * (its shifts and factors are those of C. Wellons' published search for such mixers), so that a step is a function of its arguments;
+ * give every step another seed.  Magnitudes below 2^-9 codes, 4.4e-6 of the largest of their block, are held as zero or as 2^-9 of a
+ * code: where sqrt(v) is held as zero and m is not, what is left of the update's denominator is the new gradient's part and eps, so
+ * eps is to be chosen with that in mind. */
 #define HCCLX_ADAMW_BLOCK 256
 typedef struct {
     uint64_t count;
