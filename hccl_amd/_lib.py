@@ -87,6 +87,40 @@ class AdamWStep(ctypes.Structure):
         ("step", ctypes.c_uint32), ("seed", ctypes.c_uint32), ("grad_scale", ctypes.c_void_p)]
 
 
+class Logits(ctypes.Structure):
+    """hcclx_logits_t."""
+    _fields_ = [("n", ctypes.c_uint32), ("rows", ctypes.c_uint32), ("dtype", ctypes.c_int), ("logits", _ranks_field),
+                ("columns", ctypes.POINTER(ctypes.c_uint32)), ("row_stride", ctypes.POINTER(ctypes.c_uint64))]
+
+
+class TopLogits(ctypes.Structure):
+    """hcclx_top_logits_t."""
+    _fields_ = [("logits", Logits), ("k", ctypes.c_uint32)] + [(k, ctypes.c_void_p) for k in ("values", "indices", "lse")]
+
+
+class Teacher(ctypes.Structure):
+    """hcclx_teacher_t."""
+    _fields_ = [("k", ctypes.c_uint32), ("dtype", ctypes.c_int), ("logits", ctypes.c_void_p), ("indices", ctypes.c_void_p),
+                ("temperature", ctypes.c_float)]
+
+
+class Distill(ctypes.Structure):
+    """hcclx_distill_t."""
+    _fields_ = [("logits", Logits), ("teacher", Teacher)] + [(k, ctypes.c_void_p) for k in ("weight", "loss", "stats")] + [
+        ("dlogits", _ranks_field)]
+
+
+class DistillGrad(ctypes.Structure):
+    """hcclx_distill_grad_t."""
+    _fields_ = [("logits", Logits), ("teacher", Teacher), ("weight", ctypes.c_void_p), ("stats", ctypes.c_void_p), ("dlogits", _ranks_field)]
+
+
+class Sample(ctypes.Structure):
+    """hcclx_sample_t."""
+    _fields_ = [("logits", Logits)] + [
+        (k, ctypes.c_void_p) for k in ("temperature", "top_k", "top_p", "min_p", "random", "token", "logprob")]
+
+
 _lib = None
 
 
@@ -161,7 +195,8 @@ def load():
     lib.hcclx_allgatherv.argtypes = [vpp, vpp, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint32, ctypes.c_int,
                                      ctypes.c_int, ctypes.c_void_p]
     plan_p = ctypes.POINTER(ctypes.c_void_p)
-    for name, arg in (("rms_norm", RmsNorm), ("rms_norm_grad", RmsNormGrad), ("gated_ffn", GatedFfn), ("gated_ffn_grad", GatedFfnGrad)):
+    for name, arg in (("rms_norm", RmsNorm), ("rms_norm_grad", RmsNormGrad), ("gated_ffn", GatedFfn), ("gated_ffn_grad", GatedFfnGrad),
+                      ("top_logits", TopLogits), ("distill", Distill), ("distill_grad", DistillGrad), ("sample", Sample)):
         fn = getattr(lib, f"hcclx_{name}_plan_create")
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.POINTER(arg), plan_p]

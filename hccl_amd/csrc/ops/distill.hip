@@ -1,0 +1,622 @@
+// The loss of a student against a teacher's top logits, and its gradient (include/hcclx_ops.h: hcclx_distill_*).
+//
+// With c = log2(e) / T, r a reference near the largest l c of the row and S the sum over the row of 2^(l c - r):
+//     q = 2^(l c - r) / S,   log q = (l c - r) ln 2 - log S
+// so a row needs one pass for r and S (a running reference and sum per lane, joined at the end) and one for the gradient.  Every
+// l c - r is one fused operation on the same r and c, so what rounds them cancels between a term and the sum.  What concerns the
+// teacher's k entries alone is computed in 64 bits: the loss is a small difference of logarithms.
+#include "ops/logits.h"
+
+#include <algorithm>
+#include <cmath>
+
+using namespace hcclx;
+using namespace hcclx::logits;
+
+namespace {
+
+constexpr uint32_t kThreads = 512;
+constexpr uint32_t kWaves = kThreads / 64;
+constexpr int kAhead = 4;                                        // chunks of a wavefront that are on their way together
+constexpr uint32_t kSlots = 2 * HCCLX_TOP_MAX;                   // of the table of the entries' columns
+constexpr uint32_t kEach = (HCCLX_TOP_MAX + kThreads - 1) / kThreads;   // entries of a thread
+constexpr uint32_t kFree = 0xffffffffu;
+constexpr double kLn2 = 0.69314718055994530942;
+
+struct DistillArgs {
+    Rows rows;
+    const char *teacher;
+    const int32_t *indices;
+    const float *weight;   // nullptr: 1
+    float *loss;
+    float2 *stats;         // written with the loss; read where there is none
+    float2 *parts;         // r and S of the parts of every row: [rows][nparts]
+    float *student;        // [rows][k]: the student's logits at the teacher's entries, where several workgroups share a row
+    uint32_t nparts;       // of the rows whose r and S are in `parts`
+    uint32_t k;
+    int teacher_dtype;
+    float c;               // log2(e) / T
+    double T;
+};
+
+// r and S of a set of columns: S = sum of 2^(l c - r).  r is finite or +infinity; -infinity: nothing in it (S = 0).
+struct Sum {
+    float r;
+    float s;
+};
+__device__ __forceinline__ Sum join(Sum a, Sum b)
+{
+    // (a NaN among the logits is in S, not in r)
+    const float r = fmaxf(a.r, b.r);
+    if (r == minus_infinity()) return {r, a.s + b.s};
+    return {r, a.s * exp2_fast(a.r - r) + b.s * exp2_fast(b.r - r)};
+}
+__device__ __forceinline__ Sum wave_join(Sum v)
+{
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const Sum o = {__shfl_xor(v.r, d, 64), __shfl_xor(v.s, d, 64)};
+        v = (threadIdx.x & d) == 0 ? join(v, o) : join(o, v);   // the same in every lane
+    }
+    return v;
+}
+
+// r and S over the chunks from..to of a row, of all threads (s: kWaves of them).
+template <int DT, bool ONCE>
+__device__ __forceinline__ Sum row_sum(const DistillArgs &a, uint64_t row, uint32_t from, uint32_t to, Sum *s)
+{
+    using V = Vec16<DT>;
+    constexpr int NE = V::NE;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t lane = threadIdx.x & 63;
+    Sum mine = {minus_infinity(), 0.0f};
+    for (uint32_t first = from + wave; first < to; first += kWaves * kAhead) {
+        u32x4 raw[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const uint32_t i = first + u * kWaves;
+            const Stretch t = a.rows.chunks[i < to ? i : from];
+            raw[u] = load_piece<DT, ONCE>(t.at + row * t.step, lane, i < to ? t.elems : 0);
+        }
+        float most = minus_infinity();
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            float f[NE];
+            V::unpack(raw[u], f);
+#pragma unroll
+            for (int e = 0; e < NE; ++e) most = fmaxf(most, f[e]);
+        }
+        const float r = fmaxf(mine.r, most * a.c);
+        const float ref = r == minus_infinity() ? 0.0f : r;   // (nothing yet: the terms are 2^-infinity)
+        float sum = mine.s * exp2_fast(mine.r - ref);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            float f[NE];
+            V::unpack(raw[u], f);
+#pragma unroll
+            for (int e = 0; e < NE; ++e) sum += exp2_fast(__builtin_fmaf(f[e], a.c, -ref));
+        }
+        mine = {r, sum};
+    }
+    mine = wave_join(mine);
+    if (lane == 0) s[wave] = mine;
+    __syncthreads();
+    Sum all = s[0];
+#pragma unroll
+    for (uint32_t w = 1; w < kWaves; ++w) all = join(all, s[w]);
+    __syncthreads();
+    return all;
+}
+
+__device__ __forceinline__ double teacher_logit(const DistillArgs &a, uint64_t at)
+{
+    if (a.teacher_dtype == HCCL_DATA_TYPE_FP32) return load_one<HCCL_DATA_TYPE_FP32>(a.teacher + at * 4, 0);
+    return a.teacher_dtype == HCCL_DATA_TYPE_FP16 ? load_one<HCCL_DATA_TYPE_FP16>(a.teacher + at * 2, 0)
+                                                  : load_one<HCCL_DATA_TYPE_BFP16>(a.teacher + at * 2, 0);
+}
+
+// Sum or largest of a double over all threads, in a fixed order.
+template <bool MAX>
+__device__ __forceinline__ double all_of(double v, double *s)
+{
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+        const double o = __shfl_xor(v, d, 64);
+        v = MAX ? (o > v || o != o ? o : v) : v + o;
+    }
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x / 64] = v;
+    __syncthreads();
+    v = s[0];
+#pragma unroll
+    for (uint32_t w = 1; w < kWaves; ++w) v = MAX ? (s[w] > v || s[w] != s[w] ? s[w] : v) : v + s[w];
+    __syncthreads();
+    return v;
+}
+
+// The teacher's entries of a row: thread t has the entries t, t + kThreads, ...
+struct Entries {
+    uint32_t at[kEach];    // column, or kFree: no entry, or one that names no column
+    double t[kEach];       // its logit / T
+    double p[kEach];
+    bool any;              // whether the row has one that is not minus infinity
+
+    __device__ __forceinline__ void read(const DistillArgs &a, uint64_t row)
+    {
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const uint32_t e = threadIdx.x + i * kThreads;
+            at[i] = kFree;
+            t[i] = -__builtin_inf();
+            if (e < a.k) {
+                const uint32_t c = static_cast<uint32_t>(a.indices[row * a.k + e]);
+                if (c < a.rows.vocab) {
+                    at[i] = c;
+                    t[i] = teacher_logit(a, row * a.k + e) / a.T;
+                }
+            }
+        }
+    }
+    // p of every entry, log p in t
+    __device__ __forceinline__ void normalise(double *s)
+    {
+        double most = t[0];
+#pragma unroll
+        for (uint32_t i = 1; i < kEach; ++i) most = t[i] > most || t[i] != t[i] ? t[i] : most;
+        most = all_of<true>(most, s);
+        any = !(most == -__builtin_inf());
+        double sum = 0.0;
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            p[i] = any && at[i] != kFree ? exp(t[i] - most) : 0.0;
+            sum += p[i];
+        }
+        sum = all_of<false>(sum, s);
+        const double log_sum = log(sum);
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            p[i] = any ? p[i] / sum : 0.0;
+            t[i] = t[i] - most - log_sum;
+        }
+    }
+};
+
+// Sums p over the entries that name the same column: where the entry's sum is.  Sums are of whole numbers, so that their order does not
+// show.  (p: of 2^62.)
+struct Together {
+    uint32_t *column;   // kSlots
+    unsigned long long *sum;
+    uint32_t mask;
+    __device__ __forceinline__ Together(uint32_t *c, unsigned long long *s, uint32_t k) : column(c), sum(s)
+    {
+        mask = 63;
+        while (mask + 1 < 2 * k) mask = 2 * mask + 1;
+        for (uint32_t i = threadIdx.x; i <= mask; i += kThreads) {
+            column[i] = kFree;
+            sum[i] = 0;
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ uint32_t add(uint32_t c, double p)
+    {
+        uint32_t i = (c * 2654435769u) >> 16 & mask;
+        for (;;) {   // (at most half of the slots are taken)
+            const uint32_t was = atomicCAS(&column[i], kFree, c);
+            if (was == kFree || was == c) break;
+            i = (i + 1) & mask;
+        }
+        atomicAdd(&sum[i], static_cast<unsigned long long>(p * 0x1p62));
+        return i;
+    }
+};
+
+template <int DT>
+__device__ __forceinline__ void store_piece(char *to, uint32_t lane, uint32_t elems, const float (&f)[Vec16<DT>::NE])
+{
+    using V = Vec16<DT>;
+    using S = typename V::S;
+    const uint32_t from = lane * V::NE;
+    if (from + V::NE <= elems) {
+        st16(to + lane * 16, V::pack(f));
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < V::NE; ++e) {
+        if (from + e < elems) reinterpret_cast<S *>(to)[from + e] = V::D::narrow(f[e]);
+    }
+}
+
+// Gradient of the chunks from..to of a row where p is 0: scale 2^(l c - r); or zeros.
+template <int DT, bool ZERO>
+__device__ __forceinline__ void row_gradient(const DistillArgs &a, uint64_t row, uint32_t from, uint32_t to, float r, float scale)
+{
+    using V = Vec16<DT>;
+    constexpr int NE = V::NE;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t lane = threadIdx.x & 63;
+    for (uint32_t first = from + wave; first < to; first += kWaves * kAhead) {
+        u32x4 raw[kAhead];
+        if constexpr (!ZERO) {
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const uint32_t i = first + u * kWaves;
+                const Stretch t = a.rows.chunks[i < to ? i : from];
+                raw[u] = load_piece<DT, true>(t.at + row * t.step, lane, i < to ? t.elems : 0);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const uint32_t i = first + u * kWaves;
+            if (i >= to) continue;
+            const Stretch t = a.rows.chunks[i];
+            float f[NE];
+            if constexpr (!ZERO) V::unpack(raw[u], f);
+#pragma unroll
+            for (int e = 0; e < NE; ++e) f[e] = ZERO ? 0.0f : scale * exp2_fast(__builtin_fmaf(f[e], a.c, -r));
+            store_piece<DT>(t.to + row * t.step, lane, t.elems, f);
+        }
+    }
+}
+
+struct DistillShared {
+    Sum sums[kWaves];
+    double reduce[kWaves];
+    uint32_t column[kSlots];
+    unsigned long long sum[kSlots];
+};
+
+// What is left of a row, or of its chunks from..to, once r and S are known.  student: the row's logits at the entries if not nullptr.
+template <int DT, bool LOSS, bool GRAD>
+__device__ __forceinline__ void finish(const DistillArgs &a, DistillShared &s, uint64_t row, uint32_t from, uint32_t to, Sum all, float w,
+                                       Entries &e, const float *student)
+{
+    using D = DTypeOf<DT>;
+    const Stretch *of[kEach];
+    float l[kEach];
+    // columns of these chunks
+    const uint32_t low = a.rows.chunks[from].first;
+    const uint32_t high = a.rows.chunks[to - 1].first + a.rows.chunks[to - 1].elems;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) {
+        of[i] = a.rows.ranks;
+        l[i] = 0.0f;
+        const bool mine = e.at[i] >= low && e.at[i] < high;
+        if (e.at[i] != kFree && (mine || student == nullptr)) {
+            of[i] = rank_of(a.rows, e.at[i]);
+            // (all are read before the first gradient is written: it may lie on the logits)
+            l[i] = student != nullptr ? student[threadIdx.x + i * kThreads] : load_one<DT>(of[i]->at + row * of[i]->step, e.at[i] - of[i]->first);
+        } else if (e.at[i] != kFree && LOSS) {
+            l[i] = student[threadIdx.x + i * kThreads];
+        }
+        if (!mine && GRAD && !LOSS) e.at[i] = kFree;   // (after the entries' weights are known)
+    }
+    const bool empty = all.r == minus_infinity() && all.s == 0.0f;   // every logit is minus infinity: q is 0
+    const double r = all.r;
+    const double log_s = log(static_cast<double>(all.s));
+    if constexpr (LOSS) {
+        double sum = 0.0;
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const double log_q = empty ? -__builtin_inf() : (static_cast<double>(l[i]) * a.c - r) * kLn2 - log_s;
+            if (!(e.p[i] == 0.0)) sum += e.p[i] * (e.t[i] - log_q);
+        }
+        sum = all_of<false>(sum, s.reduce);
+        if (threadIdx.x == 0) {
+            if (a.loss != nullptr) a.loss[row] = e.any ? static_cast<float>(w * a.T * a.T * sum) : 0.0f;
+            if (a.stats != nullptr) a.stats[row] = {all.r, all.s};
+        }
+    }
+    if constexpr (GRAD) {
+        const float scale = static_cast<float>(w * a.T);
+        __syncthreads();   // the entries' logits have been read
+        if (empty || !e.any) {
+            row_gradient<DT, true>(a, row, from, to, 0.0f, 0.0f);
+        } else {
+            row_gradient<DT, false>(a, row, from, to, all.r, scale / all.s);
+        }
+        if (!e.any) return;
+        Together together(s.column, s.sum, a.k);
+        uint32_t slot[kEach];
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) slot[i] = e.at[i] != kFree ? together.add(e.at[i], e.p[i]) : 0;
+        // the entries' gradients replace what the threads of their columns have written: that is in memory by then
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            if (e.at[i] < low || e.at[i] >= high) continue;
+            const double p = static_cast<double>(s.sum[slot[i]]) * 0x1p-62;
+            const double q = empty ? 0.0 : static_cast<double>(exp2_fast(__builtin_fmaf(l[i], a.c, -all.r))) / all.s;
+            reinterpret_cast<typename D::S *>(of[i]->to + row * of[i]->step)[e.at[i] - of[i]->first] =
+                D::narrow(static_cast<float>(scale * (q - p)));
+        }
+    }
+}
+
+// A row that counts nothing.
+template <int DT, bool LOSS, bool GRAD>
+__device__ __forceinline__ void nothing(const DistillArgs &a, uint64_t row, uint32_t from, uint32_t to)
+{
+    if (LOSS && threadIdx.x == 0) {
+        if (a.loss != nullptr) a.loss[row] = 0.0f;
+        if (a.stats != nullptr) a.stats[row] = {0.0f, 0.0f};
+    }
+    if (GRAD) row_gradient<DT, true>(a, row, from, to, 0.0f, 0.0f);
+}
+
+// A row per workgroup.
+template <int DT, bool GRAD>
+__global__ void __launch_bounds__(kThreads)
+k_distill_row(DistillArgs a)
+{
+    __shared__ DistillShared s;
+    const uint64_t row = blockIdx.x;
+    const uint32_t n = a.rows.nchunks;
+    const float w = a.weight != nullptr ? a.weight[row] : 1.0f;
+    if (w == 0.0f) {
+        nothing<DT, true, GRAD>(a, row, 0, n);
+        return;
+    }
+    Entries e;
+    e.read(a, row);
+    const Sum all = row_sum<DT, !GRAD>(a, row, 0, n, s.sums);
+    e.normalise(s.reduce);
+    finish<DT, true, GRAD>(a, s, row, 0, n, all, w, e, nullptr);
+}
+
+// The chunks of a part of a row, of which there are `parts`.
+struct Part {
+    uint64_t row;
+    uint32_t from;
+    uint32_t to;
+    uint32_t part;
+    __device__ __forceinline__ Part(const DistillArgs &a, uint32_t parts)
+    {
+        row = blockIdx.x / parts;
+        part = blockIdx.x % parts;
+        from = static_cast<uint32_t>(static_cast<uint64_t>(a.rows.nchunks) * part / parts);
+        to = static_cast<uint32_t>(static_cast<uint64_t>(a.rows.nchunks) * (part + 1) / parts);
+    }
+};
+
+// Several workgroups per row, two launches: r and S of every part, then what is left.
+template <int DT>
+__global__ void __launch_bounds__(kThreads)
+k_distill_sums(DistillArgs a)
+{
+    __shared__ Sum s[kWaves];
+    const Part p(a, a.nparts);
+    if (a.weight != nullptr && a.weight[p.row] == 0.0f) return;
+    if (p.part == 0) {   // the student's logits at the entries, before another workgroup writes their gradients there
+        for (uint32_t e = threadIdx.x; e < a.k; e += kThreads) {
+            const uint32_t c = static_cast<uint32_t>(a.indices[p.row * a.k + e]);
+            if (c >= a.rows.vocab) continue;
+            const Stretch *of = rank_of(a.rows, c);
+            a.student[p.row * a.k + e] = load_one<DT>(of->at + p.row * of->step, c - of->first);
+        }
+    }
+    const Sum all = row_sum<DT, false>(a, p.row, p.from, p.to, s);
+    if (threadIdx.x == 0) a.parts[p.row * a.nparts + p.part] = {all.r, all.s};
+}
+
+// grid: `parts` workgroups per row.  SAVED: r and S are those that the loss saved.
+template <int DT, bool SAVED, bool GRAD>
+__global__ void __launch_bounds__(kThreads)
+k_distill_parts(DistillArgs a, uint32_t parts)
+{
+    __shared__ DistillShared s;
+    const Part p(a, parts);
+    const float w = a.weight != nullptr ? a.weight[p.row] : 1.0f;
+    Sum all = {0.0f, 0.0f};
+    if (w != 0.0f) {
+        if constexpr (SAVED) {
+            const float2 v = a.stats[p.row];
+            all = {v.x, v.y};
+        } else {
+            const float2 *of = a.parts + p.row * a.nparts;
+            all = {of[0].x, of[0].y};
+            for (uint32_t i = 1; i < a.nparts; ++i) all = join(all, {of[i].x, of[i].y});
+        }
+    }
+    const bool none = w == 0.0f || (SAVED && all.r == 0.0f && all.s == 0.0f);   // (a row that counted has S >= 1/2, is empty or NaN)
+    if (!SAVED && p.part == 0) {
+        if (none) {
+            nothing<DT, true, GRAD>(a, p.row, p.from, p.to);
+            return;
+        }
+        Entries e;
+        e.read(a, p.row);
+        e.normalise(s.reduce);
+        finish<DT, true, GRAD>(a, s, p.row, p.from, p.to, all, w, e, a.student + p.row * a.k);
+    } else if constexpr (GRAD) {
+        if (none) {
+            nothing<DT, false, true>(a, p.row, p.from, p.to);
+            return;
+        }
+        Entries e;
+        e.read(a, p.row);
+        e.normalise(s.reduce);
+        finish<DT, false, true>(a, s, p.row, p.from, p.to, all, w, e, SAVED ? nullptr : a.student + p.row * a.k);
+    }
+}
+
+// Workgroups that share a row.
+uint32_t parts_of(uint32_t rows, uint32_t nchunks, uint32_t cus)
+{
+    const uint32_t fill = rows >= cus ? 1 : cus / rows;
+    return std::max(1u, std::min(fill, nchunks / (kWaves * 2)));
+}
+
+struct DistillWork : PlanWork {
+    DistillArgs args{};
+    Table table;
+    DeviceBlock scratch;   // parts, student
+    uint32_t parts = 1;
+    int dtype = 0;
+    bool saved = false;    // the gradient from what the loss saved
+    bool grad = false;
+
+    template <int DT>
+    void run(hipStream_t st) const
+    {
+        const uint32_t rows = args.rows.rows;
+        const dim3 grid(rows * parts), block(kThreads);
+        if (saved) {
+            HCCLX_LAUNCH((k_distill_parts<DT, true, true>), grid, block, 0, st, args, parts);
+        } else if (parts == 1) {
+            if (grad) {
+                HCCLX_LAUNCH((k_distill_row<DT, true>), grid, block, 0, st, args);
+            } else {
+                HCCLX_LAUNCH((k_distill_row<DT, false>), grid, block, 0, st, args);
+            }
+        } else {
+            HCCLX_LAUNCH((k_distill_sums<DT>), grid, block, 0, st, args);
+            if (grad) {
+                HCCLX_LAUNCH((k_distill_parts<DT, false, true>), grid, block, 0, st, args, parts);
+            } else {
+                HCCLX_LAUNCH((k_distill_parts<DT, false, false>), dim3(rows), block, 0, st, args, 1u);
+            }
+        }
+    }
+
+    int launch(const DeviceCtx *, hipStream_t st) const override
+    {
+        if (args.rows.rows == 0) return HCCL_SUCCESS;
+        if (dtype == HCCL_DATA_TYPE_FP32) {
+            run<HCCL_DATA_TYPE_FP32>(st);
+        } else if (dtype == HCCL_DATA_TYPE_FP16) {
+            run<HCCL_DATA_TYPE_FP16>(st);
+        } else {
+            run<HCCL_DATA_TYPE_BFP16>(st);
+        }
+        const hipError_t e = hipGetLastError();
+        return e == hipSuccess ? HCCL_SUCCESS : fail_hip(e, "distillation kernels");
+    }
+};
+
+// What a loss and a gradient have in common.
+int prepare(const hcclx_logits_t &l, const hcclx_teacher_t &t, const float *weight, void *const *dlogits, std::unique_ptr<DistillWork> *work)
+{
+    uint32_t vocab = 0;
+    int rc = logits::check(l, dlogits, &vocab);
+    if (rc != HCCL_SUCCESS) return rc;
+    if (t.k == 0 || t.k > HCCLX_TOP_MAX) return fail(HCCL_E_PARA, "k outside 1.." + std::to_string(HCCLX_TOP_MAX));
+    if (t.dtype != HCCL_DATA_TYPE_FP32 && t.dtype != HCCL_DATA_TYPE_FP16 && t.dtype != HCCL_DATA_TYPE_BFP16) {
+        return fail(HCCL_E_NOT_SUPPORT, "the teacher's logits are fp32, fp16 or bf16");
+    }
+    if (!(t.temperature >= 1e-6f && t.temperature <= 1e6f)) return fail(HCCL_E_PARA, "temperature outside 1e-6 .. 1e6");
+    const bool none = l.rows == 0;
+    if ((rc = check_array(t.logits, dtype_size(t.dtype), none, "teacher")) != HCCL_SUCCESS) return rc;
+    if ((rc = check_array(t.indices, 4, none, "indices")) != HCCL_SUCCESS) return rc;
+    if ((rc = check_array(weight, 4, true, "weight")) != HCCL_SUCCESS) return rc;
+    const uint64_t rows = l.rows;
+    if (dlogits != nullptr) {
+        if ((rc = check_gradients(l, dlogits)) != HCCL_SUCCESS) return rc;
+        if ((rc = check_apart(l, "dlogits", dlogits, "teacher", t.logits, rows * t.k * dtype_size(t.dtype))) != HCCL_SUCCESS) return rc;
+        if ((rc = check_apart(l, "dlogits", dlogits, "indices", t.indices, rows * t.k * 4)) != HCCL_SUCCESS) return rc;
+        if ((rc = check_apart(l, "dlogits", dlogits, "weight", weight, rows * 4)) != HCCL_SUCCESS) return rc;
+    }
+    auto w = std::make_unique<DistillWork>();
+    w->args.teacher = static_cast<const char *>(t.logits);
+    w->args.indices = t.indices;
+    w->args.weight = weight;
+    w->args.k = t.k;
+    w->args.teacher_dtype = t.dtype;
+    w->args.T = t.temperature;
+    w->args.c = static_cast<float>(1.4426950408889634074 / t.temperature);
+    w->args.rows.vocab = vocab;
+    w->dtype = l.dtype;
+    w->grad = dlogits != nullptr;
+    *work = std::move(w);
+    return HCCL_SUCCESS;
+}
+
+// Bytes of the rows' logits.
+uint64_t row_bytes(const hcclx_logits_t &l, uint32_t vocab) { return static_cast<uint64_t>(l.rows) * vocab * dtype_size(l.dtype); }
+
+int make_distill(const hcclx_distill_t &d, hcclx_plan_t **plan)
+{
+    std::unique_ptr<DistillWork> w;
+    int rc = prepare(d.logits, d.teacher, d.weight, d.dlogits, &w);
+    if (rc != HCCL_SUCCESS) return rc;
+    const hcclx_logits_t &l = d.logits;
+    const uint64_t rows = l.rows;
+    const uint64_t loss_bytes = rows * sizeof(float), stats_bytes = rows * sizeof(float2);
+    if ((rc = check_array(d.loss, 4, true, "loss")) != HCCL_SUCCESS) return rc;
+    if ((rc = check_array(d.stats, 8, true, "stats")) != HCCL_SUCCESS) return rc;
+    struct {
+        const char *what;
+        void *p;
+        uint64_t bytes;
+    } const out[2] = {{"loss", d.loss, loss_bytes}, {"stats", d.stats, stats_bytes}};
+    for (const auto &o : out) {
+        if ((rc = check_apart(l, "logits", l.logits, o.what, o.p, o.bytes)) != HCCL_SUCCESS) return rc;
+        if ((rc = check_apart(l, "dlogits", d.dlogits, o.what, o.p, o.bytes)) != HCCL_SUCCESS) return rc;
+        if ((rc = check_apart(o.what, o.p, o.bytes, "teacher", d.teacher.logits, rows * d.teacher.k * dtype_size(d.teacher.dtype))) != HCCL_SUCCESS) return rc;
+        if ((rc = check_apart(o.what, o.p, o.bytes, "indices", d.teacher.indices, rows * d.teacher.k * 4)) != HCCL_SUCCESS) return rc;
+        if ((rc = check_apart(o.what, o.p, o.bytes, "weight", d.weight, rows * 4)) != HCCL_SUCCESS) return rc;
+    }
+    if ((rc = check_apart("loss", d.loss, loss_bytes, "stats", d.stats, stats_bytes)) != HCCL_SUCCESS) return rc;
+    DeviceCtx *ctx = device_ctx();
+    if (!ctx) return HCCL_E_RUNTIME;
+    const uint32_t vocab = w->args.rows.vocab;
+    if ((rc = lay_out(l, d.dlogits, vocab, &w->table)) != HCCL_SUCCESS) return rc;
+    w->args.rows = w->table.rows;
+    w->args.loss = d.loss;
+    w->args.stats = reinterpret_cast<float2 *>(d.stats);
+    uint64_t held = w->table.bytes;
+    if (rows != 0) w->parts = parts_of(l.rows, w->args.rows.nchunks, static_cast<uint32_t>(ctx->num_cus));
+    if (w->parts > 1) {
+        w->args.nparts = w->parts;
+        const uint64_t sums = rows * w->parts * sizeof(float2);
+        const uint64_t bytes = sums + rows * d.teacher.k * sizeof(float);
+        if ((rc = w->scratch.get(bytes)) != HCCL_SUCCESS) return rc;
+        w->args.parts = reinterpret_cast<float2 *>(w->scratch.p);
+        w->args.student = reinterpret_cast<float *>(w->scratch.p + sums);
+        held += bytes;
+    }
+    const uint64_t algo = row_bytes(l, vocab) * (1 + w->grad);
+    return plan_of(ctx, std::move(w), algo, held, plan);
+}
+
+int make_distill_grad(const hcclx_distill_grad_t &d, hcclx_plan_t **plan)
+{
+    std::unique_ptr<DistillWork> w;
+    if (d.dlogits == nullptr) return fail(HCCL_E_PTR, "dlogits pointer array is null");
+    int rc = prepare(d.logits, d.teacher, d.weight, d.dlogits, &w);
+    if (rc != HCCL_SUCCESS) return rc;
+    const hcclx_logits_t &l = d.logits;
+    if ((rc = check_array(d.stats, 8, l.rows == 0, "stats")) != HCCL_SUCCESS) return rc;
+    if ((rc = check_apart(l, "dlogits", d.dlogits, "stats", d.stats, l.rows * sizeof(float2))) != HCCL_SUCCESS) return rc;
+    DeviceCtx *ctx = device_ctx();
+    if (!ctx) return HCCL_E_RUNTIME;
+    const uint32_t vocab = w->args.rows.vocab;
+    if ((rc = lay_out(l, d.dlogits, vocab, &w->table)) != HCCL_SUCCESS) return rc;
+    w->args.rows = w->table.rows;
+    w->args.stats = reinterpret_cast<float2 *>(const_cast<float *>(d.stats));
+    w->saved = true;
+    if (l.rows != 0) w->parts = parts_of(l.rows, w->args.rows.nchunks, static_cast<uint32_t>(ctx->num_cus));
+    const uint64_t held = w->table.bytes;
+    return plan_of(ctx, std::move(w), 2 * row_bytes(l, vocab), held, plan);
+}
+
+}  // namespace
+
+extern "C" {
+
+int hcclx_distill_plan_create(const hcclx_distill_t *distill, hcclx_plan_t **plan)
+{
+    if (plan == nullptr) return fail(HCCL_E_PTR, "plan is null");
+    *plan = nullptr;
+    if (distill == nullptr) return fail(HCCL_E_PTR, "distill is null");
+    return guarded([&] { return make_distill(*distill, plan); });
+}
+
+int hcclx_distill_grad_plan_create(const hcclx_distill_grad_t *distill, hcclx_plan_t **plan)
+{
+    if (plan == nullptr) return fail(HCCL_E_PTR, "plan is null");
+    *plan = nullptr;
+    if (distill == nullptr) return fail(HCCL_E_PTR, "distill is null");
+    return guarded([&] { return make_distill_grad(*distill, plan); });
+}
+
+}  // extern "C"

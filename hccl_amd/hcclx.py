@@ -345,3 +345,68 @@ class AdamWPlan(_OperatorPlan):
         rc = self._step(self._h, ctypes.byref(args), stream)
         if rc:
             check(rc)
+
+
+# ---- The output layer, its columns split over the ranks (hcclx_logits_t).  logits: lists of device addresses, one per rank; columns:
+# how many of them each rank has; strides: elements from one row of a rank to the next, without them its columns. -------------
+
+TOP_MAX = 1024       # entries of a list of largest logits
+
+
+def _logits(logits, columns, rows, dtype, strides):
+    n = len(logits)
+    for what, of in (("columns", columns), ("strides", strides)):
+        if of is not None and len(of) != n:
+            raise ValueError(f"{what} has {len(of)} numbers for {n} ranks")
+    return _lib.Logits(n, rows, int(dtype), _ptr_array(logits), (ctypes.c_uint32 * n)(*columns),
+                       None if strides is None else (ctypes.c_uint64 * n)(*strides))
+
+
+def _teacher(k, dtype, teacher, indices, temperature):
+    return _lib.Teacher(k, int(dtype), teacher or None, indices or None, temperature)
+
+
+class TopLogitsPlan(_OperatorPlan):
+    """The k largest logits of every row in descending order (values, of the logits' type), of equal ones the first, the numbers of
+    their columns (indices, 32-bit) and, where lse is given, log sum exp of the row (hcclx_top_logits_t)."""
+
+    def __init__(self, logits, columns, rows, k, dtype, values, indices, lse=0, strides=None):
+        a = _lib.TopLogits(_logits(logits, columns, rows, dtype, strides), k, values or None, indices or None, lse or None)
+        self._create("hcclx_top_logits_plan_create", ctypes.byref(a))
+
+
+class DistillPlan(_OperatorPlan):
+    """The loss of every row against a teacher's k largest logits (teacher, of teacher_dtype, and indices as TopLogitsPlan leaves
+    them): weight T^2 KL(softmax(teacher / T), softmax(logits / T)) (hcclx_distill_t).  weight: a float per row, 0 for masked ones, or
+    left out.  dlogits: a list of addresses, one per rank, for the gradients in the same launch; or stats, two floats per row, for
+    DistillGradPlan."""
+
+    def __init__(self, logits, columns, rows, teacher, indices, k, dtype, loss=0, teacher_dtype=None, temperature=1.0, weight=0, stats=0,
+                 dlogits=None, strides=None):
+        a = _lib.Distill(_logits(logits, columns, rows, dtype, strides),
+                         _teacher(k, dtype if teacher_dtype is None else teacher_dtype, teacher, indices, temperature), weight or None,
+                         loss or None, stats or None, _ranks("dlogits", dlogits, len(logits)))
+        self._create("hcclx_distill_plan_create", ctypes.byref(a))
+
+
+class DistillGradPlan(_OperatorPlan):
+    """The gradients of DistillPlan's loss from the stats that it left; weight is what a row's gradient is multiplied with
+    (hcclx_distill_grad_t)."""
+
+    def __init__(self, logits, columns, rows, teacher, indices, k, dtype, stats, dlogits, teacher_dtype=None, temperature=1.0, weight=0,
+                 strides=None):
+        a = _lib.DistillGrad(_logits(logits, columns, rows, dtype, strides),
+                             _teacher(k, dtype if teacher_dtype is None else teacher_dtype, teacher, indices, temperature), weight or None,
+                             stats or None, _ranks("dlogits", dlogits, len(logits)))
+        self._create("hcclx_distill_grad_plan_create", ctypes.byref(a))
+
+
+class SamplePlan(_OperatorPlan):
+    """A token for every row (tokens, 32-bit, -1 where there is nothing to draw) from the caller's random numbers (a float in [0, 1) per
+    row) under the row's temperature, top_k, top_p and min_p, device addresses of one number per row, each of which may be left out;
+    logprob: the logarithm of the probability with which the token was drawn (hcclx_sample_t)."""
+
+    def __init__(self, logits, columns, rows, dtype, random, tokens, temperature=0, top_k=0, top_p=0, min_p=0, logprob=0, strides=None):
+        a = _lib.Sample(_logits(logits, columns, rows, dtype, strides), temperature or None, top_k or None, top_p or None, min_p or None,
+                        random or None, tokens or None, logprob or None)
+        self._create("hcclx_sample_plan_create", ctypes.byref(a))

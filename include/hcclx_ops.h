@@ -1,12 +1,14 @@
 /*
  * hcclx_ops.h -- operators that stand next to the collectives of a training or serving step, for n virtual ranks whose
- * buffers live in one GPU's HBM: the norm in front of an MoE exchange, the experts' feed-forward block behind it, and the
- * AdamW step on a shard of reduced gradients.  No counterpart in the reference, whose callers bring these themselves.
+ * buffers live in one GPU's HBM: the norm in front of an MoE exchange, the experts' feed-forward block behind it, the
+ * AdamW step on a shard of reduced gradients, and the output layer whose columns the ranks share: its largest logits, a loss
+ * against a teacher's, and the draw of the next token.  No counterpart in the reference, whose callers bring these themselves.
  *
  * Every operator is a plan (hcclx.h): created once from shapes and device pointers, launched any number of times on any
  * stream, also into a HIP graph that is being captured, destroyed with hcclx_plan_destroy.  Arrays of pointers are host
  * arrays and are copied; what they point to has to outlive the plan.  A plan that has device memory of its own (the
- * experts' block, the norm's gradient) has one copy of it: two launches of such a plan must not overlap in time.
+ * experts' block, the norm's gradient, the operators of the output layer) has one copy of it: two launches of such a plan must not
+ * overlap in time.
  * Elements lie back to back; a buffer is aligned to its element where nothing else is said.  Refusals: HCCL_E_PTR for a
  * missing pointer, HCCL_E_PARA for a size or alignment, HCCL_E_NOT_SUPPORT for a type.
  */
@@ -182,6 +184,100 @@ int hcclx_adamw_plan_create(const hcclx_adamw_tensor_t *tensors, uint32_t ntenso
 /* Launches a plan made by hcclx_adamw_plan_create (hcclx_plan_launch refuses it: it has no step).  Captured into a HIP graph,
  * the values of *step are those of the capture. */
 int hcclx_adamw_step(const hcclx_plan_t *plan, const hcclx_adamw_step_t *step, void *stream);
+
+/* ---- Logits whose columns are split over the ranks --------------------------------------------------------------------
+ * Every rank holds some columns of all rows: row r of the output layer is row r of rank 0, of rank 1 and so on, side by side, and its
+ * columns are numbered through.  Types: fp32, fp16, bf16.  What lies between a rank's rows is neither read nor written, so ranks may
+ * hold columns of one matrix.  What the operators below write may not overlap what they read, or each other (HCCL_E_PARA), but where
+ * it is said. */
+#define HCCLX_LOGITS_MAX_COLUMNS (1u << 24) /* of all ranks together */
+#define HCCLX_TOP_MAX 1024                  /* entries of a list of largest logits */
+typedef struct {
+    uint32_t n;                 /* ranks, 1 .. 64 */
+    uint32_t rows;              /* up to 2^22 - 1, of very many columns fewer; 0: nothing to do */
+    int dtype;
+    const void *const *logits;  /* aligned to their element; not looked at where a rank has no columns */
+    const uint32_t *columns;    /* host: columns of each rank */
+    const uint64_t *row_stride; /* host: elements from one row of a rank to the next, below 2^32; NULL: its columns */
+} hcclx_logits_t;
+
+/* The k largest logits of every row, in descending order, of equal ones the first; NaN counts as -infinity, -0 as 0.
+ *     lse = log sum exp(logit) of the row, so that value - lse is the logarithm of a probability.  Summed in 32 bits, joined in 64. */
+typedef struct {
+    hcclx_logits_t logits;
+    uint32_t k;       /* 1 .. HCCLX_TOP_MAX, no more than there are columns */
+    void *values;     /* rows x k, of the logits' type */
+    int32_t *indices; /* rows x k: numbers of the columns */
+    float *lse;       /* rows; NULL: not wanted */
+} hcclx_top_logits_t;
+int hcclx_top_logits_plan_create(const hcclx_top_logits_t *top, hcclx_plan_t **plan);
+
+/* Distillation from a teacher's largest logits.  For every row, with T the temperature:
+ *     p = softmax(teacher / T) over the row's k entries,   q = softmax(logits / T) over all columns
+ *     loss    = weight T^2 sum over the entries of p (log p - log q[indices])
+ *     dlogits = weight T (q - the sum of p over the entries that name the column)
+ * Entries whose index is no column's (-1, say) are left out, and a row without any entry but those, or but logits of -infinity, has
+ * loss 0 and gradients 0; a column may be named by several entries.  A row of weight 0 (a masked token) is not read, whatever it holds:
+ * loss 0, gradients 0.  NaN and +infinity in a row that counts make its loss and gradients NaN.  The sum over the row's columns is held
+ * in 32 bits, what concerns the entries alone in 64.
+ *
+ * stats: two floats per row for hcclx_distill_grad_plan_create, 8-byte aligned.  dlogits: one pointer per rank, rows as far apart as
+ * the logits', and each may be that rank's logits.  A program that knows the weights before the loss gets the gradients in the same
+ * launch that way, without another pass over the logits. */
+typedef struct {
+    uint32_t k;             /* 1 .. HCCLX_TOP_MAX */
+    int dtype;              /* fp32, fp16 or bf16 */
+    const void *logits;     /* rows x k */
+    const int32_t *indices; /* rows x k */
+    float temperature;      /* 1e-6 .. 1e6 */
+} hcclx_teacher_t;
+typedef struct {
+    hcclx_logits_t logits;
+    hcclx_teacher_t teacher;
+    const float *weight;   /* rows; NULL: 1 */
+    float *loss;           /* rows; NULL: not wanted */
+    float *stats;          /* rows x 2; NULL: not wanted */
+    void *const *dlogits;  /* NULL: not wanted */
+} hcclx_distill_t;
+int hcclx_distill_plan_create(const hcclx_distill_t *distill, hcclx_plan_t **plan);
+
+/* Its gradient alone, from what the loss left in stats for the same logits and teacher.  weight: what the row's gradient is
+ * multiplied with, the loss's weight times what reaches the loss.  A row that the loss passed over for its weight of 0 has
+ * gradients 0 whatever its weight is here. */
+typedef struct {
+    hcclx_logits_t logits;
+    hcclx_teacher_t teacher;
+    const float *weight;
+    const float *stats;
+    void *const *dlogits;
+} hcclx_distill_grad_t;
+int hcclx_distill_grad_plan_create(const hcclx_distill_grad_t *distill, hcclx_plan_t **plan);
+
+/* Draws a token for every row.  With w = exp((logit - the row's largest) / temperature), what stays of a row is
+ *     of the order of hcclx_top_logits_t (descending, of equal logits the first)   the first top_k,
+ *     of those the shortest beginning whose w are top_p of theirs or more          (one token at least),
+ *     of those the ones with w >= min_p                                            (the first always);
+ * and the token is the first, in order of the columns, at which the running sum of the w that stay is more than random times all of
+ * them.  Settings are read on the device, one per row:
+ *     temperature  0, negative or NaN: the row's first largest logit; NULL: 1
+ *     top_k        0 or less, or as many as there are columns: all; NULL: all
+ *     top_p        1 or more, or NaN: all; 0 or less: one; NULL: all
+ *     min_p        0 or less, or NaN: all; more than 1 counts as 1; NULL: all
+ *     random       in [0, 1) from the caller's generator, so that a draw is a function of its arguments (outside: the nearest end; NaN: 0)
+ * NaN counts as -infinity and is never drawn; a row of nothing else gets token -1 and logprob -infinity.  Of +infinities one is drawn.
+ * w are computed in 64 bits and summed as multiples of 2^-38 or less (2^-45 for 131072 columns), so that sums do not go by their order;
+ * what is less than half of that is never drawn. */
+typedef struct {
+    hcclx_logits_t logits;
+    const float *temperature;
+    const int32_t *top_k;
+    const float *top_p;
+    const float *min_p;
+    const float *random;
+    int32_t *token;  /* rows */
+    float *logprob;  /* rows: log(w / the sum of what stays), of the token; NULL: not wanted */
+} hcclx_sample_t;
+int hcclx_sample_plan_create(const hcclx_sample_t *sample, hcclx_plan_t **plan);
 
 #ifdef __cplusplus
 }
