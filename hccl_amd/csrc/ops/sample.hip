@@ -23,9 +23,6 @@ namespace {
 
 constexpr uint32_t kGroup = 64;          // columns
 constexpr uint32_t kRunWaves = 4;        // of a workgroup of the first launch, a run each
-constexpr uint32_t kThreads = 512;       // of the second
-constexpr uint32_t kWaves = kThreads / 64;
-constexpr uint32_t kBins = 4 * kThreads;
 constexpr uint32_t kList = 2048;         // elements that are sorted at once
 constexpr uint32_t kMostGroups = HCCLX_TOP_MAX + HCCLX_TOP_MAX / 2 + 32;
 constexpr uint32_t kNucleus = 256;       // listed where no top_k bounds the list
@@ -188,6 +185,15 @@ k_logit_runs(SelectArgs a, uint32_t parts)
 
 typedef unsigned long long u64;
 
+// What a list holds of an element, so that larger ones come first in its order: number, ~place.  A place counts kChunk for each chunk in
+// front of the element's; places are in the order of the columns.
+template <int DT>
+__device__ __forceinline__ uint32_t column_of(const SelectArgs &a, u64 x)
+{
+    const uint32_t place = ~static_cast<uint32_t>(x);
+    return a.rows.chunks[place / kChunk<DT>].first + place % kChunk<DT>;
+}
+
 struct Range {
     uint32_t low;      // numbers (without their idle bits) that are left, both included
     uint32_t high;
@@ -197,46 +203,77 @@ struct Range {
     u64 weight_inside;
 };
 
+constexpr uint32_t kBins = 2048;
+constexpr uint32_t kMostChunks = 1024;   // of a row whose cut is found by levels
+constexpr uint32_t kMostWaves = 16;
 struct Shared {
     union {
         struct {
-            uint32_t count[kBins];
             u64 weight[kBins];
+            uint32_t count[kBins];
         } bins;
         struct {
-            u64 listed[kList];   // (number, ~column), in the order of the columns
+            u64 listed[kList];   // in the order of the columns
             u64 sorted[kList];
         } list;
         struct {
-            u64 weight[kThreads];   // of the wavefronts' pieces of a row
-            uint32_t equal[kThreads];
+            u64 weight[kMostChunks];   // of the chunks of a row
+            uint32_t equal[kMostChunks];
         } walk;
+        struct {
+            u64 listed[kList];
+            u64 sorted[kList];
+            u64 weight[kMostChunks];   // of the chunks: what is over the cut
+            uint32_t count[kBins];     // of the levels
+        } wide;
     };
+    double powers[64];   // 2^(-i / 64)
     uint32_t groups[kMostGroups];
-    u64 part[2][kWaves];
-    double part64[kWaves];
-    uint32_t part32[2][kWaves];
+    u64 part[2][kMostWaves];
+    double part64[kMostWaves];
+    uint32_t part32[2][kMostWaves];
     Range range;
     uint32_t word[4];
-    u64 wide;
+    u64 one;
 };
 
-// Sums over the threads before this one, and over all.  (Two barriers; s: kWaves.)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t v)
+{
+    return v + __builtin_amdgcn_update_dpp(0u, v, CTRL, ROWS, 0xf, false);
+}
+// Sums over the lanes up to this one.
+__device__ __forceinline__ uint32_t wave_sums(uint32_t v)
+{
+    v = dpp_add<0x111, 0xf>(v);   // row_shr 1, 2, 4, 8
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);   // lane 15 of rows 0 and 2 to the rows behind
+    return dpp_add<0x143, 0xc>(v);   // lane 31 to rows 2 and 3
+}
 template <typename T>
+__device__ __forceinline__ T wave_sums(T v)
+{
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const T o = __shfl_up(v, d, 64);
+        if ((threadIdx.x & 63) >= static_cast<uint32_t>(d)) v += o;
+    }
+    return v;
+}
+
+// Sums over the threads before this one, and over all.  (Two barriers; s: a word per wavefront.)
+template <int NT, typename T>
 __device__ __forceinline__ T before(T v, T *s, T *all)
 {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-    T sum = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const T o = __shfl_up(sum, d, 64);
-        if (lane >= static_cast<uint32_t>(d)) sum += o;
-    }
+    const T sum = wave_sums(v);
     if (lane == 63) s[wave] = sum;
     __syncthreads();
     T from = 0, whole = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < kWaves; ++w) {
+    for (uint32_t w = 0; w < NT / 64; ++w) {
         from += w < wave ? s[w] : T(0);
         whole += s[w];
     }
@@ -244,313 +281,412 @@ __device__ __forceinline__ T before(T v, T *s, T *all)
     *all = whole;
     return from + sum - v;
 }
-__device__ __forceinline__ uint32_t most_of(uint32_t v, uint32_t *s)
-{
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(v, d, 64)));
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x / 64] = v;
-    __syncthreads();
-    v = s[0];
-#pragma unroll
-    for (uint32_t w = 1; w < kWaves; ++w) v = max(v, s[w]);
-    __syncthreads();
-    return v;
-}
-
-// One round of the search: the numbers in the range are counted (and weighed) into kBins stretches of it; the range becomes the one in
-// which the running count (BY_WEIGHT: weight) from the top reaches what target() says, given the weight in the range.
-// each(f): f(number, weight) for every number that there is.
-template <bool BY_WEIGHT, typename Each, typename Target>
-__device__ __forceinline__ void narrow(Range &r, Shared &s, Each &&each, Target &&target)
-{
-    const uint32_t width = r.high - r.low;
-    const uint32_t shift = width < kBins ? 0 : 32 - __clz(width) - 11;   // kBins = 2^11
-    static_assert(kBins == 2048, "");
-    for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) {
-        s.bins.count[i] = 0;
-        if (BY_WEIGHT) s.bins.weight[i] = 0;
-    }
-    __syncthreads();
-    each([&](uint32_t n, auto &&weight) {
-        if (n < r.low || n > r.high) return;
-        const uint32_t bin = (n - r.low) >> shift;
-        atomicAdd(&s.bins.count[bin], 1u);
-        if constexpr (BY_WEIGHT) {
-            const u64 w = weight();
-            if (w != 0) atomicAdd(&s.bins.weight[bin], w);
-        }
-    });
-    __syncthreads();
-    // from the top: thread t has four stretches
-    constexpr uint32_t kMine = kBins / kThreads;
-    uint32_t count[kMine];
-    u64 weight[kMine];
-    uint32_t counts = 0;
-    u64 weights = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kMine; ++i) {
-        const uint32_t bin = kBins - 1 - (threadIdx.x * kMine + i);
-        counts += count[i] = s.bins.count[bin];
-        weights += weight[i] = BY_WEIGHT ? s.bins.weight[bin] : 0;
-    }
-    uint32_t all;
-    u64 whole = 0;
-    uint32_t c = before(counts, s.part32[0], &all);
-    u64 w = BY_WEIGHT ? before(weights, s.part[0], &whole) : 0;
-    const u64 there = BY_WEIGHT ? r.weight_above + whole : r.above + all;
-    const u64 asked = target(whole);
-    const u64 aim = asked < there ? asked : there;   // (all of it, where there is less)
-    c += r.above;
-    w += r.weight_above;
-#pragma unroll
-    for (uint32_t i = 0; i < kMine; ++i) {
-        const u64 at = BY_WEIGHT ? w : c;
-        const u64 add = BY_WEIGHT ? weight[i] : count[i];
-        if (at < aim && at + add >= aim) {
-            const uint32_t bin = kBins - 1 - (threadIdx.x * kMine + i);
-            const uint32_t low = r.low + (bin << shift);
-            const uint32_t last = low + ((1u << shift) - 1);
-            s.range = {low, last < r.high ? last : r.high, c, count[i], w, weight[i]};
-        }
-        c += count[i];
-        w += weight[i];
-    }
-    __syncthreads();
-    r = s.range;
-}
 
 // A lane's vector of a group: lanes kGroup / NE in a row hold one.
 struct Piece {
     u32x4 raw;
-    uint32_t first;   // column
+    uint32_t place;
     uint32_t have;    // elements that exist
 };
-template <int DT>
-__device__ __forceinline__ Piece piece_of(const SelectArgs &a, uint64_t row, uint32_t group, bool there)
-{
-    constexpr uint32_t NE = Vec16<DT>::NE;
-    constexpr uint32_t kPer = kChunk<DT> / kGroup;
-    const Stretch t = a.rows.chunks[there ? group / kPer : 0];
-    const uint32_t lane = group % kPer * (kGroup / NE) + threadIdx.x % (kGroup / NE);   // of the chunk
-    const uint32_t at = lane * NE;
-    Piece p;
-    p.have = !there || at >= t.elems ? 0 : t.elems - at < NE ? t.elems - at : NE;
-    p.first = t.first + at;
-    p.raw = load_piece<DT, false>(t.at + row * t.step, lane, there ? t.elems : 0);
-    return p;
-}
 
-template <int DT>
+template <int DT, int NT>
 struct Row {
     using V = Vec16<DT>;
     static constexpr uint32_t NE = V::NE;
     static constexpr uint32_t kPer = kChunk<DT> / kGroup;
-    static constexpr uint32_t kTurn = kThreads / (kGroup / NE);   // groups of a turn
+    static constexpr uint32_t kLanes = kGroup / NE;
+    static constexpr uint32_t kTurn = NT / kLanes;   // groups of a turn
+    static constexpr uint32_t kShift = kIdle<DT>;
+    static constexpr uint32_t kWaves = NT / 64;
+    static constexpr uint32_t kHeld = 4096 / NT;     // groups of a thread whose largest it holds, where all find room
+
     const SelectArgs &a;
+    Shared &s;
     const uint64_t row;
     const uint32_t *most;
     const uint32_t ngroups;
+    uint32_t held[kHeld];
     uint32_t top;      // the largest number of the row
     double top_value;
-    double c;          // log2(e) / T
+    double c;          // log2(e) / T, where weights are asked for
 
-    __device__ __forceinline__ Row(const SelectArgs &args, uint64_t r)
-        : a(args), row(r), most(args.most + r * args.rows.nchunks * kPer), ngroups(args.rows.nchunks * kPer)
+    __device__ __forceinline__ Row(const SelectArgs &args, Shared &shared)
+        : a(args), s(shared), row(blockIdx.x), most(args.most + row * args.rows.nchunks * kPer), ngroups(args.rows.nchunks * kPer)
     {
+        // (rows of the largest are whole vectors: a chunk has four or eight groups)
+        static_assert(kHeld % 4 == 0, "");
+        uint32_t t = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kHeld; i += 4) {
+            const uint32_t at = threadIdx.x * kHeld + i;
+            const u32x4 v = at < ngroups ? *reinterpret_cast<const u32x4 *>(most + at) : u32x4{kNone, kNone, kNone, kNone};
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                held[i + j] = v[j];
+                t = max(t, v[j]);
+            }
+        }
+        for (uint32_t i = NT * kHeld + threadIdx.x; i < ngroups; i += NT) t = max(t, most[i]);
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) t = max(t, static_cast<uint32_t>(__shfl_xor(t, d, 64)));
+        if ((threadIdx.x & 63) == 0) s.part32[1][threadIdx.x / 64] = t;
+        __syncthreads();
+        t = s.part32[1][0];
+#pragma unroll
+        for (uint32_t w = 1; w < kWaves; ++w) t = max(t, s.part32[1][w]);
+        top = t;
+        top_value = value_of(top);
     }
-    __device__ __forceinline__ double share(uint32_t number) const   // exp((l - most) / T)
-    {
-        return number == top ? 1.0 : exp2_exact((static_cast<double>(value_of(number)) - top_value) * c);
-    }
-    __device__ __forceinline__ u64 weight(uint32_t number) const { return static_cast<u64>(rint(ldexp(share(number), static_cast<int>(a.bits)))); }
 
-    // f(number, weight) of the elements of n groups: those of the list, or (nullptr) all
+    // f(group, its largest) of neighbouring groups per thread, in their order
     template <typename F>
-    __device__ __forceinline__ void each(const uint32_t *list, uint32_t n, F &&f) const
+    __device__ __forceinline__ void each_group(F &&f) const
+    {
+        if (ngroups <= NT * kHeld) {
+#pragma unroll
+            for (uint32_t i = 0; i < kHeld; ++i) f(threadIdx.x * kHeld + i, held[i]);   // (kNone behind the last)
+        } else {
+            const uint32_t each = (ngroups + NT - 1) / NT;
+            const uint32_t from = min(threadIdx.x * each, ngroups), to = min(from + each, ngroups);
+            for (uint32_t i = from; i < to; ++i) f(i, most[i]);
+        }
+    }
+
+    // Has to be called by all threads before the first share() or weight().
+    __device__ __forceinline__ void weigh_with(double per_logit)
+    {
+        c = per_logit;
+        if (threadIdx.x < 64) s.powers[threadIdx.x] = exp2_exact(threadIdx.x / -64.0);
+        __syncthreads();
+    }
+    // exp((l - most) / T), times 2^up: 2^(-y / 64) with y = n + f, |f| <= 1/2, is a power out of the table and five terms of the power series,
+    // the first omitted of which is below 2^-54.  What is below 2^-53 of the largest is 0, as is what is no number.
+    __device__ __forceinline__ double share(float l, int up) const
+    {
+        const double y = (top_value - l) * (64.0 * c);
+        if (number_of(l) == top) return ldexp(1.0, up);
+        if (!(y < 53.0 * 64.0)) return 0.0;
+        const double n = rint(y);
+        const double z = (y - n) * (-0.69314718055994530942 / 64);
+        double p = 1.0 / 120;
+        p = __builtin_fma(p, z, 1.0 / 24);
+        p = __builtin_fma(p, z, 1.0 / 6);
+        p = __builtin_fma(p, z, 0.5);
+        p = __builtin_fma(p, z, 1.0);
+        p = __builtin_fma(p, z, 1.0);
+        const int whole = static_cast<int>(n);
+        return ldexp(p * s.powers[whole & 63], up - (whole >> 6));
+    }
+    __device__ __forceinline__ double share(uint32_t number) const { return share(value_of(number), 0); }
+    // The same times 2^bits as a whole number: 2^52 added, the last place of a double is 1.
+    __device__ __forceinline__ u64 weight(float l) const
+    {
+        return static_cast<u64>(__double_as_longlong(share(l, static_cast<int>(a.bits)) + 0x1p52)) & ((u64(1) << 52) - 1);
+    }
+    __device__ __forceinline__ u64 weight(uint32_t number) const { return weight(value_of(number)); }
+
+    __device__ __forceinline__ Piece piece(uint32_t group, bool there) const
+    {
+        const uint32_t chunk = there ? group / kPer : 0;
+        const Stretch t = a.rows.chunks[chunk];
+        const uint32_t lane = group % kPer * kLanes + threadIdx.x % kLanes;   // of the chunk
+        const uint32_t at = lane * NE;
+        Piece p;
+        p.have = !there || at >= t.elems ? 0 : t.elems - at < NE ? t.elems - at : NE;
+        p.place = chunk * kChunk<DT> + at;
+        p.raw = load_piece<DT, false>(t.at + row * t.step, lane, there ? t.elems : 0);
+        return p;
+    }
+
+    // f(piece, values) of the vectors of n groups: those of the list, or (nullptr) all
+    template <typename F>
+    __device__ __forceinline__ void each_piece(const uint32_t *list, uint32_t n, F &&f) const
     {
         constexpr int kAhead = 4;
-        for (uint32_t g = threadIdx.x / (kGroup / NE); g < n; g += kTurn * kAhead) {
+        for (uint32_t g = threadIdx.x / kLanes; g < n; g += kTurn * kAhead) {
             Piece p[kAhead];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 const uint32_t i = g + u * kTurn;
-                p[u] = piece_of<DT>(a, row, i < n ? (list != nullptr ? list[i] : i) : 0, i < n);
+                p[u] = piece(i < n ? (list != nullptr ? list[i] : i) : 0, i < n);
             }
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 float v[NE];
                 V::unpack(p[u].raw, v);
-#pragma unroll
-                for (uint32_t e = 0; e < NE; ++e) {
-                    if (e >= p[u].have) continue;
-                    const uint32_t number = number_of(no_nan(v[e]));
-                    f(number >> kIdle<DT>, [&] { return weight(number); });
-                }
+                f(p[u], v);
             }
         }
     }
-};
-
-// The first `k` (kList at most) of the order, more if that is as easy: s.list.listed holds them in the order of their columns, the
-// number of them is returned.
-template <int DT>
-__device__ __forceinline__ uint32_t list_first(const Row<DT> &r, Shared &s, uint32_t k)
-{
-    constexpr uint32_t NE = Row<DT>::NE;
-    constexpr uint32_t kTurn = Row<DT>::kTurn;
-    constexpr uint32_t kShift = kIdle<DT>;
-    // Groups: those whose largest reaches `low`.
-    Range g = {0, r.top >> kShift, 0, r.ngroups, 0, 0};
-    uint32_t equal = 0xffffffffu;   // of the groups whose largest is low, the first so many
-    const uint32_t enough = max(k + k / 2 + 32, kList / kGroup);
-    if (g.inside > enough) {
-        g.low = kLeast >> kShift;
-        do {
-            narrow<false>(g, s, [&](auto &&f) {
-                for (uint32_t i = threadIdx.x; i < r.ngroups; i += kThreads) f(r.most[i] >> kShift, [] { return u64(0); });
-            }, [&](u64) { return u64(k); });
-        } while (g.above + g.inside > enough && g.low != g.high);
-        if (g.above + g.inside > enough) equal = k - g.above;
-    }
-    // listed in their order: a thread looks at neighbours
-    uint32_t ngroups = 0;
+    // f(number without idle bits, weight) of their elements
+    template <typename F>
+    __device__ __forceinline__ void each(const uint32_t *list, uint32_t n, F &&f) const
     {
-        const uint32_t each = (r.ngroups + kThreads - 1) / kThreads;
-        const uint32_t from = min(threadIdx.x * each, r.ngroups), to = min(from + each, r.ngroups);
-        uint32_t over = 0, same = 0;
-        for (uint32_t i = from; i < to; ++i) {
-            const uint32_t n = r.most[i];
-            const bool there = n != kNone;
-            over += there && n >> kShift > g.low;
-            same += there && n >> kShift == g.low;
-        }
-        u64 all;
-        const u64 packed = before(static_cast<u64>(over) << 32 | same, s.part[0], &all);
-        uint32_t same_before = static_cast<uint32_t>(packed);
-        uint32_t at = static_cast<uint32_t>(packed >> 32) + min(same_before, equal);
-        ngroups = static_cast<uint32_t>(all >> 32) + min(static_cast<uint32_t>(all), equal);
-        for (uint32_t i = from; i < to; ++i) {
-            const uint32_t n = r.most[i];
-            if (n == kNone || n >> kShift < g.low) continue;
-            if (n >> kShift == g.low && same_before++ >= equal) continue;
-            if (at < kMostGroups) s.groups[at] = i;
-            ++at;
-        }
-        ngroups = min(ngroups, kMostGroups);   // (never more: `enough` and k bound them)
-        __syncthreads();
+        each_piece(list, n, [&](const Piece &p, const float (&v)[NE]) {
+#pragma unroll
+            for (uint32_t e = 0; e < NE; ++e) {
+                if (e >= p.have) continue;
+                const uint32_t number = number_of(no_nan(v[e]));
+                f(number >> kShift, [&] { return weight(number); });
+            }
+        });
     }
-    // Elements: those that reach low, if they fit; else those of a narrower range.
-    Range e = {g.low, r.top >> kShift, 0, 0, 0, 0};
-    equal = 0xffffffffu;
-    for (;;) {
-        uint32_t n = 0, over_all = 0, same_all = 0;
-        for (uint32_t turn = 0; turn < ngroups && n <= kList; turn += kTurn) {
-            const uint32_t i = turn + threadIdx.x / (kGroup / NE);
-            const Piece p = piece_of<DT>(r.a, r.row, i < ngroups ? s.groups[i] : 0, i < ngroups);
+
+    // One round of the search: the numbers in the range are counted (and weighed) into kBins stretches of it; the range becomes the one in
+    // which the running count (BY_WEIGHT: weight) from the top reaches what target() says, given the weight in the range.
+    // all(f): f(number, weight) for every number that there is.
+    template <bool BY_WEIGHT, typename All, typename Target>
+    __device__ __forceinline__ void narrow(Range &r, All &&all, Target &&target) const
+    {
+        const uint32_t width = r.high - r.low;
+        const uint32_t shift = width < kBins ? 0 : 32 - __clz(width) - 11;
+        static_assert(kBins == 1u << 11, "");
+        for (uint32_t i = threadIdx.x; i < kBins; i += NT) {
+            s.bins.count[i] = 0;
+            if (BY_WEIGHT) s.bins.weight[i] = 0;
+        }
+        __syncthreads();
+        all([&](uint32_t n, auto &&weight) {
+            if (n < r.low || n > r.high) return;
+            const uint32_t bin = (n - r.low) >> shift;
+            atomicAdd(&s.bins.count[bin], 1u);
+            if constexpr (BY_WEIGHT) {
+                const u64 w = weight();
+                if (w != 0) atomicAdd(&s.bins.weight[bin], w);
+            }
+        });
+        __syncthreads();
+        // from the top: neighbours per thread
+        constexpr uint32_t kMine = kBins / NT;
+        uint32_t count[kMine];
+        u64 weight[kMine];
+        uint32_t counts = 0;
+        u64 weights = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kMine; ++i) {
+            const uint32_t bin = kBins - 1 - (threadIdx.x * kMine + i);
+            counts += count[i] = s.bins.count[bin];
+            weights += weight[i] = BY_WEIGHT ? s.bins.weight[bin] : 0;
+        }
+        uint32_t all_count;
+        u64 whole = 0;
+        uint32_t c = before<NT>(counts, s.part32[0], &all_count);
+        u64 w = BY_WEIGHT ? before<NT>(weights, s.part[0], &whole) : 0;
+        const u64 there = BY_WEIGHT ? r.weight_above + whole : r.above + all_count;
+        const u64 asked = target(whole);
+        const u64 aim = asked < there ? asked : there;   // (all of it, where there is less)
+        c += r.above;
+        w += r.weight_above;
+#pragma unroll
+        for (uint32_t i = 0; i < kMine; ++i) {
+            const u64 at = BY_WEIGHT ? w : c;
+            const u64 add = BY_WEIGHT ? weight[i] : count[i];
+            if (at < aim && at + add >= aim) {
+                const uint32_t bin = kBins - 1 - (threadIdx.x * kMine + i);
+                const uint32_t low = r.low + (bin << shift);
+                const uint32_t last = low + ((1u << shift) - 1);
+                s.range = {low, last < r.high ? last : r.high, c, count[i], w, weight[i]};
+            }
+            c += count[i];
+            w += weight[i];
+        }
+        __syncthreads();
+        r = s.range;
+    }
+
+    // Lists the elements of the groups s.groups[0 .. n) that reach `low`, of those that are it the first `equal`, in the order of the
+    // columns; returns how many there are, or a number over kList as soon as they are known to be more.
+    __device__ __forceinline__ uint32_t list(uint32_t n, uint32_t low, uint32_t equal) const
+    {
+        uint32_t listed = 0, over_all = 0, same_all = 0;
+        for (uint32_t turn = 0; turn < n && listed <= kList; turn += kTurn) {
+            const uint32_t i = turn + threadIdx.x / kLanes;
+            const Piece p = piece(i < n ? s.groups[i] : 0, i < n);
             float v[NE];
-            Row<DT>::V::unpack(p.raw, v);
+            V::unpack(p.raw, v);
             uint32_t number[NE];
             uint32_t over = 0, same = 0;
 #pragma unroll
             for (uint32_t j = 0; j < NE; ++j) {
                 number[j] = number_of(no_nan(v[j]));
-                over += j < p.have && number[j] >> kShift > e.low;
-                same += j < p.have && number[j] >> kShift == e.low;
+                over += j < p.have && number[j] >> kShift > low;
+                same += j < p.have && number[j] >> kShift == low;
             }
             uint32_t all;
-            const uint32_t packed = before(over << 16 | same, s.part32[0], &all);   // (of at most kThreads * NE elements)
+            const uint32_t packed = before<NT>(over << 16 | same, s.part32[0], &all);   // (of at most NT * NE elements)
             uint32_t same_before = same_all + (packed & 0xffffu);
             uint32_t at = over_all + (packed >> 16) + min(same_before, equal);
 #pragma unroll
             for (uint32_t j = 0; j < NE; ++j) {
-                if (j >= p.have || number[j] >> kShift < e.low) continue;
-                if (number[j] >> kShift == e.low && same_before++ >= equal) continue;
-                if (at < kList) s.list.listed[at] = static_cast<u64>(number[j]) << 32 | static_cast<uint32_t>(~(p.first + j));
+                if (j >= p.have || number[j] >> kShift < low) continue;
+                if (number[j] >> kShift == low && same_before++ >= equal) continue;
+                if (at < kList) s.list.listed[at] = static_cast<u64>(number[j]) << 32 | static_cast<uint32_t>(~(p.place + j));
                 ++at;
             }
             over_all += all >> 16;
             same_all += all & 0xffffu;
-            n = over_all + min(same_all, equal);
+            listed = over_all + min(same_all, equal);
         }
         __syncthreads();
-        if (n <= kList) return n;
-        e.above = e.inside = 0;
-        do {
-            narrow<false>(e, s, [&](auto &&f) { r.each(s.groups, ngroups, f); }, [&](u64) { return u64(k); });
-        } while (e.above + e.inside > kList && e.low != e.high);
-        if (e.above + e.inside > kList) equal = k - e.above;
-        e.high = r.top >> kShift;
+        return listed;
     }
-}
 
-// Sorts s.list.listed[0 .. n) into s.list.sorted, descending.
-__device__ __forceinline__ void sort_list(Shared &s, uint32_t n)
-{
-    uint32_t size = 64;
-    while (size < n) size *= 2;
-    for (uint32_t i = threadIdx.x; i < size; i += kThreads) s.list.sorted[i] = i < n ? s.list.listed[i] : 0;
-    __syncthreads();
-    for (uint32_t width = 2; width <= size; width *= 2) {
-        for (uint32_t step = width / 2; step >= 1; step /= 2) {
-            for (uint32_t t = threadIdx.x; t < size / 2; t += kThreads) {
-                const uint32_t i = (t & ~(step - 1)) * 2 + (t & (step - 1));
-                const u64 x = s.list.sorted[i], y = s.list.sorted[i + step];
-                const bool down = (i & width) == 0;
-                if ((x < y) == down) {
-                    s.list.sorted[i] = y;
-                    s.list.sorted[i + step] = x;
-                }
-            }
+    // The first `k` (HCCLX_TOP_MAX at most) of the order, and others if that is as easy: s.list.listed holds them in the order of their
+    // columns, the number of them is returned.  sure: how many of them are the first of the order.
+    __device__ __forceinline__ uint32_t list_first(uint32_t k, uint32_t *sure) const
+    {
+        // Groups: those whose largest reaches `low`.
+        constexpr uint32_t kNoEnd = 0xffffffffu;
+        Range g = {0, top >> kShift, 0, ngroups, 0, 0};
+        uint32_t equal = kNoEnd;   // of the groups whose largest is low, the first so many
+        const uint32_t enough = max(k + k / 2 + 32, kList / kGroup);
+        if (ngroups > enough) {
+            g.low = kLeast >> kShift;
+            do {
+                narrow<false>(g, [&](auto &&f) { each_group([&](uint32_t, uint32_t n) { f(n >> kShift, [] { return u64(0); }); }); },
+                              [&](u64) { return u64(k); });
+            } while (g.above + g.inside > enough && g.low != g.high);
+            if (g.above + g.inside > enough) equal = k - g.above;   // (groups left out may hold what is listed of the others)
+        }
+        uint32_t n = 0;
+        {
+            uint32_t over = 0, same = 0;
+            each_group([&](uint32_t, uint32_t m) {
+                over += m != kNone && m >> kShift > g.low;
+                same += m != kNone && m >> kShift == g.low;
+            });
+            // (over: at most `enough`; both fit)
+            static_assert(kMostGroups < 4096 && HCCLX_LOGITS_MAX_COLUMNS / kGroup + 8 * kMostRanks < 1 << 20, "");
+            uint32_t all;
+            const uint32_t packed = before<NT>(over << 20 | same, s.part32[0], &all);
+            uint32_t same_before = packed & 0xfffffu;
+            uint32_t at = (packed >> 20) + min(same_before, equal);
+            n = min((all >> 20) + min(all & 0xfffffu, equal), kMostGroups);   // (never more: `enough` and k bound them)
+            each_group([&](uint32_t i, uint32_t m) {
+                if (m == kNone || m >> kShift < g.low) return;
+                if (m >> kShift == g.low && same_before++ >= equal) return;
+                if (at < kMostGroups) s.groups[at] = i;
+                ++at;
+            });
             __syncthreads();
         }
+        // Elements that reach what all groups reach, if they fit.
+        if (g.low != 0 || n * kGroup <= kList) {
+            const uint32_t listed = list(n, g.low, kNoEnd);
+            *sure = equal == kNoEnd ? listed : k;
+            if (listed <= kList) return listed;
+        }
+        // The same again with the vectors of the groups in the groups' place: where there are k, elements reach the k-th vector's largest.
+        Range e = {g.low, top >> kShift, 0, 0, 0, 0};
+        do {
+            narrow<false>(e, [&](auto &&f) {
+                each_piece(s.groups, n, [&](const Piece &p, const float (&v)[NE]) {
+                    if (p.have == 0) return;
+                    float m = minus_infinity();
+#pragma unroll
+                    for (uint32_t j = 0; j < NE; ++j) m = fmaxf(m, v[j]);
+                    f(number_of(m) >> kShift, [] { return u64(0); });
+                });
+            }, [&](u64) { return u64(k); });
+        } while (e.above + e.inside > k + k / 2 + 32 && e.low != e.high);
+        const bool vectors = e.above + e.inside >= k;
+        if (vectors) {
+            const uint32_t listed = list(n, e.low, kNoEnd);
+            *sure = equal == kNoEnd ? listed : k;
+            if (listed <= kList) return listed;
+        }
+        // Elements themselves.
+        e = {vectors ? e.low : g.low, top >> kShift, 0, 0, 0, 0};
+        do {
+            narrow<false>(e, [&](auto &&f) { each(s.groups, n, f); }, [&](u64) { return u64(k); });
+        } while (e.above + e.inside > kList && e.low != e.high);
+        const uint32_t listed = list(n, e.low, e.above + e.inside > kList ? k - e.above : kNoEnd);
+        *sure = equal == kNoEnd ? listed : k;
+        return listed;
     }
-}
 
-// The row's largest number.
-template <int DT>
-__device__ __forceinline__ uint32_t top_of(const Row<DT> &r, Shared &s)
-{
-    uint32_t top = 0;
-    for (uint32_t i = threadIdx.x; i < r.ngroups; i += kThreads) top = max(top, r.most[i]);
-    return most_of(top, s.part32[0]);
-}
+    // Sorts s.list.listed[0 .. n) into s.list.sorted, descending.
+    __device__ __forceinline__ void sort(uint32_t n) const
+    {
+        uint32_t size = 64;
+        while (size < n) size *= 2;
+        const uint32_t t = threadIdx.x;
+        if (size <= NT) {   // an element per thread; a wavefront's own steps need no barrier
+            u64 x = t < n ? s.list.listed[t] : 0;
+            for (uint32_t width = 2; width <= size; width *= 2) {
+                for (uint32_t step = width / 2; step >= 1; step /= 2) {
+                    u64 y;
+                    if (step >= 64) {
+                        s.list.sorted[t] = x;
+                        __syncthreads();
+                        y = s.list.sorted[t ^ step];
+                        __syncthreads();
+                    } else {
+                        y = __shfl_xor(x, static_cast<int>(step), 64);
+                    }
+                    const bool larger = ((t & step) == 0) == ((t & width) == 0);
+                    x = (x > y) == larger ? x : y;
+                }
+            }
+            s.list.sorted[t] = x;
+            __syncthreads();
+            return;
+        }
+        for (uint32_t i = t; i < size; i += NT) s.list.sorted[i] = i < n ? s.list.listed[i] : 0;
+        __syncthreads();
+        for (uint32_t width = 2; width <= size; width *= 2) {
+            for (uint32_t step = width / 2; step >= 1; step /= 2) {
+                for (uint32_t k = t; k < size / 2; k += NT) {
+                    const uint32_t i = (k & ~(step - 1)) * 2 + (k & (step - 1));
+                    const u64 x = s.list.sorted[i], y = s.list.sorted[i + step];
+                    const bool down = (i & width) == 0;
+                    if ((x < y) == down) {
+                        s.list.sorted[i] = y;
+                        s.list.sorted[i + step] = x;
+                    }
+                }
+                __syncthreads();
+            }
+        }
+    }
 
-template <int DT>
-__global__ void __launch_bounds__(kThreads)
+    // whole: the sum of what could have been drawn, of exp((l - most) / T).
+    __device__ __forceinline__ void write_choice(uint32_t column, uint32_t number, double whole) const
+    {
+        a.choice.token[row] = static_cast<int32_t>(column);
+        if (a.choice.logprob != nullptr) {
+            const double x = number == top ? 0.0 : (static_cast<double>(value_of(number)) - top_value) * c * 0.69314718055994530942;
+            a.choice.logprob[row] = static_cast<float>(x - log(whole));
+        }
+    }
+    __device__ __forceinline__ double run_sum(uint32_t i) const   // of a run, of exp((l - most) / T)
+    {
+        const Run run = a.runs[row * a.nruns + i];
+        return run.most == static_cast<float>(top_value) ? run.sum : run.sum * exp2_exact((static_cast<double>(run.most) - top_value) * c);
+    }
+};
+
+template <int DT, int NT>
+__global__ void __launch_bounds__(NT)
 k_top_logits(SelectArgs a)
 {
     using D = DTypeOf<DT>;
     __shared__ Shared s;
-    Row<DT> r(a, blockIdx.x);
-    r.top = top_of(r, s);
-    const uint32_t n = list_first(r, s, a.k);
-    sort_list(s, n);
-    for (uint32_t i = threadIdx.x; i < a.k; i += kThreads) {
+    Row<DT, NT> r(a, s);
+    uint32_t sure;
+    r.sort(r.list_first(a.k, &sure));
+    for (uint32_t i = threadIdx.x; i < a.k; i += NT) {
         const u64 x = s.list.sorted[i];
         reinterpret_cast<typename D::S *>(a.values)[r.row * a.k + i] = D::narrow(value_of(static_cast<uint32_t>(x >> 32)));
-        a.indices[r.row * a.k + i] = static_cast<int32_t>(~static_cast<uint32_t>(x));
+        a.indices[r.row * a.k + i] = static_cast<int32_t>(column_of<DT>(a, x));
     }
     if (a.lse != nullptr) {
-        const float most = value_of(r.top);
+        r.c = 1.4426950408889634074;   // (of runs alone)
         double sum = 0.0;
-        for (uint32_t i = threadIdx.x; i < a.nruns; i += kThreads) {
-            const Run run = a.runs[r.row * a.nruns + i];
-            sum += run.most == most ? run.sum : run.sum * exp2_exact((static_cast<double>(run.most) - most) * 1.4426950408889634074);
-        }
+        for (uint32_t i = threadIdx.x; i < a.nruns; i += NT) sum += r.run_sum(i);
         double all;
-        (void)before(sum, s.part64, &all);
-        if (threadIdx.x == 0) a.lse[r.row] = static_cast<float>(most + log(all));
-    }
-}
-
-// whole: the sum of what could have been drawn, of exp((l - most) / T).
-template <int DT>
-__device__ __forceinline__ void write_choice(const SelectArgs &a, const Row<DT> &r, uint32_t column, uint32_t number, double whole)
-{
-    a.choice.token[r.row] = static_cast<int32_t>(column);
-    if (a.choice.logprob != nullptr) {
-        const double x = number == r.top ? 0.0 : (static_cast<double>(value_of(number)) - r.top_value) * r.c * 0.69314718055994530942;
-        a.choice.logprob[r.row] = static_cast<float>(x - log(whole));
+        (void)before<NT>(sum, s.part64, &all);
+        if (threadIdx.x == 0) a.lse[r.row] = static_cast<float>(r.top_value + log(all));
     }
 }
 
@@ -561,6 +697,8 @@ __device__ __forceinline__ u64 aim_of(float u, u64 whole)
     if (!(t > 0.0)) return 0;
     return t >= static_cast<double>(whole) ? whole - 1 : min(static_cast<u64>(t), whole - 1);
 }
+// What of `whole` top_p asks for.
+__device__ __forceinline__ u64 part_of(double p, double whole) { return p > 0.0 ? static_cast<u64>(ceil(p * whole)) : 0; }
 
 // What stays of a row that no list holds: numbers over `cut`, the first `equal` of those that are it, and of them all what is `least`
 // times as probable as the first.
@@ -570,14 +708,14 @@ struct Kept {
     double least;
 };
 
-// Draws among them: the wavefronts' pieces of the row are weighed, kWalk turns at a time, and the one that the aim lies in is gone
+// Draws among them: the wavefronts' pieces of the row are weighed, NT of them at a time, and the one that the aim lies in is gone
 // through.  A first walk finds the whole.
-template <int DT>
-__device__ __forceinline__ void draw_kept(const SelectArgs &a, const Row<DT> &r, Shared &s, const Kept &kept, float u)
+template <int DT, int NT>
+__device__ __forceinline__ void draw_kept(const SelectArgs &a, const Row<DT, NT> &r, Shared &s, const Kept &kept, float u)
 {
-    constexpr uint32_t NE = Row<DT>::NE;
+    using R = Row<DT, NT>;
+    constexpr uint32_t NE = R::NE;
     constexpr uint32_t kShift = kIdle<DT>;
-    constexpr uint32_t kWalk = kThreads / kWaves;   // turns
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
     const bool drop = kept.least > 0.0;
     auto weight = [&](uint32_t number) {
@@ -588,17 +726,17 @@ __device__ __forceinline__ void draw_kept(const SelectArgs &a, const Row<DT> &r,
     for (int find = 0; find < 2; ++find) {
         u64 weight_before = 0;
         uint32_t equal_before = 0;
-        for (uint32_t first = 0; first < a.rows.nchunks; first += kThreads) {   // kWalk turns of kWaves chunks
+        for (uint32_t first = 0; first < a.rows.nchunks; first += NT) {
             u64 equal_weight = 0;   // of one element at the cut
-            for (uint32_t turn = 0; turn < kWalk; ++turn) {
-                const uint32_t chunk = first + turn * kWaves + wave;
+            for (uint32_t turn = 0; turn < NT / R::kWaves; ++turn) {
+                const uint32_t chunk = first + turn * R::kWaves + wave;
                 u64 sum = 0;
                 uint32_t same = 0;
                 if (chunk < a.rows.nchunks) {
                     const Stretch t = a.rows.chunks[chunk];
                     const u32x4 raw = load_piece<DT, false>(t.at + r.row * t.step, lane, t.elems);
                     float v[NE];
-                    Row<DT>::V::unpack(raw, v);
+                    R::V::unpack(raw, v);
 #pragma unroll
                     for (uint32_t e = 0; e < NE; ++e) {
                         const uint32_t number = number_of(no_nan(v[e]));
@@ -617,21 +755,21 @@ __device__ __forceinline__ void draw_kept(const SelectArgs &a, const Row<DT> &r,
                     same += __shfl_xor(same, d, 64);
                 }
                 if (lane == 0) {
-                    s.walk.weight[turn * kWaves + wave] = sum;
-                    s.walk.equal[turn * kWaves + wave] = same;
+                    s.walk.weight[turn * R::kWaves + wave] = sum;
+                    s.walk.equal[turn * R::kWaves + wave] = same;
                 }
             }
-            if (equal_weight != 0) s.wide = equal_weight;   // (all that do write the same)
+            if (equal_weight != 0) s.one = equal_weight;   // (all that do write the same)
             __syncthreads();
-            const u64 one = s.wide;
+            const u64 one = s.one;
             const u64 sum = s.walk.weight[threadIdx.x];
             const uint32_t same = s.walk.equal[threadIdx.x];
             uint32_t same_all;
-            const uint32_t same_before = equal_before + before(same, s.part32[0], &same_all);
+            const uint32_t same_before = equal_before + before<NT>(same, s.part32[0], &same_all);
             const uint32_t taken = min(same_before + same, kept.equal) - min(same_before, kept.equal);
             u64 sum_all;
             const u64 mine = sum + taken * one;
-            const u64 at = weight_before + before(mine, s.part[0], &sum_all);
+            const u64 at = weight_before + before<NT>(mine, s.part[0], &sum_all);
             if (find == 1 && aim >= at && aim - at < mine) {
                 s.word[0] = first + threadIdx.x;   // the chunk
                 s.word[1] = same_before;
@@ -651,17 +789,11 @@ __device__ __forceinline__ void draw_kept(const SelectArgs &a, const Row<DT> &r,
     const Stretch t = a.rows.chunks[s.word[0]];
     const u32x4 raw = load_piece<DT, false>(t.at + r.row * t.step, lane, t.elems);
     float v[NE];
-    Row<DT>::V::unpack(raw, v);
+    R::V::unpack(raw, v);
     uint32_t same = 0;
 #pragma unroll
     for (uint32_t e = 0; e < NE; ++e) same += lane * NE + e < t.elems && number_of(no_nan(v[e])) >> kShift == kept.cut;
-    uint32_t same_before = same;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(same_before, d, 64);
-        if (lane >= static_cast<uint32_t>(d)) same_before += o;
-    }
-    same_before += s.word[1] - same;
+    uint32_t same_before = wave_sums(same) + s.word[1] - same;
     u64 w[NE];
     u64 sum = 0;
 #pragma unroll
@@ -671,47 +803,37 @@ __device__ __forceinline__ void draw_kept(const SelectArgs &a, const Row<DT> &r,
         if (in && number >> kShift == kept.cut) in = same_before++ < kept.equal;
         sum += w[e] = in ? weight(number) : 0;
     }
-    u64 at = sum;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const u64 o = __shfl_up(at, d, 64);
-        if (lane >= static_cast<uint32_t>(d)) at += o;
-    }
-    at += s.part[1][0] - sum;
+    u64 at = wave_sums(sum) + s.part[1][0] - sum;
 #pragma unroll
     for (uint32_t e = 0; e < NE; ++e) {
         if (aim >= at && aim - at < w[e]) {
-            write_choice(a, r, t.first + lane * NE + e, number_of(no_nan(v[e])), ldexp(static_cast<double>(whole), -static_cast<int>(a.bits)));
+            r.write_choice(t.first + lane * NE + e, number_of(no_nan(v[e])), ldexp(static_cast<double>(whole), -static_cast<int>(a.bits)));
         }
         at += w[e];
     }
 }
 
 // No filter: the run in which the running sum passes u x the whole, then the element.
-template <int DT>
-__device__ __forceinline__ void draw_all(const SelectArgs &a, const Row<DT> &r, Shared &s, float u)
+template <int DT, int NT>
+__device__ __forceinline__ void draw_all(const SelectArgs &a, const Row<DT, NT> &r, Shared &s, float u)
 {
-    constexpr uint32_t NE = Row<DT>::NE;
+    using R = Row<DT, NT>;
+    constexpr uint32_t NE = R::NE;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-    const Run *runs = a.runs + r.row * a.nruns;
-    const uint32_t each = (a.nruns + kThreads - 1) / kThreads;
+    const uint32_t each = (a.nruns + NT - 1) / NT;
     const uint32_t from = min(threadIdx.x * each, a.nruns), to = min(from + each, a.nruns);
-    auto sum_of = [&](uint32_t i) {
-        const Run run = runs[i];
-        return run.most == static_cast<float>(r.top_value) ? run.sum : run.sum * exp2_exact((static_cast<double>(run.most) - r.top_value) * r.c);
-    };
     double mine = 0.0;
-    for (uint32_t i = from; i < to; ++i) mine += sum_of(i);
+    for (uint32_t i = from; i < to; ++i) mine += r.run_sum(i);
     double whole;
-    const double begin = before(mine, s.part64, &whole);
+    const double begin = before<NT>(mine, s.part64, &whole);
     double at = begin;
     double aim = static_cast<double>(u) * whole;
     if (!(aim > 0.0)) aim = 0.0;
     // the last run that begins at or before the aim and has anything (sums are rounded: the aim may lie behind all)
-    if (threadIdx.x == 0) s.word[0] = 0;
+    if (threadIdx.x == 0) s.word[0] = s.word[1] = 0;
     __syncthreads();
     for (uint32_t i = from; i < to; ++i) {
-        const double w = sum_of(i);
+        const double w = r.run_sum(i);
         if (w > 0.0 && at <= aim) atomicMax(&s.word[0], i + 1);
         at += w;
     }
@@ -719,7 +841,7 @@ __device__ __forceinline__ void draw_all(const SelectArgs &a, const Row<DT> &r, 
     const uint32_t run = s.word[0] - 1;
     if (run >= from && run < to) {
         at = begin;
-        for (uint32_t i = from; i < run; ++i) at += sum_of(i);
+        for (uint32_t i = from; i < run; ++i) at += r.run_sum(i);
         s.part64[0] = at;
     }
     __syncthreads();
@@ -732,7 +854,7 @@ __device__ __forceinline__ void draw_all(const SelectArgs &a, const Row<DT> &r, 
     const uint32_t elems = there ? t.elems : 0;
     const u32x4 raw = load_piece<DT, false>(t.at + r.row * t.step, lane, elems);
     float v[NE];
-    Row<DT>::V::unpack(raw, v);
+    R::V::unpack(raw, v);
     double w[NE];
     double sum = 0.0;
 #pragma unroll
@@ -741,9 +863,7 @@ __device__ __forceinline__ void draw_all(const SelectArgs &a, const Row<DT> &r, 
         sum += w[e];
     }
     double all;
-    at += before(sum, s.part64, &all);
-    if (threadIdx.x == 0) s.word[1] = 0;
-    __syncthreads();
+    at += before<NT>(sum, s.part64, &all);
 #pragma unroll
     for (uint32_t e = 0; e < NE; ++e) {
         if (w[e] > 0.0 && at <= aim) atomicMax(&s.word[1], threadIdx.x * NE + e + 1);
@@ -754,23 +874,291 @@ __device__ __forceinline__ void draw_all(const SelectArgs &a, const Row<DT> &r, 
     if (place / NE != threadIdx.x) return;
 #pragma unroll
     for (uint32_t e = 0; e < NE; ++e) {
-        if (place % NE == e) write_choice(a, r, t.first + lane * NE + e, number_of(no_nan(v[e])), whole);
+        if (place % NE == e) r.write_choice(t.first + lane * NE + e, number_of(no_nan(v[e])), whole);
     }
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kThreads)
+// What stays of a row is more than a list holds: elements are counted by levels, 64 to a power of two of their weight; the level that
+// the cut lies in is found by the counts, for top_k exactly, for top_p with a level's middle for its weights, which is wrong by a level now
+// and then; the elements over that level are weighed chunk by chunk, and those in it are listed and sorted.  That says where the cut is, or
+// in which direction to look for it.  sure: so many first elements are in s.list.sorted.
+// Returns false, and nothing is drawn, where a level holds more than a list, or the cut is behind the last.
+template <int DT, int NT>
+__device__ __forceinline__ bool draw_wide(const SelectArgs &a, const Row<DT, NT> &r, Shared &s, const RowChoice &choice, float u, u64 p_of_whole,
+                                          uint32_t sure)
+{
+    using R = Row<DT, NT>;
+    constexpr uint32_t NE = R::NE;
+    constexpr uint32_t kMine = kBins / NT;
+    constexpr uint32_t kListed = kList / NT;
+    constexpr uint32_t kChunks = kMostChunks / NT;
+    constexpr uint32_t kNoLevel = 0xffffffffu;
+    constexpr int kAhead = 4;
+    constexpr int kRounds = 8;
+    if (a.rows.nchunks > kMostChunks) return false;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const float top = static_cast<float>(r.top_value);
+    const float scale = static_cast<float>(64.0 * r.c);
+    auto level_of = [&](float l) {   // (NaN: the distance of infinities, or of minus infinity times 0)
+        const uint32_t v = static_cast<uint32_t>(fminf((top - l) * scale, static_cast<float>(kBins - 1)));
+        return number_of(l) == r.top ? 0 : v;
+    };
+    const double unit = ldexp(1.0, -static_cast<int>(a.bits));
+    const bool by_level = choice.by_k || choice.by_p;
+    bool only_least = !by_level;   // of all filters min_p alone
+    uint32_t level = kNoLevel;     // the cut's
+    uint32_t level_count = 0, level_over = 0;   // elements in it, and over it
+    double level_weight = 0.0, weight_over = 0.0;   // by the middles
+    uint32_t counts[kMine];
+    uint32_t over_mine = 0;
+    double weight_mine = 0.0;
+    auto middles = [&](uint32_t l, uint32_t count) { return count * ldexp(s.powers[l & 63] * 0.99459942348363317565, -static_cast<int>(l >> 6)); };
+    // Of the levels low .. high - 1 the first at which the running count reaches top_k, or the running weight and `more` reaches aim; or else the
+    // last that holds anything.
+    auto find_level = [&](bool by_count, double more, double aim, uint32_t low, uint32_t high) {
+        if (threadIdx.x == 0) {
+            s.word[0] = kNoLevel;
+            s.word[1] = 0;
+        }
+        __syncthreads();
+        uint32_t n = over_mine;
+        double w = weight_mine;
+#pragma unroll
+        for (uint32_t i = 0; i < kMine; ++i) {
+            const uint32_t l = threadIdx.x * kMine + i;
+            n += counts[i];
+            w += middles(l, counts[i]);
+            if (l < low || l >= high || counts[i] == 0) continue;
+            if (by_count ? n >= choice.k : w + more >= aim) atomicMin(&s.word[0], l);
+            atomicMax(&s.word[1], l + 1);
+        }
+        __syncthreads();
+        level = min(s.word[0], s.word[1] - 1);   // (none: kNoLevel)
+        __syncthreads();
+        if (level == kNoLevel) return;
+        n = over_mine;
+        w = weight_mine;
+#pragma unroll
+        for (uint32_t i = 0; i < kMine; ++i) {
+            const uint32_t l = threadIdx.x * kMine + i;
+            if (l == level) {
+                s.word[0] = counts[i];
+                s.word[1] = n;
+                s.part64[0] = middles(l, counts[i]);
+                s.part64[1] = w;
+            }
+            n += counts[i];
+            w += middles(l, counts[i]);
+        }
+        __syncthreads();
+        level_count = s.word[0];
+        level_over = s.word[1];
+        level_weight = s.part64[0];
+        weight_over = s.part64[1];
+        __syncthreads();
+    };
+    uint32_t low = 0, high = kBins;   // levels that are left
+    u64 aim_p = p_of_whole;
+    if (by_level) {
+        // what the list says of the levels that it holds whole
+        u64 listed_mine = 0, listed = 0;
+        if (sure != 0) {
+            low = level_of(value_of(static_cast<uint32_t>(s.list.sorted[sure - 1] >> 32)));
+            for (uint32_t i = threadIdx.x; i < sure; i += NT) {
+                const float l = value_of(static_cast<uint32_t>(s.list.sorted[i] >> 32));
+                if (level_of(l) < low) listed_mine += r.weight(l);
+            }
+        }
+        (void)before<NT>(listed_mine, s.part[0], &listed);
+        for (uint32_t i = threadIdx.x; i < kBins; i += NT) s.wide.count[i] = 0;
+        __syncthreads();
+        r.each_piece(nullptr, r.ngroups, [&](const Piece &p, const float (&v)[NE]) {
+#pragma unroll
+            for (uint32_t e = 0; e < NE; ++e) {
+                if (e < p.have) atomicAdd(&s.wide.count[level_of(no_nan(v[e]))], 1u);
+            }
+        });
+        __syncthreads();
+        uint32_t sum = 0, all;
+        double w = 0.0, whole, listed_middles = 0.0, others;
+#pragma unroll
+        for (uint32_t i = 0; i < kMine; ++i) {
+            const uint32_t l = threadIdx.x * kMine + i;
+            sum += counts[i] = s.wide.count[l];
+            const double m = middles(l, counts[i]);
+            w += m;
+            if (l < low) listed_middles += m;
+        }
+        over_mine = before<NT>(sum, s.part32[0], &all);
+        weight_mine = before<NT>(w, s.part64, &whole);
+        (void)before<NT>(listed_middles, s.part64, &others);
+        if (choice.by_k) {
+            find_level(true, 0.0, 0.0, 0, high);
+            high = level + 1;
+        } else {
+            find_level(false, listed * unit - others, aim_p * unit, low, high);
+        }
+    }
+    bool count_known = !choice.by_k;
+    u64 last = 0;   // the last that stays of the level's, as the list has it
+    for (int round = 0;; ++round) {
+        if (!only_least && (level >= kBins - 1 || level_count > kList || round == kRounds)) return false;
+        // weights over the level by chunks, and the level's list
+        if (threadIdx.x == 0) s.word[3] = 0;
+        __syncthreads();
+        for (uint32_t first = wave; first < a.rows.nchunks; first += R::kWaves * kAhead) {
+            u32x4 raw[kAhead];
+            uint32_t elems[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const uint32_t chunk = first + k * R::kWaves;
+                const Stretch t = a.rows.chunks[chunk < a.rows.nchunks ? chunk : 0];
+                elems[k] = chunk < a.rows.nchunks ? t.elems : 0;
+                raw[k] = load_piece<DT, false>(t.at + r.row * t.step, lane, elems[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const uint32_t chunk = first + k * R::kWaves;
+                float v[NE];
+                R::V::unpack(raw[k], v);
+                u64 sum = 0;
+#pragma unroll
+                for (uint32_t e = 0; e < NE; ++e) {
+                    if (lane * NE + e >= elems[k]) continue;
+                    const float l = no_nan(v[e]);
+                    const uint32_t at = level_of(l);
+                    if (only_least) {
+                        if (r.share(l, 0) >= choice.least) sum += r.weight(l);
+                    } else if (at < level) {
+                        sum += r.weight(l);
+                    } else if (at == level) {
+                        const uint32_t i = atomicAdd(&s.word[3], 1u);
+                        if (i < kList) s.wide.listed[i] = static_cast<u64>(number_of(l)) << 32 | static_cast<uint32_t>(~(chunk * kChunk<DT> + lane * NE + e));
+                    }
+                }
+#pragma unroll
+                for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
+                if (lane == 0 && chunk < a.rows.nchunks) s.wide.weight[chunk] = sum;
+            }
+        }
+        __syncthreads();
+        if (only_least) break;
+        u64 sum = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kChunks; ++i) {
+            const uint32_t chunk = threadIdx.x * kChunks + i;
+            if (chunk < a.rows.nchunks) sum += s.wide.weight[chunk];
+        }
+        u64 above;
+        (void)before<NT>(sum, s.part[0], &above);
+        r.sort(level_count);
+        u64 w[kListed];
+        sum = 0;
+        uint32_t stay = choice.by_k && level + 1 == high && !count_known ? choice.k - level_over : level_count;
+#pragma unroll
+        for (uint32_t i = 0; i < kListed; ++i) {
+            const uint32_t place = threadIdx.x * kListed + i;
+            sum += w[i] = place < stay ? r.weight(static_cast<uint32_t>(s.wide.sorted[place] >> 32)) : 0;
+        }
+        u64 inside;
+        u64 at = above + before<NT>(sum, s.part[0], &inside);
+        if (!count_known) {
+            count_known = true;
+            aim_p = part_of(choice.p, static_cast<double>(above + inside));
+        }
+        if (choice.by_p) {
+            const bool up = aim_p <= above && level_over != 0;
+            if (up || (above + inside < aim_p && level + 1 < high)) {
+                const double more = (up ? above : above + inside) * unit - (up ? weight_over : weight_over + level_weight);
+                (up ? high : low) = up ? level : level + 1;
+                find_level(false, more, aim_p * unit, low, high);
+                if (level == kNoLevel) return false;
+                continue;
+            }
+            uint32_t keep = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kListed; ++i) {
+                const uint32_t place = threadIdx.x * kListed + i;
+                keep += place < stay && ((level_over == 0 && place == 0) || at < aim_p);
+                at += w[i];
+            }
+            (void)before<NT>(keep, s.part32[0], &stay);
+        }
+        last = s.wide.sorted[stay - 1];
+        if (choice.by_min && !(r.share(static_cast<uint32_t>(last >> 32)) >= choice.least)) {
+            only_least = true;   // it asks for more than the others
+            continue;
+        }
+        // those of the level that stay, to their chunks
+#pragma unroll
+        for (uint32_t i = 0; i < kListed; ++i) {
+            const uint32_t place = threadIdx.x * kListed + i;
+            if (place < stay && w[i] != 0) atomicAdd(&s.wide.weight[~static_cast<uint32_t>(s.wide.sorted[place]) / kChunk<DT>], w[i]);
+        }
+        __syncthreads();
+        break;
+    }
+    // the chunk, then the element
+    u64 sum = 0;
+    u64 w[kChunks];
+#pragma unroll
+    for (uint32_t i = 0; i < kChunks; ++i) {
+        const uint32_t chunk = threadIdx.x * kChunks + i;
+        sum += w[i] = chunk < a.rows.nchunks ? s.wide.weight[chunk] : 0;
+    }
+    u64 whole;
+    u64 at = before<NT>(sum, s.part[0], &whole);
+    const u64 aim = aim_of(u, whole);
+#pragma unroll
+    for (uint32_t i = 0; i < kChunks; ++i) {
+        if (aim >= at && aim - at < w[i]) {
+            s.word[0] = threadIdx.x * kChunks + i;
+            s.part[1][0] = at;
+        }
+        at += w[i];
+    }
+    __syncthreads();
+    if (wave != 0) return true;
+    const uint32_t chunk = s.word[0];
+    const Stretch t = a.rows.chunks[chunk];
+    const u32x4 raw = load_piece<DT, false>(t.at + r.row * t.step, lane, t.elems);
+    float v[NE];
+    R::V::unpack(raw, v);
+    u64 each[NE];
+    sum = 0;
+#pragma unroll
+    for (uint32_t e = 0; e < NE; ++e) {
+        const float l = no_nan(v[e]);
+        bool in = lane * NE + e < t.elems;
+        if (only_least) {
+            in = in && r.share(l, 0) >= choice.least;
+        } else {
+            const uint32_t of = level_of(l);
+            const u64 x = static_cast<u64>(number_of(l)) << 32 | static_cast<uint32_t>(~(chunk * kChunk<DT> + lane * NE + e));
+            in = in && (of < level || (of == level && x >= last));
+        }
+        sum += each[e] = in ? r.weight(l) : 0;
+    }
+    at = wave_sums(sum) + s.part[1][0] - sum;
+#pragma unroll
+    for (uint32_t e = 0; e < NE; ++e) {
+        if (aim >= at && aim - at < each[e]) r.write_choice(t.first + lane * NE + e, number_of(no_nan(v[e])), static_cast<double>(whole) * unit);
+        at += each[e];
+    }
+    return true;
+}
+
+template <int DT, int NT>
+__global__ void __launch_bounds__(NT)
 k_sample(SelectArgs a)
 {
-    constexpr uint32_t kMine = kList / kThreads;
+    constexpr uint32_t kMine = kList / NT;
     constexpr uint32_t kShift = kIdle<DT>;
     __shared__ Shared s;
-    Row<DT> r(a, blockIdx.x);
-    const RowChoice choice(a.choice, r.row, a.rows.vocab);
-    const float u = a.choice.random[r.row];
-    r.top = top_of(r, s);
-    r.top_value = value_of(r.top);
-    r.c = choice.c;
+    const RowChoice choice(a.choice, blockIdx.x, a.rows.vocab);
+    const float u = a.choice.random[blockIdx.x];
+    Row<DT, NT> r(a, s);
+    r.weigh_with(choice.c);
     if (r.top <= kLeast) {   // nothing to choose from
         if (threadIdx.x == 0) {
             a.choice.token[r.row] = -1;
@@ -785,18 +1173,16 @@ k_sample(SelectArgs a)
     u64 p_of_whole = 0;   // the weight that top_p asks for, where it is of the whole row
     if (choice.by_p && !choice.by_k) {
         double mine = 0.0;
-        for (uint32_t i = threadIdx.x; i < a.nruns; i += kThreads) {
-            const Run run = a.runs[r.row * a.nruns + i];
-            mine += run.most == static_cast<float>(r.top_value) ? run.sum : run.sum * exp2_exact((static_cast<double>(run.most) - r.top_value) * r.c);
-        }
+        for (uint32_t i = threadIdx.x; i < a.nruns; i += NT) mine += r.run_sum(i);
         double whole;
-        (void)before(mine, s.part64, &whole);
-        p_of_whole = choice.p > 0.0 ? static_cast<u64>(ceil(ldexp(choice.p * whole, static_cast<int>(a.bits)))) : 0;
+        (void)before<NT>(mine, s.part64, &whole);
+        p_of_whole = part_of(choice.p, ldexp(whole, static_cast<int>(a.bits)));
     }
+    uint32_t sure = 0;
     if (!choice.by_k || choice.k <= HCCLX_TOP_MAX) {
-        const uint32_t n = list_first(r, s, choice.by_k ? choice.k : min(kNucleus, a.rows.vocab));
-        sort_list(s, n);
-        const uint32_t limit = choice.by_k ? choice.k : n;
+        const uint32_t n = r.list_first(choice.by_k ? choice.k : min(kNucleus, a.rows.vocab), &sure);
+        r.sort(n);
+        const uint32_t limit = choice.by_k ? choice.k : sure;
         u64 w[kMine];
         u64 sum = 0;
 #pragma unroll
@@ -805,8 +1191,8 @@ k_sample(SelectArgs a)
             sum += w[i] = at < limit ? r.weight(static_cast<uint32_t>(s.list.sorted[at] >> 32)) : 0;
         }
         u64 whole;
-        u64 at = before(sum, s.part[0], &whole);
-        if (choice.by_k) p_of_whole = choice.p > 0.0 ? static_cast<u64>(ceil(choice.p * static_cast<double>(whole))) : 0;
+        u64 at = before<NT>(sum, s.part[0], &whole);
+        if (choice.by_k) p_of_whole = part_of(choice.p, static_cast<double>(whole));
         uint32_t keep = 0;
 #pragma unroll
         for (uint32_t i = 0; i < kMine; ++i) {
@@ -818,8 +1204,8 @@ k_sample(SelectArgs a)
             at += w[i];
         }
         uint32_t kept;
-        (void)before(keep, s.part32[0], &kept);
-        if (choice.by_k || kept < n || n == a.rows.vocab) {
+        (void)before<NT>(keep, s.part32[0], &kept);
+        if (choice.by_k || kept < sure || n == a.rows.vocab) {
             const u64 last = s.list.sorted[kept - 1];
             sum = 0;
 #pragma unroll
@@ -828,20 +1214,21 @@ k_sample(SelectArgs a)
                 const u64 x = place < n ? s.list.listed[place] : 0;
                 sum += w[i] = place < n && x >= last ? r.weight(static_cast<uint32_t>(x >> 32)) : 0;
             }
-            at = before(sum, s.part[0], &whole);
+            at = before<NT>(sum, s.part[0], &whole);
             const u64 aim = aim_of(u, whole);
 #pragma unroll
             for (uint32_t i = 0; i < kMine; ++i) {
                 if (aim >= at && aim - at < w[i]) {
                     const u64 x = s.list.listed[threadIdx.x * kMine + i];
-                    write_choice(a, r, ~static_cast<uint32_t>(x), static_cast<uint32_t>(x >> 32), ldexp(static_cast<double>(whole), -static_cast<int>(a.bits)));
+                    r.write_choice(column_of<DT>(a, x), static_cast<uint32_t>(x >> 32), ldexp(static_cast<double>(whole), -static_cast<int>(a.bits)));
                 }
                 at += w[i];
             }
             return;
         }
-        __syncthreads();   // the list makes room
     }
+    if (draw_wide(a, r, s, choice, u, p_of_whole, sure)) return;
+    __syncthreads();   // the lists make room
     // More stays than a list holds: the cut is searched among all elements.
     Kept stay = {0, 0xffffffffu, choice.by_min ? choice.least : 0.0};
     auto all = [&](auto &&f) { r.each(nullptr, r.ngroups, f); };
@@ -849,7 +1236,7 @@ k_sample(SelectArgs a)
     uint32_t cut_count = 0;
     if (choice.by_k) {
         do {
-            narrow<false>(range, s, all, [&](u64) { return u64(choice.k); });
+            r.template narrow<false>(range, all, [&](u64) { return u64(choice.k); });
         } while (range.low != range.high);
         stay.cut = range.low;
         stay.equal = choice.k - range.above;
@@ -862,11 +1249,8 @@ k_sample(SelectArgs a)
         // (what is equal to the cut of top_k and does not stay is at the end of the order)
         const u64 over = choice.by_k && cut_count > stay.equal ? (cut_count - stay.equal) * r.weight(stay.cut << kShift | (stay.cut >> (31 - kShift) != 0 ? 0 : (1u << kShift) - 1)) : 0;
         do {
-            narrow<true>(range, s, all, [&](u64 whole) {
-                if (first) {
-                    aim = choice.by_k && choice.p > 0.0 ? static_cast<u64>(ceil(choice.p * static_cast<double>(whole - over))) : p_of_whole;
-                    aim = max(u64(1), min(aim, whole));
-                }
+            r.template narrow<true>(range, all, [&](u64 whole) {
+                if (first) aim = max(u64(1), min(choice.by_k ? part_of(choice.p, static_cast<double>(whole - over)) : p_of_whole, whole));
                 return aim;
             });
             first = false;
@@ -877,7 +1261,7 @@ k_sample(SelectArgs a)
         stay.equal = stay.cut == range.low && choice.by_k ? min(stay.equal, equal) : equal;
         stay.cut = range.low;
     }
-    if (threadIdx.x == 0) s.wide = 0;
+    if (threadIdx.x == 0) s.one = 0;
     __syncthreads();
     draw_kept(a, r, s, stay, u);
 }
@@ -891,6 +1275,7 @@ struct SelectWork : PlanWork {
     int dtype = 0;
     bool sample = false;
     uint32_t parts = 1;    // workgroups of the first launch per row
+    uint32_t threads = 512;   // of a workgroup of the second
 
     template <int DT, int U>
     void runs(hipStream_t st) const
@@ -913,10 +1298,25 @@ struct SelectWork : PlanWork {
             case 4: runs<DT, 4>(st); break;
             default: runs<DT, 8>(st); break;
         }
-        if (sample) {
-            HCCLX_LAUNCH((k_sample<DT>), dim3(args.rows.rows), dim3(kThreads), 0, st, args);
+        const dim3 grid(args.rows.rows);
+        if (threads == 1024) {
+            if (sample) {
+                HCCLX_LAUNCH((k_sample<DT, 1024>), grid, dim3(1024), 0, st, args);
+            } else {
+                HCCLX_LAUNCH((k_top_logits<DT, 1024>), grid, dim3(1024), 0, st, args);
+            }
+        } else if (threads == 512) {
+            if (sample) {
+                HCCLX_LAUNCH((k_sample<DT, 512>), grid, dim3(512), 0, st, args);
+            } else {
+                HCCLX_LAUNCH((k_top_logits<DT, 512>), grid, dim3(512), 0, st, args);
+            }
         } else {
-            HCCLX_LAUNCH((k_top_logits<DT>), dim3(args.rows.rows), dim3(kThreads), 0, st, args);
+            if (sample) {
+                HCCLX_LAUNCH((k_sample<DT, 256>), grid, dim3(256), 0, st, args);
+            } else {
+                HCCLX_LAUNCH((k_top_logits<DT, 256>), grid, dim3(256), 0, st, args);
+            }
         }
     }
 
@@ -952,8 +1352,8 @@ int finish(const hcclx_logits_t &l, uint32_t vocab, bool sums, std::unique_ptr<S
     w->parts = parts();
     if (static_cast<uint64_t>(l.rows) * w->parts * kRunWaves * 64 > 0xffffffffull) return fail(HCCL_E_PARA, "too many rows of so many columns");
     a.nruns = (a.rows.nchunks + a.per_run - 1) / a.per_run;
-    a.bits = 62;
-    for (uint64_t n = 1; n < vocab; n *= 2) --a.bits;
+    a.bits = 51;   // a weight is below 2^52, the sum of all below 2^62
+    while (vocab > 1ull << (62 - a.bits)) --a.bits;
     const uint64_t runs = sums ? static_cast<uint64_t>(l.rows) * a.nruns * sizeof(Run) : 0;
     const uint32_t per = 64 * (16 / dtype_size(l.dtype)) / kGroup;
     const uint64_t most = static_cast<uint64_t>(l.rows) * a.rows.nchunks * per * sizeof(uint32_t);

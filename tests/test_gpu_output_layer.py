@@ -479,3 +479,16 @@ def test_rows_behind_4_gib():
     want, grad, bound, grad_bound = L.distill(last, values[-1].double(), indices[-1], 1.0, 1.0)
     assert abs(float(loss[-1]) - want) <= bound + O.E * abs(want)
     O.assert_close(whole[-1], grad, grad_bound)
+
+
+@pytest.mark.parametrize("dtype", [T.FP32, T.BFP16])
+def test_top_p_among_groups_that_are_as_large(dtype):
+    """More groups of 64 columns reach the same value than are looked at, and most groups hold it more than once: what is listed of
+    some groups is not the beginning of the order."""
+    vocab = 64 * 700
+    row = torch.full((vocab,), -1.0, device=DEV)
+    row[::64] = 2.0
+    row[5::192] = 2.0
+    row[torch.arange(9, vocab, 640)] = 3.0
+    for settings in (dict(top_p=0.3), dict(top_p=0.55), dict(top_p=0.6), dict(min_p=0.3), dict(top_k=300), dict(top_k=900)):
+        check_draws(row, shares(vocab, 2), dtype, most=40, **settings)
