@@ -25,7 +25,7 @@ constexpr uint32_t kGroup = 64;          // columns
 constexpr uint32_t kRunWaves = 4;        // of a workgroup of the first launch, a run each
 constexpr uint32_t kList = 2048;         // elements that are sorted at once
 constexpr uint32_t kMostGroups = HCCLX_TOP_MAX + HCCLX_TOP_MAX / 2 + 32;
-constexpr uint32_t kNucleus = 256;       // listed where no top_k bounds the list
+constexpr uint32_t kNucleus = 192;       // listed where no top_k bounds the list
 constexpr uint32_t kNone = 0;            // the number of what does not exist
 constexpr uint32_t kLeast = 0x007fffffu;   // of minus infinity
 
@@ -76,6 +76,76 @@ template <int DT> constexpr uint32_t kIdle = DT == HCCL_DATA_TYPE_BFP16 ? 16 : D
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) { return dpp_or<CTRL>(v, v); }
 
+typedef unsigned long long u64;
+
+// v of the lane that DPP control CTRL names, in the rows of 16 lanes that ROWS names; 0 elsewhere.
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T dpp_or_zero(T v)
+{
+    static_assert(sizeof(T) == 4 || sizeof(T) == 8, "");
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+    } else {
+        const u64 x = __builtin_bit_cast(u64, v);
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROWS, 0xf, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(x >> 32), CTRL, ROWS, 0xf, false);
+        return __builtin_bit_cast(T, static_cast<u64>(hi) << 32 | lo);
+    }
+}
+// v of the last lane.
+template <typename T>
+__device__ __forceinline__ T of_last_lane(T v)
+{
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+    } else {
+        const u64 x = __builtin_bit_cast(u64, v);
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(x), 63);
+        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(x >> 32), 63);
+        return __builtin_bit_cast(T, static_cast<u64>(hi) << 32 | lo);
+    }
+}
+// Sums over the lanes up to this one, and over all; the largest.  All in registers (through LDS a step takes ten times as long).
+template <typename T>
+__device__ __forceinline__ T wave_sums(T v)
+{
+    v += dpp_or_zero<0x111, 0xf>(v);   // row_shr 1, 2, 4, 8
+    v += dpp_or_zero<0x112, 0xf>(v);
+    v += dpp_or_zero<0x114, 0xf>(v);
+    v += dpp_or_zero<0x118, 0xf>(v);
+    v += dpp_or_zero<0x142, 0xa>(v);   // lane 15 of rows 0 and 2 to the rows behind
+    v += dpp_or_zero<0x143, 0xc>(v);   // lane 31 to rows 2 and 3
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ T wave_total(T v) { return of_last_lane(wave_sums(v)); }
+__device__ __forceinline__ uint32_t wave_most(uint32_t v)
+{
+    v = max(v, dpp_or_zero<0x111, 0xf>(v));
+    v = max(v, dpp_or_zero<0x112, 0xf>(v));
+    v = max(v, dpp_or_zero<0x114, 0xf>(v));
+    v = max(v, dpp_or_zero<0x118, 0xf>(v));
+    v = max(v, dpp_or_zero<0x142, 0xa>(v));
+    return of_last_lane(max(v, dpp_or_zero<0x143, 0xc>(v)));
+}
+
+// 2^(up - y / 64) for y >= 0: y = n + f with |f| <= 1/2, a power out of the table (64 of them) and five terms of the power series, the
+// first omitted of which is below 2^-54.  What is below 2^-53, or no number, is 0.
+__device__ __forceinline__ double power(const double *powers, double y, int up)
+{
+    if (!(y < 53.0 * 64.0)) return 0.0;
+    const double n = rint(y);
+    const double z = (y - n) * (-0.69314718055994530942 / 64);
+    double p = 1.0 / 120;
+    p = __builtin_fma(p, z, 1.0 / 24);
+    p = __builtin_fma(p, z, 1.0 / 6);
+    p = __builtin_fma(p, z, 0.5);
+    p = __builtin_fma(p, z, 1.0);
+    p = __builtin_fma(p, z, 1.0);
+    const int whole = static_cast<int>(n);
+    return ldexp(p * powers[whole & 63], up - (whole >> 6));
+}
+
 struct RowChoice {
     bool greedy;
     bool by_k;
@@ -119,6 +189,11 @@ k_logit_runs(SelectArgs a, uint32_t parts)
     const uint32_t run = blockIdx.x % parts * kRunWaves + wave;
     const uint32_t lane = threadIdx.x & 63;
     const uint32_t from = run * U;
+    __shared__ double s_powers[64];
+    if constexpr (KIND == kRunChoice) {
+        if (threadIdx.x < 64) s_powers[threadIdx.x] = exp2_exact(threadIdx.x / -64.0);
+        __syncthreads();
+    }
     if (from >= a.rows.nchunks) return;
     u32x4 raw[U];
     uint32_t elems[U];
@@ -153,18 +228,22 @@ k_logit_runs(SelectArgs a, uint32_t parts)
 #pragma unroll
         for (int d = 8; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
         double sum = 0.0;
-        if (most == minus_infinity()) {
-        } else if constexpr (KIND == kRunSum) {
+        if constexpr (KIND == kRunSum) {
+            // (bounded: minus infinity and NaN become a term of 0, and infinity has a distance of 0 from itself)
+            constexpr float kBound = 0x1.fffffep+125f;
+            const float c = 1.44269504f;
+            const float ref = fminf(fmaxf(most, -kBound), kBound) * c;
             float s = 0.0f;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 float f[NE];
                 V::unpack(raw[u], f);
 #pragma unroll
-                for (int e = 0; e < NE; ++e) s += no_nan(f[e]) == most ? 1.0f : exp2_fast((no_nan(f[e]) - most) * 1.44269504f);
+                for (int e = 0; e < NE; ++e) s += exp2_fast(__builtin_fmaf(fminf(fmaxf(f[e], -kBound), kBound), c, -ref));
             }
-            sum = wave_sum(s);
-        } else {
+            sum = most == minus_infinity() ? 0.0 : static_cast<double>(wave_sum(s));
+        } else if (most != minus_infinity()) {
+            const double step = 64.0 * choice.c;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 float f[NE];
@@ -172,18 +251,16 @@ k_logit_runs(SelectArgs a, uint32_t parts)
 #pragma unroll
                 for (int e = 0; e < NE; ++e) {
                     const float l = no_nan(f[e]);
-                    sum += l == most ? 1.0 : exp2_exact((static_cast<double>(l) - most) * choice.c);
+                    sum += l == most ? 1.0 : power(s_powers, (static_cast<double>(most) - l) * step, 0);
                 }
             }
-            sum = wave_sum64(sum);
+            sum = wave_total(sum);
         }
         if (lane == 0) a.runs[row * a.nruns + run] = {sum, most, 0};
     }
 }
 
 // ---- the second launch ---------------------------------------------------------------------------------------------------
-
-typedef unsigned long long u64;
 
 // What a list holds of an element, so that larger ones come first in its order: number, ~place.  A place counts kChunk for each chunk in
 // front of the element's; places are in the order of the columns.
@@ -204,8 +281,13 @@ struct Range {
 };
 
 constexpr uint32_t kBins = 2048;
-constexpr uint32_t kMostChunks = 1024;   // of a row whose cut is found by levels
-constexpr uint32_t kMostWaves = 16;
+constexpr uint32_t kSpan = 4;            // chunks that are weighed together
+constexpr uint32_t kMostSpans = 512;     // of a row whose cut is found by levels
+constexpr uint32_t kCounted = 256;       // elements of a list that is put in order by counting
+constexpr uint32_t kMostWaves = 8;
+constexpr uint32_t kCached = 320;        // chunks whose places in the row are kept in LDS
+constexpr uint32_t kNoEnd = 0xffffffffu;
+
 struct Shared {
     union {
         struct {
@@ -217,70 +299,28 @@ struct Shared {
             u64 sorted[kList];
         } list;
         struct {
-            u64 weight[kMostChunks];   // of the chunks of a row
-            uint32_t equal[kMostChunks];
+            u64 weight[512];   // of the chunks of a row
+            uint32_t equal[512];
         } walk;
         struct {
             u64 listed[kList];
             u64 sorted[kList];
-            u64 weight[kMostChunks];   // of the chunks: what is over the cut
-            uint32_t count[kBins];     // of the levels
+            u64 weight[kMostSpans];      // of the spans: what is over the cut
+            uint32_t count[kBins];       // of the levels
+            float queue[kMostWaves][128];
         } wide;
     };
     double powers[64];   // 2^(-i / 64)
+    uint64_t at[kCached];
+    uint32_t elems[kCached];
     uint32_t groups[kMostGroups];
     u64 part[2][kMostWaves];
-    double part64[kMostWaves];
-    uint32_t part32[2][kMostWaves];
+    uint32_t most[kMostWaves];
     Range range;
+    u64 word64[2];
     uint32_t word[4];
     u64 one;
 };
-
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp_add(uint32_t v)
-{
-    return v + __builtin_amdgcn_update_dpp(0u, v, CTRL, ROWS, 0xf, false);
-}
-// Sums over the lanes up to this one.
-__device__ __forceinline__ uint32_t wave_sums(uint32_t v)
-{
-    v = dpp_add<0x111, 0xf>(v);   // row_shr 1, 2, 4, 8
-    v = dpp_add<0x112, 0xf>(v);
-    v = dpp_add<0x114, 0xf>(v);
-    v = dpp_add<0x118, 0xf>(v);
-    v = dpp_add<0x142, 0xa>(v);   // lane 15 of rows 0 and 2 to the rows behind
-    return dpp_add<0x143, 0xc>(v);   // lane 31 to rows 2 and 3
-}
-template <typename T>
-__device__ __forceinline__ T wave_sums(T v)
-{
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const T o = __shfl_up(v, d, 64);
-        if ((threadIdx.x & 63) >= static_cast<uint32_t>(d)) v += o;
-    }
-    return v;
-}
-
-// Sums over the threads before this one, and over all.  (Two barriers; s: a word per wavefront.)
-template <int NT, typename T>
-__device__ __forceinline__ T before(T v, T *s, T *all)
-{
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-    const T sum = wave_sums(v);
-    if (lane == 63) s[wave] = sum;
-    __syncthreads();
-    T from = 0, whole = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < NT / 64; ++w) {
-        from += w < wave ? s[w] : T(0);
-        whole += s[w];
-    }
-    __syncthreads();
-    *all = whole;
-    return from + sum - v;
-}
 
 // A lane's vector of a group: lanes kGroup / NE in a row hold one.
 struct Piece {
@@ -299,6 +339,7 @@ struct Row {
     static constexpr uint32_t kShift = kIdle<DT>;
     static constexpr uint32_t kWaves = NT / 64;
     static constexpr uint32_t kHeld = 4096 / NT;     // groups of a thread whose largest it holds, where all find room
+    static_assert(kWaves <= kMostWaves && kHeld % 4 == 0, "");
 
     const SelectArgs &a;
     Shared &s;
@@ -309,13 +350,13 @@ struct Row {
     uint32_t top;      // the largest number of the row
     double top_value;
     double c;          // log2(e) / T, where weights are asked for
+    uint32_t flip;     // which partial sums are free
 
     __device__ __forceinline__ Row(const SelectArgs &args, Shared &shared)
-        : a(args), s(shared), row(blockIdx.x), most(args.most + row * args.rows.nchunks * kPer), ngroups(args.rows.nchunks * kPer)
+        : a(args), s(shared), row(blockIdx.x), most(args.most + row * args.rows.nchunks * kPer), ngroups(args.rows.nchunks * kPer), c(0.0), flip(0)
     {
-        // (rows of the largest are whole vectors: a chunk has four or eight groups)
-        static_assert(kHeld % 4 == 0, "");
         uint32_t t = 0;
+        // (rows of the largest are whole vectors: a chunk has four or eight groups)
 #pragma unroll
         for (uint32_t i = 0; i < kHeld; i += 4) {
             const uint32_t at = threadIdx.x * kHeld + i;
@@ -326,16 +367,51 @@ struct Row {
                 t = max(t, v[j]);
             }
         }
+        if (a.rows.nchunks <= kCached) {
+            for (uint32_t i = threadIdx.x; i < a.rows.nchunks; i += NT) {
+                const Stretch of = a.rows.chunks[i];
+                s.at[i] = reinterpret_cast<uint64_t>(of.at + row * of.step);
+                s.elems[i] = of.elems;
+            }
+        }
+        if (threadIdx.x < 64) s.powers[threadIdx.x] = exp2_exact(threadIdx.x / -64.0);
         for (uint32_t i = NT * kHeld + threadIdx.x; i < ngroups; i += NT) t = max(t, most[i]);
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) t = max(t, static_cast<uint32_t>(__shfl_xor(t, d, 64)));
-        if ((threadIdx.x & 63) == 0) s.part32[1][threadIdx.x / 64] = t;
+        t = wave_most(t);
+        if ((threadIdx.x & 63) == 0) s.most[threadIdx.x / 64] = t;
         __syncthreads();
-        t = s.part32[1][0];
+        t = s.most[0];
 #pragma unroll
-        for (uint32_t w = 1; w < kWaves; ++w) t = max(t, s.part32[1][w]);
+        for (uint32_t w = 1; w < kWaves; ++w) t = max(t, s.most[w]);
         top = t;
         top_value = value_of(top);
+    }
+
+    // Sums over the threads before this one, and over all.  One barrier: partial sums alternate between two places, and who is here for the
+    // third time has seen everybody leave the first.
+    template <typename T>
+    __device__ __forceinline__ T before(T v, T *all)
+    {
+        T *part = reinterpret_cast<T *>(s.part[flip]);
+        flip ^= 1;
+        const uint32_t wave = threadIdx.x / 64;
+        const T sum = wave_sums(v);
+        if ((threadIdx.x & 63) == 63) part[wave] = sum;
+        __syncthreads();
+        T from = 0, whole = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; ++w) {
+            from += w < wave ? part[w] : T(0);
+            whole += part[w];
+        }
+        *all = whole;
+        return from + sum - v;
+    }
+    template <typename T>
+    __device__ __forceinline__ T total(T v)
+    {
+        T all;
+        (void)before(v, &all);
+        return all;
     }
 
     // f(group, its largest) of neighbouring groups per thread, in their order
@@ -352,30 +428,10 @@ struct Row {
         }
     }
 
-    // Has to be called by all threads before the first share() or weight().
-    __device__ __forceinline__ void weigh_with(double per_logit)
-    {
-        c = per_logit;
-        if (threadIdx.x < 64) s.powers[threadIdx.x] = exp2_exact(threadIdx.x / -64.0);
-        __syncthreads();
-    }
-    // exp((l - most) / T), times 2^up: 2^(-y / 64) with y = n + f, |f| <= 1/2, is a power out of the table and five terms of the power series,
-    // the first omitted of which is below 2^-54.  What is below 2^-53 of the largest is 0, as is what is no number.
+    // exp((l - most) / T) times 2^up
     __device__ __forceinline__ double share(float l, int up) const
     {
-        const double y = (top_value - l) * (64.0 * c);
-        if (number_of(l) == top) return ldexp(1.0, up);
-        if (!(y < 53.0 * 64.0)) return 0.0;
-        const double n = rint(y);
-        const double z = (y - n) * (-0.69314718055994530942 / 64);
-        double p = 1.0 / 120;
-        p = __builtin_fma(p, z, 1.0 / 24);
-        p = __builtin_fma(p, z, 1.0 / 6);
-        p = __builtin_fma(p, z, 0.5);
-        p = __builtin_fma(p, z, 1.0);
-        p = __builtin_fma(p, z, 1.0);
-        const int whole = static_cast<int>(n);
-        return ldexp(p * s.powers[whole & 63], up - (whole >> 6));
+        return static_cast<double>(l) == top_value ? ldexp(1.0, up) : power(s.powers, (top_value - l) * (64.0 * c), up);
     }
     __device__ __forceinline__ double share(uint32_t number) const { return share(value_of(number), 0); }
     // The same times 2^bits as a whole number: 2^52 added, the last place of a double is 1.
@@ -385,16 +441,28 @@ struct Row {
     }
     __device__ __forceinline__ u64 weight(uint32_t number) const { return weight(value_of(number)); }
 
+    // Where the row's part of a chunk lies, and how much it has.
+    __device__ __forceinline__ const char *chunk_at(uint32_t chunk, uint32_t *elems) const
+    {
+        if (a.rows.nchunks <= kCached) {
+            *elems = s.elems[chunk];
+            return reinterpret_cast<const char *>(s.at[chunk]);
+        }
+        const Stretch t = a.rows.chunks[chunk];
+        *elems = t.elems;
+        return t.at + row * t.step;
+    }
     __device__ __forceinline__ Piece piece(uint32_t group, bool there) const
     {
         const uint32_t chunk = there ? group / kPer : 0;
-        const Stretch t = a.rows.chunks[chunk];
+        uint32_t elems;
+        const char *at = chunk_at(chunk, &elems);
         const uint32_t lane = group % kPer * kLanes + threadIdx.x % kLanes;   // of the chunk
-        const uint32_t at = lane * NE;
+        const uint32_t first = lane * NE;
         Piece p;
-        p.have = !there || at >= t.elems ? 0 : t.elems - at < NE ? t.elems - at : NE;
-        p.place = chunk * kChunk<DT> + at;
-        p.raw = load_piece<DT, false>(t.at + row * t.step, lane, there ? t.elems : 0);
+        p.have = !there || first >= elems ? 0 : elems - first < NE ? elems - first : NE;
+        p.place = chunk * kChunk<DT> + first;
+        p.raw = load_piece<DT, false>(at, lane, there ? elems : 0);
         return p;
     }
 
@@ -436,7 +504,7 @@ struct Row {
     // which the running count (BY_WEIGHT: weight) from the top reaches what target() says, given the weight in the range.
     // all(f): f(number, weight) for every number that there is.
     template <bool BY_WEIGHT, typename All, typename Target>
-    __device__ __forceinline__ void narrow(Range &r, All &&all, Target &&target) const
+    __device__ __forceinline__ void narrow(Range &r, All &&all, Target &&target)
     {
         const uint32_t width = r.high - r.low;
         const uint32_t shift = width < kBins ? 0 : 32 - __clz(width) - 11;
@@ -470,8 +538,8 @@ struct Row {
         }
         uint32_t all_count;
         u64 whole = 0;
-        uint32_t c = before<NT>(counts, s.part32[0], &all_count);
-        u64 w = BY_WEIGHT ? before<NT>(weights, s.part[0], &whole) : 0;
+        uint32_t c = before(counts, &all_count);
+        u64 w = BY_WEIGHT ? before(weights, &whole) : 0;
         const u64 there = BY_WEIGHT ? r.weight_above + whole : r.above + all_count;
         const u64 asked = target(whole);
         const u64 aim = asked < there ? asked : there;   // (all of it, where there is less)
@@ -494,12 +562,61 @@ struct Row {
         r = s.range;
     }
 
-    // Lists the elements of the groups s.groups[0 .. n) that reach `low`, of those that are it the first `equal`, in the order of the
-    // columns; returns how many there are, or a number over kList as soon as they are known to be more.
-    __device__ __forceinline__ uint32_t list(uint32_t n, uint32_t low, uint32_t equal) const
+    __device__ __forceinline__ void put(uint32_t at, float l, uint32_t place) const
     {
-        uint32_t listed = 0, over_all = 0, same_all = 0;
-        for (uint32_t turn = 0; turn < n && listed <= kList; turn += kTurn) {
+        if (at < kList) s.list.listed[at] = static_cast<u64>(number_of(l)) << 32 | static_cast<uint32_t>(~place);
+    }
+    // Lists the elements of the groups s.groups[0 .. n) that reach `low`, in the order of the columns; returns how many there are, or a
+    // number over kList as soon as they are known to be more.
+    __device__ __forceinline__ uint32_t list(uint32_t n, uint32_t low)
+    {
+        constexpr int kAhead = 4;   // turns that are read and counted together, 16 bits of a sum for each
+        static_assert(NT * NE < 1 << 16, "");
+        // (the least value of the number; the numbers of minus infinity and below are all values')
+        const float least = low <= kLeast >> kShift ? minus_infinity() : value_of(low << kShift);
+        uint32_t listed = 0;
+        for (uint32_t turn = 0; turn < n && listed <= kList; turn += kTurn * kAhead) {
+            Piece p[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const uint32_t i = turn + u * kTurn + threadIdx.x / kLanes;
+                p[u] = piece(i < n ? s.groups[i] : 0, i < n);
+            }
+            float v[kAhead][NE];
+            u64 counts = 0;
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                V::unpack(p[u].raw, v[u]);
+                uint32_t count = 0;
+#pragma unroll
+                for (uint32_t j = 0; j < NE; ++j) {
+                    v[u][j] = no_nan(v[u][j]);
+                    count += j < p[u].have && v[u][j] >= least;
+                }
+                counts |= static_cast<u64>(count) << (16 * u);
+            }
+            u64 all;
+            u64 mine = before(counts, &all);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                uint32_t at = listed + static_cast<uint32_t>(mine & 0xffffu);
+#pragma unroll
+                for (uint32_t j = 0; j < NE; ++j) {
+                    if (j < p[u].have && v[u][j] >= least) put(at++, v[u][j], p[u].place + j);
+                }
+                listed += static_cast<uint32_t>(all & 0xffffu);
+                mine >>= 16;
+                all >>= 16;
+            }
+        }
+        __syncthreads();
+        return listed;
+    }
+    // The same where of the elements that are `low` the first `equal` are wanted: a turn after the other.
+    __device__ __forceinline__ uint32_t list_ties(uint32_t n, uint32_t low, uint32_t equal)
+    {
+        uint32_t over_all = 0, same_all = 0;
+        for (uint32_t turn = 0; turn < n; turn += kTurn) {
             const uint32_t i = turn + threadIdx.x / kLanes;
             const Piece p = piece(i < n ? s.groups[i] : 0, i < n);
             float v[NE];
@@ -508,35 +625,32 @@ struct Row {
             uint32_t over = 0, same = 0;
 #pragma unroll
             for (uint32_t j = 0; j < NE; ++j) {
-                number[j] = number_of(no_nan(v[j]));
-                over += j < p.have && number[j] >> kShift > low;
-                same += j < p.have && number[j] >> kShift == low;
+                number[j] = number_of(no_nan(v[j])) >> kShift;
+                over += j < p.have && number[j] > low;
+                same += j < p.have && number[j] == low;
             }
             uint32_t all;
-            const uint32_t packed = before<NT>(over << 16 | same, s.part32[0], &all);   // (of at most NT * NE elements)
+            const uint32_t packed = before(over << 16 | same, &all);
             uint32_t same_before = same_all + (packed & 0xffffu);
             uint32_t at = over_all + (packed >> 16) + min(same_before, equal);
 #pragma unroll
             for (uint32_t j = 0; j < NE; ++j) {
-                if (j >= p.have || number[j] >> kShift < low) continue;
-                if (number[j] >> kShift == low && same_before++ >= equal) continue;
-                if (at < kList) s.list.listed[at] = static_cast<u64>(number[j]) << 32 | static_cast<uint32_t>(~(p.place + j));
-                ++at;
+                if (j >= p.have || number[j] < low) continue;
+                if (number[j] == low && same_before++ >= equal) continue;
+                put(at++, no_nan(v[j]), p.place + j);
             }
             over_all += all >> 16;
             same_all += all & 0xffffu;
-            listed = over_all + min(same_all, equal);
         }
         __syncthreads();
-        return listed;
+        return over_all + min(same_all, equal);
     }
 
     // The first `k` (HCCLX_TOP_MAX at most) of the order, and others if that is as easy: s.list.listed holds them in the order of their
     // columns, the number of them is returned.  sure: how many of them are the first of the order.
-    __device__ __forceinline__ uint32_t list_first(uint32_t k, uint32_t *sure) const
+    __device__ __forceinline__ uint32_t list_first(uint32_t k, uint32_t *sure)
     {
         // Groups: those whose largest reaches `low`.
-        constexpr uint32_t kNoEnd = 0xffffffffu;
         Range g = {0, top >> kShift, 0, ngroups, 0, 0};
         uint32_t equal = kNoEnd;   // of the groups whose largest is low, the first so many
         const uint32_t enough = max(k + k / 2 + 32, kList / kGroup);
@@ -558,7 +672,7 @@ struct Row {
             // (over: at most `enough`; both fit)
             static_assert(kMostGroups < 4096 && HCCLX_LOGITS_MAX_COLUMNS / kGroup + 8 * kMostRanks < 1 << 20, "");
             uint32_t all;
-            const uint32_t packed = before<NT>(over << 20 | same, s.part32[0], &all);
+            const uint32_t packed = before(over << 20 | same, &all);
             uint32_t same_before = packed & 0xfffffu;
             uint32_t at = (packed >> 20) + min(same_before, equal);
             n = min((all >> 20) + min(all & 0xfffffu, equal), kMostGroups);   // (never more: `enough` and k bound them)
@@ -571,36 +685,32 @@ struct Row {
             __syncthreads();
         }
         // Elements that reach what all groups reach, if they fit.
-        if (g.low != 0 || n * kGroup <= kList) {
-            const uint32_t listed = list(n, g.low, kNoEnd);
-            *sure = equal == kNoEnd ? listed : k;
-            if (listed <= kList) return listed;
-        }
-        // The same again with the vectors of the groups in the groups' place: where there are k, elements reach the k-th vector's largest.
-        Range e = {g.low, top >> kShift, 0, 0, 0, 0};
-        do {
-            narrow<false>(e, [&](auto &&f) {
-                each_piece(s.groups, n, [&](const Piece &p, const float (&v)[NE]) {
-                    if (p.have == 0) return;
-                    float m = minus_infinity();
+        uint32_t listed = kNoEnd;
+        uint32_t low = g.low;
+        if (low != 0 || n * kGroup <= kList) listed = list(n, low);
+        if (listed > kList) {
+            // The same again with the vectors of the groups in the groups' place: where there are k, elements reach the k-th vector's largest.
+            Range e = {low, top >> kShift, 0, 0, 0, 0};
+            do {
+                narrow<false>(e, [&](auto &&f) {
+                    each_piece(s.groups, n, [&](const Piece &p, const float (&v)[NE]) {
+                        if (p.have == 0) return;
+                        float m = minus_infinity();
 #pragma unroll
-                    for (uint32_t j = 0; j < NE; ++j) m = fmaxf(m, v[j]);
-                    f(number_of(m) >> kShift, [] { return u64(0); });
-                });
-            }, [&](u64) { return u64(k); });
-        } while (e.above + e.inside > k + k / 2 + 32 && e.low != e.high);
-        const bool vectors = e.above + e.inside >= k;
-        if (vectors) {
-            const uint32_t listed = list(n, e.low, kNoEnd);
-            *sure = equal == kNoEnd ? listed : k;
-            if (listed <= kList) return listed;
+                        for (uint32_t j = 0; j < NE; ++j) m = fmaxf(m, v[j]);
+                        f(number_of(m) >> kShift, [] { return u64(0); });
+                    });
+                }, [&](u64) { return u64(k); });
+            } while (e.above + e.inside > k + k / 2 + 32 && e.low != e.high);
+            if (e.above + e.inside >= k) listed = list(n, low = e.low);
         }
-        // Elements themselves.
-        e = {vectors ? e.low : g.low, top >> kShift, 0, 0, 0, 0};
-        do {
-            narrow<false>(e, [&](auto &&f) { each(s.groups, n, f); }, [&](u64) { return u64(k); });
-        } while (e.above + e.inside > kList && e.low != e.high);
-        const uint32_t listed = list(n, e.low, e.above + e.inside > kList ? k - e.above : kNoEnd);
+        if (listed > kList) {   // elements themselves
+            Range e = {low, top >> kShift, 0, 0, 0, 0};
+            do {
+                narrow<false>(e, [&](auto &&f) { each(s.groups, n, f); }, [&](u64) { return u64(k); });
+            } while (e.above + e.inside > kList && e.low != e.high);
+            listed = e.above + e.inside > kList ? list_ties(n, e.low, k - e.above) : list(n, e.low);
+        }
         *sure = equal == kNoEnd ? listed : k;
         return listed;
     }
@@ -650,6 +760,48 @@ struct Row {
         }
     }
 
+    // A short list (n <= kCounted), thread t < n: how many elements come before s.list.listed[t], and their weight, given the element's own.
+    // The threads share out the comparisons, whose sums meet in LDS.  (WEIGH false: the number alone.)
+    template <bool WEIGH>
+    __device__ __forceinline__ uint32_t count_before(uint32_t n, u64 own, u64 *weight_before)
+    {
+        static_assert(3 * kCounted <= kList && kCounted <= kMostGroups && kCounted <= NT, "");
+        u64 *const weights = s.list.sorted, *const sums = s.list.sorted + kCounted;
+        uint32_t *const ranks = s.groups;
+        if (threadIdx.x < kCounted) {
+            if (WEIGH) {
+                weights[threadIdx.x] = threadIdx.x < n ? own : 0;
+                sums[threadIdx.x] = 0;
+            }
+            ranks[threadIdx.x] = 0;
+            if (threadIdx.x >= n && threadIdx.x < ((n + 7) & ~7u)) s.list.listed[threadIdx.x] = 0;   // (comes before nothing)
+        }
+        __syncthreads();
+        uint32_t each = 64;   // threads of a share: all elements
+        while (each < n) each *= 2;
+        const uint32_t i = threadIdx.x & (each - 1);
+        const uint32_t shares = NT / each;
+        const uint32_t eights = (n + 7) / 8;
+        if (i < n) {
+            const u64 x = s.list.listed[i];
+            uint32_t rank = 0;
+            u64 sum = 0;
+            for (uint32_t k = threadIdx.x / each; k < eights; k += shares) {
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j) {
+                    const bool first = s.list.listed[k * 8 + j] > x;
+                    rank += first;
+                    if (WEIGH) sum += first ? weights[k * 8 + j] : 0;
+                }
+            }
+            atomicAdd(&ranks[i], rank);
+            if (WEIGH) atomicAdd(&sums[i], sum);
+        }
+        __syncthreads();
+        if (WEIGH) *weight_before = threadIdx.x < kCounted ? sums[threadIdx.x] : 0;
+        return threadIdx.x < kCounted ? ranks[threadIdx.x] : 0;
+    }
+
     // whole: the sum of what could have been drawn, of exp((l - most) / T).
     __device__ __forceinline__ void write_choice(uint32_t column, uint32_t number, double whole) const
     {
@@ -662,7 +814,7 @@ struct Row {
     __device__ __forceinline__ double run_sum(uint32_t i) const   // of a run, of exp((l - most) / T)
     {
         const Run run = a.runs[row * a.nruns + i];
-        return run.most == static_cast<float>(top_value) ? run.sum : run.sum * exp2_exact((static_cast<double>(run.most) - top_value) * c);
+        return run.sum * share(run.most, 0);
     }
 };
 
@@ -673,20 +825,25 @@ k_top_logits(SelectArgs a)
     using D = DTypeOf<DT>;
     __shared__ Shared s;
     Row<DT, NT> r(a, s);
+    r.c = 1.4426950408889634074;   // (of the sum)
     uint32_t sure;
-    r.sort(r.list_first(a.k, &sure));
-    for (uint32_t i = threadIdx.x; i < a.k; i += NT) {
-        const u64 x = s.list.sorted[i];
-        reinterpret_cast<typename D::S *>(a.values)[r.row * a.k + i] = D::narrow(value_of(static_cast<uint32_t>(x >> 32)));
-        a.indices[r.row * a.k + i] = static_cast<int32_t>(column_of<DT>(a, x));
+    const uint32_t n = r.list_first(a.k, &sure);
+    auto write = [&](uint32_t place, u64 x) {
+        reinterpret_cast<typename D::S *>(a.values)[r.row * a.k + place] = D::narrow(value_of(static_cast<uint32_t>(x >> 32)));
+        a.indices[r.row * a.k + place] = static_cast<int32_t>(column_of<DT>(a, x));
+    };
+    if (n <= kCounted) {
+        const uint32_t place = r.template count_before<false>(n, 0, nullptr);
+        if (threadIdx.x < n && place < a.k) write(place, s.list.listed[threadIdx.x]);
+    } else {
+        r.sort(n);
+        for (uint32_t i = threadIdx.x; i < a.k; i += NT) write(i, s.list.sorted[i]);
     }
     if (a.lse != nullptr) {
-        r.c = 1.4426950408889634074;   // (of runs alone)
         double sum = 0.0;
         for (uint32_t i = threadIdx.x; i < a.nruns; i += NT) sum += r.run_sum(i);
-        double all;
-        (void)before<NT>(sum, s.part64, &all);
-        if (threadIdx.x == 0) a.lse[r.row] = static_cast<float>(r.top_value + log(all));
+        sum = r.total(sum);
+        if (threadIdx.x == 0) a.lse[r.row] = static_cast<float>(r.top_value + log(sum));
     }
 }
 
@@ -708,14 +865,15 @@ struct Kept {
     double least;
 };
 
-// Draws among them: the wavefronts' pieces of the row are weighed, NT of them at a time, and the one that the aim lies in is gone
-// through.  A first walk finds the whole.
+// Draws among them: the chunks of the row are weighed, 512 at a time, and the one that the aim lies in is gone through.  A first walk
+// finds the whole.
 template <int DT, int NT>
-__device__ __forceinline__ void draw_kept(const SelectArgs &a, const Row<DT, NT> &r, Shared &s, const Kept &kept, float u)
+__device__ __forceinline__ void draw_kept(const SelectArgs &a, Row<DT, NT> &r, Shared &s, const Kept &kept, float u)
 {
     using R = Row<DT, NT>;
     constexpr uint32_t NE = R::NE;
     constexpr uint32_t kShift = kIdle<DT>;
+    constexpr uint32_t kWalk = NT < 512 ? NT : 512;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
     const bool drop = kept.least > 0.0;
     auto weight = [&](uint32_t number) {
@@ -726,10 +884,10 @@ __device__ __forceinline__ void draw_kept(const SelectArgs &a, const Row<DT, NT>
     for (int find = 0; find < 2; ++find) {
         u64 weight_before = 0;
         uint32_t equal_before = 0;
-        for (uint32_t first = 0; first < a.rows.nchunks; first += NT) {
+        for (uint32_t first = 0; first < a.rows.nchunks; first += kWalk) {
             u64 equal_weight = 0;   // of one element at the cut
-            for (uint32_t turn = 0; turn < NT / R::kWaves; ++turn) {
-                const uint32_t chunk = first + turn * R::kWaves + wave;
+            for (uint32_t at = wave; at < kWalk; at += R::kWaves) {
+                const uint32_t chunk = first + at;
                 u64 sum = 0;
                 uint32_t same = 0;
                 if (chunk < a.rows.nchunks) {
@@ -749,31 +907,28 @@ __device__ __forceinline__ void draw_kept(const SelectArgs &a, const Row<DT, NT>
                         }
                     }
                 }
-#pragma unroll
-                for (int d = 32; d >= 1; d >>= 1) {
-                    sum += __shfl_xor(sum, d, 64);
-                    same += __shfl_xor(same, d, 64);
-                }
+                sum = wave_total(sum);
+                same = wave_total(same);
                 if (lane == 0) {
-                    s.walk.weight[turn * R::kWaves + wave] = sum;
-                    s.walk.equal[turn * R::kWaves + wave] = same;
+                    s.walk.weight[at] = sum;
+                    s.walk.equal[at] = same;
                 }
             }
             if (equal_weight != 0) s.one = equal_weight;   // (all that do write the same)
             __syncthreads();
             const u64 one = s.one;
-            const u64 sum = s.walk.weight[threadIdx.x];
-            const uint32_t same = s.walk.equal[threadIdx.x];
+            const u64 sum = threadIdx.x < kWalk ? s.walk.weight[threadIdx.x] : 0;
+            const uint32_t same = threadIdx.x < kWalk ? s.walk.equal[threadIdx.x] : 0;
             uint32_t same_all;
-            const uint32_t same_before = equal_before + before<NT>(same, s.part32[0], &same_all);
+            const uint32_t same_before = equal_before + r.before(same, &same_all);
             const uint32_t taken = min(same_before + same, kept.equal) - min(same_before, kept.equal);
             u64 sum_all;
             const u64 mine = sum + taken * one;
-            const u64 at = weight_before + before<NT>(mine, s.part[0], &sum_all);
+            const u64 at = weight_before + r.before(mine, &sum_all);
             if (find == 1 && aim >= at && aim - at < mine) {
                 s.word[0] = first + threadIdx.x;   // the chunk
                 s.word[1] = same_before;
-                s.part[1][0] = at;
+                s.word64[0] = at;
             }
             weight_before += sum_all;
             equal_before += same_all;
@@ -803,7 +958,7 @@ __device__ __forceinline__ void draw_kept(const SelectArgs &a, const Row<DT, NT>
         if (in && number >> kShift == kept.cut) in = same_before++ < kept.equal;
         sum += w[e] = in ? weight(number) : 0;
     }
-    u64 at = wave_sums(sum) + s.part[1][0] - sum;
+    u64 at = wave_sums(sum) + s.word64[0] - sum;
 #pragma unroll
     for (uint32_t e = 0; e < NE; ++e) {
         if (aim >= at && aim - at < w[e]) {
@@ -815,7 +970,7 @@ __device__ __forceinline__ void draw_kept(const SelectArgs &a, const Row<DT, NT>
 
 // No filter: the run in which the running sum passes u x the whole, then the element.
 template <int DT, int NT>
-__device__ __forceinline__ void draw_all(const SelectArgs &a, const Row<DT, NT> &r, Shared &s, float u)
+__device__ __forceinline__ void draw_all(const SelectArgs &a, Row<DT, NT> &r, Shared &s, float u)
 {
     using R = Row<DT, NT>;
     constexpr uint32_t NE = R::NE;
@@ -824,14 +979,13 @@ __device__ __forceinline__ void draw_all(const SelectArgs &a, const Row<DT, NT> 
     const uint32_t from = min(threadIdx.x * each, a.nruns), to = min(from + each, a.nruns);
     double mine = 0.0;
     for (uint32_t i = from; i < to; ++i) mine += r.run_sum(i);
+    if (threadIdx.x == 0) s.word[0] = s.word[1] = 0;
     double whole;
-    const double begin = before<NT>(mine, s.part64, &whole);
+    const double begin = r.before(mine, &whole);
     double at = begin;
     double aim = static_cast<double>(u) * whole;
     if (!(aim > 0.0)) aim = 0.0;
     // the last run that begins at or before the aim and has anything (sums are rounded: the aim may lie behind all)
-    if (threadIdx.x == 0) s.word[0] = s.word[1] = 0;
-    __syncthreads();
     for (uint32_t i = from; i < to; ++i) {
         const double w = r.run_sum(i);
         if (w > 0.0 && at <= aim) atomicMax(&s.word[0], i + 1);
@@ -842,11 +996,8 @@ __device__ __forceinline__ void draw_all(const SelectArgs &a, const Row<DT, NT> 
     if (run >= from && run < to) {
         at = begin;
         for (uint32_t i = from; i < run; ++i) at += r.run_sum(i);
-        s.part64[0] = at;
+        s.word64[0] = __builtin_bit_cast(u64, at);
     }
-    __syncthreads();
-    at = s.part64[0];
-    __syncthreads();
     // its chunks, one for each wavefront
     const uint32_t chunk = run * a.per_run + wave;
     const bool there = wave < a.per_run && chunk < a.rows.nchunks;
@@ -859,11 +1010,12 @@ __device__ __forceinline__ void draw_all(const SelectArgs &a, const Row<DT, NT> 
     double sum = 0.0;
 #pragma unroll
     for (uint32_t e = 0; e < NE; ++e) {
-        w[e] = lane * NE + e < elems ? r.share(number_of(no_nan(v[e]))) : 0.0;
+        w[e] = lane * NE + e < elems ? r.share(no_nan(v[e]), 0) : 0.0;
         sum += w[e];
     }
     double all;
-    at += before<NT>(sum, s.part64, &all);
+    at = r.before(sum, &all);
+    at += __builtin_bit_cast(double, s.word64[0]);
 #pragma unroll
     for (uint32_t e = 0; e < NE; ++e) {
         if (w[e] > 0.0 && at <= aim) atomicMax(&s.word[1], threadIdx.x * NE + e + 1);
@@ -878,41 +1030,56 @@ __device__ __forceinline__ void draw_all(const SelectArgs &a, const Row<DT, NT> 
     }
 }
 
-// What stays of a row is more than a list holds: elements are counted by levels, 64 to a power of two of their weight; the level that
+// What stays of a row is more than a list holds.  Elements are counted by levels, 64 to a power of two of their weight.  The level that
 // the cut lies in is found by the counts, for top_k exactly, for top_p with a level's middle for its weights, which is wrong by a level now
-// and then; the elements over that level are weighed chunk by chunk, and those in it are listed and sorted.  That says where the cut is, or
-// in which direction to look for it.  sure: so many first elements are in s.list.sorted.
+// and then; the elements over that level are weighed, a span of chunks at a time, and those in it are listed and sorted.  That says where
+// the cut is, or in which direction to look for it.  sure: so many first elements are in s.list.sorted.
 // Returns false, and nothing is drawn, where a level holds more than a list, or the cut is behind the last.
+//
+// Weights take some forty instructions of 64 bits, and few elements are over the cut: a wavefront collects what it finds in a queue
+// and weighs 64 at a time.
 template <int DT, int NT>
-__device__ __forceinline__ bool draw_wide(const SelectArgs &a, const Row<DT, NT> &r, Shared &s, const RowChoice &choice, float u, u64 p_of_whole,
-                                          uint32_t sure)
+__device__ __forceinline__ bool draw_wide(const SelectArgs &a, Row<DT, NT> &r, Shared &s, const RowChoice &choice, float u, u64 p_of_whole, uint32_t sure)
 {
     using R = Row<DT, NT>;
     constexpr uint32_t NE = R::NE;
     constexpr uint32_t kMine = kBins / NT;
     constexpr uint32_t kListed = kList / NT;
-    constexpr uint32_t kChunks = kMostChunks / NT;
+    constexpr uint32_t kSpans = kMostSpans / NT < 1 ? 1 : kMostSpans / NT;
     constexpr uint32_t kNoLevel = 0xffffffffu;
-    constexpr int kAhead = 4;
     constexpr int kRounds = 8;
-    if (a.rows.nchunks > kMostChunks) return false;
+    static_assert(R::kWaves >= kSpan, "a wavefront for each chunk of a span");
+    const uint32_t nspans = (a.rows.nchunks + kSpan - 1) / kSpan;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const float top = static_cast<float>(r.top_value);
     const float scale = static_cast<float>(64.0 * r.c);
-    auto level_of = [&](float l) {   // (NaN: the distance of infinities, or of minus infinity times 0)
-        const uint32_t v = static_cast<uint32_t>(fminf((top - l) * scale, static_cast<float>(kBins - 1)));
-        return number_of(l) == r.top ? 0 : v;
+    if (nspans > kMostSpans || top == __builtin_inff() || !(scale >= 0x1p-80f && scale <= 0x1p80f)) return false;
+    // (minus infinity: the conversion is to the nearest that there is)
+    auto level_of = [&](float l) { return min(static_cast<uint32_t>(fminf((top - l) * scale, 65536.0f)), kBins - 1); };
+    // the least value of a level over `level`: numbers fall with it, so the first of them is searched, 64 places at a time
+    auto least_over = [&](uint32_t level) {
+        uint32_t low = kLeast, high = r.top;   // low: at the level or below it, high: over it
+        while (high - low > 1) {
+            const uint32_t step = (high - low + 63) / 64;
+            const uint32_t n = low + (lane + 1) * step;
+            const bool below = n < high && n > low && level_of(value_of(n)) >= level;
+            const uint32_t many = __popcll(__ballot(below));
+            const uint32_t next = low + many * step;
+            high = min(next + step, high);
+            low = next;
+        }
+        return value_of(high);
     };
     const double unit = ldexp(1.0, -static_cast<int>(a.bits));
     const bool by_level = choice.by_k || choice.by_p;
     bool only_least = !by_level;   // of all filters min_p alone
     uint32_t level = kNoLevel;     // the cut's
-    uint32_t level_count = 0, level_over = 0;   // elements in it, and over it
+    uint32_t level_count = 0, level_over = 0;       // elements in it, and over it
     double level_weight = 0.0, weight_over = 0.0;   // by the middles
     uint32_t counts[kMine];
+    double middle[kMine];
     uint32_t over_mine = 0;
     double weight_mine = 0.0;
-    auto middles = [&](uint32_t l, uint32_t count) { return count * ldexp(s.powers[l & 63] * 0.99459942348363317565, -static_cast<int>(l >> 6)); };
     // Of the levels low .. high - 1 the first at which the running count reaches top_k, or the running weight and `more` reaches aim; or else the
     // last that holds anything.
     auto find_level = [&](bool by_count, double more, double aim, uint32_t low, uint32_t high) {
@@ -927,75 +1094,83 @@ __device__ __forceinline__ bool draw_wide(const SelectArgs &a, const Row<DT, NT>
         for (uint32_t i = 0; i < kMine; ++i) {
             const uint32_t l = threadIdx.x * kMine + i;
             n += counts[i];
-            w += middles(l, counts[i]);
+            w += middle[i];
             if (l < low || l >= high || counts[i] == 0) continue;
             if (by_count ? n >= choice.k : w + more >= aim) atomicMin(&s.word[0], l);
             atomicMax(&s.word[1], l + 1);
         }
         __syncthreads();
         level = min(s.word[0], s.word[1] - 1);   // (none: kNoLevel)
-        __syncthreads();
-        if (level == kNoLevel) return;
-        n = over_mine;
-        w = weight_mine;
+        if (level / kMine == threadIdx.x) {
+            n = over_mine;
+            w = weight_mine;
 #pragma unroll
-        for (uint32_t i = 0; i < kMine; ++i) {
-            const uint32_t l = threadIdx.x * kMine + i;
-            if (l == level) {
-                s.word[0] = counts[i];
-                s.word[1] = n;
-                s.part64[0] = middles(l, counts[i]);
-                s.part64[1] = w;
+            for (uint32_t i = 0; i < kMine; ++i) {
+                if (threadIdx.x * kMine + i == level) {
+                    s.word[2] = counts[i];
+                    s.word[3] = n;
+                    s.word64[0] = __builtin_bit_cast(u64, middle[i]);
+                    s.word64[1] = __builtin_bit_cast(u64, w);
+                }
+                n += counts[i];
+                w += middle[i];
             }
-            n += counts[i];
-            w += middles(l, counts[i]);
         }
         __syncthreads();
-        level_count = s.word[0];
-        level_over = s.word[1];
-        level_weight = s.part64[0];
-        weight_over = s.part64[1];
-        __syncthreads();
+        level_count = s.word[2];
+        level_over = s.word[3];
+        level_weight = __builtin_bit_cast(double, s.word64[0]);
+        weight_over = __builtin_bit_cast(double, s.word64[1]);
     };
     uint32_t low = 0, high = kBins;   // levels that are left
     u64 aim_p = p_of_whole;
     if (by_level) {
         // what the list says of the levels that it holds whole
-        u64 listed_mine = 0, listed = 0;
+        u64 listed = 0;
         if (sure != 0) {
             low = level_of(value_of(static_cast<uint32_t>(s.list.sorted[sure - 1] >> 32)));
             for (uint32_t i = threadIdx.x; i < sure; i += NT) {
                 const float l = value_of(static_cast<uint32_t>(s.list.sorted[i] >> 32));
-                if (level_of(l) < low) listed_mine += r.weight(l);
+                if (level_of(l) < low) listed += r.weight(l);
             }
         }
-        (void)before<NT>(listed_mine, s.part[0], &listed);
         for (uint32_t i = threadIdx.x; i < kBins; i += NT) s.wide.count[i] = 0;
         __syncthreads();
+        // What is so improbable that even as many as there are columns hold no more than 1 - top_p of the whole lies behind the cut.
+        float far = minus_infinity();
+        if (!choice.by_k) {
+            const double behind = (static_cast<double>(p_of_whole) / choice.p - static_cast<double>(p_of_whole)) * unit / a.rows.vocab;
+            if (behind > 0.0) far = static_cast<float>(r.top_value + log2(behind) / r.c - 2.0 / scale);
+        }
         r.each_piece(nullptr, r.ngroups, [&](const Piece &p, const float (&v)[NE]) {
 #pragma unroll
             for (uint32_t e = 0; e < NE; ++e) {
-                if (e < p.have) atomicAdd(&s.wide.count[level_of(no_nan(v[e]))], 1u);
+                if (e < p.have && v[e] >= far) atomicAdd(&s.wide.count[level_of(v[e])], 1u);
             }
         });
         __syncthreads();
         uint32_t sum = 0, all;
-        double w = 0.0, whole, listed_middles = 0.0, others;
+        double w = 0.0, whole;
 #pragma unroll
         for (uint32_t i = 0; i < kMine; ++i) {
             const uint32_t l = threadIdx.x * kMine + i;
             sum += counts[i] = s.wide.count[l];
-            const double m = middles(l, counts[i]);
-            w += m;
-            if (l < low) listed_middles += m;
+            w += middle[i] = counts[i] * ldexp(s.powers[l & 63] * 0.99459942348363317565, -static_cast<int>(l >> 6));   // (2^(-1 / 128))
         }
-        over_mine = before<NT>(sum, s.part32[0], &all);
-        weight_mine = before<NT>(w, s.part64, &whole);
-        (void)before<NT>(listed_middles, s.part64, &others);
+        over_mine = r.before(sum, &all);
+        weight_mine = r.before(w, &whole);
         if (choice.by_k) {
             find_level(true, 0.0, 0.0, 0, high);
             high = level + 1;
         } else {
+            if (low / kMine == threadIdx.x) {
+                w = weight_mine;
+#pragma unroll
+                for (uint32_t i = 0; i < kMine; ++i) w += threadIdx.x * kMine + i < low ? middle[i] : 0.0;
+                s.word64[0] = __builtin_bit_cast(u64, w);
+            }
+            listed = r.total(listed);
+            const double others = __builtin_bit_cast(double, s.word64[0]);
             find_level(false, listed * unit - others, aim_p * unit, low, high);
         }
     }
@@ -1003,65 +1178,83 @@ __device__ __forceinline__ bool draw_wide(const SelectArgs &a, const Row<DT, NT>
     u64 last = 0;   // the last that stays of the level's, as the list has it
     for (int round = 0;; ++round) {
         if (!only_least && (level >= kBins - 1 || level_count > kList || round == kRounds)) return false;
-        // weights over the level by chunks, and the level's list
-        if (threadIdx.x == 0) s.word[3] = 0;
+        // weights over the level by spans, and the level's list
+        float over = minus_infinity(), in = minus_infinity();
+        if (!only_least) {
+            over = level == 0 ? __builtin_inff() : least_over(level);
+            in = least_over(level + 1);
+        }
         __syncthreads();
-        for (uint32_t first = wave; first < a.rows.nchunks; first += R::kWaves * kAhead) {
-            u32x4 raw[kAhead];
-            uint32_t elems[kAhead];
+        if (threadIdx.x == 0) s.word[2] = 0;
+        __syncthreads();
+        float *const queue = s.wide.queue[wave];
+        for (uint32_t span = wave; span < nspans; span += R::kWaves) {
+            u32x4 raw[kSpan];
+            uint32_t elems[kSpan];
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                const uint32_t chunk = first + k * R::kWaves;
-                const Stretch t = a.rows.chunks[chunk < a.rows.nchunks ? chunk : 0];
-                elems[k] = chunk < a.rows.nchunks ? t.elems : 0;
-                raw[k] = load_piece<DT, false>(t.at + r.row * t.step, lane, elems[k]);
+            for (uint32_t k = 0; k < kSpan; ++k) {
+                const uint32_t chunk = span * kSpan + k;
+                const char *at = r.chunk_at(chunk < a.rows.nchunks ? chunk : 0, &elems[k]);
+                elems[k] = chunk < a.rows.nchunks ? elems[k] : 0;
+                raw[k] = load_piece<DT, false>(at, lane, elems[k]);
             }
+            u64 sum = 0;
+            uint32_t queued = 0;
+            auto weigh = [&](bool live, float l) {
+                if (only_least && !(r.share(l, 0) >= choice.least)) live = false;
+                sum += live ? r.weight(l) : 0;
+            };
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                const uint32_t chunk = first + k * R::kWaves;
+            for (uint32_t k = 0; k < kSpan; ++k) {
                 float v[NE];
                 R::V::unpack(raw[k], v);
-                u64 sum = 0;
 #pragma unroll
                 for (uint32_t e = 0; e < NE; ++e) {
-                    if (lane * NE + e >= elems[k]) continue;
-                    const float l = no_nan(v[e]);
-                    const uint32_t at = level_of(l);
-                    if (only_least) {
-                        if (r.share(l, 0) >= choice.least) sum += r.weight(l);
-                    } else if (at < level) {
-                        sum += r.weight(l);
-                    } else if (at == level) {
-                        const uint32_t i = atomicAdd(&s.word[3], 1u);
-                        if (i < kList) s.wide.listed[i] = static_cast<u64>(number_of(l)) << 32 | static_cast<uint32_t>(~(chunk * kChunk<DT> + lane * NE + e));
+                    const bool there = lane * NE + e < elems[k];
+                    const uint64_t who = __ballot(there && v[e] >= over);
+                    if (!only_least && there && v[e] >= in && !(v[e] >= over)) {
+                        const uint32_t i = atomicAdd(&s.word[2], 1u);
+                        const uint32_t place = (span * kSpan + k) * kChunk<DT> + lane * NE + e;
+                        if (i < kList) s.wide.listed[i] = static_cast<u64>(number_of(v[e])) << 32 | static_cast<uint32_t>(~place);
+                    }
+                    if (who == 0) continue;
+                    const uint32_t at = queued + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(who >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(who), 0));
+                    if (who >> lane & 1) queue[at] = v[e];
+                    queued += __popcll(who);
+                    if (queued >= 64) {
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                        queued -= 64;
+                        weigh(true, queue[queued + lane]);
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                     }
                 }
-#pragma unroll
-                for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
-                if (lane == 0 && chunk < a.rows.nchunks) s.wide.weight[chunk] = sum;
             }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (queued != 0) weigh(lane < queued, queue[lane < queued ? lane : 0]);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            sum = wave_total(sum);
+            if (lane == 0) s.wide.weight[span] = sum;
         }
         __syncthreads();
         if (only_least) break;
         u64 sum = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < kChunks; ++i) {
-            const uint32_t chunk = threadIdx.x * kChunks + i;
-            if (chunk < a.rows.nchunks) sum += s.wide.weight[chunk];
+        for (uint32_t i = 0; i < kSpans; ++i) {
+            const uint32_t span = threadIdx.x * kSpans + i;
+            if (span < nspans) sum += s.wide.weight[span];
         }
-        u64 above;
-        (void)before<NT>(sum, s.part[0], &above);
+        const u64 above = r.total(sum);
         r.sort(level_count);
         u64 w[kListed];
         sum = 0;
-        uint32_t stay = choice.by_k && level + 1 == high && !count_known ? choice.k - level_over : level_count;
+        uint32_t stay = choice.by_k && !count_known ? choice.k - level_over : level_count;
 #pragma unroll
         for (uint32_t i = 0; i < kListed; ++i) {
             const uint32_t place = threadIdx.x * kListed + i;
             sum += w[i] = place < stay ? r.weight(static_cast<uint32_t>(s.wide.sorted[place] >> 32)) : 0;
         }
         u64 inside;
-        u64 at = above + before<NT>(sum, s.part[0], &inside);
+        u64 at = above + r.before(sum, &inside);
         if (!count_known) {
             count_known = true;
             aim_p = part_of(choice.p, static_cast<double>(above + inside));
@@ -1082,46 +1275,47 @@ __device__ __forceinline__ bool draw_wide(const SelectArgs &a, const Row<DT, NT>
                 keep += place < stay && ((level_over == 0 && place == 0) || at < aim_p);
                 at += w[i];
             }
-            (void)before<NT>(keep, s.part32[0], &stay);
+            stay = r.total(keep);
         }
         last = s.wide.sorted[stay - 1];
         if (choice.by_min && !(r.share(static_cast<uint32_t>(last >> 32)) >= choice.least)) {
             only_least = true;   // it asks for more than the others
             continue;
         }
-        // those of the level that stay, to their chunks
+        // those of the level that stay, to their spans
 #pragma unroll
         for (uint32_t i = 0; i < kListed; ++i) {
             const uint32_t place = threadIdx.x * kListed + i;
-            if (place < stay && w[i] != 0) atomicAdd(&s.wide.weight[~static_cast<uint32_t>(s.wide.sorted[place]) / kChunk<DT>], w[i]);
+            if (place < stay && w[i] != 0) atomicAdd(&s.wide.weight[~static_cast<uint32_t>(s.wide.sorted[place]) / (kSpan * kChunk<DT>)], w[i]);
         }
         __syncthreads();
         break;
     }
-    // the chunk, then the element
+    // the span, then the element: a wavefront for each chunk
     u64 sum = 0;
-    u64 w[kChunks];
+    u64 w[kSpans];
 #pragma unroll
-    for (uint32_t i = 0; i < kChunks; ++i) {
-        const uint32_t chunk = threadIdx.x * kChunks + i;
-        sum += w[i] = chunk < a.rows.nchunks ? s.wide.weight[chunk] : 0;
+    for (uint32_t i = 0; i < kSpans; ++i) {
+        const uint32_t span = threadIdx.x * kSpans + i;
+        sum += w[i] = span < nspans ? s.wide.weight[span] : 0;
     }
     u64 whole;
-    u64 at = before<NT>(sum, s.part[0], &whole);
+    u64 at = r.before(sum, &whole);
     const u64 aim = aim_of(u, whole);
 #pragma unroll
-    for (uint32_t i = 0; i < kChunks; ++i) {
+    for (uint32_t i = 0; i < kSpans; ++i) {
         if (aim >= at && aim - at < w[i]) {
-            s.word[0] = threadIdx.x * kChunks + i;
-            s.part[1][0] = at;
+            s.word[0] = threadIdx.x * kSpans + i;
+            s.word64[0] = at;
         }
         at += w[i];
     }
     __syncthreads();
-    if (wave != 0) return true;
-    const uint32_t chunk = s.word[0];
-    const Stretch t = a.rows.chunks[chunk];
-    const u32x4 raw = load_piece<DT, false>(t.at + r.row * t.step, lane, t.elems);
+    const uint32_t chunk = s.word[0] * kSpan + wave;
+    const bool there = wave < kSpan && chunk < a.rows.nchunks;
+    const Stretch t = a.rows.chunks[there ? chunk : 0];
+    const uint32_t elems = there ? t.elems : 0;
+    const u32x4 raw = load_piece<DT, false>(t.at + r.row * t.step, lane, elems);
     float v[NE];
     R::V::unpack(raw, v);
     u64 each[NE];
@@ -1129,7 +1323,7 @@ __device__ __forceinline__ bool draw_wide(const SelectArgs &a, const Row<DT, NT>
 #pragma unroll
     for (uint32_t e = 0; e < NE; ++e) {
         const float l = no_nan(v[e]);
-        bool in = lane * NE + e < t.elems;
+        bool in = lane * NE + e < elems;
         if (only_least) {
             in = in && r.share(l, 0) >= choice.least;
         } else {
@@ -1139,7 +1333,8 @@ __device__ __forceinline__ bool draw_wide(const SelectArgs &a, const Row<DT, NT>
         }
         sum += each[e] = in ? r.weight(l) : 0;
     }
-    at = wave_sums(sum) + s.part[1][0] - sum;
+    u64 all;
+    at = s.word64[0] + r.before(sum, &all);
 #pragma unroll
     for (uint32_t e = 0; e < NE; ++e) {
         if (aim >= at && aim - at < each[e]) r.write_choice(t.first + lane * NE + e, number_of(no_nan(v[e])), static_cast<double>(whole) * unit);
@@ -1158,7 +1353,7 @@ k_sample(SelectArgs a)
     const RowChoice choice(a.choice, blockIdx.x, a.rows.vocab);
     const float u = a.choice.random[blockIdx.x];
     Row<DT, NT> r(a, s);
-    r.weigh_with(choice.c);
+    r.c = choice.c;
     if (r.top <= kLeast) {   // nothing to choose from
         if (threadIdx.x == 0) {
             a.choice.token[r.row] = -1;
@@ -1170,67 +1365,86 @@ k_sample(SelectArgs a)
         draw_all(a, r, s, u);
         return;
     }
+    const double unit = ldexp(1.0, -static_cast<int>(a.bits));
     u64 p_of_whole = 0;   // the weight that top_p asks for, where it is of the whole row
     if (choice.by_p && !choice.by_k) {
         double mine = 0.0;
         for (uint32_t i = threadIdx.x; i < a.nruns; i += NT) mine += r.run_sum(i);
-        double whole;
-        (void)before<NT>(mine, s.part64, &whole);
-        p_of_whole = part_of(choice.p, ldexp(whole, static_cast<int>(a.bits)));
+        p_of_whole = part_of(choice.p, ldexp(r.total(mine), static_cast<int>(a.bits)));
     }
     uint32_t sure = 0;
     if (!choice.by_k || choice.k <= HCCLX_TOP_MAX) {
         const uint32_t n = r.list_first(choice.by_k ? choice.k : min(kNucleus, a.rows.vocab), &sure);
-        r.sort(n);
         const uint32_t limit = choice.by_k ? choice.k : sure;
-        u64 w[kMine];
-        u64 sum = 0;
+        if (n <= kCounted) {
+            const u64 x = threadIdx.x < n ? s.list.listed[threadIdx.x] : 0;
+            const float l = value_of(static_cast<uint32_t>(x >> 32));
+            const u64 w = threadIdx.x < n ? r.weight(l) : 0;
+            u64 weight_before;
+            const uint32_t place = r.template count_before<true>(n, w, &weight_before);
+            const bool first = threadIdx.x < n && place < limit;
+            if (choice.by_k && choice.by_p) p_of_whole = part_of(choice.p, static_cast<double>(r.total(first ? w : 0)));
+            bool in = first;
+            if (choice.by_p) in = in && (place == 0 || weight_before < p_of_whole);
+            if (choice.by_min) in = in && (place == 0 || r.share(l, 0) >= choice.least);
+            if (choice.by_k || n == a.rows.vocab || r.total(static_cast<uint32_t>(in)) < sure) {
+                u64 whole;
+                const u64 at = r.before(in ? w : 0, &whole);
+                const u64 aim = aim_of(u, whole);
+                if (in && aim >= at && aim - at < w) r.write_choice(column_of<DT>(a, x), static_cast<uint32_t>(x >> 32), static_cast<double>(whole) * unit);
+                return;
+            }
+            r.sort(n);
+        } else {
+            r.sort(n);
+            u64 w[kMine];
+            u64 sum = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < kMine; ++i) {
-            const uint32_t at = threadIdx.x * kMine + i;
-            sum += w[i] = at < limit ? r.weight(static_cast<uint32_t>(s.list.sorted[at] >> 32)) : 0;
-        }
-        u64 whole;
-        u64 at = before<NT>(sum, s.part[0], &whole);
-        if (choice.by_k) p_of_whole = part_of(choice.p, static_cast<double>(whole));
-        uint32_t keep = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < kMine; ++i) {
-            const uint32_t place = threadIdx.x * kMine + i;
-            bool in = place < limit;
-            if (choice.by_p) in = in && (place == 0 || at < p_of_whole);
-            if (choice.by_min) in = in && (place == 0 || r.share(static_cast<uint32_t>(s.list.sorted[place] >> 32)) >= choice.least);
-            keep += in;
-            at += w[i];
-        }
-        uint32_t kept;
-        (void)before<NT>(keep, s.part32[0], &kept);
-        if (choice.by_k || kept < sure || n == a.rows.vocab) {
-            const u64 last = s.list.sorted[kept - 1];
-            sum = 0;
+            for (uint32_t i = 0; i < kMine; ++i) {
+                const uint32_t at = threadIdx.x * kMine + i;
+                sum += w[i] = at < limit ? r.weight(static_cast<uint32_t>(s.list.sorted[at] >> 32)) : 0;
+            }
+            u64 whole;
+            u64 at = r.before(sum, &whole);
+            if (choice.by_k) p_of_whole = part_of(choice.p, static_cast<double>(whole));
+            uint32_t keep = 0;
 #pragma unroll
             for (uint32_t i = 0; i < kMine; ++i) {
                 const uint32_t place = threadIdx.x * kMine + i;
-                const u64 x = place < n ? s.list.listed[place] : 0;
-                sum += w[i] = place < n && x >= last ? r.weight(static_cast<uint32_t>(x >> 32)) : 0;
-            }
-            at = before<NT>(sum, s.part[0], &whole);
-            const u64 aim = aim_of(u, whole);
-#pragma unroll
-            for (uint32_t i = 0; i < kMine; ++i) {
-                if (aim >= at && aim - at < w[i]) {
-                    const u64 x = s.list.listed[threadIdx.x * kMine + i];
-                    r.write_choice(column_of<DT>(a, x), static_cast<uint32_t>(x >> 32), ldexp(static_cast<double>(whole), -static_cast<int>(a.bits)));
-                }
+                bool in = place < limit;
+                if (choice.by_p) in = in && (place == 0 || at < p_of_whole);
+                if (choice.by_min) in = in && (place == 0 || r.share(static_cast<uint32_t>(s.list.sorted[place] >> 32)) >= choice.least);
+                keep += in;
                 at += w[i];
             }
-            return;
+            const uint32_t kept = r.total(keep);
+            if (choice.by_k || kept < sure || n == a.rows.vocab) {
+                const u64 last = s.list.sorted[kept - 1];
+                sum = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < kMine; ++i) {
+                    const uint32_t place = threadIdx.x * kMine + i;
+                    const u64 x = place < n ? s.list.listed[place] : 0;
+                    sum += w[i] = place < n && x >= last ? r.weight(static_cast<uint32_t>(x >> 32)) : 0;
+                }
+                at = r.before(sum, &whole);
+                const u64 aim = aim_of(u, whole);
+#pragma unroll
+                for (uint32_t i = 0; i < kMine; ++i) {
+                    if (aim >= at && aim - at < w[i]) {
+                        const u64 x = s.list.listed[threadIdx.x * kMine + i];
+                        r.write_choice(column_of<DT>(a, x), static_cast<uint32_t>(x >> 32), static_cast<double>(whole) * unit);
+                    }
+                    at += w[i];
+                }
+                return;
+            }
         }
     }
     if (draw_wide(a, r, s, choice, u, p_of_whole, sure)) return;
     __syncthreads();   // the lists make room
-    // More stays than a list holds: the cut is searched among all elements.
-    Kept stay = {0, 0xffffffffu, choice.by_min ? choice.least : 0.0};
+    // A level holds more than a list: the cut is searched by numbers, among all elements.
+    Kept stay = {0, kNoEnd, choice.by_min ? choice.least : 0.0};
     auto all = [&](auto &&f) { r.each(nullptr, r.ngroups, f); };
     Range range = {kLeast >> kShift, r.top >> kShift, 0, 0, 0, 0};
     uint32_t cut_count = 0;
@@ -1299,13 +1513,7 @@ struct SelectWork : PlanWork {
             default: runs<DT, 8>(st); break;
         }
         const dim3 grid(args.rows.rows);
-        if (threads == 1024) {
-            if (sample) {
-                HCCLX_LAUNCH((k_sample<DT, 1024>), grid, dim3(1024), 0, st, args);
-            } else {
-                HCCLX_LAUNCH((k_top_logits<DT, 1024>), grid, dim3(1024), 0, st, args);
-            }
-        } else if (threads == 512) {
+        if (threads == 512) {
             if (sample) {
                 HCCLX_LAUNCH((k_sample<DT, 512>), grid, dim3(512), 0, st, args);
             } else {
