@@ -12,6 +12,10 @@
 // 2048 equal stretches of the range that is left, which leaves one of them, and so on: three rounds at most.
 //
 // Weights of the draw are whole numbers too, exp((l - most) / T) 2^s from 64-bit arithmetic: their sums do not go by the order.
+//
+// A row whose draw goes by more than such a list is left to a third and a fourth launch, which put several workgroups on a row: its
+// elements are counted by levels, 64 to a power of two of their weight, which says in which level the cut lies; then those over that
+// level are weighed, and those in it are listed and sorted.  (One workgroup for such a row, behind its list: TIMES_OLD.)
 #include "ops/logits.h"
 
 #include <algorithm>
@@ -25,7 +29,7 @@ constexpr uint32_t kGroup = 64;          // columns
 constexpr uint32_t kRunWaves = 4;        // of a workgroup of the first launch, a run each
 constexpr uint32_t kList = 2048;         // elements that are sorted at once
 constexpr uint32_t kMostGroups = HCCLX_TOP_MAX + HCCLX_TOP_MAX / 2 + 32;
-constexpr uint32_t kNucleus = 192;       // listed where no top_k bounds the list
+constexpr uint32_t kNucleus = 64;       // listed where no top_k bounds the list
 constexpr uint32_t kNone = 0;            // the number of what does not exist
 constexpr uint32_t kLeast = 0x007fffffu;   // of minus infinity
 
@@ -46,6 +50,29 @@ struct Run {
     uint32_t unused;
 };
 
+// A row that is left to the launches behind the second.
+struct Wide {
+    uint32_t wide;     // 0: it is not
+    uint32_t top;      // its largest number
+    unsigned long long p_of_whole;
+};
+
+// What a part of such a row holds nearer than the band, and how many in it.
+struct Found {
+    unsigned long long weight;
+    uint32_t over;
+    uint32_t listed;
+};
+
+// Distances of the elements that the cut lies among: low .. high - 1.  Those nearer all stay, those further don't.
+struct Band {
+    float low;
+    float high;
+    bool by_level;   // by top_k or top_p
+    bool by_min;
+    bool known;      // false: the cut is not found by levels
+};
+
 struct SelectArgs {
     Rows rows;
     uint32_t *most;     // [rows][nchunks * groups of a chunk]: the numbers of the groups' largest
@@ -53,6 +80,17 @@ struct SelectArgs {
     uint32_t nruns;
     uint32_t per_run;   // chunks
     uint32_t bits;      // s
+    // rows that are left to the launches behind the second, of the `batch` rows from `first` on
+    struct Wide *wide;  // [batch]
+    unsigned long long *levels;   // [batch][kLevels]
+    struct Band *bands;           // [batch]
+    struct Found *found;          // [batch][wide_parts]
+    unsigned long long *listed;   // [batch][wide_parts][kList]: the elements that the cut lies among
+    unsigned long long *spans;    // [batch][kMostSpans]: weights over them
+    uint32_t span;      // chunks that are weighed together
+    uint32_t nspans;
+    uint32_t wide_parts;   // workgroups of a row
+    uint32_t first;
     // the largest
     uint32_t k;
     char *values;
@@ -130,12 +168,13 @@ __device__ __forceinline__ uint32_t wave_most(uint32_t v)
 }
 
 // 2^(up - y / 64) for y >= 0: y = n + f with |f| <= 1/2, a power out of the table (64 of them) and five terms of the power series, the
-// first omitted of which is below 2^-54.  What is below 2^-53, or no number, is 0.
+// first omitted of which is below 2^-54.  What is below 2^-53, or no number, is 0.  (No branch: several of them run side by side.)
 __device__ __forceinline__ double power(const double *powers, double y, int up)
 {
-    if (!(y < 53.0 * 64.0)) return 0.0;
-    const double n = rint(y);
-    const double z = (y - n) * (-0.69314718055994530942 / 64);
+    constexpr double kEnd = 53.0 * 64.0;
+    const double in = __builtin_fmin(y, kEnd);   // (of NaN kEnd)
+    const double n = rint(in);
+    const double z = (in - n) * (-0.69314718055994530942 / 64);
     double p = 1.0 / 120;
     p = __builtin_fma(p, z, 1.0 / 24);
     p = __builtin_fma(p, z, 1.0 / 6);
@@ -143,7 +182,10 @@ __device__ __forceinline__ double power(const double *powers, double y, int up)
     p = __builtin_fma(p, z, 1.0);
     p = __builtin_fma(p, z, 1.0);
     const int whole = static_cast<int>(n);
-    return ldexp(p * powers[whole & 63], up - (whole >> 6));
+    // (the product is a normal number between 2^-1 and 2^1: its exponent is added to)
+    const double q = p * powers[whole & 63];
+    const u64 r = __builtin_bit_cast(u64, q) + (static_cast<u64>(static_cast<uint32_t>(up - (whole >> 6)) << 20) << 32);
+    return in < kEnd ? __builtin_bit_cast(double, r) : 0.0;
 }
 
 struct RowChoice {
@@ -251,7 +293,8 @@ k_logit_runs(SelectArgs a, uint32_t parts)
 #pragma unroll
                 for (int e = 0; e < NE; ++e) {
                     const float l = no_nan(f[e]);
-                    sum += l == most ? 1.0 : power(s_powers, (static_cast<double>(most) - l) * step, 0);
+                    const double w = power(s_powers, (static_cast<double>(most) - l) * step, 0);
+                    sum += l == most ? 1.0 : w;
                 }
             }
             sum = wave_total(sum);
@@ -281,12 +324,15 @@ struct Range {
 };
 
 constexpr uint32_t kBins = 2048;
-constexpr uint32_t kSpan = 4;            // chunks that are weighed together
-constexpr uint32_t kMostSpans = 512;     // of a row whose cut is found by levels
+constexpr uint32_t kLevels = 2048;
+constexpr uint32_t kBatch = 4096;        // rows that have memory for a wide draw at a time, 52 KB each and more where they are few
+constexpr uint32_t kMostParts = 32;      // workgroups of a wide row
+constexpr uint32_t kMostSpans = 512;
 constexpr uint32_t kCounted = 256;       // elements of a list that is put in order by counting
 constexpr uint32_t kMostWaves = 8;
 constexpr uint32_t kCached = 320;        // chunks whose places in the row are kept in LDS
 constexpr uint32_t kNoEnd = 0xffffffffu;
+constexpr uint32_t kQueue = 512;          // elements of a chunk that a wavefront weighs
 
 struct Shared {
     union {
@@ -303,11 +349,9 @@ struct Shared {
             uint32_t equal[512];
         } walk;
         struct {
-            u64 listed[kList];
-            u64 sorted[kList];
-            u64 weight[kMostSpans];      // of the spans: what is over the cut
-            uint32_t count[kBins];       // of the levels
-            float queue[kMostWaves][128];
+            u64 listed[kList];   // (where list.listed is)
+            float queue[kMostWaves][kQueue];   // (where list.sorted is, which comes later)
+            u64 weight[kMostSpans];   // of the spans: what stays
         } wide;
     };
     double powers[64];   // 2^(-i / 64)
@@ -316,6 +360,7 @@ struct Shared {
     uint32_t groups[kMostGroups];
     u64 part[2][kMostWaves];
     uint32_t most[kMostWaves];
+    uint32_t least[kMostWaves];
     Range range;
     u64 word64[2];
     uint32_t word[4];
@@ -329,61 +374,24 @@ struct Piece {
     uint32_t have;    // elements that exist
 };
 
-template <int DT, int NT>
-struct Row {
-    using V = Vec16<DT>;
-    static constexpr uint32_t NE = V::NE;
-    static constexpr uint32_t kPer = kChunk<DT> / kGroup;
-    static constexpr uint32_t kLanes = kGroup / NE;
-    static constexpr uint32_t kTurn = NT / kLanes;   // groups of a turn
-    static constexpr uint32_t kShift = kIdle<DT>;
+// What the threads of a workgroup do together about a row.
+template <int NT>
+struct Team {
     static constexpr uint32_t kWaves = NT / 64;
-    static constexpr uint32_t kHeld = 4096 / NT;     // groups of a thread whose largest it holds, where all find room
-    static_assert(kWaves <= kMostWaves && kHeld % 4 == 0, "");
+    static_assert(kWaves <= kMostWaves, "");
 
     const SelectArgs &a;
     Shared &s;
     const uint64_t row;
-    const uint32_t *most;
-    const uint32_t ngroups;
-    uint32_t held[kHeld];
     uint32_t top;      // the largest number of the row
     double top_value;
     double c;          // log2(e) / T, where weights are asked for
     uint32_t flip;     // which partial sums are free
 
-    __device__ __forceinline__ Row(const SelectArgs &args, Shared &shared)
-        : a(args), s(shared), row(blockIdx.x), most(args.most + row * args.rows.nchunks * kPer), ngroups(args.rows.nchunks * kPer), c(0.0), flip(0)
+    __device__ __forceinline__ Team(const SelectArgs &args, Shared &shared, uint64_t of, uint32_t largest, double scale)
+        : a(args), s(shared), row(of), top(largest), top_value(value_of(largest)), c(scale), flip(0)
     {
-        uint32_t t = 0;
-        // (rows of the largest are whole vectors: a chunk has four or eight groups)
-#pragma unroll
-        for (uint32_t i = 0; i < kHeld; i += 4) {
-            const uint32_t at = threadIdx.x * kHeld + i;
-            const u32x4 v = at < ngroups ? *reinterpret_cast<const u32x4 *>(most + at) : u32x4{kNone, kNone, kNone, kNone};
-#pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) {
-                held[i + j] = v[j];
-                t = max(t, v[j]);
-            }
-        }
-        if (a.rows.nchunks <= kCached) {
-            for (uint32_t i = threadIdx.x; i < a.rows.nchunks; i += NT) {
-                const Stretch of = a.rows.chunks[i];
-                s.at[i] = reinterpret_cast<uint64_t>(of.at + row * of.step);
-                s.elems[i] = of.elems;
-            }
-        }
         if (threadIdx.x < 64) s.powers[threadIdx.x] = exp2_exact(threadIdx.x / -64.0);
-        for (uint32_t i = NT * kHeld + threadIdx.x; i < ngroups; i += NT) t = max(t, most[i]);
-        t = wave_most(t);
-        if ((threadIdx.x & 63) == 0) s.most[threadIdx.x / 64] = t;
-        __syncthreads();
-        t = s.most[0];
-#pragma unroll
-        for (uint32_t w = 1; w < kWaves; ++w) t = max(t, s.most[w]);
-        top = t;
-        top_value = value_of(top);
     }
 
     // Sums over the threads before this one, and over all.  One barrier: partial sums alternate between two places, and who is here for the
@@ -414,6 +422,195 @@ struct Row {
         return all;
     }
 
+    // exp((l - most) / T) times 2^up
+    __device__ __forceinline__ double share(float l, int up) const
+    {
+        const double far = power(s.powers, (top_value - l) * (64.0 * c), up);
+        return static_cast<double>(l) == top_value ? ldexp(1.0, up) : far;   // (of infinities too)
+    }
+    __device__ __forceinline__ double share(uint32_t number) const { return share(value_of(number), 0); }
+    // The same times 2^bits as a whole number: 2^52 added, the last place of a double is 1.
+    __device__ __forceinline__ u64 weight(float l) const
+    {
+        return static_cast<u64>(__double_as_longlong(share(l, static_cast<int>(a.bits)) + 0x1p52)) & ((u64(1) << 52) - 1);
+    }
+    __device__ __forceinline__ u64 weight(uint32_t number) const { return weight(value_of(number)); }
+
+    // Sorts s.list.listed[0 .. n) into s.list.sorted, descending.
+    __device__ __forceinline__ void sort(uint32_t n) const
+    {
+        uint32_t size = 64;
+        while (size < n) size *= 2;
+        const uint32_t t = threadIdx.x;
+        if (size <= NT) {   // an element per thread; a wavefront's own steps need no barrier
+            u64 x = t < n ? s.list.listed[t] : 0;
+            for (uint32_t width = 2; width <= size; width *= 2) {
+                for (uint32_t step = width / 2; step >= 1; step /= 2) {
+                    u64 y;
+                    if (step >= 64) {
+                        s.list.sorted[t] = x;
+                        __syncthreads();
+                        y = s.list.sorted[t ^ step];
+                        __syncthreads();
+                    } else {
+                        y = __shfl_xor(x, static_cast<int>(step), 64);
+                    }
+                    const bool larger = ((t & step) == 0) == ((t & width) == 0);
+                    x = (x > y) == larger ? x : y;
+                }
+            }
+            s.list.sorted[t] = x;
+            __syncthreads();
+            return;
+        }
+        for (uint32_t i = t; i < size; i += NT) s.list.sorted[i] = i < n ? s.list.listed[i] : 0;
+        __syncthreads();
+        for (uint32_t width = 2; width <= size; width *= 2) {
+            for (uint32_t step = width / 2; step >= 1; step /= 2) {
+                for (uint32_t k = t; k < size / 2; k += NT) {
+                    const uint32_t i = (k & ~(step - 1)) * 2 + (k & (step - 1));
+                    const u64 x = s.list.sorted[i], y = s.list.sorted[i + step];
+                    const bool down = (i & width) == 0;
+                    if ((x < y) == down) {
+                        s.list.sorted[i] = y;
+                        s.list.sorted[i + step] = x;
+                    }
+                }
+                __syncthreads();
+            }
+        }
+    }
+
+    // A short list (n <= kCounted), thread t < n: how many elements come before s.list.listed[t], and their weight, given the element's own.
+    // The threads share out the comparisons, whose sums meet in LDS.  (WEIGH false: the number alone.)
+    template <bool WEIGH>
+    __device__ __forceinline__ uint32_t count_before(uint32_t n, u64 own, u64 *weight_before)
+    {
+        static_assert(3 * kCounted <= kList && kCounted <= kMostGroups && kCounted <= NT, "");
+        u64 *const weights = s.list.sorted, *const sums = s.list.sorted + kCounted;
+        uint32_t *const ranks = s.groups;
+        if (threadIdx.x < kCounted) {
+            if (WEIGH) {
+                weights[threadIdx.x] = threadIdx.x < n ? own : 0;
+                sums[threadIdx.x] = 0;
+            }
+            ranks[threadIdx.x] = 0;
+            if (threadIdx.x >= n && threadIdx.x < ((n + 7) & ~7u)) s.list.listed[threadIdx.x] = 0;   // (comes before nothing)
+        }
+        __syncthreads();
+        uint32_t each = 64;   // threads of a share: all elements
+        while (each < n) each *= 2;
+        const uint32_t i = threadIdx.x & (each - 1);
+        const uint32_t shares = NT / each;
+        const uint32_t eights = (n + 7) / 8;
+        if (i < n) {
+            const u64 x = s.list.listed[i];
+            uint32_t rank = 0;
+            u64 sum = 0;
+            for (uint32_t k = threadIdx.x / each; k < eights; k += shares) {
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j) {
+                    const bool first = s.list.listed[k * 8 + j] > x;
+                    rank += first;
+                    if (WEIGH) sum += first ? weights[k * 8 + j] : 0;
+                }
+            }
+            atomicAdd(&ranks[i], rank);
+            if (WEIGH) atomicAdd(&sums[i], sum);
+        }
+        __syncthreads();
+        if (WEIGH) *weight_before = threadIdx.x < kCounted ? sums[threadIdx.x] : 0;
+        return threadIdx.x < kCounted ? ranks[threadIdx.x] : 0;
+    }
+
+    // whole: the sum of what could have been drawn, of exp((l - most) / T).
+    __device__ __forceinline__ void write_choice(uint32_t column, uint32_t number, double whole) const
+    {
+        a.choice.token[row] = static_cast<int32_t>(column);
+        if (a.choice.logprob != nullptr) {
+            const double x = number == top ? 0.0 : (static_cast<double>(value_of(number)) - top_value) * c * 0.69314718055994530942;
+            a.choice.logprob[row] = static_cast<float>(x - log(whole));
+        }
+    }
+    __device__ __forceinline__ double run_sum(uint32_t i) const   // of a run, of exp((l - most) / T)
+    {
+        const Run run = a.runs[row * a.nruns + i];
+        return run.sum * share(run.most, 0);
+    }
+};
+
+template <int DT, int NT>
+struct Row : Team<NT> {
+    using V = Vec16<DT>;
+    using B = Team<NT>;
+    using B::a;
+    using B::s;
+    using B::row;
+    using B::top;
+    using B::top_value;
+    using B::before;
+    using B::total;
+    using B::weight;
+    using B::kWaves;
+    static constexpr uint32_t NE = V::NE;
+    static constexpr uint32_t kPer = kChunk<DT> / kGroup;
+    static constexpr uint32_t kLanes = kGroup / NE;
+    static constexpr uint32_t kTurn = NT / kLanes;   // groups of a turn
+    static constexpr uint32_t kShift = kIdle<DT>;
+    static constexpr uint32_t kHeld = 4096 / NT;     // groups of a thread whose largest it holds, where all find room
+    static_assert(kHeld % 4 == 0, "");
+
+    const uint32_t *most;
+    const uint32_t ngroups;
+    uint32_t held[kHeld];
+    uint32_t bottom;   // the least of the groups' largest
+
+    __device__ __forceinline__ Row(const SelectArgs &args, Shared &shared, uint64_t of)
+        : Team<NT>(args, shared, of, 0, 0.0), most(args.most + of * args.rows.nchunks * kPer), ngroups(args.rows.nchunks * kPer)
+    {
+        uint32_t t = 0, least = kNoEnd;
+        // (rows of the largest are whole vectors: a chunk has four or eight groups)
+#pragma unroll
+        for (uint32_t i = 0; i < kHeld; i += 4) {
+            const uint32_t at = threadIdx.x * kHeld + i;
+            const u32x4 v = at < ngroups ? *reinterpret_cast<const u32x4 *>(most + at) : u32x4{kNone, kNone, kNone, kNone};
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                held[i + j] = v[j];
+                t = max(t, v[j]);
+                least = min(least, v[j] != kNone ? v[j] : kNoEnd);
+            }
+        }
+        if (a.rows.nchunks <= kCached) {
+            for (uint32_t i = threadIdx.x; i < a.rows.nchunks; i += NT) {
+                const Stretch of = a.rows.chunks[i];
+                s.at[i] = reinterpret_cast<uint64_t>(of.at + row * of.step);
+                s.elems[i] = of.elems;
+            }
+        }
+        for (uint32_t i = NT * kHeld + threadIdx.x; i < ngroups; i += NT) {
+            t = max(t, most[i]);
+            least = min(least, most[i] != kNone ? most[i] : kNoEnd);
+        }
+        t = wave_most(t);
+        least = ~wave_most(~least);
+        if ((threadIdx.x & 63) == 0) {
+            s.most[threadIdx.x / 64] = t;
+            s.least[threadIdx.x / 64] = least;
+        }
+        __syncthreads();
+        t = s.most[0];
+        least = s.least[0];
+#pragma unroll
+        for (uint32_t w = 1; w < kWaves; ++w) {
+            t = max(t, s.most[w]);
+            least = min(least, s.least[w]);
+        }
+        top = t;
+        bottom = least;
+        top_value = value_of(top);
+    }
+
     // f(group, its largest) of neighbouring groups per thread, in their order
     template <typename F>
     __device__ __forceinline__ void each_group(F &&f) const
@@ -427,19 +624,6 @@ struct Row {
             for (uint32_t i = from; i < to; ++i) f(i, most[i]);
         }
     }
-
-    // exp((l - most) / T) times 2^up
-    __device__ __forceinline__ double share(float l, int up) const
-    {
-        return static_cast<double>(l) == top_value ? ldexp(1.0, up) : power(s.powers, (top_value - l) * (64.0 * c), up);
-    }
-    __device__ __forceinline__ double share(uint32_t number) const { return share(value_of(number), 0); }
-    // The same times 2^bits as a whole number: 2^52 added, the last place of a double is 1.
-    __device__ __forceinline__ u64 weight(float l) const
-    {
-        return static_cast<u64>(__double_as_longlong(share(l, static_cast<int>(a.bits)) + 0x1p52)) & ((u64(1) << 52) - 1);
-    }
-    __device__ __forceinline__ u64 weight(uint32_t number) const { return weight(value_of(number)); }
 
     // Where the row's part of a chunk lies, and how much it has.
     __device__ __forceinline__ const char *chunk_at(uint32_t chunk, uint32_t *elems) const
@@ -655,12 +839,13 @@ struct Row {
         uint32_t equal = kNoEnd;   // of the groups whose largest is low, the first so many
         const uint32_t enough = max(k + k / 2 + 32, kList / kGroup);
         if (ngroups > enough) {
-            g.low = kLeast >> kShift;
+            g.low = bottom >> kShift;
             do {
                 narrow<false>(g, [&](auto &&f) { each_group([&](uint32_t, uint32_t n) { f(n >> kShift, [] { return u64(0); }); }); },
                               [&](u64) { return u64(k); });
             } while (g.above + g.inside > enough && g.low != g.high);
             if (g.above + g.inside > enough) equal = k - g.above;   // (groups left out may hold what is listed of the others)
+            if (g.above + g.inside < k) g.low = 0;   // (fewer groups than k: many ranks of few columns)
         }
         uint32_t n = 0;
         {
@@ -715,107 +900,6 @@ struct Row {
         return listed;
     }
 
-    // Sorts s.list.listed[0 .. n) into s.list.sorted, descending.
-    __device__ __forceinline__ void sort(uint32_t n) const
-    {
-        uint32_t size = 64;
-        while (size < n) size *= 2;
-        const uint32_t t = threadIdx.x;
-        if (size <= NT) {   // an element per thread; a wavefront's own steps need no barrier
-            u64 x = t < n ? s.list.listed[t] : 0;
-            for (uint32_t width = 2; width <= size; width *= 2) {
-                for (uint32_t step = width / 2; step >= 1; step /= 2) {
-                    u64 y;
-                    if (step >= 64) {
-                        s.list.sorted[t] = x;
-                        __syncthreads();
-                        y = s.list.sorted[t ^ step];
-                        __syncthreads();
-                    } else {
-                        y = __shfl_xor(x, static_cast<int>(step), 64);
-                    }
-                    const bool larger = ((t & step) == 0) == ((t & width) == 0);
-                    x = (x > y) == larger ? x : y;
-                }
-            }
-            s.list.sorted[t] = x;
-            __syncthreads();
-            return;
-        }
-        for (uint32_t i = t; i < size; i += NT) s.list.sorted[i] = i < n ? s.list.listed[i] : 0;
-        __syncthreads();
-        for (uint32_t width = 2; width <= size; width *= 2) {
-            for (uint32_t step = width / 2; step >= 1; step /= 2) {
-                for (uint32_t k = t; k < size / 2; k += NT) {
-                    const uint32_t i = (k & ~(step - 1)) * 2 + (k & (step - 1));
-                    const u64 x = s.list.sorted[i], y = s.list.sorted[i + step];
-                    const bool down = (i & width) == 0;
-                    if ((x < y) == down) {
-                        s.list.sorted[i] = y;
-                        s.list.sorted[i + step] = x;
-                    }
-                }
-                __syncthreads();
-            }
-        }
-    }
-
-    // A short list (n <= kCounted), thread t < n: how many elements come before s.list.listed[t], and their weight, given the element's own.
-    // The threads share out the comparisons, whose sums meet in LDS.  (WEIGH false: the number alone.)
-    template <bool WEIGH>
-    __device__ __forceinline__ uint32_t count_before(uint32_t n, u64 own, u64 *weight_before)
-    {
-        static_assert(3 * kCounted <= kList && kCounted <= kMostGroups && kCounted <= NT, "");
-        u64 *const weights = s.list.sorted, *const sums = s.list.sorted + kCounted;
-        uint32_t *const ranks = s.groups;
-        if (threadIdx.x < kCounted) {
-            if (WEIGH) {
-                weights[threadIdx.x] = threadIdx.x < n ? own : 0;
-                sums[threadIdx.x] = 0;
-            }
-            ranks[threadIdx.x] = 0;
-            if (threadIdx.x >= n && threadIdx.x < ((n + 7) & ~7u)) s.list.listed[threadIdx.x] = 0;   // (comes before nothing)
-        }
-        __syncthreads();
-        uint32_t each = 64;   // threads of a share: all elements
-        while (each < n) each *= 2;
-        const uint32_t i = threadIdx.x & (each - 1);
-        const uint32_t shares = NT / each;
-        const uint32_t eights = (n + 7) / 8;
-        if (i < n) {
-            const u64 x = s.list.listed[i];
-            uint32_t rank = 0;
-            u64 sum = 0;
-            for (uint32_t k = threadIdx.x / each; k < eights; k += shares) {
-#pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) {
-                    const bool first = s.list.listed[k * 8 + j] > x;
-                    rank += first;
-                    if (WEIGH) sum += first ? weights[k * 8 + j] : 0;
-                }
-            }
-            atomicAdd(&ranks[i], rank);
-            if (WEIGH) atomicAdd(&sums[i], sum);
-        }
-        __syncthreads();
-        if (WEIGH) *weight_before = threadIdx.x < kCounted ? sums[threadIdx.x] : 0;
-        return threadIdx.x < kCounted ? ranks[threadIdx.x] : 0;
-    }
-
-    // whole: the sum of what could have been drawn, of exp((l - most) / T).
-    __device__ __forceinline__ void write_choice(uint32_t column, uint32_t number, double whole) const
-    {
-        a.choice.token[row] = static_cast<int32_t>(column);
-        if (a.choice.logprob != nullptr) {
-            const double x = number == top ? 0.0 : (static_cast<double>(value_of(number)) - top_value) * c * 0.69314718055994530942;
-            a.choice.logprob[row] = static_cast<float>(x - log(whole));
-        }
-    }
-    __device__ __forceinline__ double run_sum(uint32_t i) const   // of a run, of exp((l - most) / T)
-    {
-        const Run run = a.runs[row * a.nruns + i];
-        return run.sum * share(run.most, 0);
-    }
 };
 
 template <int DT, int NT>
@@ -824,7 +908,7 @@ k_top_logits(SelectArgs a)
 {
     using D = DTypeOf<DT>;
     __shared__ Shared s;
-    Row<DT, NT> r(a, s);
+    Row<DT, NT> r(a, s, blockIdx.x);
     r.c = 1.4426950408889634074;   // (of the sum)
     uint32_t sure;
     const uint32_t n = r.list_first(a.k, &sure);
@@ -986,11 +1070,14 @@ __device__ __forceinline__ void draw_all(const SelectArgs &a, Row<DT, NT> &r, Sh
     double aim = static_cast<double>(u) * whole;
     if (!(aim > 0.0)) aim = 0.0;
     // the last run that begins at or before the aim and has anything (sums are rounded: the aim may lie behind all)
+    uint32_t last = 0;
     for (uint32_t i = from; i < to; ++i) {
-        const double w = r.run_sum(i);
-        if (w > 0.0 && at <= aim) atomicMax(&s.word[0], i + 1);
+        const double w = each == 1 ? mine : r.run_sum(i);
+        if (w > 0.0 && at <= aim) last = i + 1;
         at += w;
     }
+    last = wave_most(last);
+    if (lane == 0 && last != 0) atomicMax(&s.word[0], last);
     __syncthreads();
     const uint32_t run = s.word[0] - 1;
     if (run >= from && run < to) {
@@ -1016,11 +1103,14 @@ __device__ __forceinline__ void draw_all(const SelectArgs &a, Row<DT, NT> &r, Sh
     double all;
     at = r.before(sum, &all);
     at += __builtin_bit_cast(double, s.word64[0]);
+    last = 0;
 #pragma unroll
     for (uint32_t e = 0; e < NE; ++e) {
-        if (w[e] > 0.0 && at <= aim) atomicMax(&s.word[1], threadIdx.x * NE + e + 1);
+        if (w[e] > 0.0 && at <= aim) last = threadIdx.x * NE + e + 1;
         at += w[e];
     }
+    last = wave_most(last);
+    if (lane == 0 && last != 0) atomicMax(&s.word[1], last);
     __syncthreads();
     const uint32_t place = s.word[1] - 1;
     if (place / NE != threadIdx.x) return;
@@ -1030,329 +1120,551 @@ __device__ __forceinline__ void draw_all(const SelectArgs &a, Row<DT, NT> &r, Sh
     }
 }
 
-// What stays of a row is more than a list holds.  Elements are counted by levels, 64 to a power of two of their weight.  The level that
-// the cut lies in is found by the counts, for top_k exactly, for top_p with a level's middle for its weights, which is wrong by a level now
-// and then; the elements over that level are weighed, a span of chunks at a time, and those in it are listed and sorted.  That says where
-// the cut is, or in which direction to look for it.  sure: so many first elements are in s.list.sorted.
-// Returns false, and nothing is drawn, where a level holds more than a list, or the cut is behind the last.
-//
-// Weights take some forty instructions of 64 bits, and few elements are over the cut: a wavefront collects what it finds in a queue
-// and weighs 64 at a time.
+// The cut is searched by numbers, among all elements, and chunks are weighed: right for every row, but one workgroup goes through all
+// of it several times.
 template <int DT, int NT>
-__device__ __forceinline__ bool draw_wide(const SelectArgs &a, Row<DT, NT> &r, Shared &s, const RowChoice &choice, float u, u64 p_of_whole, uint32_t sure)
+__device__ __forceinline__ void draw_by_numbers(const SelectArgs &a, Row<DT, NT> &r, Shared &s, const RowChoice &choice, float u, u64 p_of_whole)
 {
-    using R = Row<DT, NT>;
-    constexpr uint32_t NE = R::NE;
-    constexpr uint32_t kMine = kBins / NT;
-    constexpr uint32_t kListed = kList / NT;
-    constexpr uint32_t kSpans = kMostSpans / NT < 1 ? 1 : kMostSpans / NT;
-    constexpr uint32_t kNoLevel = 0xffffffffu;
-    constexpr int kRounds = 8;
-    static_assert(R::kWaves >= kSpan, "a wavefront for each chunk of a span");
-    const uint32_t nspans = (a.rows.nchunks + kSpan - 1) / kSpan;
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const float top = static_cast<float>(r.top_value);
-    const float scale = static_cast<float>(64.0 * r.c);
-    if (nspans > kMostSpans || top == __builtin_inff() || !(scale >= 0x1p-80f && scale <= 0x1p80f)) return false;
-    // (minus infinity: the conversion is to the nearest that there is)
-    auto level_of = [&](float l) { return min(static_cast<uint32_t>(fminf((top - l) * scale, 65536.0f)), kBins - 1); };
-    // the least value of a level over `level`: numbers fall with it, so the first of them is searched, 64 places at a time
-    auto least_over = [&](uint32_t level) {
-        uint32_t low = kLeast, high = r.top;   // low: at the level or below it, high: over it
-        while (high - low > 1) {
-            const uint32_t step = (high - low + 63) / 64;
-            const uint32_t n = low + (lane + 1) * step;
-            const bool below = n < high && n > low && level_of(value_of(n)) >= level;
-            const uint32_t many = __popcll(__ballot(below));
-            const uint32_t next = low + many * step;
-            high = min(next + step, high);
-            low = next;
-        }
-        return value_of(high);
-    };
-    const double unit = ldexp(1.0, -static_cast<int>(a.bits));
-    const bool by_level = choice.by_k || choice.by_p;
-    bool only_least = !by_level;   // of all filters min_p alone
-    uint32_t level = kNoLevel;     // the cut's
-    uint32_t level_count = 0, level_over = 0;       // elements in it, and over it
-    double level_weight = 0.0, weight_over = 0.0;   // by the middles
-    uint32_t counts[kMine];
-    double middle[kMine];
-    uint32_t over_mine = 0;
-    double weight_mine = 0.0;
-    // Of the levels low .. high - 1 the first at which the running count reaches top_k, or the running weight and `more` reaches aim; or else the
-    // last that holds anything.
-    auto find_level = [&](bool by_count, double more, double aim, uint32_t low, uint32_t high) {
-        if (threadIdx.x == 0) {
-            s.word[0] = kNoLevel;
-            s.word[1] = 0;
-        }
-        __syncthreads();
-        uint32_t n = over_mine;
-        double w = weight_mine;
-#pragma unroll
-        for (uint32_t i = 0; i < kMine; ++i) {
-            const uint32_t l = threadIdx.x * kMine + i;
-            n += counts[i];
-            w += middle[i];
-            if (l < low || l >= high || counts[i] == 0) continue;
-            if (by_count ? n >= choice.k : w + more >= aim) atomicMin(&s.word[0], l);
-            atomicMax(&s.word[1], l + 1);
-        }
-        __syncthreads();
-        level = min(s.word[0], s.word[1] - 1);   // (none: kNoLevel)
-        if (level / kMine == threadIdx.x) {
-            n = over_mine;
-            w = weight_mine;
-#pragma unroll
-            for (uint32_t i = 0; i < kMine; ++i) {
-                if (threadIdx.x * kMine + i == level) {
-                    s.word[2] = counts[i];
-                    s.word[3] = n;
-                    s.word64[0] = __builtin_bit_cast(u64, middle[i]);
-                    s.word64[1] = __builtin_bit_cast(u64, w);
-                }
-                n += counts[i];
-                w += middle[i];
-            }
-        }
-        __syncthreads();
-        level_count = s.word[2];
-        level_over = s.word[3];
-        level_weight = __builtin_bit_cast(double, s.word64[0]);
-        weight_over = __builtin_bit_cast(double, s.word64[1]);
-    };
-    uint32_t low = 0, high = kBins;   // levels that are left
-    u64 aim_p = p_of_whole;
-    if (by_level) {
-        // what the list says of the levels that it holds whole
-        u64 listed = 0;
-        if (sure != 0) {
-            low = level_of(value_of(static_cast<uint32_t>(s.list.sorted[sure - 1] >> 32)));
-            for (uint32_t i = threadIdx.x; i < sure; i += NT) {
-                const float l = value_of(static_cast<uint32_t>(s.list.sorted[i] >> 32));
-                if (level_of(l) < low) listed += r.weight(l);
-            }
-        }
-        for (uint32_t i = threadIdx.x; i < kBins; i += NT) s.wide.count[i] = 0;
-        __syncthreads();
-        // What is so improbable that even as many as there are columns hold no more than 1 - top_p of the whole lies behind the cut.
-        float far = minus_infinity();
-        if (!choice.by_k) {
-            const double behind = (static_cast<double>(p_of_whole) / choice.p - static_cast<double>(p_of_whole)) * unit / a.rows.vocab;
-            if (behind > 0.0) far = static_cast<float>(r.top_value + log2(behind) / r.c - 2.0 / scale);
-        }
-        r.each_piece(nullptr, r.ngroups, [&](const Piece &p, const float (&v)[NE]) {
-#pragma unroll
-            for (uint32_t e = 0; e < NE; ++e) {
-                if (e < p.have && v[e] >= far) atomicAdd(&s.wide.count[level_of(v[e])], 1u);
-            }
-        });
-        __syncthreads();
-        uint32_t sum = 0, all;
-        double w = 0.0, whole;
-#pragma unroll
-        for (uint32_t i = 0; i < kMine; ++i) {
-            const uint32_t l = threadIdx.x * kMine + i;
-            sum += counts[i] = s.wide.count[l];
-            w += middle[i] = counts[i] * ldexp(s.powers[l & 63] * 0.99459942348363317565, -static_cast<int>(l >> 6));   // (2^(-1 / 128))
-        }
-        over_mine = r.before(sum, &all);
-        weight_mine = r.before(w, &whole);
-        if (choice.by_k) {
-            find_level(true, 0.0, 0.0, 0, high);
-            high = level + 1;
-        } else {
-            if (low / kMine == threadIdx.x) {
-                w = weight_mine;
-#pragma unroll
-                for (uint32_t i = 0; i < kMine; ++i) w += threadIdx.x * kMine + i < low ? middle[i] : 0.0;
-                s.word64[0] = __builtin_bit_cast(u64, w);
-            }
-            listed = r.total(listed);
-            const double others = __builtin_bit_cast(double, s.word64[0]);
-            find_level(false, listed * unit - others, aim_p * unit, low, high);
-        }
+    constexpr uint32_t kShift = kIdle<DT>;
+    __syncthreads();   // the lists make room
+    Kept stay = {0, kNoEnd, choice.by_min ? choice.least : 0.0};
+    auto all = [&](auto &&f) { r.each(nullptr, r.ngroups, f); };
+    Range range = {kLeast >> kShift, r.top >> kShift, 0, 0, 0, 0};
+    uint32_t cut_count = 0;
+    if (choice.by_k) {
+        do {
+            r.template narrow<false>(range, all, [&](u64) { return u64(choice.k); });
+        } while (range.low != range.high);
+        stay.cut = range.low;
+        stay.equal = choice.k - range.above;
+        cut_count = range.inside;
     }
-    bool count_known = !choice.by_k;
-    u64 last = 0;   // the last that stays of the level's, as the list has it
-    for (int round = 0;; ++round) {
-        if (!only_least && (level >= kBins - 1 || level_count > kList || round == kRounds)) return false;
-        // weights over the level by spans, and the level's list
-        float over = minus_infinity(), in = minus_infinity();
-        if (!only_least) {
-            over = level == 0 ? __builtin_inff() : least_over(level);
-            in = least_over(level + 1);
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) s.word[2] = 0;
-        __syncthreads();
-        float *const queue = s.wide.queue[wave];
-        for (uint32_t span = wave; span < nspans; span += R::kWaves) {
-            u32x4 raw[kSpan];
-            uint32_t elems[kSpan];
-#pragma unroll
-            for (uint32_t k = 0; k < kSpan; ++k) {
-                const uint32_t chunk = span * kSpan + k;
-                const char *at = r.chunk_at(chunk < a.rows.nchunks ? chunk : 0, &elems[k]);
-                elems[k] = chunk < a.rows.nchunks ? elems[k] : 0;
-                raw[k] = load_piece<DT, false>(at, lane, elems[k]);
-            }
-            u64 sum = 0;
-            uint32_t queued = 0;
-            auto weigh = [&](bool live, float l) {
-                if (only_least && !(r.share(l, 0) >= choice.least)) live = false;
-                sum += live ? r.weight(l) : 0;
-            };
-#pragma unroll
-            for (uint32_t k = 0; k < kSpan; ++k) {
-                float v[NE];
-                R::V::unpack(raw[k], v);
-#pragma unroll
-                for (uint32_t e = 0; e < NE; ++e) {
-                    const bool there = lane * NE + e < elems[k];
-                    const uint64_t who = __ballot(there && v[e] >= over);
-                    if (!only_least && there && v[e] >= in && !(v[e] >= over)) {
-                        const uint32_t i = atomicAdd(&s.word[2], 1u);
-                        const uint32_t place = (span * kSpan + k) * kChunk<DT> + lane * NE + e;
-                        if (i < kList) s.wide.listed[i] = static_cast<u64>(number_of(v[e])) << 32 | static_cast<uint32_t>(~place);
-                    }
-                    if (who == 0) continue;
-                    const uint32_t at = queued + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(who >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(who), 0));
-                    if (who >> lane & 1) queue[at] = v[e];
-                    queued += __popcll(who);
-                    if (queued >= 64) {
-                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                        queued -= 64;
-                        weigh(true, queue[queued + lane]);
-                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                    }
-                }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            if (queued != 0) weigh(lane < queued, queue[lane < queued ? lane : 0]);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            sum = wave_total(sum);
-            if (lane == 0) s.wide.weight[span] = sum;
-        }
-        __syncthreads();
-        if (only_least) break;
-        u64 sum = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < kSpans; ++i) {
-            const uint32_t span = threadIdx.x * kSpans + i;
-            if (span < nspans) sum += s.wide.weight[span];
-        }
-        const u64 above = r.total(sum);
-        r.sort(level_count);
-        u64 w[kListed];
-        sum = 0;
-        uint32_t stay = choice.by_k && !count_known ? choice.k - level_over : level_count;
-#pragma unroll
-        for (uint32_t i = 0; i < kListed; ++i) {
-            const uint32_t place = threadIdx.x * kListed + i;
-            sum += w[i] = place < stay ? r.weight(static_cast<uint32_t>(s.wide.sorted[place] >> 32)) : 0;
-        }
-        u64 inside;
-        u64 at = above + r.before(sum, &inside);
-        if (!count_known) {
-            count_known = true;
-            aim_p = part_of(choice.p, static_cast<double>(above + inside));
-        }
-        if (choice.by_p) {
-            const bool up = aim_p <= above && level_over != 0;
-            if (up || (above + inside < aim_p && level + 1 < high)) {
-                const double more = (up ? above : above + inside) * unit - (up ? weight_over : weight_over + level_weight);
-                (up ? high : low) = up ? level : level + 1;
-                find_level(false, more, aim_p * unit, low, high);
-                if (level == kNoLevel) return false;
-                continue;
-            }
-            uint32_t keep = 0;
-#pragma unroll
-            for (uint32_t i = 0; i < kListed; ++i) {
-                const uint32_t place = threadIdx.x * kListed + i;
-                keep += place < stay && ((level_over == 0 && place == 0) || at < aim_p);
-                at += w[i];
-            }
-            stay = r.total(keep);
-        }
-        last = s.wide.sorted[stay - 1];
-        if (choice.by_min && !(r.share(static_cast<uint32_t>(last >> 32)) >= choice.least)) {
-            only_least = true;   // it asks for more than the others
-            continue;
-        }
-        // those of the level that stay, to their spans
-#pragma unroll
-        for (uint32_t i = 0; i < kListed; ++i) {
-            const uint32_t place = threadIdx.x * kListed + i;
-            if (place < stay && w[i] != 0) atomicAdd(&s.wide.weight[~static_cast<uint32_t>(s.wide.sorted[place]) / (kSpan * kChunk<DT>)], w[i]);
-        }
-        __syncthreads();
-        break;
+    if (choice.by_p) {
+        range = {stay.cut > kLeast >> kShift ? stay.cut : kLeast >> kShift, r.top >> kShift, 0, 0, 0, 0};
+        u64 aim = 0;
+        bool first = true;
+        // (what is equal to the cut of top_k and does not stay is at the end of the order)
+        const u64 over = choice.by_k && cut_count > stay.equal ? (cut_count - stay.equal) * r.weight(stay.cut << kShift | (stay.cut >> (31 - kShift) != 0 ? 0 : (1u << kShift) - 1)) : 0;
+        do {
+            r.template narrow<true>(range, all, [&](u64 whole) {
+                if (first) aim = max(u64(1), min(choice.by_k ? part_of(choice.p, static_cast<double>(whole - over)) : p_of_whole, whole));
+                return aim;
+            });
+            first = false;
+        } while (range.low != range.high);
+        const u64 one = range.inside != 0 ? range.weight_inside / range.inside : 1;
+        const u64 need = one != 0 ? (aim - range.weight_above + one - 1) / one : 1;
+        const uint32_t equal = static_cast<uint32_t>(min(need, static_cast<u64>(range.inside)));
+        stay.equal = stay.cut == range.low && choice.by_k ? min(stay.equal, equal) : equal;
+        stay.cut = range.low;
     }
-    // the span, then the element: a wavefront for each chunk
-    u64 sum = 0;
-    u64 w[kSpans];
-#pragma unroll
-    for (uint32_t i = 0; i < kSpans; ++i) {
-        const uint32_t span = threadIdx.x * kSpans + i;
-        sum += w[i] = span < nspans ? s.wide.weight[span] : 0;
-    }
-    u64 whole;
-    u64 at = r.before(sum, &whole);
-    const u64 aim = aim_of(u, whole);
-#pragma unroll
-    for (uint32_t i = 0; i < kSpans; ++i) {
-        if (aim >= at && aim - at < w[i]) {
-            s.word[0] = threadIdx.x * kSpans + i;
-            s.word64[0] = at;
-        }
-        at += w[i];
-    }
+    if (threadIdx.x == 0) s.one = 0;
     __syncthreads();
-    const uint32_t chunk = s.word[0] * kSpan + wave;
-    const bool there = wave < kSpan && chunk < a.rows.nchunks;
-    const Stretch t = a.rows.chunks[there ? chunk : 0];
-    const uint32_t elems = there ? t.elems : 0;
-    const u32x4 raw = load_piece<DT, false>(t.at + r.row * t.step, lane, elems);
-    float v[NE];
-    R::V::unpack(raw, v);
-    u64 each[NE];
-    sum = 0;
-#pragma unroll
-    for (uint32_t e = 0; e < NE; ++e) {
-        const float l = no_nan(v[e]);
-        bool in = lane * NE + e < elems;
-        if (only_least) {
-            in = in && r.share(l, 0) >= choice.least;
-        } else {
-            const uint32_t of = level_of(l);
-            const u64 x = static_cast<u64>(number_of(l)) << 32 | static_cast<uint32_t>(~(chunk * kChunk<DT> + lane * NE + e));
-            in = in && (of < level || (of == level && x >= last));
-        }
-        sum += each[e] = in ? r.weight(l) : 0;
-    }
-    u64 all;
-    at = s.word64[0] + r.before(sum, &all);
-#pragma unroll
-    for (uint32_t e = 0; e < NE; ++e) {
-        if (aim >= at && aim - at < each[e]) r.write_choice(t.first + lane * NE + e, number_of(no_nan(v[e])), static_cast<double>(whole) * unit);
-        at += each[e];
-    }
-    return true;
+    draw_kept(a, r, s, stay, u);
 }
 
+// Distances from the row's largest in levels.
+struct Distance {
+    float top;
+    float scale;   // 64 log2(e) / T
+    bool fits;     // whether a row has levels
+    __device__ __forceinline__ Distance(double top_value, double c) : top(static_cast<float>(top_value)), scale(static_cast<float>(64.0 * c))
+    {
+        fits = top != __builtin_inff() && scale >= 0x1p-80f && scale <= 0x1p80f;
+    }
+    __device__ __forceinline__ float operator()(float l) const { return (top - l) * scale; }   // (NaN of NaN)
+};
+// (minus infinity: the conversion is to the nearest that there is)
+__device__ __forceinline__ uint32_t level_of(float x) { return min(static_cast<uint32_t>(fminf(x, 65536.0f)), kLevels - 1); }
+
+// What a level holds is one word: its elements, times 2^40, and what they lack of the weight that they would have at the level's upper
+// end, in parts of 2^22 of that: 1 - 2^(-f / 64) for an element f of a level further down, of which two terms do.  Rounding to such
+// parts costs the sum over a level some 2^-23 of itself at random, so which level holds the cut of top_p is known but for one in many
+// thousands of rows; the fourth launch finds out.
+constexpr float kLack = 0x1p22f;
+__device__ __forceinline__ u64 level_entry(float x, uint32_t level)
+{
+    const float z = (x - static_cast<float>(level)) * static_cast<float>(0.69314718055994530942 / 64);
+    return u64(1) << 40 | static_cast<uint32_t>(rintf((z - 0.5f * z * z) * kLack));
+}
+__device__ __forceinline__ uint32_t entry_count(u64 e) { return static_cast<uint32_t>(e >> 40); }
+__device__ __forceinline__ double entry_weight(u64 e, double at_end)
+{
+    return at_end * (entry_count(e) - static_cast<double>(e & ((u64(1) << 40) - 1)) * (1.0 / kLack));
+}
+
+// Whether the third and fourth launch can draw from a row: not where the weight that top_p asks for goes by a cut of top_k.
+__device__ __forceinline__ bool is_wide(const RowChoice &choice, double top_value)
+{
+    return !(choice.by_k && choice.by_p) && Distance(top_value, choice.c).fits;
+}
+
+// The chunks first .. last - 1 of a part of the third and fourth launch.
+struct WidePart {
+    uint32_t slot;
+    uint32_t from;   // spans
+    uint32_t to;
+    __device__ __forceinline__ explicit WidePart(const SelectArgs &a) : slot(blockIdx.x / a.wide_parts)
+    {
+        const uint32_t part = blockIdx.x % a.wide_parts;
+        from = a.nspans * part / a.wide_parts;
+        to = a.nspans * (part + 1) / a.wide_parts;
+    }
+};
+
+// The third launch: the elements of a part by levels.
+template <int DT, int NT>
+__global__ void __launch_bounds__(NT)
+k_sample_levels(SelectArgs a)
+{
+    using V = Vec16<DT>;
+    constexpr uint32_t NE = V::NE;
+    constexpr uint32_t kWaves = NT / 64;
+    constexpr int kAhead = 4;
+    __shared__ u64 s_levels[kLevels];
+    const WidePart part(a);
+    const Wide &w = a.wide[part.slot];
+    if (w.wide == 0) return;
+    const uint64_t row = a.first + part.slot;
+    const RowChoice choice(a.choice, row, a.rows.vocab);
+    if (!choice.by_k && !choice.by_p) return;   // (min_p says itself how far it reaches)
+    for (uint32_t i = threadIdx.x; i < kLevels; i += NT) s_levels[i] = 0;
+    const double top_value = value_of(w.top);
+    const Distance distance(top_value, choice.c);
+    // What is so improbable that even as many as there are columns hold no more than 1 - top_p of the whole lies behind the cut.
+    float far = __builtin_inff();
+    if (!choice.by_k) {
+        const double behind = (static_cast<double>(w.p_of_whole) / choice.p - static_cast<double>(w.p_of_whole)) * ldexp(1.0, -static_cast<int>(a.bits)) / a.rows.vocab;
+        if (behind > 0.0) far = static_cast<float>(-64.0 * log2(behind)) + 2.0f;
+    }
+    __syncthreads();
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t to = min(part.to * a.span, a.rows.nchunks);
+    for (uint32_t first = part.from * a.span + __builtin_amdgcn_readfirstlane(threadIdx.x / 64); first < to; first += kWaves * kAhead) {
+        u32x4 raw[kAhead];
+        uint32_t elems[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const uint32_t i = first + k * kWaves;
+            const Stretch t = a.rows.chunks[i < to ? i : first];
+            elems[k] = i < to ? t.elems : 0;
+            raw[k] = load_piece<DT, false>(t.at + row * t.step, lane, elems[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            float v[NE];
+            V::unpack(raw[k], v);
+#pragma unroll
+            for (uint32_t e = 0; e < NE; ++e) {
+                const float x = distance(v[e]);
+                if (!(x <= far) || lane * NE + e >= elems[k]) continue;
+                const uint32_t level = level_of(x);
+                // (what is in the last one is not told apart)
+                atomicAdd(&s_levels[level], level == kLevels - 1 ? u64(1) << 40 : level_entry(x, level));
+            }
+        }
+    }
+    __syncthreads();
+    u64 *all = a.levels + static_cast<uint64_t>(part.slot) * kLevels;
+    for (uint32_t i = threadIdx.x; i < kLevels; i += NT) {
+        if (s_levels[i] != 0) atomicAdd(&all[i], s_levels[i]);
+    }
+}
+
+template <int NT>
+__device__ __forceinline__ Band band_of(const SelectArgs &a, Team<NT> &r, Shared &s, const RowChoice &choice, const Wide &w, const u64 *levels)
+{
+    constexpr uint32_t kMine = kLevels / NT;
+    const Distance distance(r.top_value, r.c);
+    Band band = {-1.0f, __builtin_inff(), choice.by_k || choice.by_p, choice.by_min, true};
+    if (band.by_level) {
+        // levels are as far apart as the rounded scale has them
+        const double apart = r.c / static_cast<double>(distance.scale);
+        if (threadIdx.x == 0) s.word[0] = kLevels;
+        uint32_t counts[kMine];
+        double weights[kMine];
+        uint32_t count = 0, all;
+        double weight = 0.0, whole;
+#pragma unroll
+        for (uint32_t i = 0; i < kMine; ++i) {
+            const uint32_t level = threadIdx.x * kMine + i;
+            const u64 e = levels[level];
+            count += counts[i] = entry_count(e);
+            weight += weights[i] = counts[i] == 0 ? 0.0 : entry_weight(e, exp2_exact(-(level * apart)));
+        }
+        count = r.before(count, &all);
+        weight = r.before(weight, &whole);
+        const double aim = ldexp(static_cast<double>(w.p_of_whole), -static_cast<int>(a.bits));
+#pragma unroll
+        for (uint32_t i = 0; i < kMine; ++i) {
+            const bool by_k = choice.by_k && count < choice.k && count + counts[i] >= choice.k;
+            const bool by_p = !choice.by_k && weight < aim && weight + weights[i] >= aim;
+            if (counts[i] != 0 && (by_k || by_p)) s.word[0] = threadIdx.x * kMine + i;
+            count += counts[i];
+            weight += weights[i];
+        }
+        __syncthreads();
+        const uint32_t level = s.word[0];
+        __syncthreads();
+        band.known = level < kLevels - 1;
+        band.low = static_cast<float>(level);
+        band.high = static_cast<float>(level + 1);
+    }
+    if (band.by_min && band.known) {
+        // (distances are good to 2^-22 of themselves, and none that matters is over 2^14)
+        const float at = static_cast<float>(-log2(choice.least) / r.c * static_cast<double>(distance.scale));
+        const float low = at - 0.01f, high = at + 0.01f;
+        if (!band.by_level || high <= band.low) {
+            band.by_level = false;
+            band.low = low;
+            band.high = high;
+        } else if (low >= band.high) {
+            band.by_min = false;
+        } else {
+            band.low = fminf(low, band.low);
+            band.high = fmaxf(high, band.high);
+        }
+    }
+    return band;
+}
+
+// Weighs a wavefront's chunk: the elements nearer than the band (their weight is returned in every lane, their number is added to `over`), and
+// lists those in it.  Few of many elements may be that near, and a weight takes some thirty instructions of 64 bits: they are
+// gathered in LDS, and weighed by all lanes.
+template <int DT, int NT>
+__device__ __forceinline__ u64 weigh_chunk(const Team<NT> &r, Shared &s, const Distance &distance, const Band &band, uint32_t chunk, u32x4 raw,
+                                           uint32_t elems, uint32_t *over)
+{
+    using V = Vec16<DT>;
+    constexpr uint32_t NE = V::NE;
+    static_assert(64 * NE <= kQueue, "");
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    float *const queue = s.wide.queue[wave];
+    float v[NE];
+    V::unpack(raw, v);
+    uint32_t near = 0, in = 0;
+#pragma unroll
+    for (uint32_t e = 0; e < NE; ++e) {
+        const float x = distance(v[e]);
+        const bool there = lane * NE + e < elems;
+        near |= (there && x < band.low ? 1u : 0u) << e;
+        in |= (there && x >= band.low && x < band.high ? 1u : 0u) << e;
+    }
+    if (in != 0) {
+        uint32_t at = atomicAdd(&s.word[2], static_cast<uint32_t>(__popc(in)));
+#pragma unroll
+        for (uint32_t e = 0; e < NE; ++e) {
+            if ((in >> e & 1) == 0) continue;
+            const uint32_t place = chunk * kChunk<DT> + lane * NE + e;
+            if (at < kList) s.wide.listed[at] = static_cast<u64>(number_of(v[e])) << 32 | static_cast<uint32_t>(~place);
+            ++at;
+        }
+    }
+    const uint32_t mine = __popc(near);
+    const uint32_t sums = wave_sums(mine);
+    const uint32_t found = of_last_lane(sums);
+    uint32_t at = sums - mine;
+#pragma unroll
+    for (uint32_t e = 0; e < NE; ++e) {
+        if (near >> e & 1) queue[at++] = v[e];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    u64 sum = 0;
+    for (uint32_t i = 0; i < found; i += 128) {
+        const uint32_t first = i + lane, second = first + 64;
+        const u64 one = r.weight(queue[min(first, found - 1)]), two = r.weight(queue[min(second, found - 1)]);
+        sum += (first < found ? one : 0) + (second < found ? two : 0);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    *over += found;
+    return wave_total(sum);
+}
+
+// What stays of a list whose elements the threads hold, kListed each (key 0: none): those from the returned key on.  `skip` of them stay (top_k), or
+// those before whose place in the order the weight is less than `aim`.  As by Row::narrow: keys are counted and weighed into equal
+// stretches of their range, which leaves one of them.
+template <int NT, int N>
+__device__ __forceinline__ u64 last_that_stays(Team<NT> &r, Shared &s, const u64 (&key)[N], const u64 (&weight)[N], bool by_count, uint32_t stay, u64 aim)
+{
+    constexpr uint32_t kMine = kBins / NT;
+    if (threadIdx.x == 0) {
+        s.word64[0] = ~u64(0);
+        s.word64[1] = 0;
+    }
+    __syncthreads();
+    u64 low = ~u64(0), high = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (key[i] == 0) continue;
+        low = min(low, key[i]);
+        high = max(high, key[i]);
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+        low = min(low, static_cast<u64>(__shfl_xor(low, d, 64)));
+        high = max(high, static_cast<u64>(__shfl_xor(high, d, 64)));
+    }
+    if ((threadIdx.x & 63) == 0) {
+        atomicMin(&s.word64[0], low);
+        atomicMax(&s.word64[1], high);
+    }
+    __syncthreads();
+    low = s.word64[0];
+    high = s.word64[1];
+    uint32_t count_before = 0;
+    u64 weight_before = 0;
+    while (low != high) {
+        const u64 width = high - low;
+        const uint32_t shift = width < kBins ? 0 : 64 - __clzll(static_cast<long long>(width)) - 11;
+        for (uint32_t i = threadIdx.x; i < kBins; i += NT) {
+            s.bins.count[i] = 0;
+            s.bins.weight[i] = 0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (key[i] < low || key[i] > high) continue;
+            const uint32_t bin = static_cast<uint32_t>((key[i] - low) >> shift);
+            atomicAdd(&s.bins.count[bin], 1u);
+            if (weight[i] != 0) atomicAdd(&s.bins.weight[bin], weight[i]);
+        }
+        __syncthreads();
+        uint32_t counts = 0, all;
+        u64 weights = 0, whole;
+#pragma unroll
+        for (uint32_t i = 0; i < kMine; ++i) {
+            const uint32_t bin = kBins - 1 - (threadIdx.x * kMine + i);
+            counts += s.bins.count[bin];
+            weights += s.bins.weight[bin];
+        }
+        uint32_t c = count_before + r.before(counts, &all);
+        u64 w = weight_before + r.before(weights, &whole);
+#pragma unroll
+        for (uint32_t i = 0; i < kMine; ++i) {
+            const uint32_t bin = kBins - 1 - (threadIdx.x * kMine + i);
+            const uint32_t more = s.bins.count[bin];
+            const u64 add = s.bins.weight[bin];
+            if (more != 0 && (by_count ? c < stay && c + more >= stay : w < aim && w + add >= aim)) {
+                s.range = {bin, 0, c, more, w, 0};
+            }
+            c += more;
+            w += add;
+        }
+        __syncthreads();
+        const Range found = s.range;
+        count_before = found.above;
+        weight_before = found.weight_above;
+        const u64 begin = low + (static_cast<u64>(found.low) << shift);
+        high = min(high, begin + ((u64(1) << shift) - 1));
+        low = begin;
+        if (found.inside == 1) {   // its own key
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (key[i] >= low && key[i] <= high) s.one = key[i];
+            }
+            __syncthreads();
+            return s.one;
+        }
+        __syncthreads();
+    }
+    return low;
+}
+
+// The fourth launch: weights of a part's spans, and the list of what the cut lies among.
+template <int DT, int NT>
+__global__ void __launch_bounds__(NT)
+k_sample_weigh(SelectArgs a)
+{
+    constexpr uint32_t kWaves = NT / 64;
+    constexpr uint32_t kAhead = 4;
+    static_assert(NT >= kMostSpans, "a thread for each span");
+    __shared__ Shared s;
+    const WidePart part(a);
+    const Wide wide = a.wide[part.slot];
+    if (wide.wide == 0) return;
+    const uint64_t row = a.first + part.slot;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t first = part.from * a.span, to = min(part.to * a.span, a.rows.nchunks);
+    u32x4 raw[kAhead];
+    uint32_t elems[kAhead];
+    const auto load = [&](uint32_t chunk) {
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k) {
+            const uint32_t i = chunk + k * kWaves;
+            const Stretch t = a.rows.chunks[i < to ? i : first];
+            elems[k] = i < to ? t.elems : 0;
+            raw[k] = load_piece<DT, false>(t.at + row * t.step, lane, elems[k]);
+        }
+    };
+    load(first + wave);   // (on its way while the band is found)
+    const RowChoice choice(a.choice, row, a.rows.vocab);
+    Team<NT> r(a, s, row, wide.top, choice.c);
+    const Distance distance(r.top_value, r.c);
+    if (threadIdx.x < part.to - part.from) s.wide.weight[threadIdx.x] = 0;
+    if (threadIdx.x == 0) s.word[2] = 0;
+    const Band band = band_of(a, r, s, choice, wide, a.levels + static_cast<uint64_t>(part.slot) * kLevels);
+    if (blockIdx.x % a.wide_parts == 0 && threadIdx.x == 0) a.bands[part.slot] = band;
+    if (!band.known) return;
+    __syncthreads();
+    u64 weight = 0;
+    uint32_t over = 0;
+    for (uint32_t chunk = first + wave; chunk < to; chunk += kWaves * kAhead) {
+        if (chunk != first + wave) load(chunk);
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k) {
+            const uint32_t i = chunk + k * kWaves;
+            if (i >= to) break;
+            const u64 sum = weigh_chunk<DT>(r, s, distance, band, i, raw[k], elems[k], &over);
+            weight += sum;
+            if (lane == 0 && sum != 0) atomicAdd(&s.wide.weight[i / a.span - part.from], sum);
+        }
+    }
+    weight = r.total(lane == 0 ? weight : 0);
+    over = r.total(lane == 0 ? over : 0);
+    if (threadIdx.x < part.to - part.from) a.spans[static_cast<uint64_t>(part.slot) * kMostSpans + part.from + threadIdx.x] = s.wide.weight[threadIdx.x];
+    const uint32_t listed = s.word[2];
+    for (uint32_t i = threadIdx.x; i < min(listed, kList); i += NT) a.listed[static_cast<uint64_t>(blockIdx.x) * kList + i] = s.wide.listed[i];
+    if (threadIdx.x == 0) a.found[blockIdx.x] = {weight, over, listed};
+}
+
+// The fifth launch: the cut, and the draw.
+template <int DT, int NT>
+__global__ void __launch_bounds__(NT)
+k_sample_wide(SelectArgs a)
+{
+    using V = Vec16<DT>;
+    constexpr uint32_t NE = V::NE;
+    constexpr uint32_t kWaves = NT / 64;
+    constexpr uint32_t kListed = kList / NT;
+    __shared__ Shared s;
+    const Wide wide = a.wide[blockIdx.x];
+    if (wide.wide == 0) return;
+    const uint64_t row = a.first + blockIdx.x;
+    const RowChoice choice(a.choice, row, a.rows.vocab);
+    const float u = a.choice.random[row];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const u64 p_of_whole = wide.p_of_whole;
+    const Band band = a.bands[blockIdx.x];
+    uint32_t n = kNoEnd, before_band = 0, mine = 0;
+    u64 above = 0;
+    if (band.known) {
+        Found f = {0, 0, 0};
+        if (lane < a.wide_parts) f = a.found[blockIdx.x * a.wide_parts + lane];
+        static_assert(kMostParts <= 64 && (kMostParts & (kMostParts - 1)) == 0, "");
+        mine = wave_sums(f.listed) - f.listed;   // in front of the part's
+        n = wave_total(f.listed);
+        before_band = wave_total(f.over);
+        above = wave_total(static_cast<u64>(f.weight));
+    }
+    if (n <= kList) {
+        Team<NT> r(a, s, row, wide.top, choice.c);
+        const Distance distance(r.top_value, r.c);
+        const u64 *const spans = a.spans + static_cast<uint64_t>(blockIdx.x) * kMostSpans;
+        if (threadIdx.x < 64) s.groups[lane] = lane < a.wide_parts ? mine : n;   // (begins of the parts' lists)
+        __syncthreads();
+        bool right = true;   // whether the cut is where the levels had it
+        {
+            // of those that the cut lies among
+                            const auto stays = [&](u64 key, u64 last) {
+                                return key >= last && (!band.by_min || static_cast<uint32_t>(key >> 32) == r.top || r.share(static_cast<uint32_t>(key >> 32)) >= choice.least);
+                            };
+                            u64 key[kListed], w[kListed];
+                            u64 sum = 0;
+#pragma unroll
+                            for (uint32_t i = 0; i < kListed; ++i) {
+                                const uint32_t place = threadIdx.x + i * NT;
+                                uint32_t part = 0;
+#pragma unroll
+                                for (uint32_t d = kMostParts / 2; d != 0; d /= 2) part += s.groups[part + d] <= place ? d : 0;
+                                key[i] = place < n ? a.listed[(static_cast<uint64_t>(blockIdx.x) * a.wide_parts + part) * kList + place - s.groups[part]] : 0;
+                                sum += w[i] = place < n ? r.weight(static_cast<uint32_t>(key[i] >> 32)) : 0;
+                            }
+                            const u64 inside = r.total(sum);
+                            u64 last = 0;
+                            if (band.by_level) {
+                                if (choice.by_k) {
+                                    right = before_band < choice.k && before_band + n >= choice.k;
+                                } else {
+                                    right = above < p_of_whole && above + inside >= p_of_whole;
+                                }
+                                // (the cut is where the levels had it)
+                                if (right) last = last_that_stays(r, s, key, w, choice.by_k, choice.k - before_band, p_of_whole - above);
+                            }
+                            if (right) {
+                                // the spans' weights, with those of the list that stay
+                                __syncthreads();
+                                if (threadIdx.x < kMostSpans) s.wide.weight[threadIdx.x] = threadIdx.x < a.nspans ? spans[threadIdx.x] : 0;
+                                __syncthreads();
+#pragma unroll
+                                for (uint32_t i = 0; i < kListed; ++i) {
+                                    if (w[i] != 0 && stays(key[i], last)) atomicAdd(&s.wide.weight[~static_cast<uint32_t>(key[i]) / kChunk<DT> / a.span], w[i]);
+                                }
+                                __syncthreads();
+                                // the span, then the element: a wavefront for each chunk
+                                sum = threadIdx.x < kMostSpans ? s.wide.weight[threadIdx.x] : 0;
+                                u64 whole;
+                                u64 begin = r.before(sum, &whole);
+                                const u64 aim = aim_of(u, whole);
+                                if (aim >= begin && aim - begin < sum) {
+                                    s.word[0] = threadIdx.x;
+                                    s.word64[0] = begin;
+                                }
+                                __syncthreads();
+                                const uint32_t first = s.word[0] * a.span;
+                                const uint32_t to = min(first + a.span, a.rows.nchunks);
+                                begin = s.word64[0];
+                                for (uint32_t turn = first; turn < to; turn += kWaves) {
+                                    const bool there = turn + wave < to;
+                                    const uint32_t chunk = there ? turn + wave : first;
+                                    const Stretch t = a.rows.chunks[chunk];
+                                    const uint32_t elems = there ? t.elems : 0;
+                                    const u32x4 raw = load_piece<DT, false>(t.at + row * t.step, lane, elems);
+                                    float v[NE];
+                                    V::unpack(raw, v);
+                                    u64 each[NE];
+                                    sum = 0;
+#pragma unroll
+                                    for (uint32_t e = 0; e < NE; ++e) {
+                                        const float x = distance(v[e]);
+                                        const u64 key = static_cast<u64>(number_of(no_nan(v[e]))) << 32 | static_cast<uint32_t>(~(chunk * kChunk<DT> + lane * NE + e));
+                                        const bool in = lane * NE + e < elems && (x < band.low || stays(key, last));
+                                        sum += each[e] = in ? r.weight(v[e]) : 0;
+                                    }
+                                    u64 all;
+                                    u64 at_element = begin + r.before(sum, &all);
+#pragma unroll
+                                    for (uint32_t e = 0; e < NE; ++e) {
+                                        if (aim >= at_element && aim - at_element < each[e]) {
+                                            r.write_choice(t.first + lane * NE + e, number_of(v[e]), ldexp(static_cast<double>(whole), -static_cast<int>(a.bits)));
+                                        }
+                                        at_element += each[e];
+                                    }
+                                    begin += all;
+                                }
+                return;
+            }
+        }
+    }
+    // More elements than a list holds are in the cut's level, or it is another.
+    __syncthreads();
+    Row<DT, NT> r(a, s, row);
+    r.c = choice.c;
+    draw_by_numbers(a, r, s, choice, u, p_of_whole);
+}
+
+// The second launch: rows from a.first on.
 template <int DT, int NT>
 __global__ void __launch_bounds__(NT)
 k_sample(SelectArgs a)
 {
     constexpr uint32_t kMine = kList / NT;
-    constexpr uint32_t kShift = kIdle<DT>;
     __shared__ Shared s;
-    const RowChoice choice(a.choice, blockIdx.x, a.rows.vocab);
-    const float u = a.choice.random[blockIdx.x];
-    Row<DT, NT> r(a, s);
+    const uint64_t row = a.first + blockIdx.x;
+    Wide &wide = a.wide[blockIdx.x];
+    if (threadIdx.x == 0) wide.wide = 0;
+    const RowChoice choice(a.choice, row, a.rows.vocab);
+    const float u = a.choice.random[row];
+    Row<DT, NT> r(a, s, row);
     r.c = choice.c;
     if (r.top <= kLeast) {   // nothing to choose from
         if (threadIdx.x == 0) {
@@ -1394,7 +1706,6 @@ k_sample(SelectArgs a)
                 if (in && aim >= at && aim - at < w) r.write_choice(column_of<DT>(a, x), static_cast<uint32_t>(x >> 32), static_cast<double>(whole) * unit);
                 return;
             }
-            r.sort(n);
         } else {
             r.sort(n);
             u64 w[kMine];
@@ -1441,43 +1752,13 @@ k_sample(SelectArgs a)
             }
         }
     }
-    if (draw_wide(a, r, s, choice, u, p_of_whole, sure)) return;
-    __syncthreads();   // the lists make room
-    // A level holds more than a list: the cut is searched by numbers, among all elements.
-    Kept stay = {0, kNoEnd, choice.by_min ? choice.least : 0.0};
-    auto all = [&](auto &&f) { r.each(nullptr, r.ngroups, f); };
-    Range range = {kLeast >> kShift, r.top >> kShift, 0, 0, 0, 0};
-    uint32_t cut_count = 0;
-    if (choice.by_k) {
-        do {
-            r.template narrow<false>(range, all, [&](u64) { return u64(choice.k); });
-        } while (range.low != range.high);
-        stay.cut = range.low;
-        stay.equal = choice.k - range.above;
-        cut_count = range.inside;
+    if (a.wide_parts == 0 || !is_wide(choice, r.top_value)) {
+        draw_by_numbers(a, r, s, choice, u, p_of_whole);
+        return;
     }
-    if (choice.by_p) {
-        range = {stay.cut > kLeast >> kShift ? stay.cut : kLeast >> kShift, r.top >> kShift, 0, 0, 0, 0};
-        u64 aim = 0;
-        bool first = true;
-        // (what is equal to the cut of top_k and does not stay is at the end of the order)
-        const u64 over = choice.by_k && cut_count > stay.equal ? (cut_count - stay.equal) * r.weight(stay.cut << kShift | (stay.cut >> (31 - kShift) != 0 ? 0 : (1u << kShift) - 1)) : 0;
-        do {
-            r.template narrow<true>(range, all, [&](u64 whole) {
-                if (first) aim = max(u64(1), min(choice.by_k ? part_of(choice.p, static_cast<double>(whole - over)) : p_of_whole, whole));
-                return aim;
-            });
-            first = false;
-        } while (range.low != range.high);
-        const u64 one = range.inside != 0 ? range.weight_inside / range.inside : 1;
-        const u64 need = one != 0 ? (aim - range.weight_above + one - 1) / one : 1;
-        const uint32_t equal = static_cast<uint32_t>(min(need, static_cast<u64>(range.inside)));
-        stay.equal = stay.cut == range.low && choice.by_k ? min(stay.equal, equal) : equal;
-        stay.cut = range.low;
-    }
-    if (threadIdx.x == 0) s.one = 0;
-    __syncthreads();
-    draw_kept(a, r, s, stay, u);
+    u64 *const levels = a.levels + static_cast<uint64_t>(blockIdx.x) * kLevels;
+    for (uint32_t i = threadIdx.x; i < kLevels; i += NT) levels[i] = 0;
+    if (threadIdx.x == 0) wide = {1, r.top, p_of_whole};
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
@@ -1489,7 +1770,8 @@ struct SelectWork : PlanWork {
     int dtype = 0;
     bool sample = false;
     uint32_t parts = 1;    // workgroups of the first launch per row
-    uint32_t threads = 512;   // of a workgroup of the second
+    uint32_t batch = 0;         // rows whose wide ones are drawn from together
+    bool may_be_wide = false;
 
     template <int DT, int U>
     void runs(hipStream_t st) const
@@ -1512,19 +1794,20 @@ struct SelectWork : PlanWork {
             case 4: runs<DT, 4>(st); break;
             default: runs<DT, 8>(st); break;
         }
-        const dim3 grid(args.rows.rows);
-        if (threads == 512) {
-            if (sample) {
-                HCCLX_LAUNCH((k_sample<DT, 512>), grid, dim3(512), 0, st, args);
-            } else {
-                HCCLX_LAUNCH((k_top_logits<DT, 512>), grid, dim3(512), 0, st, args);
-            }
-        } else {
-            if (sample) {
-                HCCLX_LAUNCH((k_sample<DT, 256>), grid, dim3(256), 0, st, args);
-            } else {
-                HCCLX_LAUNCH((k_top_logits<DT, 256>), grid, dim3(256), 0, st, args);
-            }
+        constexpr int NT = 512;
+        if (!sample) {
+            HCCLX_LAUNCH((k_top_logits<DT, NT>), dim3(args.rows.rows), dim3(NT), 0, st, args);
+            return;
+        }
+        SelectArgs of = args;
+        for (uint32_t first = 0; first < args.rows.rows; first += batch) {
+            of.first = first;
+            const uint32_t rows = std::min(batch, args.rows.rows - first);
+            HCCLX_LAUNCH((k_sample<DT, NT>), dim3(rows), dim3(NT), 0, st, of);
+            if (!may_be_wide) continue;
+            HCCLX_LAUNCH((k_sample_levels<DT, NT>), dim3(rows * args.wide_parts), dim3(NT), 0, st, of);
+            HCCLX_LAUNCH((k_sample_weigh<DT, NT>), dim3(rows * args.wide_parts), dim3(NT), 0, st, of);
+            HCCLX_LAUNCH((k_sample_wide<DT, NT>), dim3(rows), dim3(NT), 0, st, of);
         }
     }
 
@@ -1565,10 +1848,38 @@ int finish(const hcclx_logits_t &l, uint32_t vocab, bool sums, std::unique_ptr<S
     const uint64_t runs = sums ? static_cast<uint64_t>(l.rows) * a.nruns * sizeof(Run) : 0;
     const uint32_t per = 64 * (16 / dtype_size(l.dtype)) / kGroup;
     const uint64_t most = static_cast<uint64_t>(l.rows) * a.rows.nchunks * per * sizeof(uint32_t);
-    const uint64_t held = runs + most;
+    uint64_t held = runs + most;
+    const auto more = [&](uint64_t bytes) {
+        const uint64_t at = held = (held + 15) / 16 * 16;
+        held += bytes;
+        return at;
+    };
+    uint64_t wide = 0, bands = 0, levels = 0, found = 0, listed = 0, spans = 0;
+    if (w->sample && l.rows != 0) {
+        // Rows that the list of kNucleus always does for are never wide; nor are those that no filter but a short top_k may shorten, which
+        // only the device knows.
+        w->batch = std::min(l.rows, kBatch);
+        w->may_be_wide = vocab > kNucleus && (a.choice.top_k != nullptr || a.choice.top_p != nullptr || a.choice.min_p != nullptr);
+        a.span = (a.rows.nchunks + kMostSpans - 1) / kMostSpans;
+        a.nspans = (a.rows.nchunks + a.span - 1) / a.span;
+        // Workgroups for a row that may be wide: most rows are not, and their workgroups only look.
+        a.wide_parts = !w->may_be_wide ? 0 : std::min(a.nspans, std::min(kMostParts, std::max(2u, 4096 / w->batch)));
+        wide = more(w->batch * sizeof(Wide));
+        levels = more(w->may_be_wide ? w->batch * sizeof(u64) * kLevels : 0);
+        bands = more(w->batch * sizeof(Band));
+        found = more(static_cast<uint64_t>(w->batch) * a.wide_parts * sizeof(Found));
+        listed = more(static_cast<uint64_t>(w->batch) * a.wide_parts * sizeof(u64) * kList);
+        spans = more(w->may_be_wide ? w->batch * sizeof(u64) * kMostSpans : 0);
+    }
     if (held != 0 && (rc = w->scratch.get(held)) != HCCL_SUCCESS) return rc;
     a.runs = reinterpret_cast<Run *>(w->scratch.p);
     a.most = reinterpret_cast<uint32_t *>(w->scratch.p + runs);
+    a.wide = reinterpret_cast<Wide *>(w->scratch.p + wide);
+    a.levels = reinterpret_cast<u64 *>(w->scratch.p + levels);
+    a.bands = reinterpret_cast<Band *>(w->scratch.p + bands);
+    a.found = reinterpret_cast<Found *>(w->scratch.p + found);
+    a.listed = reinterpret_cast<u64 *>(w->scratch.p + listed);
+    a.spans = reinterpret_cast<u64 *>(w->scratch.p + spans);
     const uint64_t all = held + w->table.bytes;
     return plan_of(ctx, std::move(w), static_cast<uint64_t>(l.rows) * vocab * dtype_size(l.dtype), all, plan);
 }

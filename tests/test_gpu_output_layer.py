@@ -152,6 +152,13 @@ def test_top_logits_of_64_ranks_and_a_million_columns():
     check_top(contents("coarse", 2, 650, gen(2)), shares(650, 64), T.FP32, 650)
 
 
+@pytest.mark.parametrize("dtype", [T.FP32, T.BFP16])
+@pytest.mark.parametrize("each,k", [(3, 100), (3, 192), (10, 70), (40, 300), (40, 900)])
+def test_top_logits_of_more_than_there_are_groups(each, k, dtype):
+    """Many ranks of few columns: fewer groups of neighbouring columns hold anything than entries are asked for."""
+    check_top(contents("normal", 2, 64 * each, gen(k)), [each] * 64, dtype, k)
+
+
 # ---- distillation ------------------------------------------------------------------------------------------------------------
 
 
@@ -479,6 +486,47 @@ def test_rows_behind_4_gib():
     want, grad, bound, grad_bound = L.distill(last, values[-1].double(), indices[-1], 1.0, 1.0)
     assert abs(float(loss[-1]) - want) <= bound + O.E * abs(want)
     O.assert_close(whole[-1], grad, grad_bound)
+
+
+@pytest.mark.parametrize("dtype", [T.FP32, T.BFP16])
+def test_sampling_from_ranks_of_few_columns(dtype):
+    for each in (3, 40):
+        row = contents("normal", 1, 64 * each, gen(each))[0]
+        for settings in (dict(top_k=100), dict(top_p=0.95), dict(top_p=0.5), dict(T_=3.0, min_p=0.01), dict(T_=9.0, top_k=700, top_p=0.9)):
+            check_draws(row, [each] * 64, dtype, most=12, **settings)
+
+
+@pytest.mark.parametrize("dtype", [T.FP32, T.FP16, T.BFP16])
+def test_sampling_where_two_filters_cut_nearly_the_same(dtype):
+    """min_p between, at and next to the values around which top_p or top_k cut."""
+    row = contents("steep", 1, 30000, gen(31))[0].to(TD[dtype]).float()
+    l = row.double()
+    order = L.order(l)
+    w = torch.exp((l - l.max()) / 4.0)[order]
+    c = w.cumsum(0) / w.sum()
+    for place in (700, 5000, 20000):
+        for min_p in (float(w[place]), float(w[place]) * 1.0000005, float(w[place]) * 0.9999995, float(w[place + 3]), float(w[place - 2]), float(w[place + 400])):
+            check_draws(row, shares(30000, 3), dtype, T_=4.0, min_p=min_p, top_p=float(c[place]) + 1e-6, most=8)
+            check_draws(row, shares(30000, 3), dtype, T_=4.0, min_p=min_p, top_k=place + 400, most=8)
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 20011), (150, 20011), (1100, 20011), (4200, 1501)])
+def test_many_rows_of_wide_draws(rows, vocab):
+    """Rows whose list is too short among others, more and fewer workgroups to a row."""
+    g = gen(rows)
+    x = contents("steep", rows, vocab, g)
+    s = Split(x.bfloat16(), shares(vocab, 3), T.BFP16)
+    pick = lambda *v: [v[i % len(v)] for i in range(rows)]  # noqa: E731
+    settings = dict(temperature=pick(3.0, 1.0, 2.5, 3.0, 4.0), top_p=pick(0.95, 0.9, 1.0, 0.6, 1.0), top_k=pick(0, 0, 5000, 0, 0), min_p=pick(0.0, 0.0, 0.0, 0.001, 0.002))
+    u = torch.rand(rows, device=DEV, generator=g).tolist()
+    got, logprob = draw(s, settings, u)
+    whole = s.whole()
+    as32 = lambda v: float(np.float32(v))  # noqa: E731
+    for r in [*range(0, rows, 1 if rows < 200 else 7 if rows < 2000 else 61), *range(max(0, rows - 20), rows)]:
+        l = L.plain(whole[r])
+        want = L.sample(l, settings["temperature"][r], settings["top_k"][r], as32(settings["top_p"][r]), as32(settings["min_p"][r]), u[r])
+        assert got[r] == want[0], (r, got[r], want)
+        assert abs(logprob[r] - want[1]) <= 1e-9 + 2 * O.E * abs(want[1])
 
 
 @pytest.mark.parametrize("dtype", [T.FP32, T.BFP16])
