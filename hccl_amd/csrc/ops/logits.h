@@ -103,11 +103,69 @@ __device__ __forceinline__ double exp2_exact(double y)
     return ldexp(p, static_cast<int>(n));
 }
 
-__device__ __forceinline__ double wave_sum64(double v)
+typedef unsigned long long u64;
+
+// v of the lane that DPP control CTRL names, in the rows of 16 lanes that ROWS names; 0 elsewhere.
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T dpp_or_zero(T v)
 {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
+    static_assert(sizeof(T) == 4 || sizeof(T) == 8, "");
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+    } else {
+        const u64 x = __builtin_bit_cast(u64, v);
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROWS, 0xf, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(x >> 32), CTRL, ROWS, 0xf, false);
+        return __builtin_bit_cast(T, static_cast<u64>(hi) << 32 | lo);
+    }
+}
+// v of the last lane.
+template <typename T>
+__device__ __forceinline__ T of_last_lane(T v)
+{
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+    } else {
+        const u64 x = __builtin_bit_cast(u64, v);
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(x), 63);
+        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(x >> 32), 63);
+        return __builtin_bit_cast(T, static_cast<u64>(hi) << 32 | lo);
+    }
+}
+// Sums over the lanes up to this one, and over all; the largest.  All in registers (through LDS a step takes ten times as long).
+template <typename T>
+__device__ __forceinline__ T wave_sums(T v)
+{
+    v += dpp_or_zero<0x111, 0xf>(v);   // row_shr 1, 2, 4, 8
+    v += dpp_or_zero<0x112, 0xf>(v);
+    v += dpp_or_zero<0x114, 0xf>(v);
+    v += dpp_or_zero<0x118, 0xf>(v);
+    v += dpp_or_zero<0x142, 0xa>(v);   // lane 15 of rows 0 and 2 to the rows behind
+    v += dpp_or_zero<0x143, 0xc>(v);   // lane 31 to rows 2 and 3
     return v;
+}
+template <typename T>
+__device__ __forceinline__ T wave_total(T v) { return of_last_lane(wave_sums(v)); }
+
+// The largest, or NaN if there is one.
+__device__ __forceinline__ double larger(double a, double b) { return b > a || b != b ? b : a; }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double larger_of_lane(double v)
+{
+    const u64 x = __builtin_bit_cast(u64, v);
+    const int low = static_cast<int>(x), high = static_cast<int>(x >> 32);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(low, low, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(high, high, CTRL, ROWS, 0xf, false);
+    return larger(v, __builtin_bit_cast(double, static_cast<u64>(hi) << 32 | lo));
+}
+__device__ __forceinline__ double wave_largest(double v)
+{
+    v = larger_of_lane<0x111, 0xf>(v);
+    v = larger_of_lane<0x112, 0xf>(v);
+    v = larger_of_lane<0x114, 0xf>(v);
+    v = larger_of_lane<0x118, 0xf>(v);
+    v = larger_of_lane<0x142, 0xa>(v);
+    return of_last_lane(larger_of_lane<0x143, 0xc>(v));
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------

@@ -13,9 +13,9 @@
 //
 // Weights of the draw are whole numbers too, exp((l - most) / T) 2^s from 64-bit arithmetic: their sums do not go by the order.
 //
-// A row whose draw goes by more than such a list is left to a third and a fourth launch, which put several workgroups on a row: its
-// elements are counted by levels, 64 to a power of two of their weight, which says in which level the cut lies; then those over that
-// level are weighed, and those in it are listed and sorted.  (One workgroup for such a row, behind its list: TIMES_OLD.)
+// A row whose draw goes by more than such a list is left to several workgroups.  Next to the second launch they count its elements by levels, 64 to a
+// power of two of their weight, which says in which level the cut lies; in a third those over that level are weighed and those in it are
+// listed; and a fourth finds the cut among these, and draws.
 #include "ops/logits.h"
 
 #include <algorithm>
@@ -30,6 +30,7 @@ constexpr uint32_t kRunWaves = 4;        // of a workgroup of the first launch, 
 constexpr uint32_t kList = 2048;         // elements that are sorted at once
 constexpr uint32_t kMostGroups = HCCLX_TOP_MAX + HCCLX_TOP_MAX / 2 + 32;
 constexpr uint32_t kNucleus = 64;       // listed where no top_k bounds the list
+constexpr uint32_t kLevels = 2048;       // of the weights of a row, 64 to a power of two
 constexpr uint32_t kNone = 0;            // the number of what does not exist
 constexpr uint32_t kLeast = 0x007fffffu;   // of minus infinity
 
@@ -114,49 +115,6 @@ template <int DT> constexpr uint32_t kIdle = DT == HCCL_DATA_TYPE_BFP16 ? 16 : D
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) { return dpp_or<CTRL>(v, v); }
 
-typedef unsigned long long u64;
-
-// v of the lane that DPP control CTRL names, in the rows of 16 lanes that ROWS names; 0 elsewhere.
-template <int CTRL, int ROWS, typename T>
-__device__ __forceinline__ T dpp_or_zero(T v)
-{
-    static_assert(sizeof(T) == 4 || sizeof(T) == 8, "");
-    if constexpr (sizeof(T) == 4) {
-        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
-    } else {
-        const u64 x = __builtin_bit_cast(u64, v);
-        const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROWS, 0xf, false);
-        const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(x >> 32), CTRL, ROWS, 0xf, false);
-        return __builtin_bit_cast(T, static_cast<u64>(hi) << 32 | lo);
-    }
-}
-// v of the last lane.
-template <typename T>
-__device__ __forceinline__ T of_last_lane(T v)
-{
-    if constexpr (sizeof(T) == 4) {
-        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
-    } else {
-        const u64 x = __builtin_bit_cast(u64, v);
-        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(x), 63);
-        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(x >> 32), 63);
-        return __builtin_bit_cast(T, static_cast<u64>(hi) << 32 | lo);
-    }
-}
-// Sums over the lanes up to this one, and over all; the largest.  All in registers (through LDS a step takes ten times as long).
-template <typename T>
-__device__ __forceinline__ T wave_sums(T v)
-{
-    v += dpp_or_zero<0x111, 0xf>(v);   // row_shr 1, 2, 4, 8
-    v += dpp_or_zero<0x112, 0xf>(v);
-    v += dpp_or_zero<0x114, 0xf>(v);
-    v += dpp_or_zero<0x118, 0xf>(v);
-    v += dpp_or_zero<0x142, 0xa>(v);   // lane 15 of rows 0 and 2 to the rows behind
-    v += dpp_or_zero<0x143, 0xc>(v);   // lane 31 to rows 2 and 3
-    return v;
-}
-template <typename T>
-__device__ __forceinline__ T wave_total(T v) { return of_last_lane(wave_sums(v)); }
 __device__ __forceinline__ uint32_t wave_most(uint32_t v)
 {
     v = max(v, dpp_or_zero<0x111, 0xf>(v));
@@ -213,6 +171,8 @@ struct RowChoice {
         least = mp < 1.0f ? mp : 1.0f;
         c = greedy ? 1.0 : 1.4426950408889634074 / static_cast<double>(T);
     }
+    // whether elements are counted by levels, in case that no list holds what stays
+    __device__ __forceinline__ bool by_levels() const { return by_k ? k > HCCLX_TOP_MAX && !by_p : by_p; }
     // whether the sum over the whole row is needed
     __device__ __forceinline__ bool whole() const { return !by_k && (by_p || !by_min); }
 };
@@ -226,7 +186,7 @@ k_logit_runs(SelectArgs a, uint32_t parts)
     using V = Vec16<DT>;
     constexpr int NE = V::NE;
     constexpr uint32_t kPer = kChunk<DT> / kGroup;   // groups of a chunk
-    const uint64_t row = blockIdx.x / parts;
+    const uint64_t row = a.first + blockIdx.x / parts;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t run = blockIdx.x % parts * kRunWaves + wave;
     const uint32_t lane = threadIdx.x & 63;
@@ -235,6 +195,11 @@ k_logit_runs(SelectArgs a, uint32_t parts)
     if constexpr (KIND == kRunChoice) {
         if (threadIdx.x < 64) s_powers[threadIdx.x] = exp2_exact(threadIdx.x / -64.0);
         __syncthreads();
+        if (a.wide_parts != 0 && RowChoice(a.choice, row, a.rows.vocab).by_levels()) {   // (the second launch counts)
+            const uint32_t part = blockIdx.x % parts;
+            u64 *const levels = a.levels + static_cast<uint64_t>(blockIdx.x / parts) * kLevels;
+            for (uint32_t i = kLevels * part / parts + threadIdx.x; i < kLevels * (part + 1) / parts; i += kRunWaves * 64) levels[i] = 0;
+        }
     }
     if (from >= a.rows.nchunks) return;
     u32x4 raw[U];
@@ -324,7 +289,6 @@ struct Range {
 };
 
 constexpr uint32_t kBins = 2048;
-constexpr uint32_t kLevels = 2048;
 constexpr uint32_t kBatch = 4096;        // rows that have memory for a wide draw at a time, 52 KB each and more where they are few
 constexpr uint32_t kMostParts = 32;      // workgroups of a wide row
 constexpr uint32_t kMostSpans = 512;
@@ -1180,7 +1144,7 @@ __device__ __forceinline__ uint32_t level_of(float x) { return min(static_cast<u
 // What a level holds is one word: its elements, times 2^40, and what they lack of the weight that they would have at the level's upper
 // end, in parts of 2^22 of that: 1 - 2^(-f / 64) for an element f of a level further down, of which two terms do.  Rounding to such
 // parts costs the sum over a level some 2^-23 of itself at random, so which level holds the cut of top_p is known but for one in many
-// thousands of rows; the fourth launch finds out.
+// thousands of rows; the draw finds out.
 constexpr float kLack = 0x1p22f;
 __device__ __forceinline__ u64 level_entry(float x, uint32_t level)
 {
@@ -1193,54 +1157,62 @@ __device__ __forceinline__ double entry_weight(u64 e, double at_end)
     return at_end * (entry_count(e) - static_cast<double>(e & ((u64(1) << 40) - 1)) * (1.0 / kLack));
 }
 
-// Whether the third and fourth launch can draw from a row: not where the weight that top_p asks for goes by a cut of top_k.
+// Whether several workgroups can draw from a row: not where the weight that top_p asks for goes by a cut of top_k.
 __device__ __forceinline__ bool is_wide(const RowChoice &choice, double top_value)
 {
     return !(choice.by_k && choice.by_p) && Distance(top_value, choice.c).fits;
 }
 
-// The chunks first .. last - 1 of a part of the third and fourth launch.
+// The chunks first .. last - 1 of a part of a row that may be left to several workgroups.
 struct WidePart {
     uint32_t slot;
     uint32_t from;   // spans
     uint32_t to;
-    __device__ __forceinline__ explicit WidePart(const SelectArgs &a) : slot(blockIdx.x / a.wide_parts)
+    __device__ __forceinline__ WidePart(const SelectArgs &a, uint32_t block) : slot(block / a.wide_parts)
     {
-        const uint32_t part = blockIdx.x % a.wide_parts;
+        const uint32_t part = block % a.wide_parts;
         from = a.nspans * part / a.wide_parts;
         to = a.nspans * (part + 1) / a.wide_parts;
     }
 };
 
-// The third launch: the elements of a part by levels.
+// The elements of a part by levels.  Where there are few rows, by workgroups of the second launch that have no row of their own, before it is
+// known whether levels are asked for: by then they are there (37 rows of 50021: 25 us for the draw, 41 with a launch of its own; 1 row 17
+// and 20).  Where rows fill the device that holds up the others (1024 rows of 131072: 222 us for the draw, 199 with a launch of its own,
+// which rows that are not asked leave at once).
 template <int DT, int NT>
-__global__ void __launch_bounds__(NT)
-k_sample_levels(SelectArgs a)
+__device__ __forceinline__ void count_levels(const SelectArgs &a, u64 *mine, uint32_t *most, uint32_t block)
 {
     using V = Vec16<DT>;
     constexpr uint32_t NE = V::NE;
     constexpr uint32_t kWaves = NT / 64;
     constexpr int kAhead = 4;
-    __shared__ u64 s_levels[kLevels];
-    const WidePart part(a);
-    const Wide &w = a.wide[part.slot];
-    if (w.wide == 0) return;
+    const WidePart part(a, block);
     const uint64_t row = a.first + part.slot;
     const RowChoice choice(a.choice, row, a.rows.vocab);
-    if (!choice.by_k && !choice.by_p) return;   // (min_p says itself how far it reaches)
-    for (uint32_t i = threadIdx.x; i < kLevels; i += NT) s_levels[i] = 0;
-    const double top_value = value_of(w.top);
-    const Distance distance(top_value, choice.c);
-    // What is so improbable that even as many as there are columns hold no more than 1 - top_p of the whole lies behind the cut.
+    if (!choice.by_levels()) return;
+    for (uint32_t i = threadIdx.x; i < kLevels; i += NT) mine[i] = 0;
+    const uint32_t ngroups = a.rows.nchunks * (kChunk<DT> / kGroup);
+    uint32_t top = 0;
+    for (uint32_t i = threadIdx.x * 4; i < ngroups; i += NT * 4) {
+        const u32x4 v = *reinterpret_cast<const u32x4 *>(a.most + row * ngroups + i);
+        top = max(max(top, max(v.x, v.y)), max(v.z, v.w));
+    }
+    top = wave_most(top);
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    if (lane == 0) most[wave] = top;
+    __syncthreads();
+    for (uint32_t w = 0; w < kWaves; ++w) top = max(top, most[w]);
+    const Distance distance(value_of(top), choice.c);
+    if (top <= kLeast || !distance.fits) return;
+    // What is so improbable that even as many as there are columns hold no more than 1 - top_p of the largest's weight alone lies behind the cut.
     float far = __builtin_inff();
     if (!choice.by_k) {
-        const double behind = (static_cast<double>(w.p_of_whole) / choice.p - static_cast<double>(w.p_of_whole)) * ldexp(1.0, -static_cast<int>(a.bits)) / a.rows.vocab;
+        const double behind = (1.0 - choice.p) / a.rows.vocab;
         if (behind > 0.0) far = static_cast<float>(-64.0 * log2(behind)) + 2.0f;
     }
-    __syncthreads();
-    const uint32_t lane = threadIdx.x & 63;
     const uint32_t to = min(part.to * a.span, a.rows.nchunks);
-    for (uint32_t first = part.from * a.span + __builtin_amdgcn_readfirstlane(threadIdx.x / 64); first < to; first += kWaves * kAhead) {
+    for (uint32_t first = part.from * a.span + wave; first < to; first += kWaves * kAhead) {
         u32x4 raw[kAhead];
         uint32_t elems[kAhead];
 #pragma unroll
@@ -1260,15 +1232,24 @@ k_sample_levels(SelectArgs a)
                 if (!(x <= far) || lane * NE + e >= elems[k]) continue;
                 const uint32_t level = level_of(x);
                 // (what is in the last one is not told apart)
-                atomicAdd(&s_levels[level], level == kLevels - 1 ? u64(1) << 40 : level_entry(x, level));
+                atomicAdd(&mine[level], level == kLevels - 1 ? u64(1) << 40 : level_entry(x, level));
             }
         }
     }
     __syncthreads();
-    u64 *all = a.levels + static_cast<uint64_t>(part.slot) * kLevels;
+    u64 *const all = a.levels + static_cast<uint64_t>(part.slot) * kLevels;
     for (uint32_t i = threadIdx.x; i < kLevels; i += NT) {
-        if (s_levels[i] != 0) atomicAdd(&all[i], s_levels[i]);
+        if (mine[i] != 0) atomicAdd(&all[i], mine[i]);
     }
+}
+
+template <int DT, int NT>
+__global__ void __launch_bounds__(NT)
+k_sample_levels(SelectArgs a)
+{
+    __shared__ u64 s_levels[kLevels];
+    __shared__ uint32_t s_most[NT / 64];
+    if (a.wide[blockIdx.x / a.wide_parts].wide != 0) count_levels<DT, NT>(a, s_levels, s_most, blockIdx.x);
 }
 
 template <int NT>
@@ -1470,7 +1451,7 @@ __device__ __forceinline__ u64 last_that_stays(Team<NT> &r, Shared &s, const u64
     return low;
 }
 
-// The fourth launch: weights of a part's spans, and the list of what the cut lies among.
+// The third launch: weights of a part's spans, and the list of what the cut lies among.
 template <int DT, int NT>
 __global__ void __launch_bounds__(NT)
 k_sample_weigh(SelectArgs a)
@@ -1479,7 +1460,7 @@ k_sample_weigh(SelectArgs a)
     constexpr uint32_t kAhead = 4;
     static_assert(NT >= kMostSpans, "a thread for each span");
     __shared__ Shared s;
-    const WidePart part(a);
+    const WidePart part(a, blockIdx.x);
     const Wide wide = a.wide[part.slot];
     if (wide.wide == 0) return;
     const uint64_t row = a.first + part.slot;
@@ -1527,7 +1508,7 @@ k_sample_weigh(SelectArgs a)
     if (threadIdx.x == 0) a.found[blockIdx.x] = {weight, over, listed};
 }
 
-// The fifth launch: the cut, and the draw.
+// The fourth launch: the cut, and the draw.
 template <int DT, int NT>
 __global__ void __launch_bounds__(NT)
 k_sample_wide(SelectArgs a)
@@ -1655,10 +1636,15 @@ k_sample_wide(SelectArgs a)
 // The second launch: rows from a.first on.
 template <int DT, int NT>
 __global__ void __launch_bounds__(NT)
-k_sample(SelectArgs a)
+k_sample(SelectArgs a, uint32_t rows)
 {
     constexpr uint32_t kMine = kList / NT;
     __shared__ Shared s;
+    if (blockIdx.x >= rows) {
+        static_assert(kList >= kLevels, "");
+        count_levels<DT, NT>(a, s.list.listed, s.most, blockIdx.x - rows);
+        return;
+    }
     const uint64_t row = a.first + blockIdx.x;
     Wide &wide = a.wide[blockIdx.x];
     if (threadIdx.x == 0) wide.wide = 0;
@@ -1756,8 +1742,6 @@ k_sample(SelectArgs a)
         draw_by_numbers(a, r, s, choice, u, p_of_whole);
         return;
     }
-    u64 *const levels = a.levels + static_cast<uint64_t>(blockIdx.x) * kLevels;
-    for (uint32_t i = threadIdx.x; i < kLevels; i += NT) levels[i] = 0;
     if (threadIdx.x == 0) wide = {1, r.top, p_of_whole};
 }
 
@@ -1771,12 +1755,12 @@ struct SelectWork : PlanWork {
     bool sample = false;
     uint32_t parts = 1;    // workgroups of the first launch per row
     uint32_t batch = 0;         // rows whose wide ones are drawn from together
-    bool may_be_wide = false;
+    bool apart = false;         // whether levels are counted in a launch of their own
 
     template <int DT, int U>
-    void runs(hipStream_t st) const
+    void runs(const SelectArgs &args, uint32_t rows, hipStream_t st) const
     {
-        const dim3 grid(args.rows.rows * parts), block(kRunWaves * 64);
+        const dim3 grid(rows * parts), block(kRunWaves * 64);
         if (sample) {
             HCCLX_LAUNCH((k_logit_runs<DT, U, kRunChoice>), grid, block, 0, st, args, parts);
         } else if (args.lse != nullptr) {
@@ -1786,16 +1770,21 @@ struct SelectWork : PlanWork {
         }
     }
     template <int DT>
+    void first_launch(const SelectArgs &a, uint32_t rows, hipStream_t st) const
+    {
+        switch (a.per_run) {
+            case 1: runs<DT, 1>(a, rows, st); break;
+            case 2: runs<DT, 2>(a, rows, st); break;
+            case 4: runs<DT, 4>(a, rows, st); break;
+            default: runs<DT, 8>(a, rows, st); break;
+        }
+    }
+    template <int DT>
     void run(hipStream_t st) const
     {
-        switch (args.per_run) {
-            case 1: runs<DT, 1>(st); break;
-            case 2: runs<DT, 2>(st); break;
-            case 4: runs<DT, 4>(st); break;
-            default: runs<DT, 8>(st); break;
-        }
         constexpr int NT = 512;
         if (!sample) {
+            first_launch<DT>(args, args.rows.rows, st);
             HCCLX_LAUNCH((k_top_logits<DT, NT>), dim3(args.rows.rows), dim3(NT), 0, st, args);
             return;
         }
@@ -1803,10 +1792,12 @@ struct SelectWork : PlanWork {
         for (uint32_t first = 0; first < args.rows.rows; first += batch) {
             of.first = first;
             const uint32_t rows = std::min(batch, args.rows.rows - first);
-            HCCLX_LAUNCH((k_sample<DT, NT>), dim3(rows), dim3(NT), 0, st, of);
-            if (!may_be_wide) continue;
-            HCCLX_LAUNCH((k_sample_levels<DT, NT>), dim3(rows * args.wide_parts), dim3(NT), 0, st, of);
-            HCCLX_LAUNCH((k_sample_weigh<DT, NT>), dim3(rows * args.wide_parts), dim3(NT), 0, st, of);
+            const uint32_t parts_of_all = rows * args.wide_parts;
+            first_launch<DT>(of, rows, st);
+            HCCLX_LAUNCH((k_sample<DT, NT>), dim3(rows + (apart ? 0 : parts_of_all)), dim3(NT), 0, st, of, rows);
+            if (args.wide_parts == 0) continue;
+            if (apart) HCCLX_LAUNCH((k_sample_levels<DT, NT>), dim3(parts_of_all), dim3(NT), 0, st, of);
+            HCCLX_LAUNCH((k_sample_weigh<DT, NT>), dim3(parts_of_all), dim3(NT), 0, st, of);
             HCCLX_LAUNCH((k_sample_wide<DT, NT>), dim3(rows), dim3(NT), 0, st, of);
         }
     }
@@ -1859,17 +1850,18 @@ int finish(const hcclx_logits_t &l, uint32_t vocab, bool sums, std::unique_ptr<S
         // Rows that the list of kNucleus always does for are never wide; nor are those that no filter but a short top_k may shorten, which
         // only the device knows.
         w->batch = std::min(l.rows, kBatch);
-        w->may_be_wide = vocab > kNucleus && (a.choice.top_k != nullptr || a.choice.top_p != nullptr || a.choice.min_p != nullptr);
+        const bool may_be_wide = vocab > kNucleus && (a.choice.top_k != nullptr || a.choice.top_p != nullptr || a.choice.min_p != nullptr);
         a.span = (a.rows.nchunks + kMostSpans - 1) / kMostSpans;
         a.nspans = (a.rows.nchunks + a.span - 1) / a.span;
         // Workgroups for a row that may be wide: most rows are not, and their workgroups only look.
-        a.wide_parts = !w->may_be_wide ? 0 : std::min(a.nspans, std::min(kMostParts, std::max(2u, 4096 / w->batch)));
+        a.wide_parts = !may_be_wide ? 0 : std::min(a.nspans, std::min(kMostParts, std::max(2u, 4096 / w->batch)));
+        w->apart = w->batch > static_cast<uint32_t>(ctx->num_cus);
         wide = more(w->batch * sizeof(Wide));
-        levels = more(w->may_be_wide ? w->batch * sizeof(u64) * kLevels : 0);
+        levels = more(may_be_wide ? w->batch * sizeof(u64) * kLevels : 0);
         bands = more(w->batch * sizeof(Band));
         found = more(static_cast<uint64_t>(w->batch) * a.wide_parts * sizeof(Found));
         listed = more(static_cast<uint64_t>(w->batch) * a.wide_parts * sizeof(u64) * kList);
-        spans = more(w->may_be_wide ? w->batch * sizeof(u64) * kMostSpans : 0);
+        spans = more(may_be_wide ? w->batch * sizeof(u64) * kMostSpans : 0);
     }
     if (held != 0 && (rc = w->scratch.get(held)) != HCCL_SUCCESS) return rc;
     a.runs = reinterpret_cast<Run *>(w->scratch.p);
