@@ -296,8 +296,11 @@ constexpr uint32_t kCounted = 256;       // elements of a list that is put in or
 constexpr uint32_t kMostWaves = 8;
 constexpr uint32_t kCached = 320;        // chunks whose places in the row are kept in LDS
 constexpr uint32_t kNoEnd = 0xffffffffu;
+constexpr uint32_t kStretches = 1000;    // of the range of a list's numbers
+constexpr uint32_t kMostAlike = 32;      // elements of a stretch that are put in order by counting
 constexpr uint32_t kQueue = 512;          // elements of a chunk that a wavefront weighs
 
+// What is used at different times lies in the same place: 38 KB leave a CU room for four workgroups.
 struct Shared {
     union {
         struct {
@@ -314,14 +317,23 @@ struct Shared {
         } walk;
         struct {
             u64 listed[kList];   // (where list.listed is)
-            float queue[kMostWaves][kQueue];   // (where list.sorted is, which comes later)
-            u64 weight[kMostSpans];   // of the spans: what stays
+            float queue[kMostWaves][kQueue];
         } wide;
+        struct {
+            u64 unused[kBins];
+            uint32_t unused_too[kBins];
+            uint32_t groups[kMostGroups];   // behind the bins; before anything is sorted
+        };
+    };
+    union {
+        struct {
+            uint64_t at[kCached];     // of the row's chunks
+            uint32_t elems[kCached];
+        };
+        u64 span_weight[kMostSpans];
+        uint32_t stretch[kStretches + 1];   // begins in a list that is sorted
     };
     double powers[64];   // 2^(-i / 64)
-    uint64_t at[kCached];
-    uint32_t elems[kCached];
-    uint32_t groups[kMostGroups];
     u64 part[2][kMostWaves];
     uint32_t most[kMostWaves];
     uint32_t least[kMostWaves];
@@ -330,6 +342,7 @@ struct Shared {
     uint32_t word[4];
     u64 one;
 };
+static_assert(sizeof(Shared) <= 160 * 1024 / 4, "");
 
 // A lane's vector of a group: lanes kGroup / NE in a row hold one.
 struct Piece {
@@ -400,8 +413,78 @@ struct Team {
     }
     __device__ __forceinline__ u64 weight(uint32_t number) const { return weight(value_of(number)); }
 
-    // Sorts s.list.listed[0 .. n) into s.list.sorted, descending.
-    __device__ __forceinline__ void sort(uint32_t n) const
+    // Sorts s.list.listed[0 .. n) into s.list.sorted, descending: into equal stretches of the range of their numbers, and in those by counting
+    // (301 lists of some 750 elements: SORT_TEXT).  Where many are alike, by exchanges.
+    __device__ __forceinline__ void sort(uint32_t n)
+    {
+        constexpr uint32_t kMine = kList / NT;
+        u64 key[kMine];
+        uint32_t least = kNoEnd;
+#pragma unroll
+        for (uint32_t i = 0; i < kMine; ++i) {
+            const uint32_t at = threadIdx.x + i * NT;
+            key[i] = at < n ? s.list.listed[at] : 0;
+            if (at < n) least = min(least, static_cast<uint32_t>(key[i] >> 32));
+        }
+        least = ~wave_most(~least);
+        if ((threadIdx.x & 63) == 0) s.least[threadIdx.x / 64] = least;
+        for (uint32_t i = threadIdx.x; i <= kStretches; i += NT) s.stretch[i] = 0;
+        if (threadIdx.x == 0) s.word[3] = 0;
+        __syncthreads();
+        least = s.least[0];
+#pragma unroll
+        for (uint32_t w = 1; w < kWaves; ++w) least = min(least, s.least[w]);
+        // (the largest number of the list is the row's)
+        const uint32_t each = (top - least) / kStretches + 1;
+        uint32_t bin[kMine], place[kMine];
+#pragma unroll
+        for (uint32_t i = 0; i < kMine; ++i) {
+            bin[i] = place[i] = 0;
+            if (threadIdx.x + i * NT >= n) continue;
+            bin[i] = (top - static_cast<uint32_t>(key[i] >> 32)) / each;
+            place[i] = atomicAdd(&s.stretch[bin[i]], 1u);
+            if (place[i] == kMostAlike) s.word[3] = 1;
+        }
+        __syncthreads();
+        if (s.word[3] != 0) {
+            exchange(n);
+            return;
+        }
+        constexpr uint32_t kBegins = (kStretches + NT) / NT;   // neighbours of a thread
+        uint32_t count[kBegins], sum = 0, all;
+#pragma unroll
+        for (uint32_t i = 0; i < kBegins; ++i) {
+            const uint32_t b = threadIdx.x * kBegins + i;
+            sum += count[i] = b <= kStretches ? s.stretch[b] : 0;
+        }
+        sum = before(sum, &all);
+#pragma unroll
+        for (uint32_t i = 0; i < kBegins; ++i) {
+            const uint32_t b = threadIdx.x * kBegins + i;
+            if (b <= kStretches) s.stretch[b] = sum;
+            sum += count[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < kMine; ++i) {
+            if (threadIdx.x + i * NT < n) s.list.sorted[s.stretch[bin[i]] + place[i]] = key[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < kMine; ++i) {
+            if (threadIdx.x + i * NT >= n) continue;
+            const uint32_t from = s.stretch[bin[i]], to = s.stretch[bin[i] + 1];
+            place[i] = from;
+            for (uint32_t k = from; k < to; ++k) place[i] += s.list.sorted[k] > key[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < kMine; ++i) {
+            if (threadIdx.x + i * NT < n) s.list.sorted[place[i]] = key[i];
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ void exchange(uint32_t n) const
     {
         uint32_t size = 64;
         while (size < n) size *= 2;
@@ -545,13 +628,7 @@ struct Row : Team<NT> {
                 least = min(least, v[j] != kNone ? v[j] : kNoEnd);
             }
         }
-        if (a.rows.nchunks <= kCached) {
-            for (uint32_t i = threadIdx.x; i < a.rows.nchunks; i += NT) {
-                const Stretch of = a.rows.chunks[i];
-                s.at[i] = reinterpret_cast<uint64_t>(of.at + row * of.step);
-                s.elems[i] = of.elems;
-            }
-        }
+        find_chunks();
         for (uint32_t i = NT * kHeld + threadIdx.x; i < ngroups; i += NT) {
             t = max(t, most[i]);
             least = min(least, most[i] != kNone ? most[i] : kNoEnd);
@@ -589,6 +666,15 @@ struct Row : Team<NT> {
         }
     }
 
+    __device__ __forceinline__ void find_chunks()
+    {
+        if (a.rows.nchunks > kCached) return;
+        for (uint32_t i = threadIdx.x; i < a.rows.nchunks; i += NT) {
+            const Stretch of = a.rows.chunks[i];
+            s.at[i] = reinterpret_cast<uint64_t>(of.at + row * of.step);
+            s.elems[i] = of.elems;
+        }
+    }
     // Where the row's part of a chunk lies, and how much it has.
     __device__ __forceinline__ const char *chunk_at(uint32_t chunk, uint32_t *elems) const
     {
@@ -1091,6 +1177,8 @@ __device__ __forceinline__ void draw_by_numbers(const SelectArgs &a, Row<DT, NT>
 {
     constexpr uint32_t kShift = kIdle<DT>;
     __syncthreads();   // the lists make room
+    r.find_chunks();   // (sorting has taken their place)
+    __syncthreads();
     Kept stay = {0, kNoEnd, choice.by_min ? choice.least : 0.0};
     auto all = [&](auto &&f) { r.each(nullptr, r.ngroups, f); };
     Range range = {kLeast >> kShift, r.top >> kShift, 0, 0, 0, 0};
@@ -1481,7 +1569,7 @@ k_sample_weigh(SelectArgs a)
     const RowChoice choice(a.choice, row, a.rows.vocab);
     Team<NT> r(a, s, row, wide.top, choice.c);
     const Distance distance(r.top_value, r.c);
-    if (threadIdx.x < part.to - part.from) s.wide.weight[threadIdx.x] = 0;
+    if (threadIdx.x < part.to - part.from) s.span_weight[threadIdx.x] = 0;
     if (threadIdx.x == 0) s.word[2] = 0;
     const Band band = band_of(a, r, s, choice, wide, a.levels + static_cast<uint64_t>(part.slot) * kLevels);
     if (blockIdx.x % a.wide_parts == 0 && threadIdx.x == 0) a.bands[part.slot] = band;
@@ -1497,12 +1585,12 @@ k_sample_weigh(SelectArgs a)
             if (i >= to) break;
             const u64 sum = weigh_chunk<DT>(r, s, distance, band, i, raw[k], elems[k], &over);
             weight += sum;
-            if (lane == 0 && sum != 0) atomicAdd(&s.wide.weight[i / a.span - part.from], sum);
+            if (lane == 0 && sum != 0) atomicAdd(&s.span_weight[i / a.span - part.from], sum);
         }
     }
     weight = r.total(lane == 0 ? weight : 0);
     over = r.total(lane == 0 ? over : 0);
-    if (threadIdx.x < part.to - part.from) a.spans[static_cast<uint64_t>(part.slot) * kMostSpans + part.from + threadIdx.x] = s.wide.weight[threadIdx.x];
+    if (threadIdx.x < part.to - part.from) a.spans[static_cast<uint64_t>(part.slot) * kMostSpans + part.from + threadIdx.x] = s.span_weight[threadIdx.x];
     const uint32_t listed = s.word[2];
     for (uint32_t i = threadIdx.x; i < min(listed, kList); i += NT) a.listed[static_cast<uint64_t>(blockIdx.x) * kList + i] = s.wide.listed[i];
     if (threadIdx.x == 0) a.found[blockIdx.x] = {weight, over, listed};
@@ -1574,15 +1662,15 @@ k_sample_wide(SelectArgs a)
                             if (right) {
                                 // the spans' weights, with those of the list that stay
                                 __syncthreads();
-                                if (threadIdx.x < kMostSpans) s.wide.weight[threadIdx.x] = threadIdx.x < a.nspans ? spans[threadIdx.x] : 0;
+                                if (threadIdx.x < kMostSpans) s.span_weight[threadIdx.x] = threadIdx.x < a.nspans ? spans[threadIdx.x] : 0;
                                 __syncthreads();
 #pragma unroll
                                 for (uint32_t i = 0; i < kListed; ++i) {
-                                    if (w[i] != 0 && stays(key[i], last)) atomicAdd(&s.wide.weight[~static_cast<uint32_t>(key[i]) / kChunk<DT> / a.span], w[i]);
+                                    if (w[i] != 0 && stays(key[i], last)) atomicAdd(&s.span_weight[~static_cast<uint32_t>(key[i]) / kChunk<DT> / a.span], w[i]);
                                 }
                                 __syncthreads();
                                 // the span, then the element: a wavefront for each chunk
-                                sum = threadIdx.x < kMostSpans ? s.wide.weight[threadIdx.x] : 0;
+                                sum = threadIdx.x < kMostSpans ? s.span_weight[threadIdx.x] : 0;
                                 u64 whole;
                                 u64 begin = r.before(sum, &whole);
                                 const u64 aim = aim_of(u, whole);
