@@ -53,7 +53,7 @@ struct Run {
 
 // A row that is left to the launches behind the second.
 struct Wide {
-    uint32_t wide;     // 0: it is not
+    uint32_t wide;     // 0: it is not; 2: it is, but its cut is not found by levels
     uint32_t top;      // its largest number
     unsigned long long p_of_whole;
 };
@@ -804,7 +804,7 @@ struct Row : Team<NT> {
     // number over kList as soon as they are known to be more.
     __device__ __forceinline__ uint32_t list(uint32_t n, uint32_t low)
     {
-        constexpr int kAhead = 4;   // turns that are read and counted together, 16 bits of a sum for each
+        constexpr int kAhead = 2;   // turns that are read and counted together, 16 bits of a sum for each
         static_assert(NT * NE < 1 << 16, "");
         // (the least value of the number; the numbers of minus infinity and below are all values')
         const float least = low <= kLeast >> kShift ? minus_infinity() : value_of(low << kShift);
@@ -1337,7 +1337,7 @@ k_sample_levels(SelectArgs a)
 {
     __shared__ u64 s_levels[kLevels];
     __shared__ uint32_t s_most[NT / 64];
-    if (a.wide[blockIdx.x / a.wide_parts].wide != 0) count_levels<DT, NT>(a, s_levels, s_most, blockIdx.x);
+    if (a.wide[blockIdx.x / a.wide_parts].wide == 1) count_levels<DT, NT>(a, s_levels, s_most, blockIdx.x);
 }
 
 template <int NT>
@@ -1550,7 +1550,7 @@ k_sample_weigh(SelectArgs a)
     __shared__ Shared s;
     const WidePart part(a, blockIdx.x);
     const Wide wide = a.wide[part.slot];
-    if (wide.wide == 0) return;
+    if (wide.wide != 1) return;
     const uint64_t row = a.first + part.slot;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t first = part.from * a.span, to = min(part.to * a.span, a.rows.nchunks);
@@ -1616,7 +1616,7 @@ k_sample_wide(SelectArgs a)
     const Band band = a.bands[blockIdx.x];
     uint32_t n = kNoEnd, before_band = 0, mine = 0;
     u64 above = 0;
-    if (band.known) {
+    if (wide.wide == 1 && band.known) {
         Found f = {0, 0, 0};
         if (lane < a.wide_parts) f = a.found[blockIdx.x * a.wide_parts + lane];
         static_assert(kMostParts <= 64 && (kMostParts & (kMostParts - 1)) == 0, "");
@@ -1826,11 +1826,8 @@ k_sample(SelectArgs a, uint32_t rows)
             }
         }
     }
-    if (a.wide_parts == 0 || !is_wide(choice, r.top_value)) {
-        draw_by_numbers(a, r, s, choice, u, p_of_whole);
-        return;
-    }
-    if (threadIdx.x == 0) wide = {1, r.top, p_of_whole};
+    // (never where there is no launch for it: the list held all columns)
+    if (threadIdx.x == 0) wide = {is_wide(choice, r.top_value) ? 1u : 2u, r.top, p_of_whole};
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
