@@ -1,7 +1,7 @@
 // The largest logits of a row, and the draw of the next token (include/hcclx_ops.h: hcclx_top_logits_*, hcclx_sample_*).
 //
-// Two launches.  The first reads every logit once and leaves, of every 64 neighbouring columns (a group), the largest, and for runs
-// of a few chunks the sum of exp((l - most) / T) where it is wanted.  The second, a workgroup per row, works on what that left:
+// The first launch reads every logit once and leaves, of every 64 neighbouring columns (a group), the largest, and for runs of a few chunks
+// the sum of exp((l - most) / T) where it is wanted.  The second, a workgroup per row, works on what that left:
 //
 // Of the order of a row's logits (descending, of equal ones the first), the first k lie in those k groups that come first when groups
 // are ordered the same way by their largest: an element of any other group has k elements before it.  So the k groups are found among
@@ -13,9 +13,14 @@
 //
 // Weights of the draw are whole numbers too, exp((l - most) / T) 2^s from 64-bit arithmetic: their sums do not go by the order.
 //
-// A row whose draw goes by more than such a list is left to several workgroups.  Next to the second launch they count its elements by levels, 64 to a
-// power of two of their weight, which says in which level the cut lies; in a third those over that level are weighed and those in it are
-// listed; and a fourth finds the cut among these, and draws.
+// A row whose draw goes by more than such a list is left to several workgroups.  Next to the second launch they count its elements by
+// levels of their weight, 64 to a power of two, which says in which level the cut lies; in a third those over that level are weighed and
+// those in it are listed; and a fourth finds the cut among these, and draws.  (One workgroup for all of that: 64 rows of 131072 bf16,
+// a sixth of them such, 112 us instead of 36.)
+//
+// What bounds it: the first launch, by reading (8 x 4096 x 131072 bf16 192 us, 5.6 TB/s, with a sum that keeps the vector units four fifths
+// busy); the others, by how long one row takes: some twenty steps of a workgroup, each with a barrier, and the fetch of their code.  1 row
+// of 131072 3 us + 11 us + two launches that find nothing to do.
 #include "ops/logits.h"
 
 #include <algorithm>
@@ -29,8 +34,9 @@ constexpr uint32_t kGroup = 64;          // columns
 constexpr uint32_t kRunWaves = 4;        // of a workgroup of the first launch, a run each
 constexpr uint32_t kList = 2048;         // elements that are sorted at once
 constexpr uint32_t kMostGroups = HCCLX_TOP_MAX + HCCLX_TOP_MAX / 2 + 32;
-constexpr uint32_t kNucleus = 64;       // listed where no top_k bounds the list
-constexpr uint32_t kLevels = 2048;       // of the weights of a row, 64 to a power of two
+constexpr uint32_t kNucleus = 64;        // listed where no top_k bounds the list (192: 1024 rows 212 us instead of 201, and no row less)
+constexpr uint32_t kLevels = 2048;       // of the weights of a row
+constexpr uint32_t kBand = 8192;         // elements of a cut's level, 2048 of them in each part
 constexpr uint32_t kNone = 0;            // the number of what does not exist
 constexpr uint32_t kLeast = 0x007fffffu;   // of minus infinity
 
@@ -289,7 +295,7 @@ struct Range {
 };
 
 constexpr uint32_t kBins = 2048;
-constexpr uint32_t kBatch = 4096;        // rows that have memory for a wide draw at a time, 52 KB each and more where they are few
+constexpr uint32_t kBatch = 4096;        // rows that are drawn from together: 52 KB for the wide draw of each, up to 512 KB where they are few
 constexpr uint32_t kMostParts = 32;      // workgroups of a wide row
 constexpr uint32_t kMostSpans = 512;
 constexpr uint32_t kCounted = 256;       // elements of a list that is put in order by counting
@@ -298,7 +304,7 @@ constexpr uint32_t kCached = 320;        // chunks whose places in the row are k
 constexpr uint32_t kNoEnd = 0xffffffffu;
 constexpr uint32_t kStretches = 1000;    // of the range of a list's numbers
 constexpr uint32_t kMostAlike = 32;      // elements of a stretch that are put in order by counting
-constexpr uint32_t kQueue = 512;          // elements of a chunk that a wavefront weighs
+constexpr uint32_t kQueue = 512;         // elements of a chunk that a wavefront weighs
 
 // What is used at different times lies in the same place: 38 KB leave a CU room for four workgroups.
 struct Shared {
@@ -414,7 +420,7 @@ struct Team {
     __device__ __forceinline__ u64 weight(uint32_t number) const { return weight(value_of(number)); }
 
     // Sorts s.list.listed[0 .. n) into s.list.sorted, descending: into equal stretches of the range of their numbers, and in those by counting
-    // (301 lists of some 750 elements: SORT_TEXT).  Where many are alike, by exchanges.
+    // (301 rows of 32003, lists of 700: 31 us with the first launch, 44 by exchanges alone).  Where many are alike, by exchanges.
     __device__ __forceinline__ void sort(uint32_t n)
     {
         constexpr uint32_t kMine = kList / NT;
@@ -1226,23 +1232,30 @@ struct Distance {
     }
     __device__ __forceinline__ float operator()(float l) const { return (top - l) * scale; }   // (NaN of NaN)
 };
-// (minus infinity: the conversion is to the nearest that there is)
-__device__ __forceinline__ uint32_t level_of(float x) { return min(static_cast<uint32_t>(fminf(x, 65536.0f)), kLevels - 1); }
+// 64 levels to a power of two over 24 of them, and 8 to each of the 64 behind: a top_k may reach that far down.
+constexpr uint32_t kNear = 24 * 64;
+constexpr uint32_t kStep = 8;
+__device__ __forceinline__ uint32_t level_of(float x)   // (minus infinity has the nearest whole number that there is)
+{
+    const uint32_t at = static_cast<uint32_t>(fminf(x, 65536.0f));
+    return at < kNear ? at : min(kNear + (at - kNear) / kStep, kLevels - 1);
+}
+__device__ __forceinline__ uint32_t level_begin(uint32_t level) { return level < kNear ? level : kNear + (level - kNear) * kStep; }
 
 // What a level holds is one word: its elements, times 2^40, and what they lack of the weight that they would have at the level's upper
-// end, in parts of 2^22 of that: 1 - 2^(-f / 64) for an element f of a level further down, of which two terms do.  Rounding to such
-// parts costs the sum over a level some 2^-23 of itself at random, so which level holds the cut of top_p is known but for one in many
-// thousands of rows; the draw finds out.
-constexpr float kLack = 0x1p22f;
+// end, in parts of 2^22 of that (2^18 in the wide ones, which have 2^-24 of the largest's weight): 1 - 2^(-f / 64) for an element f 64ths of a power
+// of two further down, of which two terms do.  Rounding to such parts costs the sum over a level some 2^-23 of itself at random, so which level
+// holds the cut of top_p is known but for one in many thousands of rows; the draw finds out.
+__device__ __forceinline__ float lack_of(uint32_t level) { return level < kNear ? 0x1p22f : 0x1p18f; }
 __device__ __forceinline__ u64 level_entry(float x, uint32_t level)
 {
-    const float z = (x - static_cast<float>(level)) * static_cast<float>(0.69314718055994530942 / 64);
-    return u64(1) << 40 | static_cast<uint32_t>(rintf((z - 0.5f * z * z) * kLack));
+    const float z = (x - static_cast<float>(level_begin(level))) * static_cast<float>(0.69314718055994530942 / 64);
+    return u64(1) << 40 | static_cast<uint32_t>(rintf((z - 0.5f * z * z) * lack_of(level)));
 }
 __device__ __forceinline__ uint32_t entry_count(u64 e) { return static_cast<uint32_t>(e >> 40); }
-__device__ __forceinline__ double entry_weight(u64 e, double at_end)
+__device__ __forceinline__ double entry_weight(u64 e, uint32_t level, double at_end)
 {
-    return at_end * (entry_count(e) - static_cast<double>(e & ((u64(1) << 40) - 1)) * (1.0 / kLack));
+    return at_end * (entry_count(e) - static_cast<double>(e & ((u64(1) << 40) - 1)) / lack_of(level));
 }
 
 // Whether several workgroups can draw from a row: not where the weight that top_p asks for goes by a cut of top_k.
@@ -1359,7 +1372,7 @@ __device__ __forceinline__ Band band_of(const SelectArgs &a, Team<NT> &r, Shared
             const uint32_t level = threadIdx.x * kMine + i;
             const u64 e = levels[level];
             count += counts[i] = entry_count(e);
-            weight += weights[i] = counts[i] == 0 ? 0.0 : entry_weight(e, exp2_exact(-(level * apart)));
+            weight += weights[i] = counts[i] == 0 ? 0.0 : entry_weight(e, level, exp2_exact(-(level_begin(level) * apart)));
         }
         count = r.before(count, &all);
         weight = r.before(weight, &whole);
@@ -1376,8 +1389,8 @@ __device__ __forceinline__ Band band_of(const SelectArgs &a, Team<NT> &r, Shared
         const uint32_t level = s.word[0];
         __syncthreads();
         band.known = level < kLevels - 1;
-        band.low = static_cast<float>(level);
-        band.high = static_cast<float>(level + 1);
+        band.low = static_cast<float>(level_begin(level));
+        band.high = static_cast<float>(level_begin(level + 1));
     }
     if (band.by_min && band.known) {
         // (distances are good to 2^-22 of themselves, and none that matters is over 2^14)
@@ -1596,129 +1609,129 @@ k_sample_weigh(SelectArgs a)
     if (threadIdx.x == 0) a.found[blockIdx.x] = {weight, over, listed};
 }
 
-// The fourth launch: the cut, and the draw.
-template <int DT, int NT>
-__global__ void __launch_bounds__(NT)
-k_sample_wide(SelectArgs a)
+// Draws from a row of whose band n elements are listed, N for a thread at most; `over` elements of the weight `above` are nearer.  Returns false,
+// and nothing is drawn, where the cut is not among them.
+template <int DT, int NT, int N>
+__device__ __forceinline__ bool draw_band(const SelectArgs &a, Team<NT> &r, Shared &s, const RowChoice &choice, const Band &band, float u, u64 p_of_whole,
+                                          uint32_t n, uint32_t over, u64 above)
 {
     using V = Vec16<DT>;
     constexpr uint32_t NE = V::NE;
     constexpr uint32_t kWaves = NT / 64;
-    constexpr uint32_t kListed = kList / NT;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const Distance distance(r.top_value, r.c);
+    const uint64_t slot = blockIdx.x;
+    u64 key[N], w[N];
+    u64 sum = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint32_t place = threadIdx.x + i * NT;
+        uint32_t part = 0;
+#pragma unroll
+        for (uint32_t d = kMostParts / 2; d != 0; d /= 2) part += s.groups[part + d] <= place ? d : 0;
+        key[i] = place < n ? a.listed[(slot * a.wide_parts + part) * kList + place - s.groups[part]] : 0;
+        sum += w[i] = place < n ? r.weight(static_cast<uint32_t>(key[i] >> 32)) : 0;
+    }
+    const u64 inside = r.total(sum);
+    u64 last = 0;
+    if (band.by_level) {
+        const bool right = choice.by_k ? over < choice.k && over + n >= choice.k : above < p_of_whole && above + inside >= p_of_whole;
+        if (!right) return false;
+        last = last_that_stays(r, s, key, w, choice.by_k, choice.k - over, p_of_whole - above);
+    }
+    const auto stays = [&](u64 x) {
+        return x >= last && (!band.by_min || static_cast<uint32_t>(x >> 32) == r.top || r.share(static_cast<uint32_t>(x >> 32)) >= choice.least);
+    };
+    // the spans' weights, with those of the band that stay
+    __syncthreads();
+    s.span_weight[threadIdx.x] = threadIdx.x < a.nspans ? a.spans[slot * kMostSpans + threadIdx.x] : 0;
+    static_assert(NT == kMostSpans, "a thread for each span");
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (w[i] != 0 && stays(key[i])) atomicAdd(&s.span_weight[~static_cast<uint32_t>(key[i]) / kChunk<DT> / a.span], w[i]);
+    }
+    __syncthreads();
+    // the span, then the element: a wavefront for each chunk
+    sum = s.span_weight[threadIdx.x];
+    u64 whole;
+    u64 begin = r.before(sum, &whole);
+    const u64 aim = aim_of(u, whole);
+    if (aim >= begin && aim - begin < sum) {
+        s.word[0] = threadIdx.x;
+        s.word64[0] = begin;
+    }
+    __syncthreads();
+    const uint32_t first = s.word[0] * a.span;
+    const uint32_t to = min(first + a.span, a.rows.nchunks);
+    begin = s.word64[0];
+    for (uint32_t turn = first; turn < to; turn += kWaves) {
+        const bool there = turn + wave < to;
+        const uint32_t chunk = there ? turn + wave : first;
+        const Stretch t = a.rows.chunks[chunk];
+        const uint32_t elems = there ? t.elems : 0;
+        const u32x4 raw = load_piece<DT, false>(t.at + r.row * t.step, lane, elems);
+        float v[NE];
+        V::unpack(raw, v);
+        u64 each[NE];
+        sum = 0;
+#pragma unroll
+        for (uint32_t e = 0; e < NE; ++e) {
+            const u64 x = static_cast<u64>(number_of(no_nan(v[e]))) << 32 | static_cast<uint32_t>(~(chunk * kChunk<DT> + lane * NE + e));
+            const bool in = lane * NE + e < elems && (distance(v[e]) < band.low || stays(x));
+            sum += each[e] = in ? r.weight(v[e]) : 0;
+        }
+        u64 all;
+        u64 at = begin + r.before(sum, &all);
+#pragma unroll
+        for (uint32_t e = 0; e < NE; ++e) {
+            if (aim >= at && aim - at < each[e]) {
+                r.write_choice(t.first + lane * NE + e, number_of(v[e]), ldexp(static_cast<double>(whole), -static_cast<int>(a.bits)));
+            }
+            at += each[e];
+        }
+        begin += all;
+    }
+    return true;
+}
+
+// The last launch: the cut of rows that are left to it, and the draw.
+template <int DT, int NT>
+__global__ void __launch_bounds__(NT)
+k_sample_wide(SelectArgs a)
+{
     __shared__ Shared s;
     const Wide wide = a.wide[blockIdx.x];
     if (wide.wide == 0) return;
     const uint64_t row = a.first + blockIdx.x;
     const RowChoice choice(a.choice, row, a.rows.vocab);
     const float u = a.choice.random[row];
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const u64 p_of_whole = wide.p_of_whole;
-    const Band band = a.bands[blockIdx.x];
-    uint32_t n = kNoEnd, before_band = 0, mine = 0;
-    u64 above = 0;
-    if (wide.wide == 1 && band.known) {
-        Found f = {0, 0, 0};
-        if (lane < a.wide_parts) f = a.found[blockIdx.x * a.wide_parts + lane];
-        static_assert(kMostParts <= 64 && (kMostParts & (kMostParts - 1)) == 0, "");
-        mine = wave_sums(f.listed) - f.listed;   // in front of the part's
-        n = wave_total(f.listed);
-        before_band = wave_total(f.over);
-        above = wave_total(static_cast<u64>(f.weight));
-    }
-    if (n <= kList) {
-        Team<NT> r(a, s, row, wide.top, choice.c);
-        const Distance distance(r.top_value, r.c);
-        const u64 *const spans = a.spans + static_cast<uint64_t>(blockIdx.x) * kMostSpans;
-        if (threadIdx.x < 64) s.groups[lane] = lane < a.wide_parts ? mine : n;   // (begins of the parts' lists)
-        __syncthreads();
-        bool right = true;   // whether the cut is where the levels had it
-        {
-            // of those that the cut lies among
-                            const auto stays = [&](u64 key, u64 last) {
-                                return key >= last && (!band.by_min || static_cast<uint32_t>(key >> 32) == r.top || r.share(static_cast<uint32_t>(key >> 32)) >= choice.least);
-                            };
-                            u64 key[kListed], w[kListed];
-                            u64 sum = 0;
-#pragma unroll
-                            for (uint32_t i = 0; i < kListed; ++i) {
-                                const uint32_t place = threadIdx.x + i * NT;
-                                uint32_t part = 0;
-#pragma unroll
-                                for (uint32_t d = kMostParts / 2; d != 0; d /= 2) part += s.groups[part + d] <= place ? d : 0;
-                                key[i] = place < n ? a.listed[(static_cast<uint64_t>(blockIdx.x) * a.wide_parts + part) * kList + place - s.groups[part]] : 0;
-                                sum += w[i] = place < n ? r.weight(static_cast<uint32_t>(key[i] >> 32)) : 0;
-                            }
-                            const u64 inside = r.total(sum);
-                            u64 last = 0;
-                            if (band.by_level) {
-                                if (choice.by_k) {
-                                    right = before_band < choice.k && before_band + n >= choice.k;
-                                } else {
-                                    right = above < p_of_whole && above + inside >= p_of_whole;
-                                }
-                                // (the cut is where the levels had it)
-                                if (right) last = last_that_stays(r, s, key, w, choice.by_k, choice.k - before_band, p_of_whole - above);
-                            }
-                            if (right) {
-                                // the spans' weights, with those of the list that stay
-                                __syncthreads();
-                                if (threadIdx.x < kMostSpans) s.span_weight[threadIdx.x] = threadIdx.x < a.nspans ? spans[threadIdx.x] : 0;
-                                __syncthreads();
-#pragma unroll
-                                for (uint32_t i = 0; i < kListed; ++i) {
-                                    if (w[i] != 0 && stays(key[i], last)) atomicAdd(&s.span_weight[~static_cast<uint32_t>(key[i]) / kChunk<DT> / a.span], w[i]);
-                                }
-                                __syncthreads();
-                                // the span, then the element: a wavefront for each chunk
-                                sum = threadIdx.x < kMostSpans ? s.span_weight[threadIdx.x] : 0;
-                                u64 whole;
-                                u64 begin = r.before(sum, &whole);
-                                const u64 aim = aim_of(u, whole);
-                                if (aim >= begin && aim - begin < sum) {
-                                    s.word[0] = threadIdx.x;
-                                    s.word64[0] = begin;
-                                }
-                                __syncthreads();
-                                const uint32_t first = s.word[0] * a.span;
-                                const uint32_t to = min(first + a.span, a.rows.nchunks);
-                                begin = s.word64[0];
-                                for (uint32_t turn = first; turn < to; turn += kWaves) {
-                                    const bool there = turn + wave < to;
-                                    const uint32_t chunk = there ? turn + wave : first;
-                                    const Stretch t = a.rows.chunks[chunk];
-                                    const uint32_t elems = there ? t.elems : 0;
-                                    const u32x4 raw = load_piece<DT, false>(t.at + row * t.step, lane, elems);
-                                    float v[NE];
-                                    V::unpack(raw, v);
-                                    u64 each[NE];
-                                    sum = 0;
-#pragma unroll
-                                    for (uint32_t e = 0; e < NE; ++e) {
-                                        const float x = distance(v[e]);
-                                        const u64 key = static_cast<u64>(number_of(no_nan(v[e]))) << 32 | static_cast<uint32_t>(~(chunk * kChunk<DT> + lane * NE + e));
-                                        const bool in = lane * NE + e < elems && (x < band.low || stays(key, last));
-                                        sum += each[e] = in ? r.weight(v[e]) : 0;
-                                    }
-                                    u64 all;
-                                    u64 at_element = begin + r.before(sum, &all);
-#pragma unroll
-                                    for (uint32_t e = 0; e < NE; ++e) {
-                                        if (aim >= at_element && aim - at_element < each[e]) {
-                                            r.write_choice(t.first + lane * NE + e, number_of(v[e]), ldexp(static_cast<double>(whole), -static_cast<int>(a.bits)));
-                                        }
-                                        at_element += each[e];
-                                    }
-                                    begin += all;
-                                }
-                return;
+    const uint32_t lane = threadIdx.x & 63;
+    if (wide.wide == 1) {
+        const Band band = a.bands[blockIdx.x];
+        if (band.known) {
+            Found f = {0, 0, 0};
+            if (lane < a.wide_parts) f = a.found[blockIdx.x * a.wide_parts + lane];
+            static_assert(kMostParts <= 64 && (kMostParts & (kMostParts - 1)) == 0, "");
+            const uint32_t begin = wave_sums(f.listed) - f.listed;   // of the part's list in that of all
+            const uint32_t n = wave_total(f.listed), over = wave_total(f.over);
+            const u64 above = wave_total(static_cast<u64>(f.weight));
+            if (n <= kBand && wave_most(f.listed) <= kList) {
+                if (threadIdx.x < 64) s.groups[lane] = lane < a.wide_parts ? begin : n;
+                Team<NT> r(a, s, row, wide.top, choice.c);
+                __syncthreads();
+                if (n <= kBand / 4 ? draw_band<DT, NT, kBand / 4 / NT>(a, r, s, choice, band, u, wide.p_of_whole, n, over, above)
+                                   : draw_band<DT, NT, kBand / NT>(a, r, s, choice, band, u, wide.p_of_whole, n, over, above)) {
+                    return;
+                }
             }
         }
     }
-    // More elements than a list holds are in the cut's level, or it is another.
+    // The cut's level has more elements than are listed, or the cut is in another.
     __syncthreads();
     Row<DT, NT> r(a, s, row);
     r.c = choice.c;
-    draw_by_numbers(a, r, s, choice, u, p_of_whole);
+    draw_by_numbers(a, r, s, choice, u, wide.p_of_whole);
 }
 
 // The second launch: rows from a.first on.

@@ -510,6 +510,17 @@ def test_sampling_where_two_filters_cut_nearly_the_same(dtype):
             check_draws(row, shares(30000, 3), dtype, T_=4.0, min_p=min_p, top_k=place + 400, most=8)
 
 
+@pytest.mark.parametrize("dtype", [T.FP32, T.BFP16])
+def test_sampling_from_improbable_tokens_and_dense_ones(dtype):
+    """A top_k that reaches tokens of 2^-40 of the first's weight and less; a cut among thousands of tokens of nearly the same weight."""
+    steep = contents("steep", 1, 40000, gen(41))[0] * 2
+    for settings in (dict(top_k=3000), dict(top_k=39999, T_=0.4), dict(top_k=20000, T_=0.15), dict(top_p=0.9999999, T_=0.5), dict(min_p=1e-12)):
+        check_draws(steep, shares(40000, 3), dtype, most=8, **settings)
+    flat = contents("normal", 1, 300000, gen(42))[0] * 0.25
+    for settings in (dict(top_k=150000), dict(top_p=0.5), dict(top_p=0.5, min_p=0.4), dict(top_k=150000, top_p=0.7)):
+        check_draws(flat, shares(300000, 2), dtype, most=8, **settings)
+
+
 @pytest.mark.parametrize("rows,vocab", [(1, 20011), (150, 20011), (1100, 20011), (4200, 1501)])
 def test_many_rows_of_wide_draws(rows, vocab):
     """Rows whose list is too short among others, more and fewer workgroups to a row."""
