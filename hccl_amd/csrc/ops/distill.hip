@@ -1,9 +1,9 @@
 // The loss of a student against a teacher's top logits, and its gradient (include/hcclx_ops.h: hcclx_distill_*).
 //
-// With c = log2(e) / T, r a reference near the largest l c of the row and S the sum over the row of 2^(l c - r):
-//     q = 2^(l c - r) / S,   log q = (l c - r) ln 2 - log S
-// so a row needs one pass for r and S (a running reference and sum per lane, joined at the end) and one for the gradient.  Every
-// l c - r goes by the same r, so what rounds that cancels between a term and the sum, and c is held in two floats: with one, as far off as
+// With c = log2(e) / T, r the row's largest logit and S the sum over the row of 2^((l - r) c):
+//     q = 2^((l - r) c) / S,   log q = (l - r) c ln 2 - log S
+// so a row needs one pass for r and S (a running reference and sum per lane, joined at the end) and one for the gradient.  The
+// difference comes first, so that the largest term is 1 whatever the logits' magnitude, and c is held in two floats: with one, as far off as
 // 2^-25 of itself, S of logits some 20 powers of two below the largest was off by 2e-7, which the difference q - p of a student that mostly
 // agrees showed twentyfold.  What concerns the teacher's k entries alone is computed in 64 bits: the loss is a small difference of
 // logarithms.
@@ -42,20 +42,26 @@ struct DistillArgs {
     double c64;
 };
 
-// r and S of a set of columns: S = sum of 2^(l c - r).  r is finite or +infinity; -infinity: nothing in it (S = 0).
+// r and S of a set of columns: S = sum of 2^((l - r) c).  r = -infinity: nothing in it (S = 0).
 struct Sum {
     float r;
     float s;
 };
-__device__ __forceinline__ Sum join(Sum a, Sum b)
+// (l - r) c.  (The second part of c is positive: minus infinity stays that.)
+__device__ __forceinline__ float exponent(const DistillArgs &a, float l, float r)
 {
-    // (a NaN among the logits is in S, not in r)
-    const float r = fmaxf(a.r, b.r);
-    if (r == minus_infinity()) return {r, a.s + b.s};
-    return {r, a.s * exp2_fast(a.r - r) + b.s * exp2_fast(b.r - r)};
+    const float d = l - r;
+    return __builtin_fmaf(d, a.c_low, d * a.c);
+}
+// S with the reference r, of which v.r is no more.  (A NaN among the logits is in S, not in r.)
+__device__ __forceinline__ float with(const DistillArgs &a, Sum v, float r) { return r == minus_infinity() ? v.s : v.s * exp2_fast(exponent(a, v.r, r)); }
+__device__ __forceinline__ Sum join(const DistillArgs &a, Sum v, Sum o)
+{
+    const float r = fmaxf(v.r, o.r);
+    return {r, with(a, v, r) + with(a, o, r)};
 }
 // Over a wavefront, the same in every lane: a common reference first.
-__device__ __forceinline__ Sum wave_join(Sum v)
+__device__ __forceinline__ Sum wave_join(const DistillArgs &a, Sum v)
 {
     float r = v.r;
     r = fmaxf(r, dpp_or<0x111>(r, r));
@@ -64,11 +70,8 @@ __device__ __forceinline__ Sum wave_join(Sum v)
     r = fmaxf(r, dpp_or<0x118>(r, r));
     r = fmaxf(r, dpp_or<0x142>(r, r));
     r = of_last_lane(fmaxf(r, dpp_or<0x143>(r, r)));
-    return {r, wave_total(r == minus_infinity() ? v.s : v.s * exp2_fast(v.r - r))};
+    return {r, wave_total(with(a, v, r))};
 }
-
-// l c - r.  (The second part of c is positive: minus infinity stays that.)
-__device__ __forceinline__ float exponent(const DistillArgs &a, float l, float r) { return __builtin_fmaf(l, a.c_low, __builtin_fmaf(l, a.c, -r)); }
 
 // (fmaxf first makes a quiet NaN of every operand that may be a signalling one, half as much work again.  What NaN does to the largest is
 // of no matter: it is in the sum.)
@@ -93,9 +96,9 @@ __device__ __forceinline__ Sum lane_sum(const DistillArgs &a, Sum mine, const u3
 #pragma unroll
         for (int e = 0; e < NE; e += 2) most = max3(most, f[e], f[e + 1]);
     }
-    const float r = fmaxf(mine.r, most * a.c);
+    const float r = fmaxf(mine.r, most);
     const float ref = r == minus_infinity() ? 0.0f : r;   // (nothing yet: the terms are 2^-infinity)
-    float sum = mine.s * exp2_fast(mine.r - ref);
+    float sum = mine.s * exp2_fast(exponent(a, mine.r, ref));
 #pragma unroll
     for (int u = 0; u < N; ++u) {
         float f[NE];
@@ -108,9 +111,9 @@ __device__ __forceinline__ Sum lane_sum(const DistillArgs &a, Sum mine, const u3
     return {r, sum};
 }
 template <int NT>
-__device__ __forceinline__ Sum all_sum(Sum mine, Sum *s)
+__device__ __forceinline__ Sum all_sum(const DistillArgs &a, Sum mine, Sum *s)
 {
-    mine = wave_join(mine);
+    mine = wave_join(a, mine);
     if ((threadIdx.x & 63) == 0) s[threadIdx.x / 64] = mine;
     __syncthreads();
     float r = s[0].r;
@@ -118,7 +121,7 @@ __device__ __forceinline__ Sum all_sum(Sum mine, Sum *s)
     for (uint32_t w = 1; w < NT / 64; ++w) r = fmaxf(r, s[w].r);
     float sum = 0.0f;
 #pragma unroll
-    for (uint32_t w = 0; w < NT / 64; ++w) sum += r == minus_infinity() ? s[w].s : s[w].s * exp2_fast(s[w].r - r);
+    for (uint32_t w = 0; w < NT / 64; ++w) sum += with(a, s[w], r);
     return {r, sum};
 }
 
@@ -140,7 +143,7 @@ __device__ __forceinline__ Sum row_sum(const DistillArgs &a, uint64_t row, uint3
         }
         mine = lane_sum<DT>(a, mine, raw);
     }
-    return all_sum<kThreads>(mine, s);
+    return all_sum<kThreads>(a, mine, s);
 }
 
 __device__ __forceinline__ double teacher_logit(const DistillArgs &a, uint64_t at)
@@ -171,6 +174,7 @@ struct Entries {
     double t[kEach];       // its logit / T
     double p[kEach];
     bool any;              // whether the row has one that is not minus infinity
+    bool nan;              // whether p is no number: the teacher has NaN or infinity
 
     __device__ __forceinline__ void read(const DistillArgs &a, uint64_t row)
     {
@@ -204,6 +208,7 @@ struct Entries {
         }
         sum = all_of<NT, false>(sum, s[1]);
         const double log_sum = log(sum);
+        nan = sum != sum;
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
             p[i] = any ? p[i] / sum : 0.0;
@@ -266,7 +271,7 @@ __device__ __forceinline__ void store_piece(char *to, uint32_t lane, uint32_t el
     }
 }
 
-// Gradient of the chunks from..to of a row where p is 0: scale 2^(l c - r); or zeros.
+// Gradient of the chunks from..to of a row where p is 0: scale 2^((l - r) c); or zeros.
 template <int DT, int NT, bool ZERO>
 __device__ __forceinline__ void row_gradient(const DistillArgs &a, uint64_t row, uint32_t from, uint32_t to, float r, float scale)
 {
@@ -293,7 +298,7 @@ __device__ __forceinline__ void row_gradient(const DistillArgs &a, uint64_t row,
             float f[NE];
             if constexpr (!ZERO) V::unpack(raw[u], f);
 #pragma unroll
-            for (int e = 0; e < NE; ++e) f[e] = ZERO ? 0.0f : scale * exp2_fast(DT == HCCL_DATA_TYPE_FP32 ? exponent(a, f[e], r) : __builtin_fmaf(f[e], a.c, -r));   // (16 bits do not show c_low)
+            for (int e = 0; e < NE; ++e) f[e] = ZERO ? 0.0f : scale * exp2_fast(DT == HCCL_DATA_TYPE_FP32 ? exponent(a, f[e], r) : (f[e] - r) * a.c);   // (16 bits do not show c_low)
             store_piece<DT>(t.to + row * t.step, lane, t.elems, f);
         }
     }
@@ -307,7 +312,7 @@ struct DistillShared {
 };
 
 // What is left of a row, or of its chunks from..to, once r and S are known.  student: the row's logits at the entries if not nullptr.
-// gradient(scale): writes scale 2^(l c - r) everywhere.
+// gradient(scale): writes scale 2^((l - r) c) everywhere.
 template <int DT, int NT, bool LOSS, bool GRAD, typename Gradient>
 __device__ __forceinline__ void finish(const DistillArgs &a, DistillShared &s, uint64_t row, uint32_t from, uint32_t to, Sum all, float w,
                                        Entries<NT> &e, Together<NT> &together, const float *student, Gradient &&gradient)
@@ -340,7 +345,7 @@ __device__ __forceinline__ void finish(const DistillArgs &a, DistillShared &s, u
         double sum = 0.0;
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
-            const double log_q = empty ? -__builtin_inf() : (static_cast<double>(l[i]) * a.c64 - r) * kLn2 - log_s;
+            const double log_q = empty ? -__builtin_inf() : (l[i] - r) * a.c64 * kLn2 - log_s;
             if (!(e.p[i] == 0.0)) sum += e.p[i] * (e.t[i] - log_q);
         }
         sum = all_of<NT, false>(sum, s.reduce[2]);
@@ -350,12 +355,12 @@ __device__ __forceinline__ void finish(const DistillArgs &a, DistillShared &s, u
         }
     }
     if constexpr (GRAD) {
-        const float scale = static_cast<float>(w * a.T);
+        const float scale = e.nan ? __builtin_nanf("") : static_cast<float>(w * a.T);
         if (!LOSS) __syncthreads();   // the entries' logits have been read (or by the loss's sum)
         uint32_t slot[kEach];
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) slot[i] = e.any && e.at[i] != kFree ? together.add(e.at[i], e.p[i]) : 0;
-        if (empty || !e.any) {
+        if ((empty && !e.nan) || !e.any) {
             row_gradient<DT, NT, true>(a, row, from, to, 0.0f, 0.0f);
         } else {
             gradient(scale / all.s);
@@ -368,7 +373,7 @@ __device__ __forceinline__ void finish(const DistillArgs &a, DistillShared &s, u
         for (uint32_t i = 0; i < kEach; ++i) {
             if (e.at[i] < low || e.at[i] >= high) continue;
             const double p = static_cast<double>(s.sum[slot[i]]) * 0x1p-62;
-            const double q = empty ? 0.0 : exp2(static_cast<double>(l[i]) * a.c64 - r) / all.s;
+            const double q = empty ? 0.0 : exp2((l[i] - r) * a.c64) / all.s;
             reinterpret_cast<typename D::S *>(of[i]->to + row * of[i]->step)[e.at[i] - of[i]->first] =
                 D::narrow(static_cast<float>(scale * (q - p)));
         }
@@ -459,11 +464,11 @@ k_distill_parts(DistillArgs a, uint32_t parts)
         } else {
             const float2 *of = a.parts + p.row * a.nparts;
             all = {of[0].x, of[0].y};
-            for (uint32_t i = 1; i < a.nparts; ++i) all = join(all, {of[i].x, of[i].y});
+            for (uint32_t i = 1; i < a.nparts; ++i) all = join(a, all, {of[i].x, of[i].y});
         }
     }
     const auto gradient = [&](float scale) { row_gradient<DT, kThreads, false>(a, p.row, p.from, p.to, all.r, scale); };
-    const bool none = w == 0.0f || (SAVED && all.r == 0.0f && all.s == 0.0f);   // (a row that counted has S >= 1/2, is empty or NaN)
+    const bool none = w == 0.0f || (SAVED && all.r == 0.0f && all.s == 0.0f);   // (a row that counted has S >= 1, is empty or NaN)
     if (!SAVED && p.part == 0) {
         if (none) {
             nothing<DT, kThreads, true, GRAD>(a, p.row, p.from, p.to);

@@ -265,6 +265,45 @@ def test_distillation_of_many_columns_and_a_long_list():
     check_distill(contents("steep", 257, 131072, gen(9)), shares(131072, 8), T.BFP16, 64, 2.0)
 
 
+@pytest.mark.parametrize("rows", [6, 300])
+@pytest.mark.parametrize("dtype", [T.FP32, T.BFP16])
+def test_distillation_of_a_teacher_that_is_no_number(dtype, rows):
+    """NaN or +infinity among a row's entries make its loss and all its gradients NaN, and no other row's."""
+    vocab, k = 6000, 12
+    g = gen(51)
+    s = Split(contents("steep", rows, vocab, g).to(TD[dtype]), shares(vocab, 2), dtype)
+    values, at = entries(s.whole(), k, "plain", g)
+    values[1, 3], values[2, 0], values[5, k - 1] = math.nan, INF, math.nan
+    at[5, k - 1] = -1                                                # (an entry that names no column does not count)
+    for p in s.parts:
+        p[2] = -INF                                                  # with a student who rules everything out
+    loss, stats = torch.zeros(rows, device=DEV), torch.zeros((rows, 2), device=DEV)
+    d, later = [torch.zeros_like(p) for p in s.parts], [torch.zeros_like(p) for p in s.parts]
+    held = dict(s.where, strides=None, teacher=values.data_ptr(), indices=at.data_ptr(), k=k, teacher_dtype=T.FP32)
+    hcclx.DistillPlan(s.ptrs, loss=loss.data_ptr(), stats=stats.data_ptr(), dlogits=[t.data_ptr() for t in d], **held).launch()
+    hcclx.DistillGradPlan(s.ptrs, stats=stats.data_ptr(), dlogits=[t.data_ptr() for t in later], **held).launch()
+    torch.cuda.synchronize()
+    none = torch.zeros(rows, dtype=torch.bool, device=DEV)
+    none[1] = none[2] = True
+    assert torch.equal(loss.isnan(), none)
+    for t in d + later:
+        assert torch.equal(t.isnan(), none[:, None].expand_as(t))
+
+
+@pytest.mark.parametrize("dtype", [T.FP32, T.BFP16])
+@pytest.mark.parametrize("rows", [3, 280])
+def test_distillation_of_logits_of_any_magnitude(rows, dtype):
+    """Logits around 1e30, masks of the type's lowest value, temperatures from end to end."""
+    g = gen(52)
+    x = contents("normal", rows, 5000, g)
+    x[0] *= 1e30
+    x[1] = x[1] * 1e-30
+    x[2, ::2] = torch.finfo(TD[dtype]).min
+    check_distill(x, shares(5000, 2), dtype, 20, 1.0, weights=False)
+    check_distill(x, shares(5000, 2), dtype, 20, 1e6, weights=False)
+    check_distill(contents("normal", rows, 5000, g) * 1000, shares(5000, 2), dtype, 20, 1e-6, weights=False)
+
+
 def test_gradient_against_differences():
     """Central differences of the loss, h = 1/32: their error is h^2 / 6 of the third derivative, of which q's third cumulant, at most
     0.0963, is all (T = 1), and the loss's own error, as the oracle bounds it, over h."""
