@@ -245,14 +245,26 @@ k_logit_runs(SelectArgs a, uint32_t parts)
             // (bounded: minus infinity and NaN become a term of 0, and infinity has a distance of 0 from itself)
             constexpr float kBound = 0x1.fffffep+125f;
             const float c = 1.44269504f;
-            const float ref = fminf(fmaxf(most, -kBound), kBound) * c;
+            const float most_bounded = fminf(fmaxf(most, -kBound), kBound);
             float s = 0.0f;
+            if (__builtin_fabsf(most_bounded) < 0x1p20f) {
+                const float ref = most_bounded * c;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                float f[NE];
-                V::unpack(raw[u], f);
+                for (int u = 0; u < U; ++u) {
+                    float f[NE];
+                    V::unpack(raw[u], f);
 #pragma unroll
-                for (int e = 0; e < NE; ++e) s += exp2_fast(__builtin_fmaf(fminf(fmaxf(f[e], -kBound), kBound), c, -ref));
+                    for (int e = 0; e < NE; ++e) s += exp2_fast(__builtin_fmaf(fminf(fmaxf(f[e], -kBound), kBound), c, -ref));
+                }
+                s *= exp2_fast(-__builtin_fmaf(most_bounded, c, -ref));   // (what rounding the reference did to all terms)
+            } else {   // where that is more than a part of a power of two: the difference first, one operation more
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    float f[NE];
+                    V::unpack(raw[u], f);
+#pragma unroll
+                    for (int e = 0; e < NE; ++e) s += exp2_fast((fminf(fmaxf(f[e], -kBound), kBound) - most_bounded) * c);
+                }
             }
             sum = most == minus_infinity() ? 0.0 : static_cast<double>(wave_sum(s));
         } else if (most != minus_infinity()) {

@@ -153,6 +153,15 @@ def test_top_logits_of_64_ranks_and_a_million_columns():
 
 
 @pytest.mark.parametrize("dtype", [T.FP32, T.BFP16])
+def test_top_logits_of_any_magnitude(dtype):
+    x = contents("normal", 8, 9001, gen(61))
+    for r, scale in enumerate((1e30, -1e30, 1e-30, 1e3, 1e6, 1e7, 3e37, 1.0)):
+        x[r] *= scale
+    x[7, ::2] = torch.finfo(TD[dtype]).min
+    check_top(x, shares(9001, 3), dtype, 30)
+
+
+@pytest.mark.parametrize("dtype", [T.FP32, T.BFP16])
 @pytest.mark.parametrize("each,k", [(3, 100), (3, 192), (10, 70), (40, 300), (40, 900)])
 def test_top_logits_of_more_than_there_are_groups(each, k, dtype):
     """Many ranks of few columns: fewer groups of neighbouring columns hold anything than entries are asked for."""
@@ -495,6 +504,49 @@ def test_plans_on_two_streams_at_once():
                 plan.launch(stream.cuda_stream)
     torch.cuda.synchronize()
     assert same(one[1], want[0]) and same(two[1], want[1])
+
+
+def test_a_teacher_a_student_and_an_answer():
+    """All of them one behind the other, as a step that distils and then answers uses them: a teacher's list of 32-bit logits, the loss and the
+    gradients of a student whose columns are shared differently, logits that follow the gradients, their list and a draw."""
+    rows, vocab, k, temperature, g = 40, 12001, 48, 2.0, gen(71)
+    teacher = Split(contents("steep", rows, vocab, g), shares(vocab, 2), T.FP32, pad=1)
+    student = Split((teacher.whole() * 0.5 + torch.randn((rows, vocab), device=DEV, generator=g)).bfloat16(), shares(vocab, 8), T.BFP16)
+    values, indices = torch.empty((rows, k), device=DEV), torch.empty((rows, k), device=DEV, dtype=torch.int32)
+    weight = torch.rand(rows, device=DEV, generator=g)
+    weight[::10] = 0
+    loss, d = torch.empty(rows, device=DEV), [torch.zeros_like(p) for p in student.parts]
+    best, numbers = torch.empty((rows, 5), device=DEV, dtype=torch.bfloat16), torch.empty((rows, 5), device=DEV, dtype=torch.int32)
+    random, top_p = torch.rand(rows, device=DEV, generator=g), torch.full((rows,), 0.9, device=DEV)
+    tokens, lse = torch.empty(rows, device=DEV, dtype=torch.int32), torch.empty(rows, device=DEV)
+    before = student.whole().clone()
+    where = dict(student.where, strides=None)
+    plans = [hcclx.TopLogitsPlan(teacher.ptrs, k=k, values=values.data_ptr(), indices=indices.data_ptr(), **teacher.where),
+             hcclx.DistillPlan(student.ptrs, teacher=values.data_ptr(), indices=indices.data_ptr(), k=k, teacher_dtype=T.FP32, temperature=temperature,
+                               weight=weight.data_ptr(), loss=loss.data_ptr(), dlogits=[t.data_ptr() for t in d], **where),
+             hcclx.TopLogitsPlan(student.ptrs, k=5, values=best.data_ptr(), indices=numbers.data_ptr(), lse=lse.data_ptr(), **where),
+             hcclx.SamplePlan(student.ptrs, random=random.data_ptr(), tokens=tokens.data_ptr(), top_p=top_p.data_ptr(), **where)]
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        for i, plan in enumerate(plans):
+            plan.launch(stream.cuda_stream)
+            if i == 1:
+                for p, t in zip(student.parts, d):
+                    p.sub_(t, alpha=10.0)
+    stream.synchronize()
+    gradient, after = torch.cat(d, 1), student.whole()
+    for r in range(rows):
+        l = L.plain(teacher.whole()[r])
+        assert torch.equal(indices[r].long(), L.order(l)[:k])
+        want, grad, bound, grad_bound = L.distill(before[r].double(), values[r].double(), indices[r], temperature, float(weight[r]))
+        assert abs(float(loss[r]) - want) <= bound + O.E * abs(want)
+        O.assert_close(gradient[r], grad, grad_bound, f"row {r}")
+        l = L.plain(after[r])
+        first = L.order(l)[:5]
+        assert torch.equal(numbers[r].long(), first) and torch.equal(best[r].double(), l[first])
+        want, bound = L.lse(l)
+        assert abs(float(lse[r]) - want) <= bound + O.E * abs(want)
+        assert int(tokens[r]) == L.sample(l, 1.0, 0, float(np.float32(0.9)), 0.0, float(random[r]))[0]
 
 
 def test_no_rows():
