@@ -36,7 +36,7 @@ constexpr uint32_t kList = 2048;         // elements that are sorted at once
 constexpr uint32_t kMostGroups = HCCLX_TOP_MAX + HCCLX_TOP_MAX / 2 + 32;
 constexpr uint32_t kNucleus = 64;        // listed where no top_k bounds the list (192: 1024 rows 212 us instead of 201, and no row less)
 constexpr uint32_t kLevels = 2048;       // of the weights of a row
-constexpr uint32_t kBand = 8192;         // elements of a cut's level, 2048 of them in each part
+constexpr uint32_t kBand = 8192;         // elements of a cut's level, shared out to the parts of a row
 constexpr uint32_t kNone = 0;            // the number of what does not exist
 constexpr uint32_t kLeast = 0x007fffffu;   // of minus infinity
 
@@ -92,11 +92,12 @@ struct SelectArgs {
     unsigned long long *levels;   // [batch][kLevels]
     struct Band *bands;           // [batch]
     struct Found *found;          // [batch][wide_parts]
-    unsigned long long *listed;   // [batch][wide_parts][kList]: the elements that the cut lies among
+    unsigned long long *listed;   // [batch][wide_parts][band_each]: the elements that the cut lies among
     unsigned long long *spans;    // [batch][kMostSpans]: weights over them
     uint32_t span;      // chunks that are weighed together
     uint32_t nspans;
     uint32_t wide_parts;   // workgroups of a row
+    uint32_t band_each;    // elements that a part may list
     uint32_t first;
     // the largest
     uint32_t k;
@@ -307,7 +308,7 @@ struct Range {
 };
 
 constexpr uint32_t kBins = 2048;
-constexpr uint32_t kBatch = 4096;        // rows that are drawn from together: 52 KB for the wide draw of each, up to 512 KB where they are few
+constexpr uint32_t kBatch = 4096;        // rows that are drawn from together: 85 KB for the wide draw of each, 150 KB where they are few
 constexpr uint32_t kMostParts = 32;      // workgroups of a wide row
 constexpr uint32_t kMostSpans = 512;
 constexpr uint32_t kCounted = 256;       // elements of a list that is put in order by counting
@@ -355,6 +356,7 @@ struct Shared {
     u64 part[2][kMostWaves];
     uint32_t most[kMostWaves];
     uint32_t least[kMostWaves];
+    uint32_t place[kMostWaves];
     Range range;
     u64 word64[2];
     uint32_t word[4];
@@ -1476,44 +1478,43 @@ __device__ __forceinline__ u64 weigh_chunk(const Team<NT> &r, Shared &s, const D
 
 // What stays of a list whose elements the threads hold, kListed each (key 0: none): those from the returned key on.  `skip` of them stay (top_k), or
 // those before whose place in the order the weight is less than `aim`.  As by Row::narrow: keys are counted and weighed into equal
-// stretches of their range, which leaves one of them.
+// stretches of their range, which leaves one of them: two rounds, or three where many numbers are alike.
 template <int NT, int N>
 __device__ __forceinline__ u64 last_that_stays(Team<NT> &r, Shared &s, const u64 (&key)[N], const u64 (&weight)[N], bool by_count, uint32_t stay, u64 aim)
 {
-    constexpr uint32_t kMine = kBins / NT;
-    if (threadIdx.x == 0) {
-        s.word64[0] = ~u64(0);
-        s.word64[1] = 0;
-    }
-    __syncthreads();
-    u64 low = ~u64(0), high = 0;
+    static_assert(NT == 512, "a stretch for each thread");
+    const uint32_t t = threadIdx.x;
+    uint32_t most = 0, least = kNoEnd, place = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         if (key[i] == 0) continue;
-        low = min(low, key[i]);
-        high = max(high, key[i]);
+        most = max(most, static_cast<uint32_t>(key[i] >> 32));
+        least = min(least, static_cast<uint32_t>(key[i] >> 32));
+        place = max(place, ~static_cast<uint32_t>(key[i]));
     }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-        low = min(low, static_cast<u64>(__shfl_xor(low, d, 64)));
-        high = max(high, static_cast<u64>(__shfl_xor(high, d, 64)));
-    }
-    if ((threadIdx.x & 63) == 0) {
-        atomicMin(&s.word64[0], low);
-        atomicMax(&s.word64[1], high);
+    most = wave_most(most);
+    least = ~wave_most(~least);
+    place = wave_most(place);
+    if ((t & 63) == 0) {
+        s.most[t / 64] = most;
+        s.least[t / 64] = least;
+        s.place[t / 64] = place;
     }
     __syncthreads();
-    low = s.word64[0];
-    high = s.word64[1];
+#pragma unroll
+    for (uint32_t w = 0; w < NT / 64; ++w) {
+        most = max(most, s.most[w]);
+        least = min(least, s.least[w]);
+        place = max(place, s.place[w]);
+    }
+    u64 low = static_cast<u64>(least) << 32 | static_cast<uint32_t>(~place), high = static_cast<u64>(most) << 32 | kNoEnd;
     uint32_t count_before = 0;
     u64 weight_before = 0;
     while (low != high) {
         const u64 width = high - low;
-        const uint32_t shift = width < kBins ? 0 : 64 - __clzll(static_cast<long long>(width)) - 11;
-        for (uint32_t i = threadIdx.x; i < kBins; i += NT) {
-            s.bins.count[i] = 0;
-            s.bins.weight[i] = 0;
-        }
+        const uint32_t shift = width < NT ? 0 : 64 - __clzll(static_cast<long long>(width)) - 9;
+        s.bins.count[t] = 0;
+        s.bins.weight[t] = 0;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -1523,27 +1524,14 @@ __device__ __forceinline__ u64 last_that_stays(Team<NT> &r, Shared &s, const u64
             if (weight[i] != 0) atomicAdd(&s.bins.weight[bin], weight[i]);
         }
         __syncthreads();
-        uint32_t counts = 0, all;
-        u64 weights = 0, whole;
-#pragma unroll
-        for (uint32_t i = 0; i < kMine; ++i) {
-            const uint32_t bin = kBins - 1 - (threadIdx.x * kMine + i);
-            counts += s.bins.count[bin];
-            weights += s.bins.weight[bin];
-        }
-        uint32_t c = count_before + r.before(counts, &all);
-        u64 w = weight_before + r.before(weights, &whole);
-#pragma unroll
-        for (uint32_t i = 0; i < kMine; ++i) {
-            const uint32_t bin = kBins - 1 - (threadIdx.x * kMine + i);
-            const uint32_t more = s.bins.count[bin];
-            const u64 add = s.bins.weight[bin];
-            if (more != 0 && (by_count ? c < stay && c + more >= stay : w < aim && w + add >= aim)) {
-                s.range = {bin, 0, c, more, w, 0};
-            }
-            c += more;
-            w += add;
-        }
+        const uint32_t bin = NT - 1 - t;   // from the top
+        const uint32_t more = s.bins.count[bin];
+        const u64 add = s.bins.weight[bin];
+        uint32_t all;
+        u64 whole;
+        const uint32_t c = count_before + r.before(more, &all);
+        const u64 w = weight_before + r.before(add, &whole);
+        if (more != 0 && (by_count ? c < stay && c + more >= stay : w < aim && w + add >= aim)) s.range = {bin, 0, c, more, w, 0};
         __syncthreads();
         const Range found = s.range;
         count_before = found.above;
@@ -1559,7 +1547,6 @@ __device__ __forceinline__ u64 last_that_stays(Team<NT> &r, Shared &s, const u64
             __syncthreads();
             return s.one;
         }
-        __syncthreads();
     }
     return low;
 }
@@ -1617,7 +1604,7 @@ k_sample_weigh(SelectArgs a)
     over = r.total(lane == 0 ? over : 0);
     if (threadIdx.x < part.to - part.from) a.spans[static_cast<uint64_t>(part.slot) * kMostSpans + part.from + threadIdx.x] = s.span_weight[threadIdx.x];
     const uint32_t listed = s.word[2];
-    for (uint32_t i = threadIdx.x; i < min(listed, kList); i += NT) a.listed[static_cast<uint64_t>(blockIdx.x) * kList + i] = s.wide.listed[i];
+    for (uint32_t i = threadIdx.x; i < min(listed, a.band_each); i += NT) a.listed[static_cast<uint64_t>(blockIdx.x) * a.band_each + i] = s.wide.listed[i];
     if (threadIdx.x == 0) a.found[blockIdx.x] = {weight, over, listed};
 }
 
@@ -1641,7 +1628,7 @@ __device__ __forceinline__ bool draw_band(const SelectArgs &a, Team<NT> &r, Shar
         uint32_t part = 0;
 #pragma unroll
         for (uint32_t d = kMostParts / 2; d != 0; d /= 2) part += s.groups[part + d] <= place ? d : 0;
-        key[i] = place < n ? a.listed[(slot * a.wide_parts + part) * kList + place - s.groups[part]] : 0;
+        key[i] = place < n ? a.listed[(slot * a.wide_parts + part) * a.band_each + place - s.groups[part]] : 0;
         sum += w[i] = place < n ? r.weight(static_cast<uint32_t>(key[i] >> 32)) : 0;
     }
     const u64 inside = r.total(sum);
@@ -1728,7 +1715,7 @@ k_sample_wide(SelectArgs a)
             const uint32_t begin = wave_sums(f.listed) - f.listed;   // of the part's list in that of all
             const uint32_t n = wave_total(f.listed), over = wave_total(f.over);
             const u64 above = wave_total(static_cast<u64>(f.weight));
-            if (n <= kBand && wave_most(f.listed) <= kList) {
+            if (n <= kBand && wave_most(f.listed) <= a.band_each) {
                 if (threadIdx.x < 64) s.groups[lane] = lane < a.wide_parts ? begin : n;
                 Team<NT> r(a, s, row, wide.top, choice.c);
                 __syncthreads();
@@ -1761,9 +1748,9 @@ k_sample(SelectArgs a, uint32_t rows)
     const uint64_t row = a.first + blockIdx.x;
     Wide &wide = a.wide[blockIdx.x];
     if (threadIdx.x == 0) wide.wide = 0;
+    Row<DT, NT> r(a, s, row);
     const RowChoice choice(a.choice, row, a.rows.vocab);
     const float u = a.choice.random[row];
-    Row<DT, NT> r(a, s, row);
     r.c = choice.c;
     if (r.top <= kLeast) {   // nothing to choose from
         if (threadIdx.x == 0) {
@@ -1937,10 +1924,10 @@ int finish(const hcclx_logits_t &l, uint32_t vocab, bool sums, std::unique_ptr<S
     SelectArgs &a = w->args;
     a.rows = w->table.rows;
     w->dtype = l.dtype;
-    // As many chunks per wavefront as leave every CU four workgroups.
+    // As many chunks per wavefront as leave every CU eight workgroups (64 draws of 131072 44.8 us, with four 46.2, with eight chunks 47.7).
     a.per_run = 8;
     auto parts = [&] { return (a.rows.nchunks + a.per_run * kRunWaves - 1) / (a.per_run * kRunWaves); };
-    while (a.per_run > 1 && static_cast<uint64_t>(l.rows) * parts() < 4ull * static_cast<uint32_t>(ctx->num_cus)) a.per_run /= 2;
+    while (a.per_run > 1 && static_cast<uint64_t>(l.rows) * parts() < 8ull * static_cast<uint32_t>(ctx->num_cus)) a.per_run /= 2;
     w->parts = parts();
     if (static_cast<uint64_t>(l.rows) * w->parts * kRunWaves * 64 > 0xffffffffull) return fail(HCCL_E_PARA, "too many rows of so many columns");
     a.nruns = (a.rows.nchunks + a.per_run - 1) / a.per_run;
@@ -1960,17 +1947,20 @@ int finish(const hcclx_logits_t &l, uint32_t vocab, bool sums, std::unique_ptr<S
         // Rows that the list of kNucleus always does for are never wide; nor are those that no filter but a short top_k may shorten, which
         // only the device knows.
         w->batch = std::min(l.rows, kBatch);
+        w->apart = w->batch > static_cast<uint32_t>(ctx->num_cus);
         const bool may_be_wide = vocab > kNucleus && (a.choice.top_k != nullptr || a.choice.top_p != nullptr || a.choice.min_p != nullptr);
         a.span = (a.rows.nchunks + kMostSpans - 1) / kMostSpans;
         a.nspans = (a.rows.nchunks + a.span - 1) / a.span;
-        // Workgroups for a row that may be wide: most rows are not, and their workgroups only look.
-        a.wide_parts = !may_be_wide ? 0 : std::min(a.nspans, std::min(kMostParts, std::max(2u, 4096 / w->batch)));
-        w->apart = w->batch > static_cast<uint32_t>(ctx->num_cus);
+        // Workgroups for a row that may be wide: most rows are not, and their workgroups only look.  In launches of their own eight for a row
+        // (1024 rows 194 us, with four 211, with two 240), next to the lists as many as there is room for (256 rows 76 us with eight, 80 with
+        // sixteen, 85 with 32; 1 row 17 with 32).
+        a.wide_parts = !may_be_wide ? 0 : std::min(a.nspans, w->apart ? std::clamp(8192 / w->batch, 2u, 8u) : std::clamp(2048 / w->batch, 2u, kMostParts));
+        a.band_each = std::clamp(kBand / std::max(1u, a.wide_parts), 512u, kList);
         wide = more(w->batch * sizeof(Wide));
         levels = more(may_be_wide ? w->batch * sizeof(u64) * kLevels : 0);
         bands = more(w->batch * sizeof(Band));
         found = more(static_cast<uint64_t>(w->batch) * a.wide_parts * sizeof(Found));
-        listed = more(static_cast<uint64_t>(w->batch) * a.wide_parts * sizeof(u64) * kList);
+        listed = more(static_cast<uint64_t>(w->batch) * a.wide_parts * sizeof(u64) * a.band_each);
         spans = more(may_be_wide ? w->batch * sizeof(u64) * kMostSpans : 0);
     }
     if (held != 0 && (rc = w->scratch.get(held)) != HCCL_SUCCESS) return rc;
