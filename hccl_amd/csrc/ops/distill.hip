@@ -329,11 +329,11 @@ __device__ __forceinline__ void finish(const DistillArgs &a, DistillShared &s, u
         of[i] = a.rows.ranks;
         l[i] = 0.0f;
         const bool mine = e.at[i] >= low && e.at[i] < high;
-        if (e.at[i] != kFree && (mine || student == nullptr)) {
+        if (mine) {   // (kFree is no column)
             of[i] = rank_of(a.rows, e.at[i]);
             // (all are read before the first gradient is written: it may lie on the logits)
             l[i] = student != nullptr ? student[threadIdx.x + i * NT] : load_one<DT>(of[i]->at + row * of[i]->step, e.at[i] - of[i]->first);
-        } else if (e.at[i] != kFree && LOSS) {
+        } else if (LOSS && e.at[i] != kFree) {
             l[i] = student[threadIdx.x + i * NT];
         }
         if (!mine && GRAD && !LOSS) e.at[i] = kFree;   // (after the entries' weights are known)

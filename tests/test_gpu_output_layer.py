@@ -313,6 +313,38 @@ def test_distillation_of_logits_of_any_magnitude(rows, dtype):
     check_distill(contents("normal", rows, 5000, g) * 1000, shares(5000, 2), dtype, 20, 1e-6, weights=False)
 
 
+@pytest.mark.parametrize("dtype", [T.FP32, T.BFP16])
+@pytest.mark.parametrize("rows", [1, 5, 300])
+def test_gradients_from_stats_on_the_logits(rows, dtype):
+    """The gradient of the saved sums may lie on the logits as well, by several workgroups to a row."""
+    vocab, k = 50021, 100
+    g = gen(53)
+    s = Split(contents("steep", rows, vocab, g).to(TD[dtype]), shares(vocab, 3), dtype, pad=2, skew=1)
+    values, at = entries(s.whole(), k, "twice", g)
+    weight = torch.rand(rows, device=DEV, generator=g)
+    weight[1::3] = 0
+    stats = torch.zeros((rows, 2), device=DEV)
+    held = dict(s.where, teacher=values.data_ptr(), indices=at.data_ptr(), k=k, teacher_dtype=T.FP32, weight=weight.data_ptr())
+    hcclx.DistillPlan(s.ptrs, stats=stats.data_ptr(), **held).launch()
+    apart = Split(torch.zeros_like(s.whole()), shares(vocab, 3), dtype, pad=2, skew=1)
+    hcclx.DistillGradPlan(s.ptrs, stats=stats.data_ptr(), dlogits=apart.ptrs, **held).launch()
+    hcclx.DistillGradPlan(s.ptrs, stats=stats.data_ptr(), dlogits=s.ptrs, **held).launch()
+    torch.cuda.synchronize()
+    assert bool(apart.whole().any()) and torch.equal(s.whole(), apart.whole())
+    assert s.untouched()
+
+
+def test_the_most_columns():
+    """2^24 of them: rows of 65536 chunks of 32-bit logits."""
+    vocab = 1 << 24
+    row = contents("steep", 1, vocab, gen(54))
+    check_top(row, shares(vocab, 3), T.FP32, 1024)
+    check_top(row, shares(vocab, 64), T.BFP16, 40)
+    check_distill(row, shares(vocab, 3), T.BFP16, 30, 1.5, weights=False)
+    for settings in (dict(), dict(top_k=50), dict(top_p=0.9), dict(T_=0.8, top_p=0.95), dict(top_k=100000), dict(min_p=0.0001)):
+        check_draws(row[0], shares(vocab, 3), T.FP32, most=3, **settings)
+
+
 def test_gradient_against_differences():
     """Central differences of the loss, h = 1/32: their error is h^2 / 6 of the third derivative, of which q's third cumulant, at most
     0.0963, is all (T = 1), and the loss's own error, as the oracle bounds it, over h."""
@@ -577,6 +609,15 @@ def test_rows_behind_4_gib():
     want, grad, bound, grad_bound = L.distill(last, values[-1].double(), indices[-1], 1.0, 1.0)
     assert abs(float(loss[-1]) - want) <= bound + O.E * abs(want)
     O.assert_close(whole[-1], grad, grad_bound)
+
+
+@pytest.mark.parametrize("dtype", [T.FP32, T.BFP16])
+def test_sampling_of_many_infinities(dtype):
+    row = contents("normal", 1, 30000, gen(55))[0]
+    row[7::97] = INF
+    row[11::13] = math.nan
+    for settings in (dict(), dict(top_p=0.9), dict(top_p=0.5, T_=0.3), dict(min_p=0.2), dict(top_k=200), dict(top_k=5000, top_p=0.8), dict(top_k=5000), dict(T_=0.0)):
+        check_draws(row, shares(30000, 4), dtype, most=12, **settings)
 
 
 @pytest.mark.parametrize("dtype", [T.FP32, T.BFP16])
