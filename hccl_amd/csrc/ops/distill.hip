@@ -20,6 +20,7 @@ namespace {
 constexpr uint32_t kThreads = 512;
 constexpr uint32_t kMostWaves = kThreads / 64;
 constexpr int kAhead = 4;                                        // chunks of a wavefront that are on their way together
+constexpr int kHeld = 8;                                         // vectors of a thread that holds its part of a row
 constexpr uint32_t kSlots = 2 * HCCLX_TOP_MAX;                   // of the table of the entries' columns
 constexpr uint32_t kFree = 0xffffffffu;
 constexpr double kLn2 = 0.69314718055994530942;
@@ -415,6 +416,53 @@ k_distill_row(DistillArgs a)
                                  [&](float scale) { row_gradient<DT, kThreads, false>(a, row, 0, n, all.r, scale); });
 }
 
+// The same where rows are few and short: a row stays in the threads' registers, N vectors in each, instead of being read twice.  What counts
+// there is the chain of one row (16 rows of 32000 bf16 10.3 us, read twice 11.8; of 8000 9.8 and 9.2, the code of N vectors costs more than
+// one more turn; where rows fill the device, 4096 of 32000, 190 and 145: fewer of them are there at once).
+template <int DT, int N>
+__global__ void __launch_bounds__(kThreads)
+k_distill_held(DistillArgs a)
+{
+    using V = Vec16<DT>;
+    constexpr int NE = V::NE;
+    constexpr uint32_t kWaves = kThreads / 64;
+    __shared__ DistillShared s;
+    const uint64_t row = blockIdx.x;
+    const uint32_t n = a.rows.nchunks;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t lane = threadIdx.x & 63;
+    const float w = a.weight != nullptr ? a.weight[row] : 1.0f;
+    if (w == 0.0f) {
+        nothing<DT, kThreads, true, true>(a, row, 0, n);
+        return;
+    }
+    u32x4 raw[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        const uint32_t i = wave + u * kWaves;
+        const Stretch t = a.rows.chunks[i < n ? i : 0];
+        raw[u] = load_piece<DT, true>(t.at + row * t.step, lane, i < n ? t.elems : 0);
+    }
+    Together<kThreads> together(s.column, s.sum, a.k);
+    Entries<kThreads> e;
+    e.read(a, row);
+    const Sum all = all_sum<kThreads>(a, lane_sum<DT>(a, {minus_infinity(), 0.0f}, raw), s.sums);
+    e.normalise(s.reduce);
+    finish<DT, kThreads, true, true>(a, s, row, 0, n, all, w, e, together, nullptr, [&](float scale) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const uint32_t i = wave + u * kWaves;
+            if (i >= n) break;
+            const Stretch t = a.rows.chunks[i];
+            float f[NE];
+            V::unpack(raw[u], f);
+#pragma unroll
+            for (int k = 0; k < NE; ++k) f[k] = scale * exp2_fast(DT == HCCL_DATA_TYPE_FP32 ? exponent(a, f[k], all.r) : (f[k] - all.r) * a.c);
+            store_piece<DT>(t.to + row * t.step, lane, t.elems, f);
+        }
+    });
+}
+
 // The chunks of a part of a row, of which there are `parts`.
 struct Part {
     uint64_t row;
@@ -498,7 +546,7 @@ k_distill_parts(DistillArgs a, uint32_t parts)
 uint32_t parts_of(uint32_t rows, uint32_t nchunks, uint32_t most)
 {
     const uint32_t fill = rows >= most ? 1 : most / rows;
-    // (four chunks for a wavefront: 16 rows of 32000 bf16 11.8 us in a workgroup each, 13 in three, of 131072 13 in eight and 29 in one)
+    // (four chunks for a wavefront: 16 rows of 131072 bf16 13 us in eight workgroups each, 29 in one; of 32000 13 in three, 11.8 in one)
     return std::max(1u, std::min(fill, nchunks / (kThreads / 64 * kAhead)));
 }
 
@@ -510,6 +558,7 @@ struct DistillWork : PlanWork {
     int dtype = 0;
     bool saved = false;    // the gradient from what the loss saved
     bool grad = false;
+    bool held = false;     // rows in registers
 
     template <int DT>
     void run(hipStream_t st) const
@@ -519,7 +568,9 @@ struct DistillWork : PlanWork {
         if (saved) {
             HCCLX_LAUNCH((k_distill_parts<DT, true, true>), grid, block, 0, st, args, parts);
         } else if (parts == 1) {
-            if (grad) {
+            if (held) {
+                HCCLX_LAUNCH((k_distill_held<DT, kHeld>), grid, block, 0, st, args);
+            } else if (grad) {
                 HCCLX_LAUNCH((k_distill_row<DT, true>), grid, block, 0, st, args);
             } else {
                 HCCLX_LAUNCH((k_distill_row<DT, false>), grid, block, 0, st, args);
@@ -623,7 +674,9 @@ int make_distill(const hcclx_distill_t &d, hcclx_plan_t **plan)
     w->args.loss = d.loss;
     w->args.stats = reinterpret_cast<float2 *>(d.stats);
     uint64_t held = w->table.bytes;
-    if (rows != 0) w->parts = parts_of(l.rows, w->args.rows.nchunks, static_cast<uint32_t>(ctx->num_cus));
+    const uint32_t cus = static_cast<uint32_t>(ctx->num_cus), turn = kThreads / 64 * kAhead;
+    w->held = w->grad && l.rows <= cus && w->args.rows.nchunks > turn && w->args.rows.nchunks <= kThreads / 64 * kHeld;
+    if (rows != 0 && !w->held) w->parts = parts_of(l.rows, w->args.rows.nchunks, cus);
     if (w->parts > 1) {
         w->args.nparts = w->parts;
         const uint64_t sums = rows * w->parts * sizeof(float2);
