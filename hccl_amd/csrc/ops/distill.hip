@@ -418,7 +418,7 @@ k_distill_row(DistillArgs a)
 
 // The same where rows are few and short: a row stays in the threads' registers, N vectors in each, instead of being read twice.  What counts
 // there is the chain of one row (16 rows of 32000 bf16 10.3 us, read twice 11.8; of 8000 9.8 and 9.2, the code of N vectors costs more than
-// one more turn; where rows fill the device, 4096 of 32000, 190 and 145: fewer of them are there at once).
+// one more turn), of up to the two rows that a CU has room for (500 of 32000 17.7 and 19.5, 1000 32 and 32, 4096 190 and 145).
 template <int DT, int N>
 __global__ void __launch_bounds__(kThreads)
 k_distill_held(DistillArgs a)
@@ -675,7 +675,7 @@ int make_distill(const hcclx_distill_t &d, hcclx_plan_t **plan)
     w->args.stats = reinterpret_cast<float2 *>(d.stats);
     uint64_t held = w->table.bytes;
     const uint32_t cus = static_cast<uint32_t>(ctx->num_cus), turn = kThreads / 64 * kAhead;
-    w->held = w->grad && l.rows <= cus && w->args.rows.nchunks > turn && w->args.rows.nchunks <= kThreads / 64 * kHeld;
+    w->held = w->grad && l.rows <= 2 * cus && w->args.rows.nchunks > turn && w->args.rows.nchunks <= kThreads / 64 * kHeld;
     if (rows != 0 && !w->held) w->parts = parts_of(l.rows, w->args.rows.nchunks, cus);
     if (w->parts > 1) {
         w->args.nparts = w->parts;
