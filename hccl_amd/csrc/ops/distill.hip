@@ -18,10 +18,10 @@ using namespace hcclx::logits;
 namespace {
 
 constexpr uint32_t kThreads = 512;
+constexpr uint32_t kSmall = 256;                                 // of a workgroup for a short row
 constexpr uint32_t kMostWaves = kThreads / 64;
 constexpr int kAhead = 4;                                        // chunks of a wavefront that are on their way together
 constexpr int kHeld = 8;                                         // vectors of a thread that holds its part of a row
-constexpr uint32_t kSlots = 2 * HCCLX_TOP_MAX;                   // of the table of the entries' columns
 constexpr uint32_t kFree = 0xffffffffu;
 constexpr double kLn2 = 0.69314718055994530942;
 
@@ -36,6 +36,7 @@ struct DistillArgs {
     float *student;        // [rows][k]: the student's logits at the teacher's entries, where several workgroups share a row
     uint32_t nparts;       // of the rows whose r and S are in `parts`
     uint32_t k;
+    uint32_t mask;         // slots of the table of the entries' columns, less one
     int teacher_dtype;
     float c;               // log2(e) / T: the float below it, and what is left, which is more than 0
     float c_low;
@@ -127,10 +128,10 @@ __device__ __forceinline__ Sum all_sum(const DistillArgs &a, Sum mine, Sum *s)
 }
 
 // r and S over the chunks from..to of a row, of all threads (s: one for each wavefront).
-template <int DT, bool ONCE>
+template <int DT, int NT, bool ONCE>
 __device__ __forceinline__ Sum row_sum(const DistillArgs &a, uint64_t row, uint32_t from, uint32_t to, Sum *s)
 {
-    constexpr uint32_t kWaves = kThreads / 64;
+    constexpr uint32_t kWaves = NT / 64;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t lane = threadIdx.x & 63;
     Sum mine = {minus_infinity(), 0.0f};
@@ -144,7 +145,7 @@ __device__ __forceinline__ Sum row_sum(const DistillArgs &a, uint64_t row, uint3
         }
         mine = lane_sum<DT>(a, mine, raw);
     }
-    return all_sum<kThreads>(a, mine, s);
+    return all_sum<NT>(a, mine, s);
 }
 
 __device__ __forceinline__ double teacher_logit(const DistillArgs &a, uint64_t at)
@@ -218,18 +219,23 @@ struct Entries {
     }
 };
 
+struct DistillShared {
+    Sum sums[kMostWaves];
+    double reduce[3][kMostWaves];
+};
+extern __shared__ unsigned long long s_table[];   // sums and columns of the entries, as many as the plan's k needs (Together)
+
 // Sums p over the entries that name the same column: where the entry's sum is.  Sums are of whole numbers, so that their order does not
 // show.  (p: of 2^62.)  Between the table's making and the first entry lies a barrier of the caller's.
 template <int NT>
 struct Together {
-    uint32_t *column;   // kSlots
-    unsigned long long *sum;
-    uint32_t mask;
-    __device__ __forceinline__ Together(uint32_t *c, unsigned long long *s, uint32_t k) : column(c), sum(s)
+    unsigned long long *const sum;
+    uint32_t *const column;
+    const uint32_t mask;
+    // (used: false where the launch has no memory for it)
+    __device__ __forceinline__ Together(uint32_t last, bool used) : sum(s_table), column(reinterpret_cast<uint32_t *>(s_table + last + 1)), mask(last)
     {
-        mask = 63;
-        while (mask + 1 < 2 * k) mask = 2 * mask + 1;
-        for (uint32_t i = threadIdx.x; i <= mask; i += NT) {
+        for (uint32_t i = threadIdx.x; used && i <= mask; i += NT) {
             column[i] = kFree;
             sum[i] = 0;
         }
@@ -305,13 +311,6 @@ __device__ __forceinline__ void row_gradient(const DistillArgs &a, uint64_t row,
     }
 }
 
-struct DistillShared {
-    Sum sums[kMostWaves];
-    double reduce[3][kMostWaves];
-    uint32_t column[kSlots];
-    unsigned long long sum[kSlots];
-};
-
 // What is left of a row, or of its chunks from..to, once r and S are known.  student: the row's logits at the entries if not nullptr.
 // gradient(scale): writes scale 2^((l - r) c) everywhere.
 template <int DT, int NT, bool LOSS, bool GRAD, typename Gradient>
@@ -373,7 +372,7 @@ __device__ __forceinline__ void finish(const DistillArgs &a, DistillShared &s, u
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
             if (e.at[i] < low || e.at[i] >= high) continue;
-            const double p = static_cast<double>(s.sum[slot[i]]) * 0x1p-62;
+            const double p = static_cast<double>(together.sum[slot[i]]) * 0x1p-62;
             const double q = empty ? 0.0 : exp2((l[i] - r) * a.c64) / all.s;
             reinterpret_cast<typename D::S *>(of[i]->to + row * of[i]->step)[e.at[i] - of[i]->first] =
                 D::narrow(static_cast<float>(scale * (q - p)));
@@ -395,8 +394,8 @@ __device__ __forceinline__ void nothing(const DistillArgs &a, uint64_t row, uint
 // A row per workgroup.  Bound by the bytes on their way where there are many rows: 8 ranks, 4096 x 131072 bf16, loss and gradient 478 us, 3.0 GB
 // at 6.3 TB/s, of which the gradient's second reading comes from the last-level cache (four workgroups of 512 on a CU; of 256 540 us, of
 // 1024 497, with the row kept in registers in between 586); 2048 x 65536 fp16, loss alone, 52 us, 4.6 TB/s with the vector units 67 % busy.
-template <int DT, bool GRAD>
-__global__ void __launch_bounds__(kThreads)
+template <int DT, bool GRAD, int NT>
+__global__ void __launch_bounds__(NT)
 k_distill_row(DistillArgs a)
 {
     __shared__ DistillShared s;
@@ -404,16 +403,16 @@ k_distill_row(DistillArgs a)
     const uint32_t n = a.rows.nchunks;
     const float w = a.weight != nullptr ? a.weight[row] : 1.0f;
     if (w == 0.0f) {
-        nothing<DT, kThreads, true, GRAD>(a, row, 0, n);
+        nothing<DT, NT, true, GRAD>(a, row, 0, n);
         return;
     }
-    Together<kThreads> together(s.column, s.sum, GRAD ? a.k : 0);
-    Entries<kThreads> e;
+    Together<NT> together(a.mask, GRAD);
+    Entries<NT> e;
     e.read(a, row);
-    const Sum all = row_sum<DT, !GRAD>(a, row, 0, n, s.sums);
+    const Sum all = row_sum<DT, NT, !GRAD>(a, row, 0, n, s.sums);
     e.normalise(s.reduce);
-    finish<DT, kThreads, true, GRAD>(a, s, row, 0, n, all, w, e, together, nullptr,
-                                 [&](float scale) { row_gradient<DT, kThreads, false>(a, row, 0, n, all.r, scale); });
+    finish<DT, NT, true, GRAD>(a, s, row, 0, n, all, w, e, together, nullptr,
+                                 [&](float scale) { row_gradient<DT, NT, false>(a, row, 0, n, all.r, scale); });
 }
 
 // The same where rows are few and short: a row stays in the threads' registers, N vectors in each, instead of being read twice.  What counts
@@ -423,6 +422,7 @@ template <int DT, int N>
 __global__ void __launch_bounds__(kThreads)
 k_distill_held(DistillArgs a)
 {
+    constexpr int NT = kThreads;
     using V = Vec16<DT>;
     constexpr int NE = V::NE;
     constexpr uint32_t kWaves = kThreads / 64;
@@ -443,7 +443,7 @@ k_distill_held(DistillArgs a)
         const Stretch t = a.rows.chunks[i < n ? i : 0];
         raw[u] = load_piece<DT, true>(t.at + row * t.step, lane, i < n ? t.elems : 0);
     }
-    Together<kThreads> together(s.column, s.sum, a.k);
+    Together<NT> together(a.mask, true);
     Entries<kThreads> e;
     e.read(a, row);
     const Sum all = all_sum<kThreads>(a, lane_sum<DT>(a, {minus_infinity(), 0.0f}, raw), s.sums);
@@ -494,7 +494,7 @@ k_distill_sums(DistillArgs a)
             a.student[p.row * a.k + e] = load_one<DT>(of->at + p.row * of->step, c - of->first);
         }
     }
-    const Sum all = row_sum<DT, false>(a, p.row, p.from, p.to, s);
+    const Sum all = row_sum<DT, kThreads, false>(a, p.row, p.from, p.to, s);
     if (threadIdx.x == 0) a.parts[p.row * a.nparts + p.part] = {all.r, all.s};
 }
 
@@ -503,6 +503,7 @@ template <int DT, bool SAVED, bool GRAD>
 __global__ void __launch_bounds__(kThreads)
 k_distill_parts(DistillArgs a, uint32_t parts)
 {
+    constexpr int NT = kThreads;
     __shared__ DistillShared s;
     const Part p(a, parts);
     const float w = a.weight != nullptr ? a.weight[p.row] : 1.0f;
@@ -524,7 +525,7 @@ k_distill_parts(DistillArgs a, uint32_t parts)
             nothing<DT, kThreads, true, GRAD>(a, p.row, p.from, p.to);
             return;
         }
-        Together<kThreads> together(s.column, s.sum, GRAD ? a.k : 0);
+        Together<NT> together(a.mask, GRAD);
         Entries<kThreads> e;
         e.read(a, p.row);
         e.normalise(s.reduce);
@@ -534,7 +535,7 @@ k_distill_parts(DistillArgs a, uint32_t parts)
             nothing<DT, kThreads, false, true>(a, p.row, p.from, p.to);
             return;
         }
-        Together<kThreads> together(s.column, s.sum, a.k);
+        Together<NT> together(a.mask, true);
         Entries<kThreads> e;
         e.read(a, p.row);
         e.normalise(s.reduce);
@@ -559,26 +560,34 @@ struct DistillWork : PlanWork {
     bool saved = false;    // the gradient from what the loss saved
     bool grad = false;
     bool held = false;     // rows in registers
+    bool short_rows = false;   // small workgroups
 
     template <int DT>
     void run(hipStream_t st) const
     {
         const uint32_t rows = args.rows.rows;
-        const dim3 grid(rows * parts), block(kThreads);
+        const dim3 grid(rows * parts), block(kThreads), small(kSmall);
+        const uint32_t table = (args.mask + 1) * 12;
         if (saved) {
-            HCCLX_LAUNCH((k_distill_parts<DT, true, true>), grid, block, 0, st, args, parts);
-        } else if (parts == 1) {
-            if (held) {
-                HCCLX_LAUNCH((k_distill_held<DT, kHeld>), grid, block, 0, st, args);
-            } else if (grad) {
-                HCCLX_LAUNCH((k_distill_row<DT, true>), grid, block, 0, st, args);
+            HCCLX_LAUNCH((k_distill_parts<DT, true, true>), grid, block, table, st, args, parts);
+        } else if (held) {
+            HCCLX_LAUNCH((k_distill_held<DT, kHeld>), grid, block, table, st, args);
+        } else if (parts == 1 && short_rows) {
+            if (grad) {
+                HCCLX_LAUNCH((k_distill_row<DT, true, kSmall>), grid, small, table, st, args);
             } else {
-                HCCLX_LAUNCH((k_distill_row<DT, false>), grid, block, 0, st, args);
+                HCCLX_LAUNCH((k_distill_row<DT, false, kSmall>), grid, small, 0, st, args);
+            }
+        } else if (parts == 1) {
+            if (grad) {
+                HCCLX_LAUNCH((k_distill_row<DT, true, kThreads>), grid, block, table, st, args);
+            } else {
+                HCCLX_LAUNCH((k_distill_row<DT, false, kThreads>), grid, block, 0, st, args);
             }
         } else {
             HCCLX_LAUNCH((k_distill_sums<DT>), grid, block, 0, st, args);
             if (grad) {
-                HCCLX_LAUNCH((k_distill_parts<DT, false, true>), grid, block, 0, st, args, parts);
+                HCCLX_LAUNCH((k_distill_parts<DT, false, true>), grid, block, table, st, args, parts);
             } else {
                 HCCLX_LAUNCH((k_distill_parts<DT, false, false>), dim3(rows), block, 0, st, args, 1u);
             }
@@ -634,6 +643,8 @@ int prepare(const hcclx_logits_t &l, const hcclx_teacher_t &t, const float *weig
     if (w->args.c >= w->args.c64) w->args.c = std::nextafter(w->args.c, 0.0f);
     w->args.c_low = static_cast<float>(w->args.c64 - w->args.c);
     w->args.rows.vocab = vocab;
+    w->args.mask = 63;
+    while (w->args.mask + 1 < 2 * t.k) w->args.mask = 2 * w->args.mask + 1;   // (at most half are taken)
     w->dtype = l.dtype;
     w->grad = dlogits != nullptr;
     *work = std::move(w);
@@ -676,6 +687,10 @@ int make_distill(const hcclx_distill_t &d, hcclx_plan_t **plan)
     uint64_t held = w->table.bytes;
     const uint32_t cus = static_cast<uint32_t>(ctx->num_cus), turn = kThreads / 64 * kAhead;
     w->held = w->grad && l.rows <= 2 * cus && w->args.rows.nchunks > turn && w->args.rows.nchunks <= kThreads / 64 * kHeld;
+    // Short rows: what counts is how many are there at once, and smaller workgroups find room for more (loss and gradient, 4096 rows bf16 of 5000
+    // 45 us, by workgroups of 512 62, of 32000 137 and 145, of 50000 231 and 216; the loss alone, 2048 rows fp16 of 5000 16 and 25, of 65536 51
+    // and 53, of 131072 95 and 90).
+    w->short_rows = w->args.rows.nchunks <= (w->grad ? 64 : 128);
     if (rows != 0 && !w->held) w->parts = parts_of(l.rows, w->args.rows.nchunks, cus);
     if (w->parts > 1) {
         w->args.nparts = w->parts;
