@@ -33,7 +33,8 @@ namespace {
 constexpr uint32_t kGroup = 64;          // columns
 constexpr uint32_t kRunWaves = 4;        // of a workgroup of the first launch, a run each
 constexpr uint32_t kList = 2048;         // elements that are sorted at once
-constexpr uint32_t kMostGroups = HCCLX_TOP_MAX + HCCLX_TOP_MAX / 2 + 32;
+constexpr uint32_t kSmallTop = 256;      // the longest list of a small workgroup, and the elements that it sorts
+constexpr uint32_t kSmallList = 1024;
 constexpr uint32_t kNucleus = 64;        // listed where no top_k bounds the list (192: 1024 rows 212 us instead of 201, and no row less)
 constexpr uint32_t kLevels = 2048;       // of the weights of a row
 constexpr uint32_t kBand = 8192;         // elements of a cut's level, shared out to the parts of a row
@@ -307,7 +308,6 @@ struct Range {
     u64 weight_inside;
 };
 
-constexpr uint32_t kBins = 2048;
 constexpr uint32_t kBatch = 4096;        // rows that are drawn from together: 85 KB for the wide draw of each, 150 KB where they are few
 constexpr uint32_t kMostParts = 32;      // workgroups of a wide row
 constexpr uint32_t kMostSpans = 512;
@@ -319,8 +319,12 @@ constexpr uint32_t kStretches = 1000;    // of the range of a list's numbers
 constexpr uint32_t kMostAlike = 32;      // elements of a stretch that are put in order by counting
 constexpr uint32_t kQueue = 512;         // elements of a chunk that a wavefront weighs
 
-// What is used at different times lies in the same place: 38 KB leave a CU room for four workgroups.
-struct Shared {
+// What is used at different times lies in the same place.
+template <uint32_t LIST, uint32_t GROUPS>
+struct SharedOf {
+    static constexpr uint32_t kList = LIST;        // elements of a list
+    static constexpr uint32_t kBins = LIST;        // stretches that are counted into
+    static constexpr uint32_t kMostGroups = GROUPS;
     union {
         struct {
             u64 weight[kBins];
@@ -336,12 +340,11 @@ struct Shared {
         } walk;
         struct {
             u64 listed[kList];   // (where list.listed is)
-            float queue[kMostWaves][kQueue];
+            float queue[LIST < 2048 ? 1 : kMostWaves][kQueue];
         } wide;
         struct {
-            u64 unused[kBins];
-            uint32_t unused_too[kBins];
-            uint32_t groups[kMostGroups];   // behind the bins; before anything is sorted
+            uint32_t unused[LIST * 4 - GROUPS];
+            uint32_t groups[GROUPS];   // behind the bins and what counting uses of `sorted`; before anything is sorted by exchanges
         };
     };
     union {
@@ -362,7 +365,11 @@ struct Shared {
     uint32_t word[4];
     u64 one;
 };
-static_assert(sizeof(Shared) <= 160 * 1024 / 4, "");
+constexpr uint32_t groups_for(uint32_t k) { return k + k / 2 + 32; }
+using Shared = SharedOf<kList, groups_for(HCCLX_TOP_MAX)>;            // 38 KB: four workgroups on a CU
+using SmallShared = SharedOf<kSmallList, groups_for(kSmallTop)>;      // 22 KB: seven
+template <typename S> constexpr bool kApart = S::kList * 16 - S::kMostGroups * 4 >= S::kBins * 12 && S::kList * 16 - S::kMostGroups * 4 >= S::kList * 8 + 3 * kCounted * 8;
+static_assert(kApart<Shared> && kApart<SmallShared> && sizeof(Shared) <= 160 * 1024 / 4 && sizeof(SmallShared) <= 160 * 1024 / 7, "");
 
 // A lane's vector of a group: lanes kGroup / NE in a row hold one.
 struct Piece {
@@ -372,20 +379,20 @@ struct Piece {
 };
 
 // What the threads of a workgroup do together about a row.
-template <int NT>
+template <int NT, typename S = Shared>
 struct Team {
     static constexpr uint32_t kWaves = NT / 64;
     static_assert(kWaves <= kMostWaves, "");
 
     const SelectArgs &a;
-    Shared &s;
+    S &s;
     const uint64_t row;
     uint32_t top;      // the largest number of the row
     double top_value;
     double c;          // log2(e) / T, where weights are asked for
     uint32_t flip;     // which partial sums are free
 
-    __device__ __forceinline__ Team(const SelectArgs &args, Shared &shared, uint64_t of, uint32_t largest, double scale)
+    __device__ __forceinline__ Team(const SelectArgs &args, S &shared, uint64_t of, uint32_t largest, double scale)
         : a(args), s(shared), row(of), top(largest), top_value(value_of(largest)), c(scale), flip(0)
     {
         if (threadIdx.x < 64) s.powers[threadIdx.x] = exp2_exact(threadIdx.x / -64.0);
@@ -437,7 +444,7 @@ struct Team {
     // (301 rows of 32003, lists of 700: 31 us with the first launch, 44 by exchanges alone).  Where many are alike, by exchanges.
     __device__ __forceinline__ void sort(uint32_t n)
     {
-        constexpr uint32_t kMine = kList / NT;
+        constexpr uint32_t kMine = S::kList / NT;
         u64 key[kMine];
         uint32_t least = kNoEnd;
 #pragma unroll
@@ -553,7 +560,7 @@ struct Team {
     template <bool WEIGH>
     __device__ __forceinline__ uint32_t count_before(uint32_t n, u64 own, u64 *weight_before)
     {
-        static_assert(3 * kCounted <= kList && kCounted <= kMostGroups && kCounted <= NT, "");
+        static_assert(3 * kCounted <= S::kList && kCounted <= S::kMostGroups && kCounted <= NT, "");
         u64 *const weights = s.list.sorted, *const sums = s.list.sorted + kCounted;
         uint32_t *const ranks = s.groups;
         if (threadIdx.x < kCounted) {
@@ -606,10 +613,10 @@ struct Team {
     }
 };
 
-template <int DT, int NT>
-struct Row : Team<NT> {
+template <int DT, int NT, typename S = Shared>
+struct Row : Team<NT, S> {
     using V = Vec16<DT>;
-    using B = Team<NT>;
+    using B = Team<NT, S>;
     using B::a;
     using B::s;
     using B::row;
@@ -632,8 +639,8 @@ struct Row : Team<NT> {
     uint32_t held[kHeld];
     uint32_t bottom;   // the least of the groups' largest
 
-    __device__ __forceinline__ Row(const SelectArgs &args, Shared &shared, uint64_t of)
-        : Team<NT>(args, shared, of, 0, 0.0), most(args.most + of * args.rows.nchunks * kPer), ngroups(args.rows.nchunks * kPer)
+    __device__ __forceinline__ Row(const SelectArgs &args, S &shared, uint64_t of)
+        : Team<NT, S>(args, shared, of, 0, 0.0), most(args.most + of * args.rows.nchunks * kPer), ngroups(args.rows.nchunks * kPer)
     {
         uint32_t t = 0, least = kNoEnd;
         // (rows of the largest are whole vectors: a chunk has four or eight groups)
@@ -754,16 +761,17 @@ struct Row : Team<NT> {
         });
     }
 
-    // One round of the search: the numbers in the range are counted (and weighed) into kBins stretches of it; the range becomes the one in
+    // One round of the search: the numbers in the range are counted (and weighed) into S::kBins stretches of it; the range becomes the one in
     // which the running count (BY_WEIGHT: weight) from the top reaches what target() says, given the weight in the range.
     // all(f): f(number, weight) for every number that there is.
     template <bool BY_WEIGHT, typename All, typename Target>
     __device__ __forceinline__ void narrow(Range &r, All &&all, Target &&target)
     {
         const uint32_t width = r.high - r.low;
-        const uint32_t shift = width < kBins ? 0 : 32 - __clz(width) - 11;
-        static_assert(kBins == 1u << 11, "");
-        for (uint32_t i = threadIdx.x; i < kBins; i += NT) {
+        constexpr uint32_t kBits = S::kBins == 2048 ? 11 : 10;
+        static_assert(S::kBins == 1u << kBits, "");
+        const uint32_t shift = width < S::kBins ? 0 : 32 - __clz(width) - kBits;
+        for (uint32_t i = threadIdx.x; i < S::kBins; i += NT) {
             s.bins.count[i] = 0;
             if (BY_WEIGHT) s.bins.weight[i] = 0;
         }
@@ -779,14 +787,14 @@ struct Row : Team<NT> {
         });
         __syncthreads();
         // from the top: neighbours per thread
-        constexpr uint32_t kMine = kBins / NT;
+        constexpr uint32_t kMine = S::kBins / NT;
         uint32_t count[kMine];
         u64 weight[kMine];
         uint32_t counts = 0;
         u64 weights = 0;
 #pragma unroll
         for (uint32_t i = 0; i < kMine; ++i) {
-            const uint32_t bin = kBins - 1 - (threadIdx.x * kMine + i);
+            const uint32_t bin = S::kBins - 1 - (threadIdx.x * kMine + i);
             counts += count[i] = s.bins.count[bin];
             weights += weight[i] = BY_WEIGHT ? s.bins.weight[bin] : 0;
         }
@@ -804,7 +812,7 @@ struct Row : Team<NT> {
             const u64 at = BY_WEIGHT ? w : c;
             const u64 add = BY_WEIGHT ? weight[i] : count[i];
             if (at < aim && at + add >= aim) {
-                const uint32_t bin = kBins - 1 - (threadIdx.x * kMine + i);
+                const uint32_t bin = S::kBins - 1 - (threadIdx.x * kMine + i);
                 const uint32_t low = r.low + (bin << shift);
                 const uint32_t last = low + ((1u << shift) - 1);
                 s.range = {low, last < r.high ? last : r.high, c, count[i], w, weight[i]};
@@ -818,10 +826,10 @@ struct Row : Team<NT> {
 
     __device__ __forceinline__ void put(uint32_t at, float l, uint32_t place) const
     {
-        if (at < kList) s.list.listed[at] = static_cast<u64>(number_of(l)) << 32 | static_cast<uint32_t>(~place);
+        if (at < S::kList) s.list.listed[at] = static_cast<u64>(number_of(l)) << 32 | static_cast<uint32_t>(~place);
     }
     // Lists the elements of the groups s.groups[0 .. n) that reach `low`, in the order of the columns; returns how many there are, or a
-    // number over kList as soon as they are known to be more.
+    // number over S::kList as soon as they are known to be more.
     __device__ __forceinline__ uint32_t list(uint32_t n, uint32_t low)
     {
         constexpr int kAhead = 2;   // turns that are read and counted together, 16 bits of a sum for each
@@ -829,7 +837,7 @@ struct Row : Team<NT> {
         // (the least value of the number; the numbers of minus infinity and below are all values')
         const float least = low <= kLeast >> kShift ? minus_infinity() : value_of(low << kShift);
         uint32_t listed = 0;
-        for (uint32_t turn = 0; turn < n && listed <= kList; turn += kTurn * kAhead) {
+        for (uint32_t turn = 0; turn < n && listed <= S::kList; turn += kTurn * kAhead) {
             Piece p[kAhead];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
@@ -907,7 +915,7 @@ struct Row : Team<NT> {
         // Groups: those whose largest reaches `low`.
         Range g = {0, top >> kShift, 0, ngroups, 0, 0};
         uint32_t equal = kNoEnd;   // of the groups whose largest is low, the first so many
-        const uint32_t enough = max(k + k / 2 + 32, kList / kGroup);
+        const uint32_t enough = max(k + k / 2 + 32, S::kList / kGroup);
         if (ngroups > enough) {
             g.low = bottom >> kShift;
             do {
@@ -925,16 +933,16 @@ struct Row : Team<NT> {
                 same += m != kNone && m >> kShift == g.low;
             });
             // (over: at most `enough`; both fit)
-            static_assert(kMostGroups < 4096 && HCCLX_LOGITS_MAX_COLUMNS / kGroup + 8 * kMostRanks < 1 << 20, "");
+            static_assert(S::kMostGroups < 4096 && HCCLX_LOGITS_MAX_COLUMNS / kGroup + 8 * kMostRanks < 1 << 20, "");
             uint32_t all;
             const uint32_t packed = before(over << 20 | same, &all);
             uint32_t same_before = packed & 0xfffffu;
             uint32_t at = (packed >> 20) + min(same_before, equal);
-            n = min((all >> 20) + min(all & 0xfffffu, equal), kMostGroups);   // (never more: `enough` and k bound them)
+            n = min((all >> 20) + min(all & 0xfffffu, equal), S::kMostGroups);   // (never more: `enough` and k bound them)
             each_group([&](uint32_t i, uint32_t m) {
                 if (m == kNone || m >> kShift < g.low) return;
                 if (m >> kShift == g.low && same_before++ >= equal) return;
-                if (at < kMostGroups) s.groups[at] = i;
+                if (at < S::kMostGroups) s.groups[at] = i;
                 ++at;
             });
             __syncthreads();
@@ -942,8 +950,8 @@ struct Row : Team<NT> {
         // Elements that reach what all groups reach, if they fit.
         uint32_t listed = kNoEnd;
         uint32_t low = g.low;
-        if (low != 0 || n * kGroup <= kList) listed = list(n, low);
-        if (listed > kList) {
+        if (low != 0 || n * kGroup <= S::kList) listed = list(n, low);
+        if (listed > S::kList) {
             // The same again with the vectors of the groups in the groups' place: where there are k, elements reach the k-th vector's largest.
             Range e = {low, top >> kShift, 0, 0, 0, 0};
             do {
@@ -959,12 +967,12 @@ struct Row : Team<NT> {
             } while (e.above + e.inside > k + k / 2 + 32 && e.low != e.high);
             if (e.above + e.inside >= k) listed = list(n, low = e.low);
         }
-        if (listed > kList) {   // elements themselves
+        if (listed > S::kList) {   // elements themselves
             Range e = {low, top >> kShift, 0, 0, 0, 0};
             do {
                 narrow<false>(e, [&](auto &&f) { each(s.groups, n, f); }, [&](u64) { return u64(k); });
-            } while (e.above + e.inside > kList && e.low != e.high);
-            listed = e.above + e.inside > kList ? list_ties(n, e.low, k - e.above) : list(n, e.low);
+            } while (e.above + e.inside > S::kList && e.low != e.high);
+            listed = e.above + e.inside > S::kList ? list_ties(n, e.low, k - e.above) : list(n, e.low);
         }
         *sure = equal == kNoEnd ? listed : k;
         return listed;
@@ -972,13 +980,13 @@ struct Row : Team<NT> {
 
 };
 
-template <int DT, int NT>
+template <int DT, int NT, typename S>
 __global__ void __launch_bounds__(NT)
 k_top_logits(SelectArgs a)
 {
     using D = DTypeOf<DT>;
-    __shared__ Shared s;
-    Row<DT, NT> r(a, s, blockIdx.x);
+    __shared__ S s;
+    Row<DT, NT, S> r(a, s, blockIdx.x);
     r.c = 1.4426950408889634074;   // (of the sum)
     uint32_t sure;
     const uint32_t n = r.list_first(a.k, &sure);
@@ -1852,6 +1860,7 @@ struct SelectWork : PlanWork {
     bool sample = false;
     uint32_t parts = 1;    // workgroups of the first launch per row
     uint32_t batch = 0;         // rows whose wide ones are drawn from together
+    bool small = false;         // whether many rows with short lists have small workgroups
     bool apart = false;         // whether levels are counted in a launch of their own
 
     template <int DT, int U>
@@ -1882,7 +1891,11 @@ struct SelectWork : PlanWork {
         constexpr int NT = 512;
         if (!sample) {
             first_launch<DT>(args, args.rows.rows, st);
-            HCCLX_LAUNCH((k_top_logits<DT, NT>), dim3(args.rows.rows), dim3(NT), 0, st, args);
+            if (small) {
+                HCCLX_LAUNCH((k_top_logits<DT, NT / 2, SmallShared>), dim3(args.rows.rows), dim3(NT / 2), 0, st, args);
+            } else {
+                HCCLX_LAUNCH((k_top_logits<DT, NT, Shared>), dim3(args.rows.rows), dim3(NT), 0, st, args);
+            }
             return;
         }
         SelectArgs of = args;
@@ -1942,6 +1955,9 @@ int finish(const hcclx_logits_t &l, uint32_t vocab, bool sums, std::unique_ptr<S
         held += bytes;
         return at;
     };
+    // Where rows fill the device more than three times, small workgroups for their lists, of which seven find room on a CU (64 of 4096 rows of
+    // 131072 bf16 244 us, by four large ones 255, of 5000 67 and 86; of 1000 rows 68 and 70, of 600 48 and 46.5).
+    w->small = a.k <= kSmallTop && l.rows > 3 * static_cast<uint32_t>(ctx->num_cus);
     uint64_t wide = 0, bands = 0, levels = 0, found = 0, listed = 0, spans = 0;
     if (w->sample && l.rows != 0) {
         // Rows that the list of kNucleus always does for are never wide; nor are those that no filter but a short top_k may shorten, which

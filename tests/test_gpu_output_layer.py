@@ -147,6 +147,14 @@ def test_top_logits_of_many_rows(rows, dtype):
     check_top(contents("steep", rows, 5000, gen(rows)), shares(5000, 3), dtype, 20, one=True)
 
 
+@pytest.mark.parametrize("dtype", [T.FP32, T.FP16, T.BFP16])
+@pytest.mark.parametrize("kind", KINDS)
+def test_top_logits_of_rows_that_fill_the_device(kind, dtype):
+    """Small workgroups, whose lists are shorter: up to 256 entries, rows where more than a list holds reaches the k-th."""
+    check_top(contents(kind, 800, 1201, gen(62)), shares(1201, 3), dtype, 256, pad=1)
+    check_top(contents(kind, 780, 30011, gen(63)), shares(30011, 2), dtype, 100)
+
+
 def test_top_logits_of_64_ranks_and_a_million_columns():
     check_top(contents("normal", 2, 1 << 20, gen(1)), shares(1 << 20, 64), T.BFP16, 100)
     check_top(contents("coarse", 2, 650, gen(2)), shares(650, 64), T.FP32, 650)
