@@ -393,7 +393,8 @@ __device__ __forceinline__ void nothing(const DistillArgs &a, uint64_t row, uint
 
 // A row per workgroup.  Bound by the bytes on their way where there are many rows: 8 ranks, 4096 x 131072 bf16, loss and gradient 478 us, 3.0 GB
 // at 6.3 TB/s, of which the gradient's second reading comes from the last-level cache (four workgroups of 512 on a CU; of 256 540 us, of
-// 1024 497, with the row kept in registers in between 586); 2048 x 65536 fp16, loss alone, 52 us, 4.6 TB/s with the vector units 67 % busy.
+// 1024 497, with the row kept in registers in between 586); 2048 x 65536 fp16, loss alone, 51 us, 4.8 TB/s with the vector units 60 %
+// busy.
 template <int DT, bool GRAD, int NT>
 __global__ void __launch_bounds__(NT)
 k_distill_row(DistillArgs a)
@@ -478,7 +479,8 @@ struct Part {
     }
 };
 
-// Several workgroups per row, two launches: r and S of every part, then what is left.  Bound by the chain of one row (4.5 + 8 us).
+// Several workgroups per row, two launches: r and S of every part, then what is left.  Bound by the chain of one row (16 of
+// 131072 bf16 5 + 8 us).
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
 k_distill_sums(DistillArgs a)

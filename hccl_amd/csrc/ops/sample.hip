@@ -16,11 +16,11 @@
 // A row whose draw goes by more than such a list is left to several workgroups.  Next to the second launch they count its elements by
 // levels of their weight, 64 to a power of two, which says in which level the cut lies; in a third those over that level are weighed and
 // those in it are listed; and a fourth finds the cut among these, and draws.  (One workgroup for all of that: 64 rows of 131072 bf16,
-// a sixth of them such, 112 us instead of 36.)
+// a sixth of them such, 112 us instead of 31 to 41.)
 //
-// What bounds it: the first launch, by reading (8 x 4096 x 131072 bf16 192 us, 5.6 TB/s, with a sum that keeps the vector units four fifths
+// What bounds it: the first launch, by reading (8 x 4096 x 131072 bf16 195 us, 5.5 TB/s, with a sum that keeps the vector units four fifths
 // busy); the others, by how long one row takes: some twenty steps of a workgroup, each with a barrier, and the fetch of their code.  1 row
-// of 131072 3 us + 11 us + two launches that find nothing to do.
+// of 131072 3 us + 10 us + two launches that find nothing to do.
 #include "ops/logits.h"
 
 #include <algorithm>
