@@ -258,6 +258,14 @@ def test_distillation_of_few_and_many_rows(rows, dtype, in_place):
     check_distill(contents("steep", rows, 30011, gen(rows)), shares(30011, 4), dtype, 40, 2.0, one=True, weights=rows > 1, in_place=in_place)
 
 
+@pytest.mark.parametrize("dtype", [T.FP32, T.BFP16])
+@pytest.mark.parametrize("kind", ["holes", "twice"])
+@pytest.mark.parametrize("rows,vocab,k", [(5, 3000, 1024), (600, 20001, 300), (513, 700, 64), (40, 24000, 1024)])
+def test_distillation_of_short_rows_and_long_lists(rows, vocab, k, kind, dtype):
+    """Small workgroups, several entries to a thread; rows that stay in registers."""
+    check_distill(contents("steep", rows, vocab, gen(81)), shares(vocab, 2), dtype, k, 1.0, kind, pad=1)
+
+
 @pytest.mark.parametrize("rows", [4, 270])
 @pytest.mark.parametrize("kind", ["normal", "equal", "falling", "masked", "odd", "nothing"])
 @pytest.mark.parametrize("dtype", [T.FP32, T.BFP16])
