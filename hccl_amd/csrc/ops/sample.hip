@@ -1968,9 +1968,10 @@ int finish(const hcclx_logits_t &l, uint32_t vocab, bool sums, std::unique_ptr<S
         a.span = (a.rows.nchunks + kMostSpans - 1) / kMostSpans;
         a.nspans = (a.rows.nchunks + a.span - 1) / a.span;
         // Workgroups for a row that may be wide: most rows are not, and their workgroups only look.  In launches of their own eight for a row
-        // (1024 rows 194 us, with four 211, with two 240), next to the lists as many as there is room for (256 rows 76 us with eight, 80 with
-        // sixteen, 85 with 32; 1 row 17 with 32).
-        a.wide_parts = !may_be_wide ? 0 : std::min(a.nspans, w->apart ? std::clamp(8192 / w->batch, 2u, 8u) : std::clamp(2048 / w->batch, 2u, kMostParts));
+        // (1024 rows of 131072 194 us, with four 211, with two 240), of sixteen chunks at least (of 5000 60, of a chunk at least 65); next to
+        // the lists as many as there is room for (256 rows 76 us with eight, 80 with sixteen, 85 with 32; 1 row 17 with 32).
+        const uint32_t parts = w->apart ? std::clamp(std::min(8192 / w->batch, (a.rows.nchunks + 15) / 16), 1u, 8u) : std::clamp(2048 / w->batch, 2u, kMostParts);
+        a.wide_parts = may_be_wide ? std::min(a.nspans, parts) : 0;
         a.band_each = std::clamp(kBand / std::max(1u, a.wide_parts), 512u, kList);
         wide = more(w->batch * sizeof(Wide));
         levels = more(may_be_wide ? w->batch * sizeof(u64) * kLevels : 0);
