@@ -160,7 +160,7 @@ struct RowChoice {
     bool by_p;
     bool by_min;
     uint32_t k;
-    double p;
+    float p;        // where top_p is below 1
     double least;
     double c;   // log2(e) / T
 
@@ -1009,15 +1009,34 @@ k_top_logits(SelectArgs a)
     }
 }
 
+// x times whole, for 0 < x < 1, as the whole number below or (UP) above: exactly, from the 24 bits of x and 88 of the product.  (In doubles a
+// whole of more than 2^53 was rounded first, and a border that lies at the product was on either side of it.)
+template <bool UP>
+__device__ __forceinline__ u64 share_of(float x, u64 whole)
+{
+    const uint32_t bits = __float_as_uint(x), power = max(bits >> 23, 1u);
+    const u64 m = (bits & 0x7fffffu) | (bits >> 23 != 0 ? 0x800000u : 0u);
+    const u64 low = m * whole, high = __umul64hi(m, whole);
+    const uint32_t down = 150 - power;   // x = m 2^-down: 24 or more
+    u64 n, rest;
+    if (down < 64) {
+        n = high << (64 - down) | low >> down;
+        rest = low & ((u64(1) << down) - 1);
+    } else {   // (high has 23 bits)
+        const uint32_t more = min(down - 64, 63u);
+        n = high >> more;
+        rest = low | (high & ((u64(1) << more) - 1));
+    }
+    return n + (UP && rest != 0 ? 1 : 0);
+}
 // floor(u x whole), inside the whole
 __device__ __forceinline__ u64 aim_of(float u, u64 whole)
 {
-    const double t = static_cast<double>(u) * static_cast<double>(whole);
-    if (!(t > 0.0)) return 0;
-    return t >= static_cast<double>(whole) ? whole - 1 : min(static_cast<u64>(t), whole - 1);
+    if (!(u > 0.0f)) return 0;
+    return u < 1.0f ? share_of<false>(u, whole) : whole - 1;
 }
 // What of `whole` top_p asks for.
-__device__ __forceinline__ u64 part_of(double p, double whole) { return p > 0.0 ? static_cast<u64>(ceil(p * whole)) : 0; }
+__device__ __forceinline__ u64 part_of(float p, u64 whole) { return p > 0.0f ? share_of<true>(p, whole) : 0; }
 
 // What stays of a row that no list holds: numbers over `cut`, the first `equal` of those that are it, and of them all what is `least`
 // times as probable as the first.
@@ -1227,7 +1246,7 @@ __device__ __forceinline__ void draw_by_numbers(const SelectArgs &a, Row<DT, NT>
         const u64 over = choice.by_k && cut_count > stay.equal ? (cut_count - stay.equal) * r.weight(stay.cut << kShift | (stay.cut >> (31 - kShift) != 0 ? 0 : (1u << kShift) - 1)) : 0;
         do {
             r.template narrow<true>(range, all, [&](u64 whole) {
-                if (first) aim = max(u64(1), min(choice.by_k ? part_of(choice.p, static_cast<double>(whole - over)) : p_of_whole, whole));
+                if (first) aim = max(u64(1), min(choice.by_k ? part_of(choice.p, whole - over) : p_of_whole, whole));
                 return aim;
             });
             first = false;
@@ -1331,7 +1350,7 @@ __device__ __forceinline__ void count_levels(const SelectArgs &a, u64 *mine, uin
     // What is so improbable that even as many as there are columns hold no more than 1 - top_p of the largest's weight alone lies behind the cut.
     float far = __builtin_inff();
     if (!choice.by_k) {
-        const double behind = (1.0 - choice.p) / a.rows.vocab;
+        const double behind = (1.0 - static_cast<double>(choice.p)) / a.rows.vocab;
         if (behind > 0.0) far = static_cast<float>(-64.0 * log2(behind)) + 2.0f;
     }
     const uint32_t to = min(part.to * a.span, a.rows.nchunks);
@@ -1776,7 +1795,7 @@ k_sample(SelectArgs a, uint32_t rows)
     if (choice.by_p && !choice.by_k) {
         double mine = 0.0;
         for (uint32_t i = threadIdx.x; i < a.nruns; i += NT) mine += r.run_sum(i);
-        p_of_whole = part_of(choice.p, ldexp(r.total(mine), static_cast<int>(a.bits)));
+        p_of_whole = part_of(choice.p, static_cast<u64>(ldexp(r.total(mine), static_cast<int>(a.bits))));
     }
     uint32_t sure = 0;
     if (!choice.by_k || choice.k <= HCCLX_TOP_MAX) {
@@ -1789,7 +1808,7 @@ k_sample(SelectArgs a, uint32_t rows)
             u64 weight_before;
             const uint32_t place = r.template count_before<true>(n, w, &weight_before);
             const bool first = threadIdx.x < n && place < limit;
-            if (choice.by_k && choice.by_p) p_of_whole = part_of(choice.p, static_cast<double>(r.total(first ? w : 0)));
+            if (choice.by_k && choice.by_p) p_of_whole = part_of(choice.p, r.total(first ? w : 0));
             bool in = first;
             if (choice.by_p) in = in && (place == 0 || weight_before < p_of_whole);
             if (choice.by_min) in = in && (place == 0 || r.share(l, 0) >= choice.least);
@@ -1811,7 +1830,7 @@ k_sample(SelectArgs a, uint32_t rows)
             }
             u64 whole;
             u64 at = r.before(sum, &whole);
-            if (choice.by_k) p_of_whole = part_of(choice.p, static_cast<double>(whole));
+            if (choice.by_k && choice.by_p) p_of_whole = part_of(choice.p, whole);
             uint32_t keep = 0;
 #pragma unroll
             for (uint32_t i = 0; i < kMine; ++i) {
