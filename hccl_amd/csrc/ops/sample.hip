@@ -37,6 +37,7 @@ constexpr uint32_t kSmallTop = 256;      // the longest list of a small workgrou
 constexpr uint32_t kSmallList = 1024;
 constexpr uint32_t kNucleus = 64;        // listed where no top_k bounds the list (192: 1024 rows 212 us instead of 201, and no row less)
 constexpr uint32_t kLevels = 2048;       // of the weights of a row
+constexpr uint32_t kWholeBits = 51;      // of a weight's whole number where there is no filter
 constexpr uint32_t kBand = 8192;         // elements of a cut's level, shared out to the parts of a row
 constexpr uint32_t kNone = 0;            // the number of what does not exist
 constexpr uint32_t kLeast = 0x007fffffu;   // of minus infinity
@@ -60,7 +61,7 @@ struct Run {
 
 // A row that is left to the launches behind the second.
 struct Wide {
-    uint32_t wide;     // 0: it is not; 2: it is, but its cut is not found by levels
+    uint32_t wide;     // 0: it is not; 2: it is, but its cut is not found by levels, or it has none
     uint32_t top;      // its largest number
     unsigned long long p_of_whole;
 };
@@ -181,6 +182,7 @@ struct RowChoice {
     }
     // whether elements are counted by levels, in case that no list holds what stays
     __device__ __forceinline__ bool by_levels() const { return by_k ? k > HCCLX_TOP_MAX && !by_p : by_p; }
+    __device__ __forceinline__ bool none() const { return !by_k && !by_p && !by_min; }
     // whether the sum over the whole row is needed
     __device__ __forceinline__ bool whole() const { return !by_k && (by_p || !by_min); }
 };
@@ -434,10 +436,11 @@ struct Team {
     }
     __device__ __forceinline__ double share(uint32_t number) const { return share(value_of(number), 0); }
     // The same times 2^bits as a whole number: 2^52 added, the last place of a double is 1.
-    __device__ __forceinline__ u64 weight(float l) const
+    __device__ __forceinline__ u64 weight(float l, uint32_t bits) const
     {
-        return static_cast<u64>(__double_as_longlong(share(l, static_cast<int>(a.bits)) + 0x1p52)) & ((u64(1) << 52) - 1);
+        return static_cast<u64>(__double_as_longlong(share(l, static_cast<int>(bits)) + 0x1p52)) & ((u64(1) << 52) - 1);
     }
+    __device__ __forceinline__ u64 weight(float l) const { return weight(l, a.bits); }
     __device__ __forceinline__ u64 weight(uint32_t number) const { return weight(value_of(number)); }
 
     // Sorts s.list.listed[0 .. n) into s.list.sorted, descending: into equal stretches of the range of their numbers, and in those by counting
@@ -1009,34 +1012,29 @@ k_top_logits(SelectArgs a)
     }
 }
 
-// x times whole, for 0 < x < 1, as the whole number below or (UP) above: exactly, from the 24 bits of x and 88 of the product.  (In doubles a
-// whole of more than 2^53 was rounded first, and a border that lies at the product was on either side of it.)
+typedef unsigned __int128 u128;
+
+// x times whole, for 0 < x < 1, as the whole number below or (UP) above: exactly, from the 24 bits of x and all of the product, which has 100 at
+// most.  (In doubles a whole of more than 2^53 was rounded first, and a border that lies at the product was on either side of it.)
 template <bool UP>
-__device__ __forceinline__ u64 share_of(float x, u64 whole)
+__device__ __forceinline__ u128 share_of(float x, u128 whole)
 {
     const uint32_t bits = __float_as_uint(x), power = max(bits >> 23, 1u);
     const u64 m = (bits & 0x7fffffu) | (bits >> 23 != 0 ? 0x800000u : 0u);
-    const u64 low = m * whole, high = __umul64hi(m, whole);
-    const uint32_t down = 150 - power;   // x = m 2^-down: 24 or more
-    u64 n, rest;
-    if (down < 64) {
-        n = high << (64 - down) | low >> down;
-        rest = low & ((u64(1) << down) - 1);
-    } else {   // (high has 23 bits)
-        const uint32_t more = min(down - 64, 63u);
-        n = high >> more;
-        rest = low | (high & ((u64(1) << more) - 1));
-    }
-    return n + (UP && rest != 0 ? 1 : 0);
+    const u128 product = whole * m;
+    const uint32_t down = min(150 - power, 127u);   // x = m 2^-down: 24 or more
+    const u128 n = product >> down;
+    return n + (UP && n << down != product ? 1 : 0);
 }
 // floor(u x whole), inside the whole
-__device__ __forceinline__ u64 aim_of(float u, u64 whole)
+template <typename W>
+__device__ __forceinline__ W aim_of(float u, W whole)
 {
     if (!(u > 0.0f)) return 0;
-    return u < 1.0f ? share_of<false>(u, whole) : whole - 1;
+    return u < 1.0f ? static_cast<W>(share_of<false>(u, whole)) : whole - 1;
 }
 // What of `whole` top_p asks for.
-__device__ __forceinline__ u64 part_of(float p, u64 whole) { return p > 0.0f ? share_of<true>(p, whole) : 0; }
+__device__ __forceinline__ u64 part_of(float p, u64 whole) { return p > 0.0f ? static_cast<u64>(share_of<true>(p, whole)) : 0; }
 
 // What stays of a row that no list holds: numbers over `cut`, the first `equal` of those that are it, and of them all what is `least`
 // times as probable as the first.
@@ -1149,9 +1147,83 @@ __device__ __forceinline__ void draw_kept(const SelectArgs &a, Row<DT, NT> &r, S
     }
 }
 
-// No filter: the run in which the running sum passes u x the whole, then the element.
+// No filter, by the definition: weights are multiples of 2^-51, the most that the sum of a chunk has room for in 64 bits, and sums over chunks
+// have 128.  Chunks are weighed 512 at a time, and the one that the aim lies in is gone through; a first walk finds the whole.
 template <int DT, int NT>
-__device__ __forceinline__ void draw_all(const SelectArgs &a, Row<DT, NT> &r, Shared &s, float u)
+__device__ __forceinline__ void draw_whole(const SelectArgs &a, Row<DT, NT> &r, Shared &s, float u)
+{
+    using R = Row<DT, NT>;
+    constexpr uint32_t NE = R::NE;
+    static_assert(NT == 512, "a thread for each chunk");
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    u128 aim = 0, whole = 0;
+    for (int find = 0; find < 2; ++find) {
+        u128 front = 0;
+        for (uint32_t first = 0; first < a.rows.nchunks; first += NT) {
+            for (uint32_t at = wave; at < NT; at += R::kWaves) {
+                if (find == 1 && a.rows.nchunks <= NT) break;   // (still there)
+                const uint32_t chunk = first + at;
+                u64 sum = 0;
+                if (chunk < a.rows.nchunks) {
+                    const Stretch t = a.rows.chunks[chunk];
+                    const u32x4 raw = load_piece<DT, false>(t.at + r.row * t.step, lane, t.elems);
+                    float v[NE];
+                    R::V::unpack(raw, v);
+#pragma unroll
+                    for (uint32_t e = 0; e < NE; ++e) sum += lane * NE + e < t.elems ? r.weight(no_nan(v[e]), kWholeBits) : 0;
+                }
+                sum = wave_total(sum);
+                if (lane == 0) s.walk.weight[at] = sum;
+            }
+            __syncthreads();
+            const u64 mine = s.walk.weight[threadIdx.x];
+            u64 low_all, high_all;
+            const u64 low = r.before(mine & 0xffffffffu, &low_all);
+            const u64 high = r.before(mine >> 32, &high_all);
+            const u128 at = front + (static_cast<u128>(high) << 32) + low;
+            if (find == 1 && aim >= at && aim - at < mine) {
+                s.word[0] = first + threadIdx.x;   // the chunk
+                s.word64[0] = static_cast<u64>(aim - at);
+            }
+            front += (static_cast<u128>(high_all) << 32) + low_all;
+            __syncthreads();
+        }
+        if (find == 0) {
+            whole = front;
+            aim = aim_of(u, whole);
+        }
+    }
+    if (wave != 0) return;
+    // one wavefront, one chunk
+    const Stretch t = a.rows.chunks[s.word[0]];
+    const u32x4 raw = load_piece<DT, false>(t.at + r.row * t.step, lane, t.elems);
+    float v[NE];
+    R::V::unpack(raw, v);
+    u64 w[NE];
+    u64 sum = 0;
+#pragma unroll
+    for (uint32_t e = 0; e < NE; ++e) sum += w[e] = lane * NE + e < t.elems ? r.weight(no_nan(v[e]), kWholeBits) : 0;
+    u64 at = wave_sums(sum) - sum;
+    const u64 rest = s.word64[0];
+#pragma unroll
+    for (uint32_t e = 0; e < NE; ++e) {
+        if (rest >= at && rest - at < w[e]) {
+            const double all = static_cast<double>(static_cast<u64>(whole >> 64)) * 0x1p64 + static_cast<double>(static_cast<u64>(whole));
+            r.write_choice(t.first + lane * NE + e, number_of(no_nan(v[e])), ldexp(all, -static_cast<int>(kWholeBits)));
+        }
+        at += w[e];
+    }
+}
+
+// No filter: the run in which the running sum passes u x the whole, then the element, by sums of doubles, whose order goes by the plan (how
+// many chunks a run has).  The whole numbers say the same where both of the element's borders are further from the aim than that can matter.
+// With e the error of an element in these sums, of which k are in front of a border, the distance border - u whole is off by (1 - u) times
+// the first k and u times the others' sum.  e is 2^-52 where a number is rounded, and 2^-53 of a run's largest where the run leaves it out; and
+// in parts of the whole, an exponent of up to 53 powers of two, rounded twice, is good to 2^-46.8 of its term; three of them, and 200
+// additions of doubles one behind the other, make 2^-44.3.
+// Otherwise false is returned, and nothing is drawn (for one row of 131072 columns in some millions).
+template <int DT, int NT>
+__device__ __forceinline__ bool draw_all(const SelectArgs &a, Row<DT, NT> &r, Shared &s, float u)
 {
     using R = Row<DT, NT>;
     constexpr uint32_t NE = R::NE;
@@ -1160,7 +1232,10 @@ __device__ __forceinline__ void draw_all(const SelectArgs &a, Row<DT, NT> &r, Sh
     const uint32_t from = min(threadIdx.x * each, a.nruns), to = min(from + each, a.nruns);
     double mine = 0.0;
     for (uint32_t i = from; i < to; ++i) mine += r.run_sum(i);
-    if (threadIdx.x == 0) s.word[0] = s.word[1] = 0;
+    if (threadIdx.x == 0) {
+        s.word[0] = s.word[1] = 0;
+        s.word[2] = 1;   // nothing is drawn
+    }
     double whole;
     const double begin = r.before(mine, &whole);
     double at = begin;
@@ -1200,6 +1275,7 @@ __device__ __forceinline__ void draw_all(const SelectArgs &a, Row<DT, NT> &r, Sh
     double all;
     at = r.before(sum, &all);
     at += __builtin_bit_cast(double, s.word64[0]);
+    const double first = at;
     last = 0;
 #pragma unroll
     for (uint32_t e = 0; e < NE; ++e) {
@@ -1210,11 +1286,30 @@ __device__ __forceinline__ void draw_all(const SelectArgs &a, Row<DT, NT> &r, Sh
     if (lane == 0 && last != 0) atomicMax(&s.word[1], last);
     __syncthreads();
     const uint32_t place = s.word[1] - 1;
-    if (place / NE != threadIdx.x) return;
+    if (place / NE == threadIdx.x) {
+        float l = 0.0f;
+        double its = 0.0, front = 0.0;
+        at = first;
 #pragma unroll
-    for (uint32_t e = 0; e < NE; ++e) {
-        if (place % NE == e) r.write_choice(t.first + lane * NE + e, number_of(no_nan(v[e])), whole);
+        for (uint32_t e = 0; e < NE; ++e) {
+            if (place % NE == e) {
+                l = no_nan(v[e]);
+                its = w[e];
+                front = at;
+            }
+            at += w[e];
+        }
+        const uint32_t column = t.first + (lane * NE + place % NE);
+        const double share = fmin(fmax(static_cast<double>(u), 0.0), 1.0);
+        const double gap = ((1.0 - share) * (column + 2) + share * (a.rows.vocab - column + 1)) * 0x1p-51 + whole * 0x1p-43;
+        // (at 0: nothing in front of it has any weight)
+        if ((front == 0.0 || aim - front >= gap) && front + its - aim >= gap) {
+            r.write_choice(column, number_of(l), whole);
+            s.word[2] = 0;
+        }
     }
+    __syncthreads();
+    return s.word[2] == 0;
 }
 
 // The cut is searched by numbers, among all elements, and chunks are weighed: right for every row, but one workgroup goes through all
@@ -1753,21 +1848,26 @@ k_sample_wide(SelectArgs a)
             }
         }
     }
-    // The cut's level has more elements than are listed, or the cut is in another.
+    // The cut's level has more elements than are listed, or the cut is in another.  (Or there is no cut, and what is to be drawn is next to a border.)
     __syncthreads();
     Row<DT, NT> r(a, s, row);
     r.c = choice.c;
+    if (choice.none()) {
+        draw_whole(a, r, s, u);
+        return;
+    }
     draw_by_numbers(a, r, s, choice, u, wide.p_of_whole);
 }
 
-// The second launch: rows from a.first on.
-template <int DT, int NT>
-__global__ void __launch_bounds__(NT)
+// The second launch: rows from a.first on.  ALONE: there are none behind it, since no row has a filter, or none is longer than a list.
+// (Otherwise six wavefronts for a SIMD: one register more, and a CU has two workgroups instead of three.)
+template <int DT, int NT, bool ALONE>
+__global__ void __launch_bounds__(NT, ALONE ? 4 : 6)
 k_sample(SelectArgs a, uint32_t rows)
 {
     constexpr uint32_t kMine = kList / NT;
     __shared__ Shared s;
-    if (blockIdx.x >= rows) {
+    if (!ALONE && blockIdx.x >= rows) {
         static_assert(kList >= kLevels, "");
         count_levels<DT, NT>(a, s.list.listed, s.most, blockIdx.x - rows);
         return;
@@ -1786,8 +1886,13 @@ k_sample(SelectArgs a, uint32_t rows)
         }
         return;
     }
-    if (!choice.by_k && !choice.by_p && !choice.by_min) {
-        draw_all(a, r, s, u);
+    if (choice.none()) {
+        if (draw_all(a, r, s, u)) return;
+        if constexpr (ALONE) {
+            draw_whole(a, r, s, u);
+        } else if (threadIdx.x == 0) {
+            wide = {2, r.top, 0};
+        }
         return;
     }
     const double unit = ldexp(1.0, -static_cast<int>(a.bits));
@@ -1923,8 +2028,11 @@ struct SelectWork : PlanWork {
             const uint32_t rows = std::min(batch, args.rows.rows - first);
             const uint32_t parts_of_all = rows * args.wide_parts;
             first_launch<DT>(of, rows, st);
-            HCCLX_LAUNCH((k_sample<DT, NT>), dim3(rows + (apart ? 0 : parts_of_all)), dim3(NT), 0, st, of, rows);
-            if (args.wide_parts == 0) continue;
+            if (args.wide_parts == 0) {
+                HCCLX_LAUNCH((k_sample<DT, NT, true>), dim3(rows), dim3(NT), 0, st, of, rows);
+                continue;
+            }
+            HCCLX_LAUNCH((k_sample<DT, NT, false>), dim3(rows + (apart ? 0 : parts_of_all)), dim3(NT), 0, st, of, rows);
             if (apart) HCCLX_LAUNCH((k_sample_levels<DT, NT>), dim3(parts_of_all), dim3(NT), 0, st, of);
             HCCLX_LAUNCH((k_sample_weigh<DT, NT>), dim3(parts_of_all), dim3(NT), 0, st, of);
             HCCLX_LAUNCH((k_sample_wide<DT, NT>), dim3(rows), dim3(NT), 0, st, of);

@@ -37,3 +37,66 @@ def test_half_of_a_mirrored_row(dtype, top_k, min_p, spread):
     got, _ = draw(s, dict(temperature=temperature, top_k=[top_k] * rows, min_p=[min_p] * rows), [0.5] * rows)
     want = [first_of_second_half(s.whole()[r], temperature[r], top_k, float(np.float32(min_p))) for r in range(rows)]
     assert got == want, [(r, a, b) for r, (a, b) in enumerate(zip(got, want)) if a != b]
+
+
+@pytest.mark.parametrize("dtype", [T.FP32, T.BFP16])
+@pytest.mark.parametrize("vocab,n", [(131072, 1), (120001, 5), (600000, 2)])
+def test_half_of_a_mirrored_row_without_a_filter(vocab, n, dtype):
+    """The same rows in plans of few and many rows, whose first launch sums up longer and shorter runs, with settings that filter nothing
+    and without any: the same tokens, those of the whole numbers."""
+    vocab -= vocab % 2
+    half = torch.empty((20, vocab // 2), device=DEV).exponential_(1.0, generator=gen(vocab)) * 1.6 - 4
+    rows = mirrored(half).to(TD[dtype])
+    for times in (1, 4, 8, 16):
+        s = Split(rows.repeat(times, 1), shares(vocab, n), dtype)
+        for settings in (dict(), dict(top_k=[0] * s.rows, top_p=[1.0] * s.rows)):
+            got, _ = draw(s, settings, [0.5] * s.rows)
+            assert got == [vocab // 2] * s.rows, (times, [(r, a) for r, a in enumerate(got) if a != vocab // 2])
+
+
+@pytest.mark.parametrize("vocab", [65536, 1 << 19])
+@pytest.mark.parametrize("settings", [dict(), dict(top_p=1.0), dict(min_p=0.5), dict(T_=0.25, min_p=1.0)])
+def test_equal_logits_at_every_border(vocab, settings):
+    """Token j takes [j / vocab, (j + 1) / vocab)."""
+    places = torch.randint(0, vocab, (60,), device=DEV, generator=gen(3)).tolist() + [0, 1, vocab // 2, vocab - 1]
+    rows = 2 * len(places)
+    s = Split(torch.full((rows, vocab), 3.5, device=DEV, dtype=torch.bfloat16), shares(vocab, 3), T.BFP16)
+    below = np.nextafter(np.array([(j + 1) / vocab for j in places], dtype=np.float32), np.float32(0))
+    u = [j / vocab for j in places] + below.tolist()
+    got, logprob = draw(s, {("temperature" if k == "T_" else k): [v] * rows for k, v in settings.items()}, u)
+    assert got == places * 2
+    assert np.allclose(logprob, -np.log(vocab), rtol=1e-7, atol=0)
+
+
+@pytest.mark.parametrize("vocab,bits", [(131072, 45), (600000, 42)])
+@pytest.mark.parametrize("settings", [dict(), dict(top_p=1.0, top_k=0), dict(min_p=1e-30)])
+def test_what_is_less_than_half_of_a_part_is_never_drawn(vocab, bits, settings):
+    """Weights are whole numbers of 2^-51 of the largest without a filter, otherwise of 2^-45 for 131072 columns and 2^-42 for 600000: a little
+    less than half of that is nothing, a little more is one."""
+    if "min_p" not in settings:
+        bits = 51
+    x = torch.zeros((8, vocab), device=DEV)
+    for r, (place, more) in enumerate([(vocab - 1, -0.01), (vocab - 1, 0.01), (0, -0.01), (0, 0.01)] * 2):
+        x[r] = float((-(bits + 1) + more) * np.log(2))
+        x[r, place] = 0.0
+    s = Split(x, shares(vocab, 2), T.FP32)
+    got, _ = draw(s, {k: [v] * 8 for k, v in settings.items()}, [0.0] * 4 + [1.0] * 4)
+    assert got == [vocab - 1, 0, 0, 0, vocab - 1, vocab - 1, 0, vocab - 1]
+
+
+@pytest.mark.parametrize("dtype", [T.FP32, T.FP16])
+def test_ends_of_rows_without_a_filter(dtype):
+    """0 draws the first column that has any weight, 1 and more the last."""
+    x = torch.randn((6, 40000), device=DEV, generator=gen(9))
+    x[:, 0] = x[:, -1] = -float("inf")
+    x[1, :30000] = float("nan")
+    x[2, 20000:] = -float("inf")
+    x[3] = -float("inf")
+    x[3, 777] = -3.0
+    x[4, [300, 500]] = float("inf")
+    s = Split(x.to(TD[dtype]), shares(40000, 3), dtype, pad=1)
+    for settings in (dict(), dict(min_p=[0.0] * 6)):
+        for T_ in (1.0, 2.5, float("inf")):
+            first, _ = draw(s, dict(settings, temperature=[T_] * 6), [0.0] * 6)
+            last, _ = draw(s, dict(settings, temperature=[T_] * 6), [1.0] * 3 + [2.0] * 3)
+            assert first == [1, 30000, 1, 777, 300, 1] and last == [39998, 39998, 19999, 777, 500, 39998]
