@@ -63,7 +63,8 @@ struct Run {
 struct Wide {
     uint32_t wide;     // 0: it is not; 2: it is, but its cut is not found by levels, or it has none
     uint32_t top;      // its largest number
-    unsigned long long p_of_whole;
+    unsigned long long p_low;    // between which what top_p asks for lies
+    unsigned long long p_high;
 };
 
 // What a part of such a row holds nearer than the band, and how many in it.
@@ -317,6 +318,7 @@ constexpr uint32_t kCounted = 256;       // elements of a list that is put in or
 constexpr uint32_t kMostWaves = 8;
 constexpr uint32_t kCached = 320;        // chunks whose places in the row are kept in LDS
 constexpr uint32_t kNoEnd = 0xffffffffu;
+constexpr uint32_t kNotSure = 1 << 16;   // counts for more elements than a list has
 constexpr uint32_t kStretches = 1000;    // of the range of a list's numbers
 constexpr uint32_t kMostAlike = 32;      // elements of a stretch that are put in order by counting
 constexpr uint32_t kQueue = 512;         // elements of a chunk that a wavefront weighs
@@ -1016,25 +1018,40 @@ typedef unsigned __int128 u128;
 
 // x times whole, for 0 < x < 1, as the whole number below or (UP) above: exactly, from the 24 bits of x and all of the product, which has 100 at
 // most.  (In doubles a whole of more than 2^53 was rounded first, and a border that lies at the product was on either side of it.)
-template <bool UP>
-__device__ __forceinline__ u128 share_of(float x, u128 whole)
+template <bool UP, typename W>
+__device__ __forceinline__ W share_of(float x, W whole)
 {
     const uint32_t bits = __float_as_uint(x), power = max(bits >> 23, 1u);
     const u64 m = (bits & 0x7fffffu) | (bits >> 23 != 0 ? 0x800000u : 0u);
-    const u128 product = whole * m;
     const uint32_t down = min(150 - power, 127u);   // x = m 2^-down: 24 or more
-    const u128 n = product >> down;
-    return n + (UP && n << down != product ? 1 : 0);
+    if constexpr (sizeof(W) == 8) {   // (half the operations)
+        const u64 low = m * whole, high = __umul64hi(m, whole);
+        const u64 n = down < 64 ? high << (64 - down) | low >> down : high >> (down - 64);
+        const u64 rest = down < 64 ? low << (64 - down) : low | (high & ~(~u64(0) << (down - 64)));
+        return n + (UP && rest != 0 ? 1 : 0);
+    } else {
+        const u128 product = whole * m, n = product >> down;
+        return n + (UP && n << down != product ? 1 : 0);
+    }
 }
 // floor(u x whole), inside the whole
 template <typename W>
 __device__ __forceinline__ W aim_of(float u, W whole)
 {
     if (!(u > 0.0f)) return 0;
-    return u < 1.0f ? static_cast<W>(share_of<false>(u, whole)) : whole - 1;
+    return u < 1.0f ? share_of<false>(u, whole) : whole - 1;
 }
 // What of `whole` top_p asks for.
-__device__ __forceinline__ u64 part_of(float p, u64 whole) { return p > 0.0f ? static_cast<u64>(share_of<true>(p, whole)) : 0; }
+__device__ __forceinline__ u64 part_of(float p, u64 whole) { return p > 0.0f ? share_of<true>(p, whole) : 0; }
+
+// The same of a sum over a whole row, in multiples of 2^-51, as multiples of 2^-bits.
+__device__ __forceinline__ u64 part_of_whole(const SelectArgs &a, float p, u128 whole)
+{
+    if (!(p > 0.0f)) return 0;
+    const u128 n = share_of<true>(p, whole);
+    const uint32_t down = kWholeBits - a.bits;
+    return static_cast<u64>(n >> down) + ((n >> down) << down != n ? 1 : 0);
+}
 
 // What stays of a row that no list holds: numbers over `cut`, the first `equal` of those that are it, and of them all what is `least`
 // times as probable as the first.
@@ -1147,52 +1164,60 @@ __device__ __forceinline__ void draw_kept(const SelectArgs &a, Row<DT, NT> &r, S
     }
 }
 
-// No filter, by the definition: weights are multiples of 2^-51, the most that the sum of a chunk has room for in 64 bits, and sums over chunks
-// have 128.  Chunks are weighed 512 at a time, and the one that the aim lies in is gone through; a first walk finds the whole.
+// A walk over the chunks of a row, in their order: f(chunk, what the weights in front of it sum up to, its own).  Weights are multiples of 2^-51, the
+// most that the sum of a chunk has room for in 64 bits, and sums over chunks have 128.  Returns that of the row.  AGAIN: the walk before was
+// this row's, and what it weighed last is still there.
+template <int DT, int NT, bool AGAIN, typename F>
+__device__ __forceinline__ u128 walk_whole(const SelectArgs &a, Row<DT, NT> &r, Shared &s, F &&f)
+{
+    using R = Row<DT, NT>;
+    constexpr uint32_t NE = R::NE;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    static_assert(NT == 512, "a thread for each chunk");
+    u128 front = 0;
+    for (uint32_t first = 0; first < a.rows.nchunks; first += NT) {
+        for (uint32_t at = wave; at < NT; at += R::kWaves) {
+            if (AGAIN && a.rows.nchunks <= NT) break;
+            const uint32_t chunk = first + at;
+            u64 sum = 0;
+            if (chunk < a.rows.nchunks) {
+                const Stretch t = a.rows.chunks[chunk];
+                const u32x4 raw = load_piece<DT, false>(t.at + r.row * t.step, lane, t.elems);
+                float v[NE];
+                R::V::unpack(raw, v);
+#pragma unroll
+                for (uint32_t e = 0; e < NE; ++e) sum += lane * NE + e < t.elems ? r.weight(no_nan(v[e]), kWholeBits) : 0;
+            }
+            sum = wave_total(sum);
+            if (lane == 0) s.walk.weight[at] = sum;
+        }
+        __syncthreads();
+        const u64 mine = s.walk.weight[threadIdx.x];
+        u64 low_all, high_all;
+        const u64 low = r.before(mine & 0xffffffffu, &low_all);
+        const u64 high = r.before(mine >> 32, &high_all);
+        f(first + threadIdx.x, front + (static_cast<u128>(high) << 32) + low, mine);
+        front += (static_cast<u128>(high_all) << 32) + low_all;
+        __syncthreads();
+    }
+    return front;
+}
+
+// No filter, by the definition: the chunk that the aim lies in is gone through.
 template <int DT, int NT>
 __device__ __forceinline__ void draw_whole(const SelectArgs &a, Row<DT, NT> &r, Shared &s, float u)
 {
     using R = Row<DT, NT>;
     constexpr uint32_t NE = R::NE;
-    static_assert(NT == 512, "a thread for each chunk");
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-    u128 aim = 0, whole = 0;
-    for (int find = 0; find < 2; ++find) {
-        u128 front = 0;
-        for (uint32_t first = 0; first < a.rows.nchunks; first += NT) {
-            for (uint32_t at = wave; at < NT; at += R::kWaves) {
-                if (find == 1 && a.rows.nchunks <= NT) break;   // (still there)
-                const uint32_t chunk = first + at;
-                u64 sum = 0;
-                if (chunk < a.rows.nchunks) {
-                    const Stretch t = a.rows.chunks[chunk];
-                    const u32x4 raw = load_piece<DT, false>(t.at + r.row * t.step, lane, t.elems);
-                    float v[NE];
-                    R::V::unpack(raw, v);
-#pragma unroll
-                    for (uint32_t e = 0; e < NE; ++e) sum += lane * NE + e < t.elems ? r.weight(no_nan(v[e]), kWholeBits) : 0;
-                }
-                sum = wave_total(sum);
-                if (lane == 0) s.walk.weight[at] = sum;
-            }
-            __syncthreads();
-            const u64 mine = s.walk.weight[threadIdx.x];
-            u64 low_all, high_all;
-            const u64 low = r.before(mine & 0xffffffffu, &low_all);
-            const u64 high = r.before(mine >> 32, &high_all);
-            const u128 at = front + (static_cast<u128>(high) << 32) + low;
-            if (find == 1 && aim >= at && aim - at < mine) {
-                s.word[0] = first + threadIdx.x;   // the chunk
-                s.word64[0] = static_cast<u64>(aim - at);
-            }
-            front += (static_cast<u128>(high_all) << 32) + low_all;
-            __syncthreads();
+    const u128 whole = walk_whole<DT, NT, false>(a, r, s, [](uint32_t, u128, u64) {});
+    const u128 aim = aim_of(u, whole);
+    (void)walk_whole<DT, NT, true>(a, r, s, [&](uint32_t chunk, u128 at, u64 mine) {
+        if (aim >= at && aim - at < mine) {
+            s.word[0] = chunk;
+            s.word64[0] = static_cast<u64>(aim - at);
         }
-        if (find == 0) {
-            whole = front;
-            aim = aim_of(u, whole);
-        }
-    }
+    });
     if (wave != 0) return;
     // one wavefront, one chunk
     const Stretch t = a.rows.chunks[s.word[0]];
@@ -1215,12 +1240,15 @@ __device__ __forceinline__ void draw_whole(const SelectArgs &a, Row<DT, NT> &r, 
     }
 }
 
-// No filter: the run in which the running sum passes u x the whole, then the element, by sums of doubles, whose order goes by the plan (how
-// many chunks a run has).  The whole numbers say the same where both of the element's borders are further from the aim than that can matter.
-// With e the error of an element in these sums, of which k are in front of a border, the distance border - u whole is off by (1 - u) times
-// the first k and u times the others' sum.  e is 2^-52 where a number is rounded, and 2^-53 of a run's largest where the run leaves it out; and
-// in parts of the whole, an exponent of up to 53 powers of two, rounded twice, is good to 2^-46.8 of its term; three of them, and 200
-// additions of doubles one behind the other, make 2^-44.3.
+// How far a sum of doubles over what the first launch's runs hold, whose order goes by the plan (how many chunks a run has), may be from that of the
+// multiples of 2^-51, with an error of each of n elements in it.  That is 2^-52 where a number is rounded, and 2^-53 of a run's largest where
+// the run leaves it out (taken twice).  In parts of the whole: an exponent of up to 53 powers of two, rounded twice, is good to 2^-46.8 of its
+// term; three of them, and 200 additions of doubles one behind the other, make 2^-44.3.
+__device__ __forceinline__ double slack(double n, double whole) { return n * 0x1p-51 + whole * 0x1p-43; }
+
+// No filter: the run in which the running sum passes u x the whole, then the element, by such sums.  The whole numbers say the same where both of
+// the element's borders are further from the aim than that can matter: with k elements in front of a border, the distance border - u whole
+// is off by 1 - u of the error of the first k and u of that of the others.
 // Otherwise false is returned, and nothing is drawn (for one row of 131072 columns in some millions).
 template <int DT, int NT>
 __device__ __forceinline__ bool draw_all(const SelectArgs &a, Row<DT, NT> &r, Shared &s, float u)
@@ -1301,7 +1329,7 @@ __device__ __forceinline__ bool draw_all(const SelectArgs &a, Row<DT, NT> &r, Sh
         }
         const uint32_t column = t.first + (lane * NE + place % NE);
         const double share = fmin(fmax(static_cast<double>(u), 0.0), 1.0);
-        const double gap = ((1.0 - share) * (column + 2) + share * (a.rows.vocab - column + 1)) * 0x1p-51 + whole * 0x1p-43;
+        const double gap = slack((1.0 - share) * (column + 2) + share * (a.rows.vocab - column + 1), whole);
         // (at 0: nothing in front of it has any weight)
         if ((front == 0.0 || aim - front >= gap) && front + its - aim >= gap) {
             r.write_choice(column, number_of(l), whole);
@@ -1313,9 +1341,9 @@ __device__ __forceinline__ bool draw_all(const SelectArgs &a, Row<DT, NT> &r, Sh
 }
 
 // The cut is searched by numbers, among all elements, and chunks are weighed: right for every row, but one workgroup goes through all
-// of it several times.
+// of it several times (where top_p is a part of the whole row once more, for the sum of that).
 template <int DT, int NT>
-__device__ __forceinline__ void draw_by_numbers(const SelectArgs &a, Row<DT, NT> &r, Shared &s, const RowChoice &choice, float u, u64 p_of_whole)
+__device__ __forceinline__ void draw_by_numbers(const SelectArgs &a, Row<DT, NT> &r, Shared &s, const RowChoice &choice, float u)
 {
     constexpr uint32_t kShift = kIdle<DT>;
     __syncthreads();   // the lists make room
@@ -1336,12 +1364,13 @@ __device__ __forceinline__ void draw_by_numbers(const SelectArgs &a, Row<DT, NT>
     if (choice.by_p) {
         range = {stay.cut > kLeast >> kShift ? stay.cut : kLeast >> kShift, r.top >> kShift, 0, 0, 0, 0};
         u64 aim = 0;
+        if (!choice.by_k) aim = part_of_whole(a, choice.p, walk_whole<DT, NT, false>(a, r, s, [](uint32_t, u128, u64) {}));
         bool first = true;
         // (what is equal to the cut of top_k and does not stay is at the end of the order)
         const u64 over = choice.by_k && cut_count > stay.equal ? (cut_count - stay.equal) * r.weight(stay.cut << kShift | (stay.cut >> (31 - kShift) != 0 ? 0 : (1u << kShift) - 1)) : 0;
         do {
             r.template narrow<true>(range, all, [&](u64 whole) {
-                if (first) aim = max(u64(1), min(choice.by_k ? part_of(choice.p, whole - over) : p_of_whole, whole));
+                if (first) aim = max(u64(1), min(choice.by_k ? part_of(choice.p, whole - over) : aim, whole));
                 return aim;
             });
             first = false;
@@ -1512,7 +1541,7 @@ __device__ __forceinline__ Band band_of(const SelectArgs &a, Team<NT> &r, Shared
         }
         count = r.before(count, &all);
         weight = r.before(weight, &whole);
-        const double aim = ldexp(static_cast<double>(w.p_of_whole), -static_cast<int>(a.bits));
+        const double aim = ldexp(static_cast<double>(w.p_high), -static_cast<int>(a.bits));
 #pragma unroll
         for (uint32_t i = 0; i < kMine; ++i) {
             const bool by_k = choice.by_k && count < choice.k && count + counts[i] >= choice.k;
@@ -1599,10 +1628,10 @@ __device__ __forceinline__ u64 weigh_chunk(const Team<NT> &r, Shared &s, const D
 }
 
 // What stays of a list whose elements the threads hold, kListed each (key 0: none): those from the returned key on.  `skip` of them stay (top_k), or
-// those before whose place in the order the weight is less than `aim`.  As by Row::narrow: keys are counted and weighed into equal
+// those before whose place in the order the weight is less than `aim`; *front is what is before the last of them.  As by Row::narrow: keys are counted and weighed into equal
 // stretches of their range, which leaves one of them: two rounds, or three where many numbers are alike.
 template <int NT, int N>
-__device__ __forceinline__ u64 last_that_stays(Team<NT> &r, Shared &s, const u64 (&key)[N], const u64 (&weight)[N], bool by_count, uint32_t stay, u64 aim)
+__device__ __forceinline__ u64 last_that_stays(Team<NT> &r, Shared &s, const u64 (&key)[N], const u64 (&weight)[N], bool by_count, uint32_t stay, u64 aim, u64 *front)
 {
     static_assert(NT == 512, "a stretch for each thread");
     const uint32_t t = threadIdx.x;
@@ -1657,7 +1686,7 @@ __device__ __forceinline__ u64 last_that_stays(Team<NT> &r, Shared &s, const u64
         __syncthreads();
         const Range found = s.range;
         count_before = found.above;
-        weight_before = found.weight_above;
+        *front = weight_before = found.weight_above;
         const u64 begin = low + (static_cast<u64>(found.low) << shift);
         high = min(high, begin + ((u64(1) << shift) - 1));
         low = begin;
@@ -1731,9 +1760,9 @@ k_sample_weigh(SelectArgs a)
 }
 
 // Draws from a row of whose band n elements are listed, N for a thread at most; `over` elements of the weight `above` are nearer.  Returns false,
-// and nothing is drawn, where the cut is not among them.
+// and nothing is drawn, where the cut is not among them, or top_p may ask for one more or less.
 template <int DT, int NT, int N>
-__device__ __forceinline__ bool draw_band(const SelectArgs &a, Team<NT> &r, Shared &s, const RowChoice &choice, const Band &band, float u, u64 p_of_whole,
+__device__ __forceinline__ bool draw_band(const SelectArgs &a, Team<NT> &r, Shared &s, const RowChoice &choice, const Band &band, float u, const Wide &wide,
                                           uint32_t n, uint32_t over, u64 above)
 {
     using V = Vec16<DT>;
@@ -1756,9 +1785,11 @@ __device__ __forceinline__ bool draw_band(const SelectArgs &a, Team<NT> &r, Shar
     const u64 inside = r.total(sum);
     u64 last = 0;
     if (band.by_level) {
-        const bool right = choice.by_k ? over < choice.k && over + n >= choice.k : above < p_of_whole && above + inside >= p_of_whole;
+        const bool right = choice.by_k ? over < choice.k && over + n >= choice.k : above < wide.p_low && above + inside >= wide.p_high;
         if (!right) return false;
-        last = last_that_stays(r, s, key, w, choice.by_k, choice.k - over, p_of_whole - above);
+        u64 front = 0;
+        last = last_that_stays(r, s, key, w, choice.by_k, choice.k - over, wide.p_high - above, &front);
+        if (!choice.by_k && above + front >= wide.p_low) return false;   // (what top_p asks for may be in front of it)
     }
     const auto stays = [&](u64 x) {
         return x >= last && (!band.by_min || static_cast<uint32_t>(x >> 32) == r.top || r.share(static_cast<uint32_t>(x >> 32)) >= choice.least);
@@ -1841,8 +1872,8 @@ k_sample_wide(SelectArgs a)
                 if (threadIdx.x < 64) s.groups[lane] = lane < a.wide_parts ? begin : n;
                 Team<NT> r(a, s, row, wide.top, choice.c);
                 __syncthreads();
-                if (n <= kBand / 4 ? draw_band<DT, NT, kBand / 4 / NT>(a, r, s, choice, band, u, wide.p_of_whole, n, over, above)
-                                   : draw_band<DT, NT, kBand / NT>(a, r, s, choice, band, u, wide.p_of_whole, n, over, above)) {
+                if (n <= kBand / 4 ? draw_band<DT, NT, kBand / 4 / NT>(a, r, s, choice, band, u, wide, n, over, above)
+                                   : draw_band<DT, NT, kBand / NT>(a, r, s, choice, band, u, wide, n, over, above)) {
                     return;
                 }
             }
@@ -1856,7 +1887,7 @@ k_sample_wide(SelectArgs a)
         draw_whole(a, r, s, u);
         return;
     }
-    draw_by_numbers(a, r, s, choice, u, wide.p_of_whole);
+    draw_by_numbers(a, r, s, choice, u);
 }
 
 // The second launch: rows from a.first on.  ALONE: there are none behind it, since no row has a filter, or none is longer than a list.
@@ -1891,16 +1922,21 @@ k_sample(SelectArgs a, uint32_t rows)
         if constexpr (ALONE) {
             draw_whole(a, r, s, u);
         } else if (threadIdx.x == 0) {
-            wide = {2, r.top, 0};
+            wide = {2, r.top, 0, 0};
         }
         return;
     }
     const double unit = ldexp(1.0, -static_cast<int>(a.bits));
-    u64 p_of_whole = 0;   // the weight that top_p asks for, where it is of the whole row
+    // The weight that top_p asks for lies between these two.  Of a whole row that comes from sums of doubles; where an element ends between them, the row is
+    // left to the launches behind, the last of which adds up whole numbers.
+    u64 p_low = 0, p_high = 0;
     if (choice.by_p && !choice.by_k) {
         double mine = 0.0;
         for (uint32_t i = threadIdx.x; i < a.nruns; i += NT) mine += r.run_sum(i);
-        p_of_whole = part_of(choice.p, static_cast<u64>(ldexp(r.total(mine), static_cast<int>(a.bits))));
+        mine = r.total(mine);
+        const double off = slack(a.rows.vocab, mine);
+        p_low = part_of(choice.p, static_cast<u64>(ldexp(fmax(mine - off, 0.0), static_cast<int>(a.bits))));
+        p_high = part_of(choice.p, static_cast<u64>(ldexp(mine + off, static_cast<int>(a.bits))) + 1);
     }
     uint32_t sure = 0;
     if (!choice.by_k || choice.k <= HCCLX_TOP_MAX) {
@@ -1913,11 +1949,13 @@ k_sample(SelectArgs a, uint32_t rows)
             u64 weight_before;
             const uint32_t place = r.template count_before<true>(n, w, &weight_before);
             const bool first = threadIdx.x < n && place < limit;
-            if (choice.by_k && choice.by_p) p_of_whole = part_of(choice.p, r.total(first ? w : 0));
+            // (where the list holds the whole row, bits is kWholeBits)
+            if (choice.by_p && (choice.by_k || n == a.rows.vocab)) p_low = p_high = part_of(choice.p, r.total(first ? w : 0));
             bool in = first;
-            if (choice.by_p) in = in && (place == 0 || weight_before < p_of_whole);
+            if (choice.by_p) in = in && (place == 0 || weight_before < p_high);
             if (choice.by_min) in = in && (place == 0 || r.share(l, 0) >= choice.least);
-            if (choice.by_k || n == a.rows.vocab || r.total(static_cast<uint32_t>(in)) < sure) {
+            const bool unsure = choice.by_p && in && place != 0 && weight_before >= p_low;
+            if (choice.by_k || n == a.rows.vocab || r.total(unsure ? kNotSure : static_cast<uint32_t>(in)) < sure) {
                 u64 whole;
                 const u64 at = r.before(in ? w : 0, &whole);
                 const u64 aim = aim_of(u, whole);
@@ -1935,15 +1973,15 @@ k_sample(SelectArgs a, uint32_t rows)
             }
             u64 whole;
             u64 at = r.before(sum, &whole);
-            if (choice.by_k && choice.by_p) p_of_whole = part_of(choice.p, whole);
+            if (choice.by_p && (choice.by_k || n == a.rows.vocab)) p_low = p_high = part_of(choice.p, whole);
             uint32_t keep = 0;
 #pragma unroll
             for (uint32_t i = 0; i < kMine; ++i) {
                 const uint32_t place = threadIdx.x * kMine + i;
                 bool in = place < limit;
-                if (choice.by_p) in = in && (place == 0 || at < p_of_whole);
+                if (choice.by_p) in = in && (place == 0 || at < p_high);
                 if (choice.by_min) in = in && (place == 0 || r.share(static_cast<uint32_t>(s.list.sorted[place] >> 32)) >= choice.least);
-                keep += in;
+                keep += choice.by_p && in && place != 0 && at >= p_low ? kNotSure : in;
                 at += w[i];
             }
             const uint32_t kept = r.total(keep);
@@ -1971,7 +2009,7 @@ k_sample(SelectArgs a, uint32_t rows)
         }
     }
     // (never where there is no launch for it: the list held all columns)
-    if (threadIdx.x == 0) wide = {is_wide(choice, r.top_value) ? 1u : 2u, r.top, p_of_whole};
+    if (threadIdx.x == 0) wide = {is_wide(choice, r.top_value) ? 1u : 2u, r.top, p_low, p_high};
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------

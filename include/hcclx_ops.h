@@ -265,9 +265,9 @@ int hcclx_distill_grad_plan_create(const hcclx_distill_grad_t *distill, hcclx_pl
  *     min_p        0 or less, or NaN: all; more than 1 counts as 1; NULL: all
  *     random       in [0, 1) from the caller's generator, so that a draw is a function of its arguments (outside: the nearest end; NaN: 0)
  * NaN counts as -infinity and is never drawn; a row of nothing else gets token -1 and logprob -infinity.  Of +infinities one is drawn.
- * w are computed in 64 bits and summed as whole multiples, of 2^-51 where nothing filters a row and otherwise of 2^-38 or less (2^-45 for 131072
- * columns), so that sums, and the token, do not go by their order or by the other rows of the plan; what is less than half of that is never
- * drawn. */
+ * w are computed in 64 bits and summed as whole multiples, so that sums, and the token, do not go by their order or by the other rows of the plan:
+ * of 2^-51 where all columns count (in a row without a filter, and for what top_p is a part of where there is no top_k), otherwise of 2^-38 or
+ * less (2^-45 for 131072 columns).  What is less than half of that is never drawn. */
 typedef struct {
     hcclx_logits_t logits;
     const float *temperature;

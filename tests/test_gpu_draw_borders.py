@@ -100,3 +100,18 @@ def test_ends_of_rows_without_a_filter(dtype):
             first, _ = draw(s, dict(settings, temperature=[T_] * 6), [0.0] * 6)
             last, _ = draw(s, dict(settings, temperature=[T_] * 6), [1.0] * 3 + [2.0] * 3)
             assert first == [1, 30000, 1, 777, 300, 1] and last == [39998, 39998, 19999, 777, 500, 39998]
+
+
+@pytest.mark.parametrize("seed,top_p,stay", [(3483, 0.5376677513122559, None), (2737, 0.6722675561904907, 75747), (952, 0.9737805724143982, 125109),
+                                             (1731, 0.826088011264801, 98931), (5860, 0.6229817867279053, 68836)])
+def test_top_p_next_to_where_a_token_ends(seed, top_p, stay):
+    """Descending rows of which the first `stay` tokens reach top_p of the whole by 2^-35 of it, or the one less fails it by that (which of the two,
+    the first row does not say: it is nearer than that).  random 1 draws the last that stays.  The same in plans of few and many rows."""
+    vocab = 131072
+    row = np.sort(np.random.default_rng(seed).standard_normal(vocab).astype(np.float32) * np.float32(0.25))[::-1].copy()
+    seen = set()
+    for rows in (1, 64, 128, 300):
+        s = Split(torch.from_numpy(row).to(DEV)[None].expand(rows, -1), [vocab], T.FP32)
+        for settings in (dict(), dict(min_p=[1e-9] * rows)):
+            seen |= set(draw(s, dict(settings, top_p=[top_p] * rows), [1.0] * rows)[0])
+    assert len(seen) == 1 and (stay is None or seen == {stay - 1}), seen
