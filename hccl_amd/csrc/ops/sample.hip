@@ -1561,7 +1561,7 @@ __device__ __forceinline__ Band band_of(const SelectArgs &a, Team<NT> &r, Shared
         // (distances are good to 2^-22 of themselves, and none that matters is over 2^14)
         const float at = static_cast<float>(-log2(choice.least) / r.c * static_cast<double>(distance.scale));
         const float low = at - 0.01f, high = at + 0.01f;
-        if (!band.by_level || high <= band.low) {
+        if (!band.by_level || high <= band.low) {   // (the draw finds out whether the cut of top_p is nearer than its level after all)
             band.by_level = false;
             band.low = low;
             band.high = high;
@@ -1808,6 +1808,7 @@ __device__ __forceinline__ bool draw_band(const SelectArgs &a, Team<NT> &r, Shar
     sum = s.span_weight[threadIdx.x];
     u64 whole;
     u64 begin = r.before(sum, &whole);
+    if (choice.by_p && !band.by_level && whole >= wide.p_low) return false;   // (top_p cuts off some of what min_p leaves)
     const u64 aim = aim_of(u, whole);
     if (aim >= begin && aim - begin < sum) {
         s.word[0] = threadIdx.x;

@@ -115,3 +115,31 @@ def test_top_p_next_to_where_a_token_ends(seed, top_p, stay):
         for settings in (dict(), dict(min_p=[1e-9] * rows)):
             seen |= set(draw(s, dict(settings, top_p=[top_p] * rows), [1.0] * rows)[0])
     assert len(seen) == 1 and (stay is None or seen == {stay - 1}), seen
+
+
+@pytest.mark.parametrize("later", [3, 4, 5])
+def test_top_p_where_min_p_cuts_behind_it(later):
+    """A largest token, 2^20 tokens that are less probable than min_p, and 2^21 equal ones, all over min_p, of which top_p cuts off the last `later`.
+    That is less of their weight than whole numbers of 2^-40 round them up by (w is two fifths below such a number)."""
+    many, few, bits = 1 << 21, 1 << 20, 40
+    d = next(x for x in np.arange(1538, 1542, 1 / 512) if 0.55 < np.exp(-float(np.float32(x / 92.332))) * 2.0 ** bits % 1 < 0.65)
+    d, d2 = float(np.float32(d / 92.332)), float(np.float32(1556 / 92.332))
+    w, w2 = np.exp(-d), np.exp(-d2)
+    number = int(np.rint(w * 2.0 ** bits))
+    whole = (1 << 51) + many * int(np.rint(w * 2.0 ** 51)) + few * int(np.rint(w2 * 2.0 ** 51))
+    # a top_p in the middle of the last token that it leaves, over 2^-26 of itself from that one's ends: half a step of a float
+    stay = many - later
+    for extra in range(200):                                         # (some more of the improbable ones, until a float lies there)
+        total = whole + extra * int(np.rint(w2 * 2.0 ** 51))
+        top_p = float(np.float32(((1 << bits) + (stay - 0.5) * number) * 2.0 ** (51 - bits) / total))
+        asked = -(-int(top_p * 2 ** 30) * total // 2 ** (30 + 51 - bits))
+        if (1 << bits) + (stay - 1) * number + 1000 < asked < (1 << bits) + stay * number - 1000:
+            break
+    assert int(top_p * 2 ** 30) == top_p * 2 ** 30 and -(-(asked - (1 << bits)) // number) == stay
+    vocab = 1 + few + extra + many
+    row = torch.full((1, vocab), -d2, device=DEV)
+    row[0, 0] = 0.0
+    row[0, 1 + few + extra:] = -d
+    s = Split(row, shares(vocab, 2), T.FP32)
+    got, _ = draw(s, dict(top_p=[top_p], min_p=[2.0 ** (-1546 / 64)]), [1.0])
+    assert got == [vocab - 1 - later]
