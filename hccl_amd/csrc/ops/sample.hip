@@ -38,7 +38,7 @@ constexpr uint32_t kSmallList = 1024;
 constexpr uint32_t kNucleus = 64;        // listed where no top_k bounds the list (192: 1024 rows 212 us instead of 201, and no row less)
 constexpr uint32_t kLevels = 2048;       // of the weights of a row
 constexpr uint32_t kWholeBits = 51;      // of a weight's whole number where there is no filter
-constexpr uint32_t kBand = 8192;         // elements of a cut's level, shared out to the parts of a row
+constexpr uint32_t kBand = 8192;         // elements of a cut's level, shared out to the parts of a row (each lists kList at most: of the most rows 4096)
 constexpr uint32_t kNone = 0;            // the number of what does not exist
 constexpr uint32_t kLeast = 0x007fffffu;   // of minus infinity
 
@@ -311,7 +311,7 @@ struct Range {
     u64 weight_inside;
 };
 
-constexpr uint32_t kBatch = 4096;        // rows that are drawn from together: 85 KB for the wide draw of each, 150 KB where they are few
+constexpr uint32_t kBatch = 4096;        // rows that are drawn from together: 36 to 84 KB for the wide draw of each, 150 KB where they are few
 constexpr uint32_t kMostParts = 32;      // workgroups of a wide row
 constexpr uint32_t kMostSpans = 512;
 constexpr uint32_t kCounted = 256;       // elements of a list that is put in order by counting
@@ -1346,9 +1346,6 @@ template <int DT, int NT>
 __device__ __forceinline__ void draw_by_numbers(const SelectArgs &a, Row<DT, NT> &r, Shared &s, const RowChoice &choice, float u)
 {
     constexpr uint32_t kShift = kIdle<DT>;
-    __syncthreads();   // the lists make room
-    r.find_chunks();   // (sorting has taken their place)
-    __syncthreads();
     Kept stay = {0, kNoEnd, choice.by_min ? choice.least : 0.0};
     auto all = [&](auto &&f) { r.each(nullptr, r.ngroups, f); };
     Range range = {kLeast >> kShift, r.top >> kShift, 0, 0, 0, 0};
