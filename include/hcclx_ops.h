@@ -218,8 +218,9 @@ int hcclx_top_logits_plan_create(const hcclx_top_logits_t *top, hcclx_plan_t **p
  *     dlogits = weight T (q - the sum of p over the entries that name the column)
  * Entries whose index is no column's (-1, say) are left out, and a row without any entry but those, or but logits of -infinity, has
  * loss 0 and gradients 0; a column may be named by several entries.  A row of weight 0 (a masked token) is not read, whatever it holds:
- * loss 0, gradients 0.  NaN and +infinity in a row that counts, the teacher's or the student's, make its loss and gradients NaN.  The
- * sum over the row's columns is held in 32 bits, what concerns the entries alone in 64.
+ * loss 0, gradients 0.  NaN and +infinity in a row that counts, the teacher's or the student's, make its loss and gradients NaN.  A column
+ * whose logit is -infinity has q = 0, and so has every column of a row of nothing else: with an entry of p > 0 there the loss is infinite, and its
+ * gradient - weight T p.  The sum over the row's columns is held in 32 bits, what concerns the entries alone in 64.
  *
  * stats: two floats per row for hcclx_distill_grad_plan_create, 8-byte aligned.  dlogits: one pointer per rank, rows as far apart as
  * the logits', and each may be that rank's logits.  A program that knows the weights before the loss gets the gradients in the same
