@@ -417,8 +417,10 @@ k_distill_row(DistillArgs a)
 }
 
 // The same where rows are few and short: a row stays in the threads' registers, N vectors in each, instead of being read twice.  What counts
-// there is the chain of one row (16 rows of 32000 bf16 10.3 us, read twice 11.8; of 8000 9.8 and 9.2, the code of N vectors costs more than
-// one more turn), of up to the two rows that a CU has room for (500 of 32000 17.7 and 19.5, 1000 32 and 32, 4096 190 and 145).
+// there is the chain of one row: with more chunks than a turn of the workgroup it saves a turn's wait, with fewer the code of N vectors costs
+// more than that.  16 rows bf16 of 33, 48 and 64 chunks 10.1, 9.8 and 9.9 us, read twice 11.2, 11.7 and 11.2; of 16 and 32 9.4 and 9.7, read
+// twice 8.8 and 8.7.  Of up to the two rows that a CU has room for: 512 rows of 33 to 64 chunks 15.6 to 17.1 and 15.0 to 22.5; 600 of 33 21 and
+// 18, 4096 of 33, 48 and 64 97, 103 and 113 and 78, 102 and 124.
 template <int DT, int N>
 __global__ void __launch_bounds__(kThreads)
 k_distill_held(DistillArgs a)
@@ -689,10 +691,12 @@ int make_distill(const hcclx_distill_t &d, hcclx_plan_t **plan)
     uint64_t held = w->table.bytes;
     const uint32_t cus = static_cast<uint32_t>(ctx->num_cus), turn = kThreads / 64 * kAhead;
     w->held = w->grad && l.rows <= 2 * cus && w->args.rows.nchunks > turn && w->args.rows.nchunks <= kThreads / 64 * kHeld;
-    // Short rows: what counts is how many are there at once, and smaller workgroups find room for more (loss and gradient, 4096 rows bf16 of 5000
-    // 45 us, by workgroups of 512 62, of 32000 137 and 145, of 50000 231 and 216; the loss alone, 2048 rows fp16 of 5000 16 and 25, of 65536 51
-    // and 53, of 131072 95 and 90).
-    w->short_rows = w->args.rows.nchunks <= (w->grad ? 64 : 128);
+    // Short rows: smaller workgroups find room for more of them at once.  With a gradient that pays while a row is one turn of theirs (bf16, 16 rows
+    // of 16 chunks 8.1 us, by workgroups of 512 8.8; of 24 10.6 and 8.6), or two where rows fill the device (4096 rows of 5000 35 and 53, of
+    // 16000 66 and 68, of 24000 99 and 100, of 32000 127 and 116; fp32 of 8000 59 and 63, of 16000 121 and 110).  The loss alone reads a row once:
+    // 4096 rows of 16 chunks 25 and 42, of 64 50 and 57, of 128 93 and 94, of 160 114 and 113; 1000 of 128 27 and 29; 300 of 64 10.7 and 10.7, of 128
+    // 16.8 and 15.3.
+    w->short_rows = w->args.rows.nchunks <= (!w->grad ? 128 : l.rows > 2 * cus ? 32 : 16);
     if (rows != 0 && !w->held) w->parts = parts_of(l.rows, w->args.rows.nchunks, cus);
     if (w->parts > 1) {
         w->args.nparts = w->parts;

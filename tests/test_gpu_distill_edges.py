@@ -9,7 +9,7 @@ import logits_oracle as L
 import ops_oracle as O
 from hccl_amd import hcclx
 from hccl_amd import types as T
-from test_gpu_output_layer import DEV, TD, Split, entries, gen, shares
+from test_gpu_output_layer import DEV, TD, Split, check_distill, contents, entries, gen, shares
 
 pytestmark = pytest.mark.gpu
 INF = math.inf
@@ -93,3 +93,11 @@ def test_a_student_that_rules_entries_or_everything_out(rows, vocab, dtype):
     for r in (0, 1, rows - 1):
         assert float(out[0][r]) == INF and float(out[2][r]) == INF
     check_rows(whole, values, at, weight, out, set())
+
+
+@pytest.mark.parametrize("dtype,chunk", [(T.FP32, 256), (T.BFP16, 512)])
+@pytest.mark.parametrize("rows", [5, 520])
+@pytest.mark.parametrize("chunks", [16, 24, 32, 64, 128])
+def test_lengths_on_both_sides_of_where_a_route_ends(chunks, rows, dtype, chunk):
+    for vocab in (chunks * chunk, chunks * chunk + 1):
+        check_distill(contents("steep", rows, vocab, gen(vocab)), [vocab], dtype, 30, 1.5, in_place=rows == 5)
