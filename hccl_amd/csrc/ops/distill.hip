@@ -226,7 +226,8 @@ struct DistillShared {
 extern __shared__ unsigned long long s_table[];   // sums and columns of the entries, as many as the plan's k needs (Together)
 
 // Sums p over the entries that name the same column: where the entry's sum is.  Sums are of whole numbers, so that their order does not
-// show.  (p: of 2^62.)  Between the table's making and the first entry lies a barrier of the caller's.
+// show: p is rounded to 2^-62 there, 2^-24 of what is as improbable as 2^-38.  A column that one entry names has that entry's p as it is.  Between
+// the table's making and the first entry lies a barrier of the caller's.
 template <int NT>
 struct Together {
     unsigned long long *const sum;
@@ -240,16 +241,25 @@ struct Together {
             sum[i] = 0;
         }
     }
+    static constexpr uint32_t kShared = 0x80000000u;   // (no column has this bit)
     __device__ __forceinline__ uint32_t add(uint32_t c, double p)
     {
         uint32_t i = (c * 2654435769u) >> 16 & mask;
         for (;;) {   // (at most half of the slots are taken)
             const uint32_t was = atomicCAS(&column[i], kFree, c);
-            if (was == kFree || was == c) break;
+            if (was == c) atomicOr(&column[i], kShared);
+            if (was == kFree || (was & ~kShared) == c) break;
             i = (i + 1) & mask;
         }
         atomicAdd(&sum[i], static_cast<unsigned long long>(p * 0x1p62));
         return i;
+    }
+    // The sum at i, given an entry of it.
+    __device__ __forceinline__ double of(uint32_t i, double p) const
+    {
+        const bool shared = (column[i] & kShared) != 0;
+        const double all = static_cast<double>(sum[i]) * 0x1p-62;
+        return shared ? all : p;
     }
 };
 
@@ -372,7 +382,7 @@ __device__ __forceinline__ void finish(const DistillArgs &a, DistillShared &s, u
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
             if (e.at[i] < low || e.at[i] >= high) continue;
-            const double p = static_cast<double>(together.sum[slot[i]]) * 0x1p-62;
+            const double p = together.of(slot[i], e.p[i]);
             const double q = empty ? 0.0 : exp2((l[i] - r) * a.c64) / all.s;
             reinterpret_cast<typename D::S *>(of[i]->to + row * of[i]->step)[e.at[i] - of[i]->first] =
                 D::narrow(static_cast<float>(scale * (q - p)));

@@ -101,3 +101,30 @@ def test_a_student_that_rules_entries_or_everything_out(rows, vocab, dtype):
 def test_lengths_on_both_sides_of_where_a_route_ends(chunks, rows, dtype, chunk):
     for vocab in (chunks * chunk, chunks * chunk + 1):
         check_distill(contents("steep", rows, vocab, gen(vocab)), [vocab], dtype, 30, 1.5, in_place=rows == 5)
+
+
+@pytest.mark.parametrize("dtype", [T.FP32, T.BFP16])
+@pytest.mark.parametrize("rows,vocab", ROUTES)
+def test_improbable_entries_keep_their_gradients(rows, vocab, dtype):
+    """A teacher's entries of 1 to 2^-90, a student who finds them as improbable or more: the gradients there are as good as their own size asks for.
+    Where two entries name a column, as 2^-61 asks for."""
+    k, T_, g = 40, 0.25, gen(rows + vocab + 2)
+    x = torch.randn((rows, vocab), device=DEV, generator=g) - 16
+    values = -torch.arange(k, device=DEV).float()[None].repeat(rows, 1) * 0.4
+    at = torch.stack([torch.randperm(vocab, device=DEV, generator=g)[:k] for _ in range(rows)]).to(torch.int32)
+    x[torch.arange(rows, device=DEV)[:, None], at.long()] = values - 3 * torch.rand((rows, k), device=DEV, generator=g)
+    at[:, -1] = at[:, -2]
+    s = Split(x.to(TD[dtype]), shares(vocab, 2), dtype, 3)
+    whole, d = s.whole(), Split(torch.zeros_like(s.whole()), s.columns, dtype, 3)
+    later = Split(torch.zeros_like(whole), s.columns, dtype, 3)
+    stats = torch.zeros((rows, 2), device=DEV)
+    held = dict(s.where, teacher=values.data_ptr(), indices=at.data_ptr(), k=k, teacher_dtype=T.FP32, temperature=T_)
+    hcclx.DistillPlan(s.ptrs, stats=stats.data_ptr(), dlogits=d.ptrs, **held).launch()
+    hcclx.DistillGradPlan(s.ptrs, stats=stats.data_ptr(), dlogits=later.ptrs, **held).launch()
+    torch.cuda.synchronize()
+    for r in [*range(min(rows, 7)), rows - 1]:
+        _, grad, _, bound = L.distill(whole[r].double(), values[r].double(), at[r], T_, 1.0)
+        named = at[r].long()
+        bound[named[-1]] += T_ * 2.0 ** -61
+        for got in (d, later):
+            O.assert_close(got.whole()[r][named], grad[named], bound[named], f"row {r}")
