@@ -401,10 +401,10 @@ __device__ __forceinline__ void nothing(const DistillArgs &a, uint64_t row, uint
     if (GRAD) row_gradient<DT, NT, true>(a, row, from, to, 0.0f, 0.0f);
 }
 
-// A row per workgroup.  Bound by the bytes on their way where there are many rows: 8 ranks, 4096 x 131072 bf16, loss and gradient 478 us, 3.0 GB
-// at 6.3 TB/s, of which the gradient's second reading comes from the last-level cache (four workgroups of 512 on a CU; of 256 540 us, of
-// 1024 497, with the row kept in registers in between 586); 2048 x 65536 fp16, loss alone, 51 us, 4.8 TB/s with the vector units 60 %
-// busy.
+// A row per workgroup.  Bound by the bytes on their way where there are many rows: 8 ranks, 4096 x 131072 bf16, loss and gradient 482 us, 3.0 GB
+// at 6.2 TB/s, of which the gradient's second reading comes from the last-level cache (four workgroups of 512 on a CU; of 256 540 us, of
+// 1024 497, with the row kept in registers in between 586); 2048 x 65536 fp16, loss alone, 52 us, 270 MB at
+// 5.2 TB/s, a tenth of which are lines of 128 bytes for the entries' logits, out of the caches by then.
 template <int DT, bool GRAD, int NT>
 __global__ void __launch_bounds__(NT)
 k_distill_row(DistillArgs a)
@@ -492,7 +492,7 @@ struct Part {
 };
 
 // Several workgroups per row, two launches: r and S of every part, then what is left.  Bound by the chain of one row (16 of
-// 131072 bf16 5 + 8 us).
+// 131072 bf16 12 us).
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
 k_distill_sums(DistillArgs a)
@@ -561,7 +561,7 @@ k_distill_parts(DistillArgs a, uint32_t parts)
 uint32_t parts_of(uint32_t rows, uint32_t nchunks, uint32_t most)
 {
     const uint32_t fill = rows >= most ? 1 : most / rows;
-    // (four chunks for a wavefront: 16 rows of 131072 bf16 13 us in eight workgroups each, 29 in one; of 32000 13 in three, 11.8 in one)
+    // (four chunks for a wavefront: 16 rows of 131072 bf16 12.2 us in eight workgroups each, in four 14.2, in one 29; of 32000 11.7 in three, 11.3 in one)
     return std::max(1u, std::min(fill, nchunks / (kThreads / 64 * kAhead)));
 }
 
@@ -738,7 +738,7 @@ int make_distill_grad(const hcclx_distill_grad_t &d, hcclx_plan_t **plan)
     w->args.stats = reinterpret_cast<float2 *>(const_cast<float *>(d.stats));
     w->saved = true;
     // The parts of a row have nothing to wait for: 32 workgroups for a CU, four of which it holds, even out what a last round of them leaves
-    // idle (1500 rows of 100003 fp32: 250 us, one for a row 290).
+    // idle (1500 rows of 100003 fp32: 256 us, one for a row 277).
     if (l.rows != 0) w->parts = parts_of(l.rows, w->args.rows.nchunks, 32 * static_cast<uint32_t>(ctx->num_cus));
     const uint64_t held = w->table.bytes;
     return plan_of(ctx, std::move(w), 2 * row_bytes(l, vocab), held, plan);

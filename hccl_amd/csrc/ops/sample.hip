@@ -16,9 +16,9 @@
 // A row whose draw goes by more than such a list is left to several workgroups.  Next to the second launch they count its elements by
 // levels of their weight, 64 to a power of two, which says in which level the cut lies; in a third those over that level are weighed and
 // those in it are listed; and a fourth finds the cut among these, and draws.  (One workgroup for all of that: 64 rows of 131072 bf16,
-// a sixth of them such, 112 us instead of 31 to 41.)
+// a sixth of them such, 112 us instead of 36 to 42.)
 //
-// What bounds it: the first launch, by reading (8 x 4096 x 131072 bf16 195 us, 5.5 TB/s, with a sum that keeps the vector units four fifths
+// What bounds it: the first launch, by reading (8 x 4096 x 131072 bf16 197 us, 5.5 TB/s, with a sum that keeps the vector units four fifths
 // busy); the others, by how long one row takes: some twenty steps of a workgroup, each with a barrier, and the fetch of their code.  1 row
 // of 131072 3 us + 10 us + two launches that find nothing to do.
 #include "ops/logits.h"
@@ -35,7 +35,7 @@ constexpr uint32_t kRunWaves = 4;        // of a workgroup of the first launch, 
 constexpr uint32_t kList = 2048;         // elements that are sorted at once
 constexpr uint32_t kSmallTop = 256;      // the longest list of a small workgroup, and the elements that it sorts
 constexpr uint32_t kSmallList = 1024;
-constexpr uint32_t kNucleus = 64;        // listed where no top_k bounds the list (192: 1024 rows 212 us instead of 201, and no row less)
+constexpr uint32_t kNucleus = 64;        // listed where no top_k bounds the list (192: 1024 draws 194 us instead of 186, 64 42.5 instead of 40)
 constexpr uint32_t kLevels = 2048;       // of the weights of a row
 constexpr uint32_t kWholeBits = 51;      // of a weight's whole number where there is no filter
 constexpr uint32_t kBand = 8192;         // elements of a cut's level, shared out to the parts of a row (each lists kList at most: of the most rows 4096)
@@ -1249,7 +1249,8 @@ __device__ __forceinline__ double slack(double n, double whole) { return n * 0x1
 // No filter: the run in which the running sum passes u x the whole, then the element, by such sums.  The whole numbers say the same where both of
 // the element's borders are further from the aim than that can matter: with k elements in front of a border, the distance border - u whole
 // is off by 1 - u of the error of the first k and u of that of the others.
-// Otherwise false is returned, and nothing is drawn (for one row of 131072 columns in some millions).
+// Otherwise false is returned, and nothing is drawn (for one row of 131072 columns in some millions, whose chunks are then weighed again: 76 us
+// more; 1 row takes 9 us without that).
 template <int DT, int NT>
 __device__ __forceinline__ bool draw_all(const SelectArgs &a, Row<DT, NT> &r, Shared &s, float u)
 {
@@ -1440,8 +1441,8 @@ struct WidePart {
 };
 
 // The elements of a part by levels.  Where there are few rows, by workgroups of the second launch that have no row of their own, before it is
-// known whether levels are asked for: by then they are there (37 rows of 50021: 25 us for the draw, 41 with a launch of its own; 1 row 17
-// and 20).  Where rows fill the device that holds up the others (1024 rows of 131072: 222 us for the draw, 199 with a launch of its own,
+// known whether levels are asked for: by then they are there (37 rows of 50021: 32 us for the draw, 37 with a launch of its own; 1 row 16
+// and 17.5; 256 of 131072 73 and 79).  Where rows fill the device that holds up the others (1024 rows of 131072: 225 us for the draw, 186 with a launch of its own,
 // which rows that are not asked leave at once).
 template <int DT, int NT>
 __device__ __forceinline__ void count_levels(const SelectArgs &a, u64 *mine, uint32_t *most, uint32_t block)
@@ -1624,9 +1625,9 @@ __device__ __forceinline__ u64 weigh_chunk(const Team<NT> &r, Shared &s, const D
     return wave_total(sum);
 }
 
-// What stays of a list whose elements the threads hold, kListed each (key 0: none): those from the returned key on.  `skip` of them stay (top_k), or
-// those before whose place in the order the weight is less than `aim`; *front is what is before the last of them.  As by Row::narrow: keys are counted and weighed into equal
-// stretches of their range, which leaves one of them: two rounds, or three where many numbers are alike.
+// What stays of a list whose elements the threads hold, N each (key 0: none): those from the returned key on.  `stay` of them stay (top_k), or
+// those before whose place in the order the weight is less than `aim`; *front is what is before the last of them.  As by Row::narrow: keys are
+// counted and weighed into equal stretches of their range, which leaves one of them: two rounds, or three where many numbers are alike.
 template <int NT, int N>
 __device__ __forceinline__ u64 last_that_stays(Team<NT> &r, Shared &s, const u64 (&key)[N], const u64 (&weight)[N], bool by_count, uint32_t stay, u64 aim, u64 *front)
 {
@@ -2100,7 +2101,7 @@ int finish(const hcclx_logits_t &l, uint32_t vocab, bool sums, std::unique_ptr<S
     SelectArgs &a = w->args;
     a.rows = w->table.rows;
     w->dtype = l.dtype;
-    // As many chunks per wavefront as leave every CU eight workgroups (64 draws of 131072 44.8 us, with four 46.2, with eight chunks 47.7).
+    // As many chunks per wavefront as leave every CU eight workgroups (64 draws of 131072 40.3 us, with four 39.7, with sixteen 41.0).
     a.per_run = 8;
     auto parts = [&] { return (a.rows.nchunks + a.per_run * kRunWaves - 1) / (a.per_run * kRunWaves); };
     while (a.per_run > 1 && static_cast<uint64_t>(l.rows) * parts() < 8ull * static_cast<uint32_t>(ctx->num_cus)) a.per_run /= 2;
@@ -2119,7 +2120,7 @@ int finish(const hcclx_logits_t &l, uint32_t vocab, bool sums, std::unique_ptr<S
         return at;
     };
     // Where rows fill the device more than three times, small workgroups for their lists, of which seven find room on a CU (64 of 4096 rows of
-    // 131072 bf16 244 us, by four large ones 255, of 5000 67 and 86; of 1000 rows 68 and 70, of 600 48 and 46.5).
+    // 131072 bf16 237 us, by four large ones 249, of 5000 67 and 85; of 1000 rows of 5000 22.7 and 26.1, of 600 19.1 and 18.7).
     w->small = a.k <= kSmallTop && l.rows > 3 * static_cast<uint32_t>(ctx->num_cus);
     uint64_t wide = 0, bands = 0, levels = 0, found = 0, listed = 0, spans = 0;
     if (w->sample && l.rows != 0) {
@@ -2131,8 +2132,8 @@ int finish(const hcclx_logits_t &l, uint32_t vocab, bool sums, std::unique_ptr<S
         a.span = (a.rows.nchunks + kMostSpans - 1) / kMostSpans;
         a.nspans = (a.rows.nchunks + a.span - 1) / a.span;
         // Workgroups for a row that may be wide: most rows are not, and their workgroups only look.  In launches of their own eight for a row
-        // (1024 rows of 131072 194 us, with four 211, with two 240), of sixteen chunks at least (of 5000 60, of a chunk at least 65); next to
-        // the lists as many as there is room for (256 rows 76 us with eight, 80 with sixteen, 85 with 32; 1 row 17 with 32).
+        // (1024 rows of 131072 186 us, with four 200, with two 228, with sixteen 188), of sixteen chunks at least (of 5000 65, with eight 71); next to
+        // the lists as many as there is room for (256 rows 73 us with eight, 78 with sixteen, 81 with 32; 1 row 16 with two, eight or 32).
         const uint32_t parts = w->apart ? std::clamp(std::min(8192 / w->batch, (a.rows.nchunks + 15) / 16), 1u, 8u) : std::clamp(2048 / w->batch, 2u, kMostParts);
         a.wide_parts = may_be_wide ? std::min(a.nspans, parts) : 0;
         a.band_each = std::clamp(kBand / std::max(1u, a.wide_parts), 512u, kList);
