@@ -221,7 +221,8 @@ int hcclx_top_logits_plan_create(const hcclx_top_logits_t *top, hcclx_plan_t **p
  * loss 0, gradients 0.  NaN and +infinity in a row that counts, the teacher's or the student's, make its loss and gradients NaN.  A column
  * whose logit is -infinity has q = 0, and so has every column of a row of nothing else: with an entry of p > 0 there the loss is infinite, and its
  * gradient - weight T p.  The sum over the row's columns is held in 32 bits, what concerns the entries alone in 64; where several name a column, the
- * sum of their p is one of multiples of 2^-62.  At columns that none names, what is below 2^-126 of the row's largest weight is 0.
+ * sum of their p is one of multiples of 2^-62.  So a loss is good to some 2^-20 weight T^2 beside its own last bits.  At columns that no entry names,
+ * what is below 2^-126 of the row's largest weight is 0.
  *
  * stats: two floats per row for hcclx_distill_grad_plan_create, 8-byte aligned.  dlogits: one pointer per rank, rows as far apart as
  * the logits', and each may be that rank's logits.  A program that knows the weights before the loss gets the gradients in the same

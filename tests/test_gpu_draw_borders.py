@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import logits_oracle as L
+from hccl_amd import hcclx
 from hccl_amd import types as T
 from test_gpu_output_layer import DEV, TD, Split, draw, gen, shares
 
@@ -143,3 +144,31 @@ def test_top_p_where_min_p_cuts_behind_it(later):
     s = Split(row, shares(vocab, 2), T.FP32)
     got, _ = draw(s, dict(top_p=[top_p], min_p=[2.0 ** (-1546 / 64)]), [1.0])
     assert got == [vocab - 1 - later]
+
+
+@pytest.mark.parametrize("rows", [3, 300])
+@pytest.mark.parametrize("filtered", [False, True])
+def test_borders_in_a_graph_that_is_replayed(rows, filtered):
+    """Rows over 64 ranks that are weighed again, between others, from a graph with other random numbers at every replay."""
+    vocab = 64 * 300
+    half = torch.randn((rows, vocab // 2), device=DEV, generator=gen(rows)) * 2
+    whole = mirrored(half).half()
+    s = Split(whole, [300] * 64, T.FP16, pad=1)
+    random, tokens = torch.zeros(rows, device=DEV), torch.zeros(rows, device=DEV, dtype=torch.int32)
+    neutral = torch.ones(rows, device=DEV)
+    plan = hcclx.SamplePlan(s.ptrs, random=random.data_ptr(), tokens=tokens.data_ptr(), top_p=neutral.data_ptr() if filtered else 0, **s.where)
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        plan.launch(torch.cuda.current_stream().cuda_stream)
+    l = L.plain(s.whole()[0])
+    u, middles = L.middles(l, 1.0, 0, 1.0, 0.0, 5)
+    for x, token in [(0.5, vocab // 2), *zip(u.tolist(), middles.tolist()), (1.0, vocab - 1), (0.0, 0), (0.5, vocab // 2)]:
+        random.fill_(0.5)
+        random[0] = x
+        tokens.fill_(-5)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = tokens.clone()
+        plan.launch()
+        torch.cuda.synchronize()
+        assert got.tolist() == [token] + [vocab // 2] * (rows - 1) and torch.equal(got, tokens), x
