@@ -1441,9 +1441,9 @@ struct WidePart {
 };
 
 // The elements of a part by levels.  Where there are few rows, by workgroups of the second launch that have no row of their own, before it is
-// known whether levels are asked for: by then they are there (37 rows of 50021: 32 us for the draw, 37 with a launch of its own; 1 row 16
-// and 17.5; 256 of 131072 73 and 79).  Where rows fill the device that holds up the others (1024 rows of 131072: 225 us for the draw, 186 with a launch of its own,
-// which rows that are not asked leave at once).
+// known whether levels are asked for: by then they are there (37 rows of 50021: 32 us for the draw, 37 with a launch of its own; 256 of 131072
+// 73 and 79; 1 row 16 and 17.5).  Where rows fill the device that holds up the others (1024 rows of 131072: 225 us for the draw, 186 with a
+// launch of its own, which rows that are not asked leave at once).
 template <int DT, int NT>
 __device__ __forceinline__ void count_levels(const SelectArgs &a, u64 *mine, uint32_t *most, uint32_t block)
 {
